@@ -389,6 +389,41 @@ int ody_attn_bwd_dropout(const void* q, const void* k, const void* v, const void
                          float scale, int causal, int flags, int dtype,
                          void* workspace, size_t workspace_bytes, void* stream, float p_drop, uint64_t seed);
 
+/* ---- key / value cache in pages ---------------------------------------------
+ * What a program that decodes many sequences keeps in the place of the host's cache (past_key_value of decoder/odysseus.py:215-220, which
+ * copies every key with every token): pools of pages that belong to sequences by a table, so that a sequence grows without moving.
+ *
+ * k_pages, v_pages  (pages, page_size, Hkv, D) of `dtype`, strides s*_p (page), s*_r (row of a page), s*_h (head); page_size a power of two
+ *                   from 8 on.  Layouts with heads outside of rows are given by their strides.
+ * page_table        (S, table_width) int32, rows table_stride apart: the page of places [c page_size, (c + 1) page_size) of a sequence.  An
+ *                   entry outside [0, pages) is no page: nothing is written there, its keys take no part, and nothing is read there.
+ *                   Sequences may share pages that none of them appends to.
+ * lengths           (S) int32: tokens of a sequence WITH the n new ones; below 0 as 0.  Device memory, as the table is: a captured graph
+ *                   replays with what they hold then.
+ * New token i sits at place lengths - n + i.  Where that is negative there is no token (shorter sequences of a batch are padded on the left;
+ * length 0 is a sequence that takes no part).  A place behind the table's last column has no page.
+ *
+ * ody_paged_append  qkv (S, n, Hq + 2 Hkv, D), the packed projection, strides sx_*.  q != NULL: queries and keys are rotated as ody_rope
+ *                   rotates them, by position_ids (S, n) int64, contiguous, or with NULL by their places, and inv_freq (D / 2) fp32; the queries go to q
+ *                   (S, n, Hq, D), strides sq_*, 0 where there is no token.  q == NULL: nothing is rotated.  Keys and values go to
+ *                   their pages.  Rows of pages that no new token has keep what they hold.  No two sequences may append to one row.
+ * ody_paged_attn    out (S, n, Hq, D) and lse (S, Hq, n), contiguous fp32, of q (S, n, Hq, D): token i sees the places up to its own that have a
+ *                   page, as ody_attn_fwd's causal mask with Lk = lengths has it; 0 and -inf where that is none.  Query head h reads kv head
+ *                   h / (Hq / Hkv).  workspace: ody_paged_attn_workspace_bytes(...) bytes, 256-byte aligned, of no value before or after.
+ * D in {64, 128}; bf16 and fp32; pointers and strides of qkv, q, out and the pages on 16 bytes.
+ */
+int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v_pages, const int* page_table, const int* lengths,
+                     const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,
+                     int64_t sx_s, int64_t sx_n, int64_t sx_h, int64_t sq_s, int64_t sq_n, int64_t sq_h,
+                     int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
+                     int pages, int page_size, int table_width, int64_t table_stride, int dtype, void* stream);
+size_t ody_paged_attn_workspace_bytes(int S, int n, int Hq, int Hkv, int D, int page_size, int table_width, int dtype);
+int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* lengths, void* out, float* lse,
+                   int S, int n, int Hq, int Hkv, int D, int64_t sq_s, int64_t sq_n, int64_t sq_h,
+                   int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
+                   int64_t so_s, int64_t so_n, int64_t so_h, int pages, int page_size, int table_width, int64_t table_stride,
+                   float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- optimizer ------------------------------------------------------------
  * One step of torch.optim.AdamW (the optimizer of the reference's training loop, train.py:170,216) on one
  * tensor of n elements, in one pass instead of the host framework's seven element-wise passes:

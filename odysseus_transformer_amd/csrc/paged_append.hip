@@ -1,0 +1,123 @@
+// New tokens into a key / value cache in pages, their queries and keys rotated on the way.
+#include <algorithm>
+#include <cmath>
+#include "paged.h"
+
+namespace {
+
+struct AppendParams {
+  const void* x;        // (S, n, Hq + 2 Hkv, D): the packed projection
+  void* q;              // (S, n, Hq, D), or null: nothing is rotated, and the queries stay where they are
+  const int64_t* pos;   // (S, n), or null: the tokens' places in their sequences
+  const float* inv_freq;
+  AttnStrides sx, sq;
+  int S, n, Hq, Hkv;
+};
+
+template <typename T> __device__ __forceinline__ float rounded(float x) { return (float)(T)x; }
+
+// A block takes TOKENS tokens: their angles go to LDS, then consecutive threads take consecutive vectors of a head, x[j] together
+// with x[j + D / 2].  A token before place 0 is none: its queries become 0, nothing else is written.
+template <typename T, int D, int TOKENS, bool ROTATE>
+__global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p, const PagedCache cache) {
+  constexpr int N = Vec16B<T>::N, HALF = D / 2, VECS = HALF / N;
+  typedef typename Vec16B<T>::type vec;
+  __shared__ __attribute__((aligned(16))) float cs[TOKENS][HALF], sn[TOKENS][HALF];
+  const int64_t first = (int64_t)blockIdx.x * TOKENS, all = (int64_t)p.S * p.n;
+  const int mine = (int)min((int64_t)TOKENS, all - first);
+  if (ROTATE) {
+    for (int e = threadIdx.x; e < mine * HALF; e += 256) {
+      const int t = e / HALF, j = e % HALF, s = (int)((first + t) / p.n), i = (int)((first + t) % p.n);
+      const float pos = p.pos ? (float)p.pos[first + t] : (float)(max(cache.lengths[s], 0) - p.n + i);
+      const float th = pos * p.inv_freq[j];
+      cs[t][j] = rounded<T>(cosf(th));   // rounded to the values' type before use, as ody_rope has them
+      sn[t][j] = rounded<T>(sinf(th));
+    }
+    __syncthreads();
+  }
+  const int h0 = ROTATE ? 0 : p.Hq, heads = p.Hq + 2 * p.Hkv - h0;
+  for (int v = threadIdx.x; v < mine * heads * VECS; v += 256) {
+    const int j = v % VECS * N, h = h0 + v / VECS % heads, t = v / (VECS * heads);
+    const int s = (int)((first + t) / p.n), i = (int)((first + t) % p.n);
+    const int place = max(cache.lengths[s], 0) - p.n + i;
+    const T* src = static_cast<const T*>(p.x) + s * p.sx.b + i * p.sx.l + h * p.sx.h + j;
+    T* dst;
+    if (h < p.Hq) {
+      dst = static_cast<T*>(p.q) + s * p.sq.b + i * p.sq.l + h * p.sq.h + j;
+      if (place < 0) {
+        const vec zero = {};
+        *reinterpret_cast<vec*>(dst) = zero;
+        *reinterpret_cast<vec*>(dst + HALF) = zero;
+        continue;
+      }
+    } else {
+      if (place < 0 || place >> cache.shift >= cache.width) continue;
+      const int page = cache.table[s * cache.table_stride + (place >> cache.shift)], row = place & ((1 << cache.shift) - 1);
+      if (page < 0 || page >= cache.pages) continue;
+      const bool key = h < p.Hq + p.Hkv;
+      const int hk = h - p.Hq - (key ? 0 : p.Hkv);
+      const PageStrides& st = key ? cache.sk : cache.sv;
+      dst = static_cast<T*>(key ? cache.k : cache.v) + page * st.p + row * st.r + hk * st.h + j;
+    }
+    vec a = *reinterpret_cast<const vec*>(src), b = *reinterpret_cast<const vec*>(src + HALF);
+    if (ROTATE && h < p.Hq + p.Hkv) {
+      vec a1, b1;
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const float c = cs[t][j + e], sine = sn[t][j + e], x1 = (float)a[e], x2 = (float)b[e];
+        a1[e] = (T)(x1 * c - x2 * sine);
+        b1[e] = (T)(x2 * c + x1 * sine);
+      }
+      a = a1, b = b1;
+    }
+    *reinterpret_cast<vec*>(dst) = a;
+    *reinterpret_cast<vec*>(dst + HALF) = b;
+  }
+}
+
+template <typename T, int D, int TOKENS>
+int launch(const AppendParams& p, const PagedCache& cache, hipStream_t st) {
+  const int64_t all = (int64_t)p.S * p.n;
+  const dim3 grid((unsigned)((all + TOKENS - 1) / TOKENS));
+  if (p.q) ODY_LAUNCH("paged_append", st, (paged_append_kernel<T, D, TOKENS, true>), grid, dim3(256), 0, p, cache);
+  else ODY_LAUNCH("paged_append", st, (paged_append_kernel<T, D, TOKENS, false>), grid, dim3(256), 0, p, cache);
+  return ody_check_launch("paged_append");
+}
+template <typename T>
+int by_head_dim(const AppendParams& p, int D, const PagedCache& cache, hipStream_t st) {
+  return D == 64 ? launch<T, 64, 1>(p, cache, st) : launch<T, 128, 1>(p, cache, st);
+}
+
+}  // namespace
+
+int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype, const PagedCache& c, int page_size) {
+  ODY_REQUIRE(c.k && c.v && c.table && c.lengths, ODY_ERR_NULL, "%s: k_pages, v_pages, page_table or lengths is NULL", who);
+  ODY_REQUIRE(S > 0 && n > 0 && Hq > 0 && Hkv > 0 && c.pages > 0 && c.width > 0, ODY_ERR_BAD_SHAPE,
+              "%s: sizes must be positive (S=%d n=%d Hq=%d Hkv=%d pages=%d table_width=%d)", who, S, n, Hq, Hkv, c.pages, c.width);
+  ODY_REQUIRE(Hq % Hkv == 0, ODY_ERR_BAD_SHAPE, "%s: Hq=%d is not a multiple of Hkv=%d", who, Hq, Hkv);
+  ODY_REQUIRE(D == 64 || D == 128, ODY_ERR_UNSUPPORTED, "%s: head_dim %d not built (64, 128)", who, D);
+  ODY_REQUIRE(dtype == ODY_BF16 || dtype == ODY_F32, ODY_ERR_UNSUPPORTED, "%s: dtype %d unknown", who, dtype);
+  ODY_REQUIRE(page_size >= 8 && (page_size & (page_size - 1)) == 0, ODY_ERR_UNSUPPORTED, "%s: page_size %d: a power of two from 8 on", who, page_size);
+  ODY_REQUIRE((int64_t)c.width * page_size < (int64_t)1 << 31 && (int64_t)S * n * (Hq + 2 * (int64_t)Hkv) < (int64_t)1 << 31, ODY_ERR_BAD_SHAPE,
+              "%s: 2^31 tokens of a sequence, or heads of all new tokens, and more", who);
+  ODY_REQUIRE(c.table_stride >= c.width || S == 1, ODY_ERR_BAD_SHAPE, "%s: rows of the page table overlap", who);
+  ODY_REQUIRE(paged_rows_aligned(c.k, c.sk.p, c.sk.r, c.sk.h, dtype) && paged_rows_aligned(c.v, c.sv.p, c.sv.r, c.sv.h, dtype), ODY_ERR_MISALIGNED,
+              "%s: k_pages and v_pages need 16-byte aligned pointers and strides", who);
+  return ODY_OK;
+}
+
+extern "C" int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v_pages, const int* page_table, const int* lengths,
+                                const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,
+                                int64_t sx_s, int64_t sx_n, int64_t sx_h, int64_t sq_s, int64_t sq_n, int64_t sq_h,
+                                int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
+                                int pages, int page_size, int table_width, int64_t table_stride, int dtype, void* stream) {
+  const PagedCache c{k_pages, v_pages, page_table, lengths, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride, pages, paged_shift(page_size),
+                     table_width};
+  if (int rc = paged_check("ody_paged_append", S, n, Hq, Hkv, D, dtype, c, page_size)) return rc;
+  ODY_REQUIRE(qkv && (q == nullptr || inv_freq), ODY_ERR_NULL, "ody_paged_append: qkv, or inv_freq of a rotation, is NULL");
+  ODY_REQUIRE(paged_rows_aligned(qkv, sx_s, sx_n, sx_h, dtype) && (q == nullptr || paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype)), ODY_ERR_MISALIGNED,
+              "ody_paged_append: qkv and q need 16-byte aligned pointers and strides");
+  const AppendParams p{qkv, q, position_ids, inv_freq, {sx_s, sx_n, sx_h}, {sq_s, sq_n, sq_h}, S, n, Hq, Hkv};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return dtype == ODY_BF16 ? by_head_dim<bf16>(p, D, c, st) : by_head_dim<float>(p, D, c, st);
+}

@@ -1,0 +1,396 @@
+"""A key / value cache in pages: appending with the rotation, attention over it, against 64 bits on the CPU."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _to(c, dev):
+    def move(t):   # keeps the strides: what is tested with a layout is that layout
+        return torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=dev).copy_(t)
+    return {k: move(t) if torch.is_tensor(t) else t for k, t in c.items()}
+
+
+def _inv_freq(D, base=10000.0):
+    return 1.0 / (base ** (torch.arange(0, D, 2, dtype=torch.int64).float() / D))
+
+
+def _check_attn(c, g, scale=None):
+    from odysseus_transformer_amd import ops
+    out, lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"], scale=scale)
+    torch.cuda.synchronize()
+    o, s, mean, dots = ref.attend(c, scale)
+    tol_o, tol_s = ref.attend_bounds(c, o, s, mean, dots)
+    out, lse = out.double().cpu(), lse.double().cpu()
+    none = s == -math.inf
+    assert torch.equal(lse == -math.inf, none)
+    assert (out[none.transpose(1, 2)] == 0).all()
+    bad = (out - o).abs() > tol_o
+    assert not bad.any(), f"out: {int(bad.sum())} of {bad.numel()} beyond their bounds, worst {((out - o).abs() / tol_o).max():.2f}"
+    bad = ((lse - s).abs() > tol_s) & ~none
+    assert not bad.any(), f"lse: {int(bad.sum())} beyond their bounds, worst {((lse - s).abs()[~none] / tol_s[~none]).max():.2f}"
+
+
+def _check_append(c, g, Hq, positions=None, rotate=True):
+    from odysseus_transformer_amd import ops
+    D, dtype = c["q"].shape[3], c["q"].dtype
+    f = _inv_freq(D)
+    (q, q_size), (k, k_size), v = ref.append(c, Hq, f if rotate else None, positions)
+    qkv = g["qkv"].clone()
+    got = ops.paged_append_(g["qkv"], Hq, g["k"], g["v"], g["table"], g["lengths"],
+                            position_ids=None if positions is None else positions.to(g["qkv"].device),
+                            inv_freq=f.to(g["qkv"].device) if rotate else None, rotate=rotate)
+    torch.cuda.synchronize()
+    assert torch.equal(g["qkv"], qkv), "the projection was written to"
+    assert torch.equal(g["v"].cpu(), v.to(dtype)), "values"
+    if not rotate:
+        assert got.data_ptr() == g["qkv"].data_ptr() and torch.equal(got, g["qkv"][:, :, :Hq])
+        assert torch.equal(g["k"].cpu(), k.to(dtype)), "keys"
+        return
+    half = torch.finfo(dtype).eps / 2
+    for name, have, want, size in (("q", got, q, q_size), ("k", g["k"], k, k_size)):
+        have = have.double().cpu()
+        assert torch.equal(have[size == 0], want[size == 0]), f"{name}: rows without a new token"
+        # one rounding of the result, the sum's in 32 bits, and a cosine within 2^-23 of the middle of two values of the type, which may round to either
+        # one: a step of the type of one of the two products
+        err = (have - want).abs()
+        assert (err <= half * want.abs() + (2 * half + 2 ** -22) * size).all(), name
+        # but hardly any of them do
+        assert err.norm() <= (half + 2 ** -12 * half + 2 ** -22) * want.norm() + 2 * half * size.norm() * 2 ** -4, name
+        tight = err <= half * want.abs() + 2 ** -21 * size
+        assert tight.double().mean() > 0.998, f"{name}: {1 - tight.double().mean().item():.1e} of the values are further than their rounding"
+
+
+APPEND = [
+    # lengths, n, Hq, Hkv, D, page, dtype, layout
+    ([1], 1, 1, 1, 128, 16, BF16, "rows"),
+    ([5, 0, 17, 33, 8], 1, 4, 2, 128, 8, BF16, "rows"),            # a sequence that takes no part
+    ([9, 3, 40], 9, 8, 2, 64, 16, BF16, "heads"),                  # padded on the left
+    ([300, 131, 70], 67, 6, 3, 128, 32, BF16, "mixed"),
+    ([100, 20], 33, 5, 1, 64, 64, F32, "rows"),
+    ([41, 0, 1], 7, 4, 4, 128, 8, F32, "mixed"),
+    ([2, 1], 2, 8, 8, 64, 256, F32, "heads"),
+    ([700], 700, 4, 1, 128, 128, BF16, "rows"),
+    (list(range(1, 98)), 1, 2, 1, 64, 16, BF16, "rows"),
+]
+
+
+@pytest.mark.parametrize("case", APPEND, ids=lambda c: "S%d_max%d_n%d_H%d_%d_D%d_p%d_%s_%s" % (len(c[0]), max(c[0]), *c[1:6], str(c[6])[-4:], c[7]))
+def test_append(case, dev):
+    lengths, n, Hq, Hkv, D, page, dtype, layout = case
+    print(f"append {case}", flush=True)
+    c = ref.make(lengths, n, Hq, Hkv, D, page, dtype, seed=n + Hq, layout=layout)
+    _check_append(c, _to(c, dev), Hq)
+    _check_append(c, _to(c, dev), Hq, rotate=False)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_append_with_positions_of_its_own(dtype, dev):
+    """Positions apart from the places: far ones, whose angles are products of 32 bits, of each sequence and shared by all."""
+    c = ref.make([50, 11, 30], 4, 4, 2, 128, 16, dtype, seed=3)
+    own = torch.tensor([[131071, 0, 7, 99999], [1, 2, 3, 4], [65536, 65537, 12, 0]])
+    _check_append(c, _to(c, dev), 4, positions=own)
+    g = _to(c, dev)
+    from odysseus_transformer_amd import ops
+    shared = torch.tensor([3, 4, 5, 6], device=dev)
+    a = ops.paged_append_(g["qkv"], 4, g["k"], g["v"], g["table"], g["lengths"], position_ids=shared)
+    b = ops.paged_append_(g["qkv"], 4, g["k"], g["v"], g["table"], g["lengths"], position_ids=shared.to(torch.int32).expand(3, 4).contiguous())
+    assert torch.equal(a, b)
+
+
+def test_append_rotates_as_rope_does(dev):
+    from odysseus_transformer_amd import ops
+    for dtype in (BF16, F32):
+        c = ref.make([77, 77], 77, 6, 2, 128, 16, dtype, seed=8)
+        g = _to(c, dev)
+        q = ops.paged_append_(g["qkv"], 6, g["k"], g["v"], g["table"], g["lengths"])
+        x = g["qkv"].clone()
+        ops.rope_(x, 8)
+        assert torch.equal(q, x[:, :, :6])
+        pages, rows = g["table"].long()[:, torch.arange(77) // 16], torch.arange(77, device=dev) % 16
+        assert torch.equal(g["k"][pages, rows], x[:, :, 6:8])
+
+
+ATTN = [
+    # lengths, n, Hq, Hkv, D, page, dtype, layout
+    ([1], 1, 1, 1, 128, 16, BF16, "rows"),
+    ([1], 1, 1, 1, 64, 8, F32, "rows"),
+    ([100], 1, 4, 1, 128, 16, BF16, "rows"),
+    ([5, 0, 17, 33, 8, 128, 129, 127, 31, 32], 1, 4, 2, 128, 8, BF16, "rows"),
+    ([700, 1, 64, 1029], 1, 8, 2, 64, 32, BF16, "heads"),
+    ([2000, 513, 4], 1, 32, 8, 128, 64, BF16, "mixed"),
+    ([600, 77], 1, 32, 1, 128, 16, BF16, "rows"),                 # 32 rows of one kv head
+    ([600, 77], 1, 40, 1, 64, 16, BF16, "rows"),                  # 40
+    ([400, 70], 1, 71, 1, 128, 16, BF16, "rows"),                 # 71
+    ([300, 2], 5, 7, 1, 128, 16, BF16, "rows"),                   # 35 rows, padded on the left
+    ([150, 40, 3, 0], 8, 8, 8, 64, 16, BF16, "heads"),
+    ([333], 333, 4, 1, 128, 32, BF16, "rows"),                    # a whole prompt
+    ([400, 90, 200], 130, 6, 2, 128, 64, BF16, "mixed"),
+    ([260, 129], 65, 4, 4, 64, 8, BF16, "rows"),
+    ([500, 33, 1, 0], 1, 8, 8, 64, 32, F32, "rows"),
+    ([290, 40], 1, 24, 2, 128, 16, F32, "heads"),
+    ([129, 64, 31], 6, 6, 2, 64, 8, F32, "mixed"),
+    ([150, 20], 40, 4, 2, 128, 16, F32, "rows"),
+    ([4096 + 3], 1, 8, 8, 128, 128, BF16, "rows"),
+    ([3000], 1, 2, 2, 64, 256, F32, "rows"),
+    (list(range(0, 260, 2)), 1, 2, 1, 64, 16, BF16, "rows"),      # more sequences than a wavefront has lanes
+    ([8] * 300 + [900], 1, 2, 2, 64, 8, BF16, "rows"),
+]
+_ids = lambda c: "S%d_max%d_n%d_H%d_%d_D%d_p%d_%s_%s" % (len(c[0]), max(c[0]), *c[1:6], str(c[6])[-4:], c[7])  # noqa: E731
+
+
+@pytest.mark.parametrize("case", ATTN, ids=_ids)
+def test_attn(case, dev):
+    lengths, n, Hq, Hkv, D, page, dtype, layout = case
+    print(f"attn {case}", flush=True)
+    c = ref.make(lengths, n, Hq, Hkv, D, page, dtype, seed=n + Hq + D, layout=layout)
+    _check_attn(c, _to(c, dev))
+
+
+def test_attn_scale_and_strided_queries(dev):
+    c = ref.make([90, 200], 3, 4, 2, 128, 16, BF16, seed=1)
+    g = _to(c, dev)
+    for scale in (0.25, 0.0, -0.1):
+        _check_attn(c, g, scale)
+    c["q"] = c["qkv"][:, :, :4]
+    g["q"] = g["qkv"][:, :, :4]                                   # a slice of the packed projection
+    _check_attn(c, g)
+
+
+def test_unowned_rows_are_neither_read_nor_written(dev):
+    """NaN in every row that belongs to no token, the tail of the last pages among them."""
+    from odysseus_transformer_amd import ops
+    c = ref.make([37, 5, 130], 1, 4, 2, 128, 16, BF16, seed=2)
+    owned = torch.zeros(c["k"].shape[:2], dtype=torch.bool)
+    for s, length in enumerate(c["lengths"].tolist()):
+        for j in range(length):
+            owned[ref.page_of(c, s, j)] = True
+    for t in ("k", "v"):
+        c[t][~owned] = float("nan")
+    g = _to(c, dev)
+    _check_attn(c, g)
+    ops.paged_append_(g["qkv"], 4, g["k"], g["v"], g["table"], g["lengths"])
+    for t in ("k", "v"):
+        now = g[t].cpu()
+        assert now[~owned].isnan().all()
+        assert torch.isfinite(now[owned]).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_entries_that_are_no_page(n, dev):
+    """Table entries outside the pool (below, at its end, far behind): their places hold nothing and nothing is written or read there;
+    lengths behind the last column and below zero likewise."""
+    c = ref.make([200, 100, 100, 64, 90], n, 4, 2, 64, 16, BF16, seed=5)
+    pages = c["k"].shape[0]
+    c["table"][0, 3] = -1
+    c["table"][0, 12] = pages                                     # the newest tokens'
+    c["table"][1, 0] = 2 ** 31 - 1
+    c["table"][2, :] = -2 ** 31
+    c["lengths"][3] = 2 ** 31 - 1                                 # far beyond what the table can hold
+    c["lengths"][4] = -2 ** 31
+    c["table"][3, 4:] = -1
+    if n == 1:
+        c["table"][3, 5] = c["table"][3, 1]
+    g = _to(c, dev)
+    full = dict(c, lengths=c["lengths"].clone())
+    # in 64 bits a length of 2^31 - 1 is walked by its columns only: all places of the table are before every new token
+    full["lengths"][3] = c["table"].shape[1] * 16 + n
+    _check_attn(full, g)
+    c2 = dict(full)
+    from odysseus_transformer_amd import ops
+    before = g["k"].clone(), g["v"].clone()
+    f = _inv_freq(64)
+    (q, q_size), (k, k_size), v = ref.append(c2, 4, f)
+    got = ops.paged_append_(g["qkv"], 4, g["k"], g["v"], g["table"], g["lengths"], inv_freq=f.to(dev))
+    assert torch.equal(g["v"].cpu(), v.to(BF16))
+    untouched = k_size == 0
+    assert torch.equal(g["k"].cpu()[untouched], before[0].cpu()[untouched])
+    assert (got[4] == 0).all() and torch.isfinite(got).all()
+
+
+def test_sequences_that_share_pages(dev):
+    c = ref.make([80, 80, 80], 1, 4, 2, 128, 16, BF16, seed=6)
+    c["table"][1, :4] = c["table"][0, :4]
+    c["table"][2, :5] = c["table"][0, 0]                          # one page five times
+    _check_attn(c, _to(c, dev))
+
+
+def test_infinite_and_nan_values_reach_their_own_sequence_only(dev):
+    from odysseus_transformer_amd import ops
+    c = ref.make([60, 60, 60, 60], 1, 4, 2, 128, 16, BF16, seed=7)
+    g = _to(c, dev)
+    clean, clean_lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"])
+    g["k"][int(c["table"][1, 1]), 3, 0] = float("nan")            # kv head 0: query heads 0, 1
+    g["v"][int(c["table"][2, 2]), 1, 1] = float("inf")
+    out, lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"])
+    assert out[1, 0, :2].isnan().all() and lse[1, :2].isnan().all()
+    assert torch.equal(out[1, 0, 2:], clean[1, 0, 2:])
+    assert (out[2, 0, 2:] == float("inf")).all() and torch.equal(lse[2], clean_lse[2]) and torch.equal(out[2, 0, :2], clean[2, 0, :2])
+    for s in (0, 3):
+        assert torch.equal(out[s], clean[s]) and torch.equal(lse[s], clean_lse[s])
+
+
+def test_large_scores(dev):
+    """Scores far apart, the largest last and first: no sum overflows or vanishes."""
+    for at in (0, 250, 299):
+        c = ref.make([300], 1, 2, 1, 64, 16, BF16, seed=9)
+        c["k"] *= 4
+        place = ref.page_of(c, 0, at)
+        c["k"][place] = c["q"][0, 0, 0] * 6
+        _check_attn(c, _to(c, dev))
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Pages whose elements lie more than 2^31 from the pool's start."""
+    pages, page, Hkv, D = 17000, 128, 8, 128                       # 2.2e9 elements
+    from odysseus_transformer_amd import ops
+    k = torch.zeros((pages, page, Hkv, D), dtype=BF16, device=dev)
+    v = torch.zeros((pages, page, Hkv, D), dtype=BF16, device=dev)
+    ids = [0, 16999, 16500, 3]
+    table = torch.tensor([ids], dtype=torch.int32, device=dev)
+    small = ref.make([400], 1, 16, Hkv, D, page, BF16, seed=11)
+    for c, p in enumerate(ids):
+        k[p].copy_(small["k"][int(small["table"][0, c])])
+        v[p].copy_(small["v"][int(small["table"][0, c])])
+    lengths = torch.tensor([400], dtype=torch.int32, device=dev)
+    g = _to(small, dev)
+    for n in (1, 40):
+        q = torch.randn((1, n, 16, D), device=dev).to(BF16)
+        want = ops.paged_attn(q, g["k"], g["v"], g["table"], g["lengths"])
+        got = ops.paged_attn(q, k, v, table, lengths)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    lengths += 20                                                  # into page 3 from place 384 on
+    qkv = torch.randn((1, 200, 32, D), device=dev).to(BF16)
+    ops.paged_append_(qkv, 16, k, v, table, lengths, rotate=False)
+    rows = torch.arange(220, 420, device=dev)
+    at = (torch.tensor(ids, device=dev)[rows // page], rows % page)
+    assert torch.equal(v[at], qkv[0, :, 24:]) and torch.equal(k[at], qkv[0, :, 16:24])
+
+
+def test_attends_what_was_appended_step_by_step(dev):
+    """A prompt, then single tokens, against attention over the whole sequence at once."""
+    from odysseus_transformer_amd import ops
+    L0, steps, Hq, Hkv, D, page = 45, 23, 8, 2, 128, 16
+    for dtype in (BF16, F32):
+        x = torch.randn((1, L0 + steps, Hq + 2 * Hkv, D), generator=torch.Generator().manual_seed(4)).to(dtype).to(dev)
+        whole = x.clone()
+        ops.rope_(whole, Hq + Hkv)
+        want, want_lse = ops.attn_fwd(whole[:, :, :Hq], whole[:, :, Hq:Hq + Hkv], whole[:, :, Hq + Hkv:], causal=True)
+        k, v = (torch.full((7, page, Hkv, D), float("nan"), dtype=dtype, device=dev) for _ in range(2))
+        table = torch.tensor([[4, 0, 6, 2, 5]], dtype=torch.int32, device=dev)
+        lengths = torch.zeros(1, dtype=torch.int32, device=dev)
+        out, lse = [], []
+        for a, b in [(0, L0)] + [(t, t + 1) for t in range(L0, L0 + steps)]:
+            lengths += b - a
+            q = ops.paged_append_(x[:, a:b], Hq, k, v, table, lengths)
+            o, s = ops.paged_attn(q, k, v, table, lengths)
+            out.append(o)
+            lse.append(s)
+        out, lse = torch.cat(out, 1), torch.cat(lse, 2)
+        # both round p and the result once: twice the bound of one
+        half = torch.finfo(dtype).eps / 2
+        bound = 2 * (2 * half + 1e-5) * whole[:, :, Hq + Hkv:].float().abs().amax()
+        assert (out.float() - want.float()).abs().max() <= bound
+        assert (lse - want_lse).abs().max() <= 1e-4
+
+
+def test_replayed_from_a_graph_with_other_lengths_and_pages(dev):
+    """A decoding step as a captured graph: appended to and attended with whatever table and lengths hold at the replay; two graphs that
+    take turns, eager calls between them."""
+    from odysseus_transformer_amd import ops
+    Hq, Hkv, D, page = 8, 2, 128, 16
+    base = ref.make([40, 3, 0, 90], 1, Hq, Hkv, D, page, BF16, seed=12)
+    wide = ref.make([40] * 40, 1, Hq, Hkv, D, page, BF16, seed=13)
+    sets, graphs = [_to(base, dev), _to(wide, dev)], []
+
+    def step(g):
+        q = ops.paged_append_(g["qkv"], Hq, g["k"], g["v"], g["table"], g["lengths"])
+        return ops.paged_attn(q, g["k"], g["v"], g["table"], g["lengths"])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for g in sets:
+            step(g)
+    torch.cuda.current_stream().wait_stream(side)
+    for g in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = step(g)
+        graphs.append((graph, res))
+    for turn in range(3):
+        for g, (graph, res) in zip(sets, graphs):
+            g["lengths"].copy_((g["lengths"] + 1) * (g["lengths"] > 0))
+            g["qkv"].normal_()
+            pools = g["k"].clone(), g["v"].clone()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = res[0].clone(), res[1].clone(), g["k"].clone(), g["v"].clone()
+            g["k"].copy_(pools[0])
+            g["v"].copy_(pools[1])
+            want = step(g)
+            for a, b in zip(got, (*want, g["k"], g["v"])):
+                assert torch.equal(a, b), f"turn {turn}"
+
+
+def test_calls_on_two_streams_at_once(dev):
+    from odysseus_transformer_amd import ops
+    cs = [_to(ref.make([900, 30, 411], 1, 16, 4, 128, 32, BF16, seed=20 + i), dev) for i in range(2)]
+    want = [ops.paged_attn(c["q"], c["k"], c["v"], c["table"], c["lengths"]) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, (s, c) in enumerate(zip(streams, cs)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.paged_attn(c["q"], c["k"], c["v"], c["table"], c["lengths"]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, s in got[i]:
+            assert torch.equal(o, want[i][0]) and torch.equal(s, want[i][1])
+
+
+def test_nothing_to_do(dev):
+    from odysseus_transformer_amd import ops
+    c = _to(ref.make([5, 6], 1, 4, 2, 64, 8, BF16, seed=1), dev)
+    q = ops.paged_append_(c["qkv"][:, :0], 4, c["k"], c["v"], c["table"], c["lengths"])
+    assert q.shape == (2, 0, 4, 64)
+    out, lse = ops.paged_attn(c["q"][:0], c["k"], c["v"], c["table"][:0], c["lengths"][:0])
+    assert out.shape == (0, 1, 4, 64) and lse.shape == (0, 4, 1)
+
+
+def test_refusals(dev):
+    from odysseus_transformer_amd import ops
+    from odysseus_transformer_amd._lib import OdysseusHipError
+    c = _to(ref.make([5, 6], 1, 4, 2, 64, 8, BF16, seed=1), dev)
+    args = lambda **kw: [{**c, **kw}[k] for k in ("k", "v", "table", "lengths")]  # noqa: E731
+    for kw in (dict(k=c["k"].float()), dict(v=c["v"][:, :, :1]), dict(table=c["table"].long()), dict(table=c["table"][:1]), dict(table=c["table"].t().contiguous().t()),
+               dict(lengths=c["lengths"].long()), dict(lengths=c["lengths"][:1]), dict(k=c["k"].transpose(2, 3), v=c["v"].transpose(2, 3))):
+        with pytest.raises(ValueError):
+            ops.paged_attn(c["q"], *args(**kw))
+        with pytest.raises(ValueError):
+            ops.paged_append_(c["qkv"], 4, *args(**kw))
+    with pytest.raises(ValueError):
+        ops.paged_append_(c["qkv"], 3, *args())
+    with pytest.raises(ValueError):
+        ops.paged_append_(c["qkv"], 4, *args(), position_ids=torch.zeros((2, 3), dtype=torch.int64, device=dev))
+    with pytest.raises(TypeError):
+        ops.paged_attn(c["q"].half(), c["k"].half(), c["v"].half(), c["table"], c["lengths"])
+    with pytest.raises(OdysseusHipError):          # 3 heads on 2
+        ops.paged_attn(c["q"][:, :, :3], *args())
+    with pytest.raises(OdysseusHipError):          # a page of 5 rows
+        ops.paged_attn(c["q"], *args(k=c["k"][:, :5], v=c["v"][:, :5]))
+    with pytest.raises(OdysseusHipError):          # a row that does not start on 16 bytes
+        flat = torch.zeros(c["q"].numel() + 1, dtype=BF16, device=dev)
+        ops.paged_attn(flat[1:].view(c["q"].shape), *args())
+    with pytest.raises(RuntimeError):
+        ops.paged_attn(c["q"].clone().requires_grad_(True), *args())
+    with torch.no_grad():
+        ops.paged_attn(c["q"].clone().requires_grad_(True), *args())
+    with pytest.raises(RuntimeError):
+        ops.paged_attn(c["q"].cpu(), *args())
