@@ -1,62 +1,385 @@
 // Attention of new tokens over a key / value cache in pages.
+//
+// Bound by reading K and V once.  A wavefront takes a tile of keys (32 in bf16, 16 in fp32) for all rows of a row tile (16 NT of them: the
+// query heads that share a kv head, times the new tokens) at once, and nothing but registers lies between memory and the matrix cores:
+//
+//      S^T = K Q^T          A: K rows in operand order, 16 bytes a lane        B: Q^T, in registers
+//      O^T += V^T P^T       A: V^T, the lane's own rows transposed in its registers   B: P^T = accumulator layout of S^T
+//
+// on v_mfma_f32_16x16x32_bf16 / v_mfma_f32_16x16x4_f32 (lane = 16 q + c: A row c / B column c; accumulator column c, rows 4 q .. 4 q + 3).  The key that
+// row c of a K operand stands for is chosen so that a lane's scores are those of GK keys in a row, tile + GK q ..: its P is then the B operand for the very
+// keys whose V rows this lane loads.  V rows are loaded GK at a time with 16 lanes on a row; component i of the vectors is row c of operand i, which
+// stands for column c * DV + i of V, so the transposition is bytes exchanged within a lane (bf16) or nothing at all (fp32).
+// Loads run one tile ahead of the products, the page numbers two.  A group of GK keys lies within a page: two table entries a lane and tile.
+#include <algorithm>
 #include <cmath>
 #include "paged.h"
 
 namespace {
 
-struct PagedAttnParams {
-  const void* q;   // (S, n, Hq, D)
-  void* out;       // (S, n, Hq, D)
-  float* lse;      // (S, Hq, n)
-  AttnStrides sq, so;
-  int S, n, Hq, Hkv, group;
-  float scale_log2e;
+constexpr int WAVES = 4, BLOCKS = 512;   // two blocks on each of 256 compute units
+
+template <typename T, int D> struct Tile;
+template <int D> struct Tile<bf16, D> {
+  static constexpr int KEYS = 32, GK = 8, KV = 2 * (D / 32), DV = D / 16;   // keys, keys of a group, K vectors and V columns a lane
+  typedef bf16x8 kvec;
+  typedef bf16 vvec __attribute__((ext_vector_type(DV)));
+  // K vector j of a lane: operand row c stands for key 8 (c / 4) + 4 (j / (D / 32)) + c % 4
+  __device__ static int key_row(int c, int j) { return 4 * (j / (D / 32)) + (c & 3); }
+  __device__ static int key_col(int q, int j) { return 32 * (j % (D / 32)) + 8 * q; }
+};
+template <int D> struct Tile<float, D> {
+  static constexpr int KEYS = 16, GK = 4, KV = D / 16, DV = D / 16;
+  typedef f32x4 kvec;
+  typedef float vvec __attribute__((ext_vector_type(DV)));
+  __device__ static int key_row(int c, int) { return c & 3; }
+  __device__ static int key_col(int q, int j) { return 16 * j + 4 * q; }
 };
 
-// One wavefront per (sequence, token, query head), a key after the other.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void paged_attn_kernel(const PagedAttnParams p, const PagedCache cache) {
-  constexpr int N = D / 64;
-  const int lane = threadIdx.x, h = blockIdx.x % p.Hq, i = blockIdx.x / p.Hq % p.n, s = blockIdx.x / (p.Hq * p.n), hk = h / p.group;
-  float q[N], o[N], m = -INFINITY, l = 0.f;
+struct Loaded {   // one tile of keys
+  typename Tile<T, D>::kvec k[Tile<T, D>::KV];
+  typename Tile<T, D>::vvec v[Tile<T, D>::GK];
+  bool page;      // the lane's keys, tile + GK q .., have one
+};
+
+// scores of the lane's GK keys against column c's query row
+template <int D>
+__device__ __forceinline__ void scores(const Loaded<bf16, D>& t, const bf16x8 (&qf)[D / 32], float (&x)[8]) {
 #pragma unroll
-  for (int e = 0; e < N; e++) {
-    q[e] = (float)static_cast<const T*>(p.q)[s * p.sq.b + i * p.sq.l + h * p.sq.h + lane * N + e] * p.scale_log2e;
-    o[e] = 0.f;
+  for (int st = 0; st < 2; st++) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ks++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t.k[st * (D / 32) + ks], qf[ks], s, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; r++) x[4 * st + r] = s[r];
   }
-  const int keys = min(paged_length(cache, s), max(cache.lengths[s], 0) - p.n + i + 1);
-  for (int k = 0; k < keys; k++) {
-    const int page = cache.table[s * cache.table_stride + (k >> cache.shift)], row = k & ((1 << cache.shift) - 1);
-    if (page < 0 || page >= cache.pages) continue;
-    const T* kp = static_cast<const T*>(cache.k) + page * cache.sk.p + row * cache.sk.r + hk * cache.sk.h + lane * N;
-    const T* vp = static_cast<const T*>(cache.v) + page * cache.sv.p + row * cache.sv.r + hk * cache.sv.h + lane * N;
-    float x = 0.f;
+}
+template <int D>
+__device__ __forceinline__ void scores(const Loaded<float, D>& t, const f32x4 (&qf)[D / 16], float (&x)[4]) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < N; e++) x = fmaf(q[e], (float)kp[e], x);
+  for (int j = 0; j < D / 16; j++)
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
-    const float top = fmaxf(m, x), ref = top == -INFINITY ? 0.f : top, alpha = ody_exp2(m - ref), w = ody_exp2(x - ref);
-    m = top, l = l * alpha + w;
+    for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[j][e], qf[j][e], s, 0, 0, 0);
 #pragma unroll
-    for (int e = 0; e < N; e++) o[e] = fmaf(w, (float)vp[e], o[e] * alpha);
-  }
-#pragma unroll
-  for (int e = 0; e < N; e++)
-    static_cast<T*>(p.out)[s * p.so.b + i * p.so.l + h * p.so.h + lane * N + e] = (T)(l == 0.f ? 0.f : o[e] / l);
-  if (lane == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * ODY_LN2;
+  for (int r = 0; r < 4; r++) x[r] = s[r];
 }
 
+// o[i], row c: column c * DV + i of the result
+template <int D, int NT>
+__device__ __forceinline__ void values(const Loaded<bf16, D>& t, const float (&w)[NT][8], f32x4 (&o)[NT][D / 16]) {
+  bf16x8 pb[NT];
+#pragma unroll
+  for (int m = 0; m < NT; m++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) pb[m][e] = (bf16)w[m][e];
+  unsigned v[8][D / 32];
+#pragma unroll
+  for (int j = 0; j < 8; j++) __builtin_memcpy(v[j], &t.v[j], sizeof(v[j]));
+#pragma unroll
+  for (int i = 0; i < D / 16; i++) {
+    i32x4 a;
+#pragma unroll
+    for (int j = 0; j < 4; j++) a[j] = __builtin_amdgcn_perm(v[2 * j + 1][i / 2], v[2 * j][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+    const bf16x8 af = __builtin_bit_cast(bf16x8, a);
+#pragma unroll
+    for (int m = 0; m < NT; m++) o[m][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, pb[m], o[m][i], 0, 0, 0);
+  }
+}
+template <int D, int NT>
+__device__ __forceinline__ void values(const Loaded<float, D>& t, const float (&w)[NT][4], f32x4 (&o)[NT][D / 16]) {
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int i = 0; i < D / 16; i++)
+#pragma unroll
+      for (int m = 0; m < NT; m++) o[m][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.v[r][i], w[m][r], o[m][i], 0, 0, 0);
+}
+
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel(const PagedAttnParams p, const PagedCache cache) {
+  typedef Tile<T, D> G;
+  constexpr int STEP = WAVES * G::KEYS, GK = G::GK, OP = D + 4;
+  __shared__ __attribute__((aligned(16))) float Os[WAVES][16][OP];
+  __shared__ float sm[WAVES][16 * NT], sl[WAVES][16 * NT];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q = lane >> 4;
+  const int64_t total = paged_total<STEP>(p, cache, lane) * p.Hkv;
+  const int blocks = (int)min((int64_t)gridDim.x, total), block = blockIdx.x;   // as many as have a step
+  if (block >= blocks) return;
+  int64_t pos = paged_cut(total, block, blocks);
+  const int64_t begin = pos, end = paged_cut(total, block + 1, blocks);
+  int64_t entry_first;
+  int steps, entry = paged_find<STEP>(p, cache, lane, pos, entry_first, steps);
+  int hk = (int)((pos - entry_first) / steps), step = (int)((pos - entry_first) % steps);
+
+  while (pos < end) {
+    const int s = entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * p.tile;
+    const int rows = (int)min((int64_t)p.tile, (int64_t)p.n * p.group - row0), length = paged_length(cache, s);
+    const int keys = paged_keys(p, cache, length, rt), steps_here = (int)min((int64_t)(steps - step), end - pos);
+    const T* kp = static_cast<const T*>(cache.k) + hk * cache.sk.h;
+    const T* vp = static_cast<const T*>(cache.v) + hk * cache.sv.h;
+    const int* table = cache.table + s * cache.table_stride;
+    const int in_page = (1 << cache.shift) - 1, last_group = max(keys - 1, 0) & -GK;
+
+    // ---- row 16 m + c: token (row0 + ..) / group, query head hk * group + (row0 + ..) % group
+    typename G::kvec qf[NT][D * sizeof(T) / 64];
+    int lim[NT];   // last key the row sees
+    int safe = keys - 1;
+#pragma unroll
+    for (int m = 0; m < NT; m++) {
+      const int r = row0 + min(16 * m + c, rows - 1), i = r / p.group, h = hk * p.group + r - i * p.group;
+      const T* qp = static_cast<const T*>(p.q) + s * p.sq.b + i * p.sq.l + h * p.sq.h;
+#pragma unroll
+      for (int j = 0; j < (int)(D * sizeof(T) / 64); j++) qf[m][j] = *reinterpret_cast<const typename G::kvec*>(qp + G::key_col(q, j));
+      lim[m] = min(keys - 1, length - p.n + i);
+    }
+    safe = min(safe, length - p.n + row0 / p.group);
+
+    f32x4 o[NT][D / 16];
+    float mx[NT], l[NT];
+#pragma unroll
+    for (int m = 0; m < NT; m++) {
+      mx[m] = -INFINITY, l[m] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; i++) o[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- the wavefront's tiles: keys (step + t) * STEP + wave * KEYS ..
+    const int key0 = step * STEP + wave * G::KEYS;
+    const int tiles = key0 >= keys ? 0 : min(steps_here, (keys - key0 + STEP - 1) / STEP);
+    struct Pages { int k, v; };
+    auto lookup = [&](int t) {   // of the groups that the lane's K row and V rows are in
+      const int base = key0 + min(t, tiles - 1) * STEP;
+      return Pages{table[min(base + GK * (c >> 2), last_group) >> cache.shift], table[min(base + GK * q, last_group) >> cache.shift]};
+    };
+    auto load = [&](Loaded<T, D>& t, int at, const Pages& pg) {
+      const int base = key0 + at * STEP, gk = min(base + GK * (c >> 2), last_group), gv = min(base + GK * q, last_group);
+      t.page = (unsigned)pg.v < (unsigned)cache.pages;
+      const T* kr = kp + ((unsigned)pg.k < (unsigned)cache.pages ? pg.k : 0) * cache.sk.p + (gk & in_page) * cache.sk.r;
+      const T* vr = vp + (t.page ? pg.v : 0) * cache.sv.p + (gv & in_page) * cache.sv.r + c * G::DV;
+#pragma unroll
+      for (int j = 0; j < G::KV; j++) t.k[j] = *reinterpret_cast<const typename G::kvec*>(kr + G::key_row(c, j) * cache.sk.r + G::key_col(q, j));
+#pragma unroll
+      for (int j = 0; j < GK; j++) t.v[j] = *reinterpret_cast<const typename G::vvec*>(vr + j * cache.sv.r);
+    };
+    auto compute = [&](Loaded<T, D>& t, int at) {
+      const int base = key0 + at * STEP, first = base + GK * q;   // the lane's keys
+      float w[NT][GK];
+#pragma unroll
+      for (int m = 0; m < NT; m++) scores<D>(t, qf[m], w[m]);
+#pragma unroll
+      for (int m = 0; m < NT; m++)
+#pragma unroll
+        for (int e = 0; e < GK; e++) w[m][e] *= p.scale_log2e;
+      // keys that a row does not see, that no token has, that have no page: neither their scores nor their values count, whatever lies there
+      if (base + G::KEYS - 1 > safe || !__all(t.page)) {
+        const int most = t.page ? keys - 1 : -1;
+#pragma unroll
+        for (int e = 0; e < GK; e++) {
+#pragma unroll
+          for (int m = 0; m < NT; m++)
+            if (first + e > min(lim[m], most)) w[m][e] = -INFINITY;
+          if (first + e > most) t.v[e] = typename G::vvec{};
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < NT; m++) {
+        float top = w[m][0];
+#pragma unroll
+        for (int e = 1; e < GK; e++) top = fmaxf(top, w[m][e]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float now = fmaxf(mx[m], top), ref = now == -INFINITY ? 0.f : now, alpha = ody_exp2(mx[m] - ref);
+        mx[m] = now;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < GK; e++) w[m][e] = ody_exp2(w[m][e] - ref), sum += w[m][e];
+        l[m] = l[m] * alpha + sum;   // this lane's share of the row sum
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[m][i] *= alpha;
+      }
+      values<D, NT>(t, w, o);
+    };
+    if (NT == 4) {   // two tiles do not fit the registers beside 64 rows
+      Loaded<T, D> a;
+      for (int t = 0; t < tiles; t++) {
+        load(a, t, lookup(t));
+        compute(a, t);
+      }
+    } else if (tiles > 0) {
+      Loaded<T, D> a, b;
+      load(a, 0, lookup(0));
+      Pages next = lookup(1);
+      for (int t = 0; t < tiles; t += 2) {
+        if (t + 1 < tiles) {
+          load(b, t + 1, next);
+          next = lookup(t + 2);
+        }
+        compute(a, t);
+        if (t + 1 >= tiles) break;
+        if (t + 2 < tiles) {
+          load(a, t + 2, next);
+          next = lookup(t + 3);
+        }
+        compute(b, t + 1);
+      }
+    }
+
+    // ---- the four wavefronts' results of a row: common reference, weighted sum
+#pragma unroll
+    for (int m = 0; m < NT; m++) {
+      l[m] += __shfl_xor(l[m], 16, 64);
+      l[m] += __shfl_xor(l[m], 32, 64);
+      if (q == 0) sm[wave][16 * m + c] = mx[m], sl[wave][16 * m + c] = l[m];
+    }
+    __syncthreads();
+    const bool whole = steps_here == steps;
+    const int64_t slot = (int64_t)block * 2 + (pos > begin);   // the unit that the range begins with, or the one that it ends with
+#pragma unroll
+    for (int m = 0; m < NT; m++) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) top = fmaxf(top, sm[w][16 * m + c]);
+      const float mine = ody_exp2(mx[m] - (top == -INFINITY ? 0.f : top));
+      // o[i][r] of row 4 q + r: column (4 q + r) * DV + i
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 4)
+          *reinterpret_cast<f32x4*>(&Os[wave][c][(4 * q + r) * G::DV + i]) = f32x4{o[m][i][r], o[m][i + 1][r], o[m][i + 2][r], o[m][i + 3][r]} * mine;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 16 * D / 4 / (64 * WAVES); e++) {
+        const int idx = tid + 64 * WAVES * e, row = idx / (D / 4), d4 = idx % (D / 4), r = 16 * m + row;
+        if (r >= rows) continue;
+        float t = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) t = fmaxf(t, sm[w][r]);
+        const float ref = t == -INFINITY ? 0.f : t;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+          sum += sl[w][r] * ody_exp2(sm[w][r] - ref);
+          acc += *reinterpret_cast<const f32x4*>(&Os[w][row][4 * d4]);
+        }
+        if (whole) {
+          const int i = (row0 + r) / p.group, h = hk * p.group + (row0 + r) - i * p.group;
+          acc *= sum == 0.f ? 0.f : 1.f / sum;
+          T* dst = static_cast<T*>(p.out) + s * p.so.b + i * p.so.l + h * p.so.h + 4 * d4;
+          typedef T out4 __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<out4*>(dst) = out4{(T)acc[0], (T)acc[1], (T)acc[2], (T)acc[3]};
+          if (d4 == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + i] = sum == 0.f ? -INFINITY : (t + __log2f(sum)) * ODY_LN2;
+        } else {
+          *reinterpret_cast<f32x4*>(p.part + (slot * p.tile + r) * D + 4 * d4) = acc;
+          if (d4 == 0) p.part_ml[slot * p.tile + r] = make_float2(t, sum);
+        }
+      }
+      __syncthreads();
+    }
+
+    pos += steps_here;
+    step = 0;
+    if (++hk == p.Hkv && pos < end) hk = 0, steps = paged_steps<STEP>(p, cache, ++entry);
+  }
+}
+
+// One block per row: the parts of its unit, if a cut goes through it, weighted by their sums.
+template <typename T, int D, int STEP>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p, const PagedCache cache, int most_blocks) {
+  constexpr int C4 = D / 4, GROUPS = 256 / C4;
+  __shared__ f32x4 red[GROUPS][C4];
+  __shared__ float2 red_ml[GROUPS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  // blockIdx.x: (sequence, row of all rows of a kv head, kv head)
+  const int hk = blockIdx.x % p.Hkv, row = blockIdx.x / p.Hkv % (p.n * p.group), s = blockIdx.x / p.Hkv / (p.n * p.group);
+  const int rt = row / p.tile, r = row - rt * p.tile, entry = s * p.row_tiles + rt;
+  // steps in front of this unit
+  int64_t before = 0, total = 0;
+  for (int at = 0; at < p.S * p.row_tiles; at += 64) {
+    const int e = at + lane, x = e < p.S * p.row_tiles ? paged_steps<STEP>(p, cache, e) : 0;
+    total += __builtin_amdgcn_readlane(paged_wave_scan(x, lane), 63);
+    before += __builtin_amdgcn_readlane(paged_wave_scan(e < entry ? x : 0, lane), 63);
+  }
+  const int steps = paged_steps<STEP>(p, cache, entry);
+  const int64_t first = before * p.Hkv + (int64_t)hk * steps;
+  total *= p.Hkv;
+  const int blocks = (int)min((int64_t)most_blocks, total);
+  const int b0 = paged_block_of(total, first, blocks), b1 = paged_block_of(total, first + steps - 1, blocks);
+  if (b0 == b1) return;
+  const int d4 = tid % C4, g = tid / C4;
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int b = b0 + g; b <= b1; b += GROUPS) {
+    const int64_t at = ((int64_t)b * 2 + (b == b0 && first > paged_cut(total, b, blocks))) * p.tile + r;
+    const float2 ml = p.part_ml[at];
+    const f32x4 o = *reinterpret_cast<const f32x4*>(p.part + at * D + 4 * d4);
+    const float now = fmaxf(m, ml.x), ref = now == -INFINITY ? 0.f : now, wa = ody_exp2(m - ref), wb = ody_exp2(ml.x - ref);
+    m = now, l = l * wa + ml.y * wb, acc = acc * wa + o * wb;
+  }
+  red[g][d4] = acc;
+  if (d4 == 0) red_ml[g] = make_float2(m, l);
+  __syncthreads();
+  if (g != 0) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < GROUPS; k++) top = fmaxf(top, red_ml[k].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  acc = f32x4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < GROUPS; k++) {
+    const float w = ody_exp2(red_ml[k].x - ref);
+    l += red_ml[k].y * w, acc += red[k][d4] * w;
+  }
+  acc *= l == 0.f ? 0.f : 1.f / l;
+  const int i = row / p.group, h = hk * p.group + row - i * p.group;
+  typedef T out4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<out4*>(static_cast<T*>(p.out) + s * p.so.b + i * p.so.l + h * p.so.h + 4 * d4) = out4{(T)acc[0], (T)acc[1], (T)acc[2], (T)acc[3]};
+  if (d4 == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + i] = l == 0.f ? -INFINITY : (top + __log2f(l)) * ODY_LN2;
+}
+
+// Row tiles of 16, 32 or 64.
+int row_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int step_keys(int dtype) { return WAVES * (dtype == ODY_BF16 ? 32 : 16); }
+struct Plan {
+  int tile, row_tiles, blocks;
+  bool joined;          // a cut may go through a unit
+  size_t part_bytes, ml_bytes;
+};
+Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype) {
+  const int64_t rows = (int64_t)n * group;
+  const int tile = row_tile(rows), row_tiles = (int)((rows + tile - 1) / tile);
+  const int64_t steps = std::max((int64_t)1, (most_keys + step_keys(dtype) - 1) / step_keys(dtype));   // of a unit, at most
+  const int blocks = (int)std::min((double)BLOCKS, (double)S * row_tiles * Hkv * steps);
+  const bool joined = steps > 1;
+  const size_t parts = joined ? (size_t)blocks * 2 * tile : 0;
+  return Plan{tile, row_tiles, blocks, joined, parts * D * sizeof(float), parts * sizeof(float2)};
+}
+
+template <typename T, int D, int NT>
+int launch(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
+  ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
+  int rc = ody_check_launch("paged_attn");
+  if (rc || !pl.joined) return rc;
+  ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, WAVES * Tile<T, D>::KEYS>), dim3((unsigned)(p.S * p.n * p.Hq)), dim3(256), 0, p, c, pl.blocks);
+  return ody_check_launch("paged_join");
+}
+template <typename T, int D>
+int by_rows(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
+  return pl.tile == 16 ? launch<T, D, 1>(p, c, pl, st) : pl.tile == 32 ? launch<T, D, 2>(p, c, pl, st) : launch<T, D, 4>(p, c, pl, st);
+}
 template <typename T>
-int by_head_dim(const PagedAttnParams& p, int D, const PagedCache& c, hipStream_t st) {
-  const dim3 grid((unsigned)(p.S * p.n * p.Hq));
-  if (D == 64) ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, 64>), grid, dim3(64), 0, p, c);
-  else ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, 128>), grid, dim3(64), 0, p, c);
-  return ody_check_launch("paged_attn");
+int by_head_dim(const PagedAttnParams& p, int D, const PagedCache& c, const Plan& pl, hipStream_t st) {
+  return D == 64 ? by_rows<T, 64>(p, c, pl, st) : by_rows<T, 128>(p, c, pl, st);
 }
 
 }  // namespace
 
-extern "C" size_t ody_paged_attn_workspace_bytes(int S, int n, int Hq, int Hkv, int D, int page_size, int table_width, int dtype) { return 0; }
+extern "C" size_t ody_paged_attn_workspace_bytes(int S, int n, int Hq, int Hkv, int D, int page_size, int table_width, int dtype) {
+  if (S <= 0 || n <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || page_size <= 0 || table_width <= 0) return 0;   // the call refuses these
+  const Plan pl = plan(S, n, Hq / Hkv, Hkv, D, (int64_t)page_size * table_width, dtype);
+  return pl.part_bytes + pl.ml_bytes;
+}
 
 extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* lengths, void* out,
                               float* lse, int S, int n, int Hq, int Hkv, int D, int64_t sq_s, int64_t sq_n, int64_t sq_h,
@@ -69,7 +392,13 @@ extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_
   ODY_REQUIRE(q && out && lse, ODY_ERR_NULL, "ody_paged_attn: q, out or lse is NULL");
   ODY_REQUIRE(paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype) && paged_rows_aligned(out, so_s, so_n, so_h, dtype), ODY_ERR_MISALIGNED,
               "ody_paged_attn: q and out need 16-byte aligned pointers and strides");
-  const PagedAttnParams p{q, out, lse, {sq_s, sq_n, sq_h}, {so_s, so_n, so_h}, S, n, Hq, Hkv, Hq / Hkv, scale * ODY_LOG2E};
+  const Plan pl = plan(S, n, Hq / Hkv, Hkv, D, (int64_t)page_size * table_width, dtype);
+  ODY_REQUIRE(pl.part_bytes == 0 || (workspace && workspace_bytes >= pl.part_bytes + pl.ml_bytes && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
+              ODY_ERR_WORKSPACE, "ody_paged_attn: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", pl.part_bytes + pl.ml_bytes,
+              workspace_bytes);
+  float* part = static_cast<float*>(workspace);
+  const PagedAttnParams p{q, out, lse, {sq_s, sq_n, sq_h}, {so_s, so_n, so_h}, S, n, Hq, Hkv, Hq / Hkv, scale * ODY_LOG2E, pl.row_tiles, pl.tile,
+                          part, reinterpret_cast<float2*>(static_cast<char*>(workspace) + pl.part_bytes)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == ODY_BF16 ? by_head_dim<bf16>(p, D, c, st) : by_head_dim<float>(p, D, c, st);
+  return dtype == ODY_BF16 ? by_head_dim<bf16>(p, D, c, pl, st) : by_head_dim<float>(p, D, c, pl, st);
 }
