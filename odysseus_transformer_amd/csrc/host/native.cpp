@@ -11,11 +11,12 @@
 // definition of what an op accepts and of the error it raises.
 //
 // No state but what bind() is given once: the addresses of the library's entry points, so that this module uses the library that
-// Python loaded, and six Python objects.
+// Python loaded, and seven Python objects.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/hip/HIPFunctions.h>
@@ -38,7 +39,7 @@ namespace {
   X(ody_linear_rope_ws) X(ody_linear_swiglu) X(ody_linear_swiglu_h_fused) X(ody_linear_swiglu_h)                                  \
   X(ody_linear_dgrad_swiglu_workspace_bytes) X(ody_linear_dgrad_swiglu) X(ody_attn_fwd_workspace_bytes) X(ody_attn_fwd)           \
   X(ody_attn_bwd_workspace_bytes) X(ody_attn_bwd) X(ody_attn_bwd_rope) X(ody_rope) X(ody_rope_table)           \
-  X(ody_norm_linear_rope) X(ody_norm_linear_swiglu_h)
+  X(ody_norm_linear_rope) X(ody_norm_linear_swiglu_h) X(ody_paged_append) X(ody_paged_attn) X(ody_paged_attn_workspace_bytes)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -47,6 +48,7 @@ struct Library {
 } lib;
 PyObject* arena_holder = nullptr;   // class whose attribute `instance` is the scratch arena, or None
 PyObject* scratch_fn = nullptr;     // scratch(nbytes, name, device) of ops.py
+PyObject* own_scratch_fn = nullptr; // the same, of a graph's own under capture
 PyObject* raise_fn = nullptr;       // raises for (name, status)
 PyObject* no_memory = nullptr;      // torch.OutOfMemoryError
 PyObject* never_keeps_ds = nullptr; // _never_keeps_ds() of ops.py
@@ -142,7 +144,7 @@ at::Tensor make_f32(at::IntArrayRef shape, const at::Tensor& like) { return at::
 struct Scratch {
   at::Tensor t;
   size_t bytes;
-  Scratch(size_t nbytes, const char* name, const at::Tensor& like) : bytes(nbytes) {
+  Scratch(size_t nbytes, const char* name, const at::Tensor& like, PyObject* from = nullptr) : bytes(nbytes) {
     if (nbytes == 0) return;
     PyObject* arena = PyObject_GetAttrString(arena_holder, "instance");
     if (!arena) throw PythonError{};
@@ -150,7 +152,7 @@ struct Scratch {
     Py_DECREF(arena);
     if (have) {
       PyObject* device = THPDevice_New_(like);
-      PyObject* r = PyObject_CallFunction(scratch_fn, "nsO", (Py_ssize_t)nbytes, name, device);
+      PyObject* r = PyObject_CallFunction(from ? from : scratch_fn, "nsO", (Py_ssize_t)nbytes, name, device);
       Py_XDECREF(device);
       if (!r) {
         if (!PyErr_ExceptionMatches(no_memory)) throw PythonError{};
@@ -545,6 +547,59 @@ PyObject* norm_linear_swiglu_h(Call c) {
   return wrap(h);
 }
 
+// What the two ops of a cache in pages share: x (S, n, heads, D), pages (pages, page size, kv heads, D), their table and lengths; nobody
+// waits for a gradient.
+struct Paged {
+  const at::Tensor &k, &v, &table, &lengths;
+  Paged(Call& c, Py_ssize_t i, const at::Tensor& x) : k(c.heads(i, &x)), v(c.heads(i + 1, &x)), table(c.any(i + 2)), lengths(c.any(i + 3)) {
+    need(k.sizes() == v.sizes() && k.size(3) == x.size(3));
+    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == x.size(0) && table.stride(1) == 1 && table.size(1) < INT32_MAX);
+    need(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.is_contiguous() && lengths.size(0) == x.size(0));
+    need(!at::GradMode::is_enabled() || !(x.requires_grad() || k.requires_grad() || v.requires_grad()));
+  }
+  int pages() const { return (int)k.size(0); }
+  int page_size() const { return (int)k.size(1); }
+  int columns() const { return (int)table.size(1); }
+};
+#define PAGED_TABLE(c) (c).table.data_ptr<int>(), (c).lengths.data_ptr<int>()
+#define PAGED_SHAPE(c) (c).pages(), (c).page_size(), (c).columns(), (c).table.stride(0)
+
+// (qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids or None, inv_freq or None: no rotation) -> q
+PyObject* paged_append(Call c) {
+  const at::Tensor& x = c.heads(0, nullptr);
+  const Paged pg(c, 2, x);
+  const int64_t Hq = c.whole(1), S = x.size(0), n = x.size(1), D = x.size(3), Hkv = pg.k.size(2);
+  need(Hq > 0 && x.size(2) == Hq + 2 * Hkv);
+  if (c.none(7)) {
+    need(c.none(6));
+    at::Tensor q = x.narrow(2, 0, Hq);
+    CALL(ody_paged_append, x.data_ptr(), nullptr, pg.k.data_ptr(), pg.v.data_ptr(), PAGED_TABLE(pg), nullptr, nullptr, (int)S, (int)n, (int)Hq, (int)Hkv,
+         (int)D, STRIDES(x), STRIDES(q), STRIDES(pg.k), STRIDES(pg.v), PAGED_SHAPE(pg), dt(x), (void*)c.stream);
+    return wrap(q);
+  }
+  if (!c.none(6)) need(c.any(6).dim() == 2 && c.any(6).size(0) == S);
+  const int64_t* pos = positions(c, 6, S * n);
+  const at::Tensor& f = frequencies(c, 7, D);
+  need(f.dim() == 1);
+  at::Tensor q = make({S, n, Hq, D}, x);
+  CALL(ody_paged_append, x.data_ptr(), q.data_ptr(), pg.k.data_ptr(), pg.v.data_ptr(), PAGED_TABLE(pg), pos, f.data_ptr<float>(), (int)S, (int)n, (int)Hq,
+       (int)Hkv, (int)D, STRIDES(x), STRIDES(q), STRIDES(pg.k), STRIDES(pg.v), PAGED_SHAPE(pg), dt(x), (void*)c.stream);
+  return wrap(q);
+}
+
+// (q, k_pages, v_pages, page_table, lengths, scale) -> (out, lse)
+PyObject* paged_attn(Call c) {
+  const at::Tensor& q = c.heads(0, nullptr);
+  const Paged pg(c, 1, q);
+  const int S = q.size(0), n = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = pg.k.size(2);
+  const float scale = (float)c.real(5);
+  at::Tensor out = make({S, n, Hq, D}, q), lse = make_f32({S, Hq, n}, q);
+  Scratch ws(lib.ody_paged_attn_workspace_bytes(S, n, Hq, Hkv, D, pg.page_size(), pg.columns(), dt(q)), "paged_attn_workspace", q, own_scratch_fn);
+  CALL(ody_paged_attn, q.data_ptr(), pg.k.data_ptr(), pg.v.data_ptr(), PAGED_TABLE(pg), out.data_ptr(), lse.data_ptr<float>(), S, n, Hq, Hkv, D,
+       STRIDES(q), STRIDES(pg.k), STRIDES(pg.v), STRIDES(out), PAGED_SHAPE(pg), scale, dt(q), ws.ptr(), ws.bytes, (void*)c.stream);
+  return tuple(out, lse);
+}
+
 // the raw stream that the ops above launch on
 PyObject* current_stream(Call) {
   return PyLong_FromVoidPtr((void*)c10::hip::getCurrentHIPStream(c10::hip::current_device()).stream());
@@ -563,10 +618,10 @@ PyObject* method(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (addresses by name, arena holder, scratch, raise, torch.OutOfMemoryError, _never_keeps_ds, attn_bwd)
+// (addresses by name, arena holder, scratch, raise, torch.OutOfMemoryError, _never_keeps_ds, attn_bwd, _own_scratch)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7 || !PyDict_Check(args[0])) {
-    PyErr_SetString(PyExc_TypeError, "bind(addresses, arena_holder, scratch, raise, no_memory, never_keeps_ds, attn_bwd)");
+  if (n != 8 || !PyDict_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "bind(addresses, arena_holder, scratch, raise, no_memory, never_keeps_ds, attn_bwd, own_scratch)");
     return nullptr;
   }
 #define X(name)                                                                      \
@@ -581,8 +636,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   ODY_ENTRY_POINTS(X)
 #undef X
-  PyObject** to[6] = {&arena_holder, &scratch_fn, &raise_fn, &no_memory, &never_keeps_ds, &attn_bwd_fn};
-  for (int i = 0; i < 6; i++) {
+  PyObject** to[7] = {&arena_holder, &scratch_fn, &raise_fn, &no_memory, &never_keeps_ds, &attn_bwd_fn, &own_scratch_fn};
+  for (int i = 0; i < 7; i++) {
     Py_INCREF(args[1 + i]);
     Py_XSETREF(*to[i], args[1 + i]);
   }
@@ -595,6 +650,7 @@ PyMethodDef methods[] = {
     METHOD(rmsnorm_fwd, 3), METHOD(rmsnorm_bwd, 5), METHOD(gemm, 3), METHOD(linear_residual, 3), METHOD(linear_rope, 5), METHOD(linear_swiglu, 2),
     METHOD(linear_swiglu_h, 2), METHOD(linear_dgrad_swiglu, 3), METHOD(attn_fwd, 5), METHOD(attn_bwd, 13), METHOD(flash, 5), METHOD(rope, 6), METHOD(rope_table, 5),
     METHOD(norm_linear_rope, 8), METHOD(norm_linear_swiglu_h, 4),
+    METHOD(paged_append, 8), METHOD(paged_attn, 6),
     METHOD(current_stream, 0), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_odysseus_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -35,69 +35,72 @@ struct PagedAttnParams {
 // ranges of equal length (to a step), so that blocks finish together whatever the lengths are; a unit that a cut goes through has its
 // results joined by a second kernel.  Fewer steps than blocks: a step each, for as many as there are.  Every block finds its range by itself from the lengths on the device: a captured graph replays with
 // the lengths of that time, and there is no plan to be kept.
-struct PagedUnit {
-  int s, rt;        // sequence, row tile
-  int steps;
-};
-
 // Tokens of a sequence; less than nothing is nothing.
 __device__ __forceinline__ int paged_length(const PagedCache& c, int s) { return max(0, c.lengths[s]); }
 // Keys that the last row of a row tile sees: places behind the table's last column have no page (the host checks width << shift < 2^31).
 __device__ __forceinline__ int paged_keys(const PagedAttnParams& p, const PagedCache& c, int length, int rt) {
-  const int64_t last_row = min((int64_t)(rt + 1) * p.tile, (int64_t)p.n * p.group) - 1;
-  return max(0, min(c.width << c.shift, length - p.n + (int)(last_row / p.group) + 1));
+  const int last_row = min((rt + 1) * p.tile, p.n * p.group) - 1;   // rows are below 2^31, and so is a row tile more
+  const int last = p.row_tiles == 1 ? p.n - 1 : last_row / p.group;
+  return max(0, min(c.width << c.shift, length - p.n + last + 1));
 }
 template <int STEP>
 __device__ __forceinline__ int paged_steps(const PagedAttnParams& p, const PagedCache& c, int e) {
-  const int s = e / p.row_tiles, keys = paged_keys(p, c, paged_length(c, s), e - s * p.row_tiles);
-  return max(1, (int)(((int64_t)keys + STEP - 1) / STEP));
+  const int s = p.row_tiles == 1 ? e : e / p.row_tiles, keys = paged_keys(p, c, paged_length(c, s), e - s * p.row_tiles);
+  return max(1, (keys - 1) / STEP + 1);
 }
 
-// Every lane of a wavefront: inclusive sums over its lanes.
-__device__ __forceinline__ int paged_wave_scan(int x, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
+// Inclusive sums over the lanes of a wavefront, within rows of 16 lanes and then from row to row.
+__device__ __forceinline__ int paged_wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);   // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);
   return x;
 }
-// Steps of all (sequence, row tile) pairs of one kv head.
-template <int STEP>
-__device__ __forceinline__ int64_t paged_total(const PagedAttnParams& p, const PagedCache& c, int lane) {
-  const int entries = p.S * p.row_tiles;
-  int64_t total = 0;
-  for (int at = 0; at < entries; at += 64) {
-    const int x = paged_wave_scan(at + lane < entries ? paged_steps<STEP>(p, c, at + lane) : 0, lane);
-    total += __builtin_amdgcn_readlane(x, 63);
+
+// Where the cuts are: `total` steps (below 2^31, which the host checks) over as many of the blocks as have one.
+struct PagedCuts {
+  int total, blocks, base, more;   // the first `more` blocks have base + 1 steps, the others base
+  __device__ __forceinline__ PagedCuts(int steps, int most_blocks) : total(steps), blocks(min(most_blocks, steps)) {
+    base = (unsigned)total / (unsigned)blocks, more = total - base * blocks;
   }
-  return total;
-}
-// The pair that step `pos` (of all kv heads together) belongs to, and the first step of it.
-template <int STEP>
-__device__ __forceinline__ int paged_find(const PagedAttnParams& p, const PagedCache& c, int lane, int64_t pos, int64_t& first, int& steps) {
-  const int entries = p.S * p.row_tiles;
-  int64_t before = 0;
-  for (int at = 0;; at += 64) {
-    const int mine = at + lane < entries ? paged_steps<STEP>(p, c, at + lane) : 0, x = paged_wave_scan(mine, lane);
-    const int all = __builtin_amdgcn_readlane(x, 63);
-    if (pos < (before + all) * p.Hkv || at + 64 >= entries) {
-      const int k = min(__popcll(__ballot((before + x) * p.Hkv <= pos)), min(63, entries - 1 - at));
-      steps = __builtin_amdgcn_readlane(mine, k);
-      first = (before + __builtin_amdgcn_readlane(x, k) - steps) * p.Hkv;
-      return at + k;
-    }
-    before += all;
+  __device__ __forceinline__ int at(int block) const { return block * base + min(block, more); }
+  __device__ __forceinline__ int block_of(int step) const {
+    const int heavy = more * (base + 1);
+    return step < heavy ? (int)((unsigned)step / (unsigned)(base + 1)) : more + (int)((unsigned)(step - heavy) / (unsigned)base);
   }
-}
-__device__ __forceinline__ int64_t paged_cut(int64_t total, int block, int blocks) { return total / blocks * block + total % blocks * block / blocks; }
-// The block whose range holds step `pos`.
-__device__ __forceinline__ int paged_block_of(int64_t total, int64_t pos, int blocks) {
-  int b = (int)min((int64_t)blocks - 1, (int64_t)((double)pos * blocks / (double)total));
-  while (b > 0 && paged_cut(total, b, blocks) > pos) b--;
-  while (b + 1 < blocks && paged_cut(total, b + 1, blocks) <= pos) b++;
-  return b;
-}
+};
+
+// One walk over the (sequence, row tile) pairs by a wavefront: a chunk of 64 of them, their steps and the sums so far.
+template <int STEP>
+struct PagedWalk {
+  const PagedAttnParams& p;
+  const PagedCache& c;
+  int lane, entries, at = 0, before = 0, mine = 0, sums = 0;   // sums: inclusive, of this chunk
+  __device__ __forceinline__ PagedWalk(const PagedAttnParams& p_, const PagedCache& c_, int lane_) : p(p_), c(c_), lane(lane_), entries(p_.S * p_.row_tiles) { chunk(); }
+  __device__ __forceinline__ void chunk() {
+    mine = at + lane < entries ? paged_steps<STEP>(p, c, at + lane) : 0;
+    sums = paged_wave_scan(mine);
+  }
+  __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(sums, 63); }
+  __device__ __forceinline__ bool next() {
+    if (at + 64 >= entries) return false;
+    before += all(), at += 64;
+    chunk();
+    return true;
+  }
+  __device__ __forceinline__ int total() {   // of one kv head; ends on the last chunk
+    while (next()) {}
+    return before + all();
+  }
+  __device__ __forceinline__ void rewind() {
+    if (at == 0) return;
+    at = before = 0;
+    chunk();
+  }
+};
 #endif
 
 // Host side: the checks that both entry points share.

@@ -104,19 +104,24 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
   __shared__ __attribute__((aligned(16))) float Os[WAVES][16][OP];
   __shared__ float sm[WAVES][16 * NT], sl[WAVES][16 * NT];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q = lane >> 4;
-  const int64_t total = paged_total<STEP>(p, cache, lane) * p.Hkv;
-  const int blocks = (int)min((int64_t)gridDim.x, total), block = blockIdx.x;   // as many as have a step
-  if (block >= blocks) return;
-  int64_t pos = paged_cut(total, block, blocks);
-  const int64_t begin = pos, end = paged_cut(total, block + 1, blocks);
-  int64_t entry_first;
-  int steps, entry = paged_find<STEP>(p, cache, lane, pos, entry_first, steps);
-  int hk = (int)((pos - entry_first) / steps), step = (int)((pos - entry_first) % steps);
+  PagedWalk<STEP> walk(p, cache, lane);
+  const PagedCuts cuts(walk.total() * p.Hkv, gridDim.x);
+  const int block = blockIdx.x;
+  if (block >= cuts.blocks) return;
+  const int begin = cuts.at(block), end = cuts.at(block + 1);
+  int pos = begin;
+  // the pair that the range begins in
+  walk.rewind();
+  while ((walk.before + walk.all()) * p.Hkv <= pos && walk.next()) {}
+  const int k = __popcll(__ballot((walk.before + walk.sums) * p.Hkv <= pos));
+  int entry = walk.at + k, steps = __builtin_amdgcn_readlane(walk.mine, k);
+  const int into = pos - (walk.before + __builtin_amdgcn_readlane(walk.sums, k) - steps) * p.Hkv;
+  int hk = (int)((unsigned)into / (unsigned)steps), step = into - hk * steps;
 
   while (pos < end) {
-    const int s = entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * p.tile;
-    const int rows = (int)min((int64_t)p.tile, (int64_t)p.n * p.group - row0), length = paged_length(cache, s);
-    const int keys = paged_keys(p, cache, length, rt), steps_here = (int)min((int64_t)(steps - step), end - pos);
+    const int s = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * p.tile;
+    const int rows = min(p.tile, p.n * p.group - row0), length = paged_length(cache, s);
+    const int keys = paged_keys(p, cache, length, rt), steps_here = min(steps - step, end - pos);
     const T* kp = static_cast<const T*>(cache.k) + hk * cache.sk.h;
     const T* vp = static_cast<const T*>(cache.v) + hk * cache.sv.h;
     const int* table = cache.table + s * cache.table_stride;
@@ -235,7 +240,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
     }
     __syncthreads();
     const bool whole = steps_here == steps;
-    const int64_t slot = (int64_t)block * 2 + (pos > begin);   // the unit that the range begins with, or the one that it ends with
+    const int64_t slot = 2 * block + (pos > begin);   // the unit that the range begins with, or the one that it ends with
 #pragma unroll
     for (int m = 0; m < NT; m++) {
       float top = -INFINITY;
@@ -284,58 +289,63 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
   }
 }
 
-// One block per row: the parts of its unit, if a cut goes through it, weighted by their sums.
+// One block per row: the parts of its unit, if a cut goes through it, weighted by their sums.  A wavefront finds the weights, then
+// 256 / (D / 4) threads per column vector share the parts.
 template <typename T, int D, int STEP>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p, const PagedCache cache, int most_blocks) {
   constexpr int C4 = D / 4, GROUPS = 256 / C4;
+  __shared__ float weight[BLOCKS];
   __shared__ f32x4 red[GROUPS][C4];
-  __shared__ float2 red_ml[GROUPS];
   const int tid = threadIdx.x, lane = tid & 63;
   // blockIdx.x: (sequence, row of all rows of a kv head, kv head)
-  const int hk = blockIdx.x % p.Hkv, row = blockIdx.x / p.Hkv % (p.n * p.group), s = blockIdx.x / p.Hkv / (p.n * p.group);
+  const int all_rows = p.n * p.group, hk = blockIdx.x % p.Hkv, row = blockIdx.x / p.Hkv % all_rows, s = blockIdx.x / p.Hkv / all_rows;
   const int rt = row / p.tile, r = row - rt * p.tile, entry = s * p.row_tiles + rt;
-  // steps in front of this unit
-  int64_t before = 0, total = 0;
-  for (int at = 0; at < p.S * p.row_tiles; at += 64) {
-    const int e = at + lane, x = e < p.S * p.row_tiles ? paged_steps<STEP>(p, cache, e) : 0;
-    total += __builtin_amdgcn_readlane(paged_wave_scan(x, lane), 63);
-    before += __builtin_amdgcn_readlane(paged_wave_scan(e < entry ? x : 0, lane), 63);
+  PagedWalk<STEP> walk(p, cache, lane);
+  int before = 0, steps = 0;
+  do {
+    if (entry >= walk.at && entry < walk.at + 64) {
+      steps = __builtin_amdgcn_readlane(walk.mine, entry - walk.at);
+      before = walk.before + __builtin_amdgcn_readlane(walk.sums, entry - walk.at) - steps;
+    }
+  } while (walk.next());
+  const PagedCuts cuts((walk.before + walk.all()) * p.Hkv, most_blocks);
+  const int first = before * p.Hkv + hk * steps, b0 = cuts.block_of(first), b1 = cuts.block_of(first + steps - 1), parts = b1 - b0 + 1;
+  if (parts == 1) return;
+  // part k is in slot 2 (b0 + k), but for the first where that block's range begins with another unit
+  const int first_slot = 2 * b0 + (first > cuts.at(b0));
+  auto slot = [&](int k) { return ((int64_t)(k == 0 ? first_slot : 2 * (b0 + k))) * p.tile + r; };
+  const int i = row / p.group, h = hk * p.group + row - i * p.group;
+  if (tid < 64) {
+    float m = -INFINITY, l = 0.f;
+    for (int k = lane; k < parts; k += 64) {
+      const float2 ml = p.part_ml[slot(k)];
+      const float now = fmaxf(m, ml.x), ref = now == -INFINITY ? 0.f : now;
+      l = l * ody_exp2(m - ref) + ml.y * ody_exp2(ml.x - ref), m = now;
+    }
+    float top = m;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float ref = top == -INFINITY ? 0.f : top;
+    l *= ody_exp2(m - ref);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int k = lane; k < parts; k += 64) weight[k] = ody_exp2(p.part_ml[slot(k)].x - ref) * inv;
+    if (lane == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + i] = l == 0.f ? -INFINITY : (top + __log2f(l)) * ODY_LN2;
   }
-  const int steps = paged_steps<STEP>(p, cache, entry);
-  const int64_t first = before * p.Hkv + (int64_t)hk * steps;
-  total *= p.Hkv;
-  const int blocks = (int)min((int64_t)most_blocks, total);
-  const int b0 = paged_block_of(total, first, blocks), b1 = paged_block_of(total, first + steps - 1, blocks);
-  if (b0 == b1) return;
   const int d4 = tid % C4, g = tid / C4;
-  float m = -INFINITY, l = 0.f;
+  const float* src = p.part + 4 * d4;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int b = b0 + g; b <= b1; b += GROUPS) {
-    const int64_t at = ((int64_t)b * 2 + (b == b0 && first > paged_cut(total, b, blocks))) * p.tile + r;
-    const float2 ml = p.part_ml[at];
-    const f32x4 o = *reinterpret_cast<const f32x4*>(p.part + at * D + 4 * d4);
-    const float now = fmaxf(m, ml.x), ref = now == -INFINITY ? 0.f : now, wa = ody_exp2(m - ref), wb = ody_exp2(ml.x - ref);
-    m = now, l = l * wa + ml.y * wb, acc = acc * wa + o * wb;
-  }
+  __syncthreads();
+#pragma unroll 4
+  for (int k = g; k < parts; k += GROUPS) acc += weight[k] * *reinterpret_cast<const f32x4*>(src + slot(k) * D);
   red[g][d4] = acc;
-  if (d4 == 0) red_ml[g] = make_float2(m, l);
   __syncthreads();
   if (g != 0) return;
-  float top = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < GROUPS; k++) top = fmaxf(top, red_ml[k].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  acc = f32x4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
-#pragma unroll
-  for (int k = 0; k < GROUPS; k++) {
-    const float w = ody_exp2(red_ml[k].x - ref);
-    l += red_ml[k].y * w, acc += red[k][d4] * w;
-  }
-  acc *= l == 0.f ? 0.f : 1.f / l;
-  const int i = row / p.group, h = hk * p.group + row - i * p.group;
+  for (int k = 1; k < GROUPS; k++) acc += red[k][d4];
   typedef T out4 __attribute__((ext_vector_type(4)));
   *reinterpret_cast<out4*>(static_cast<T*>(p.out) + s * p.so.b + i * p.so.l + h * p.so.h + 4 * d4) = out4{(T)acc[0], (T)acc[1], (T)acc[2], (T)acc[3]};
-  if (d4 == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + i] = l == 0.f ? -INFINITY : (top + __log2f(l)) * ODY_LN2;
 }
 
 // Row tiles of 16, 32 or 64.
@@ -344,6 +354,7 @@ int step_keys(int dtype) { return WAVES * (dtype == ODY_BF16 ? 32 : 16); }
 struct Plan {
   int tile, row_tiles, blocks;
   bool joined;          // a cut may go through a unit
+  bool fits;            // the steps can be counted
   size_t part_bytes, ml_bytes;
 };
 Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype) {
@@ -353,7 +364,7 @@ Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype)
   const int blocks = (int)std::min((double)BLOCKS, (double)S * row_tiles * Hkv * steps);
   const bool joined = steps > 1;
   const size_t parts = joined ? (size_t)blocks * 2 * tile : 0;
-  return Plan{tile, row_tiles, blocks, joined, parts * D * sizeof(float), parts * sizeof(float2)};
+  return Plan{tile, row_tiles, blocks, joined, (double)S * row_tiles * Hkv * steps < 2147483648.0, parts * D * sizeof(float), parts * sizeof(float2)};
 }
 
 template <typename T, int D, int NT>
@@ -393,6 +404,7 @@ extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_
   ODY_REQUIRE(paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype) && paged_rows_aligned(out, so_s, so_n, so_h, dtype), ODY_ERR_MISALIGNED,
               "ody_paged_attn: q and out need 16-byte aligned pointers and strides");
   const Plan pl = plan(S, n, Hq / Hkv, Hkv, D, (int64_t)page_size * table_width, dtype);
+  ODY_REQUIRE(pl.fits, ODY_ERR_BAD_SHAPE, "ody_paged_attn: 2^31 tiles of keys and more, by the table's width");
   ODY_REQUIRE(pl.part_bytes == 0 || (workspace && workspace_bytes >= pl.part_bytes + pl.ml_bytes && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
               ODY_ERR_WORKSPACE, "ody_paged_attn: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", pl.part_bytes + pl.ml_bytes,
               workspace_bytes);

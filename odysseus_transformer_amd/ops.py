@@ -494,6 +494,14 @@ def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, posi
 
     rotate: queries and keys are rotated as rope_ rotates them, by position_ids -- (S, n), or (n) for all -- or by the tokens' places; the
     queries are a new tensor.  rotate=False: they have been rotated already (linear_rope, norm_linear_rope); the result is a view of qkv."""
+    if not rotate and position_ids is not None:
+        raise ValueError("paged_append_: positions are for a rotation")
+    if qkv.is_cuda:
+        if inv_freq is None and rotate:
+            inv_freq = rope_inv_freq(qkv.shape[-1], base, qkv.device)
+        plain = native.paged_append(qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids, inv_freq if rotate else None)
+        if plain is not None:
+            return plain
     if qkv.is_cuda and qkv.device.index != torch.cuda.current_device():
         with torch.cuda.device(qkv.device):
             return paged_append_(qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids, base, inv_freq, rotate)
@@ -502,9 +510,8 @@ def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, posi
     Hkv = k_pages.shape[2]
     if n_heads <= 0 or heads != n_heads + 2 * Hkv:
         raise ValueError(f"paged_append_: {heads} heads are not {n_heads} query heads and {Hkv} heads of keys and of values")
-    if inv_freq is None and rotate:
-        inv_freq = rope_inv_freq(D, base, qkv.device)
-    check_rope_args(qkv, heads if rotate else 0, position_ids, inv_freq)
+    if rotate:
+        check_rope_args(qkv, heads, position_ids, inv_freq)
     q = torch.empty((S, n, n_heads, D), dtype=qkv.dtype, device=qkv.device) if rotate else qkv[:, :, :n_heads]
     if qkv.numel() == 0:
         return q
@@ -521,6 +528,10 @@ def paged_attn(q, k_pages, v_pages, page_table, lengths, scale: Optional[float] 
     """Attention of the n newest tokens of every sequence, q (S, n, Hq, D), over a cache in pages that holds them already (paged_append_, which
     says what the arguments are): a token sees the places up to its own.  -> out (S, n, Hq, D), lse (S, Hq, n) fp32, 0 and -inf for a
     token that sees none."""
+    if q.is_cuda:
+        plain = native.paged_attn(q, k_pages, v_pages, page_table, lengths, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale)
+        if plain is not None:
+            return plain
     if q.is_cuda and q.device.index != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return paged_attn(q, k_pages, v_pages, page_table, lengths, scale)
