@@ -22,12 +22,25 @@ struct PagedAttnParams {
   float* lse;           // (S, Hq, n)
   AttnStrides sq, so;
   int S, n, Hq, Hkv, group;
-  float scale_log2e;
+  float scale_log2e;    // above 0: a negative scale is the queries' sign, of a scale of 0 the queries are 0
+  unsigned q_keep, q_flip;   // 32 bits of a query, two values or one: kept, then flipped
   int row_tiles;        // of one (sequence, kv head): its rows, token i, query head g of the group as row i * group + g, in tiles of `tile`
   int tile;
   float* part;          // [block][2][tile][D]: results of the first and the last unit of a block's range, where they are not whole
   float2* part_ml;      // [block][2][tile]: their maxima (of scores times log2 e) and sums
+#ifdef __HIPCC__
+  template <typename V> __device__ __forceinline__ V signed_query(V q) const {
+    i32x4 x = __builtin_bit_cast(i32x4, q);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = (x[e] & q_keep) ^ q_flip;
+    return __builtin_bit_cast(V, x);
+  }
+#endif
 };
+
+// The kernel of many rows (paged_attn_chunk.hip): rows of a tile, keys of a step
+constexpr int PAGED_CHUNK_ROWS = 128, PAGED_CHUNK_KEYS = 64;
+int ody_launch_paged_chunk(const PagedAttnParams& p, int D, const PagedCache& c, int blocks, hipStream_t st);
 
 #ifdef __HIPCC__
 // ---- Division of the work.  A unit is a row tile of one (sequence, kv head); its work is a row of steps of STEP keys, up to the last key
@@ -95,10 +108,18 @@ struct PagedWalk {
     while (next()) {}
     return before + all();
   }
-  __device__ __forceinline__ void rewind() {
-    if (at == 0) return;
-    at = before = 0;
-    chunk();
+  // The pair that step `pos` of all kv heads is one of, its steps, and which kv head's and which of them it is.
+  __device__ __forceinline__ int find(int pos, int& hk, int& step, int& steps) {
+    if (at != 0) {
+      at = before = 0;
+      chunk();
+    }
+    while ((before + all()) * p.Hkv <= pos && next()) {}
+    const int k = __popcll(__ballot((before + sums) * p.Hkv <= pos));
+    steps = __builtin_amdgcn_readlane(mine, k);
+    const int into = pos - (before + __builtin_amdgcn_readlane(sums, k) - steps) * p.Hkv;
+    hk = (int)((unsigned)into / (unsigned)steps), step = into - hk * steps;
+    return at + k;
   }
 };
 #endif

@@ -109,14 +109,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
   const int block = blockIdx.x;
   if (block >= cuts.blocks) return;
   const int begin = cuts.at(block), end = cuts.at(block + 1);
-  int pos = begin;
-  // the pair that the range begins in
-  walk.rewind();
-  while ((walk.before + walk.all()) * p.Hkv <= pos && walk.next()) {}
-  const int k = __popcll(__ballot((walk.before + walk.sums) * p.Hkv <= pos));
-  int entry = walk.at + k, steps = __builtin_amdgcn_readlane(walk.mine, k);
-  const int into = pos - (walk.before + __builtin_amdgcn_readlane(walk.sums, k) - steps) * p.Hkv;
-  int hk = (int)((unsigned)into / (unsigned)steps), step = into - hk * steps;
+  int pos = begin, hk, step, steps, entry = walk.find(pos, hk, step, steps);
 
   while (pos < end) {
     const int s = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * p.tile;
@@ -136,7 +129,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
       const int r = row0 + min(16 * m + c, rows - 1), i = r / p.group, h = hk * p.group + r - i * p.group;
       const T* qp = static_cast<const T*>(p.q) + s * p.sq.b + i * p.sq.l + h * p.sq.h;
 #pragma unroll
-      for (int j = 0; j < (int)(D * sizeof(T) / 64); j++) qf[m][j] = *reinterpret_cast<const typename G::kvec*>(qp + G::key_col(q, j));
+      for (int j = 0; j < (int)(D * sizeof(T) / 64); j++) qf[m][j] = p.signed_query(*reinterpret_cast<const typename G::kvec*>(qp + G::key_col(q, j)));
       lim[m] = min(keys - 1, length - p.n + i);
     }
     safe = min(safe, length - p.n + row0 / p.group);
@@ -173,10 +166,6 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
       float w[NT][GK];
 #pragma unroll
       for (int m = 0; m < NT; m++) scores<D>(t, qf[m], w[m]);
-#pragma unroll
-      for (int m = 0; m < NT; m++)
-#pragma unroll
-        for (int e = 0; e < GK; e++) w[m][e] *= p.scale_log2e;
       // keys that a row does not see, that no token has, that have no page: neither their scores nor their values count, whatever lies there
       if (base + G::KEYS - 1 > safe || !__all(t.page)) {
         const int most = t.page ? keys - 1 : -1;
@@ -195,11 +184,11 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
         for (int e = 1; e < GK; e++) top = fmaxf(top, w[m][e]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float now = fmaxf(mx[m], top), ref = now == -INFINITY ? 0.f : now, alpha = ody_exp2(mx[m] - ref);
+        const float now = fmaxf(mx[m], top * p.scale_log2e), ref = now == -INFINITY ? 0.f : now, alpha = ody_exp2(mx[m] - ref);
         mx[m] = now;
         float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < GK; e++) w[m][e] = ody_exp2(w[m][e] - ref), sum += w[m][e];
+        for (int e = 0; e < GK; e++) w[m][e] = ody_exp2(fmaf(w[m][e], p.scale_log2e, -ref)), sum += w[m][e];
         l[m] = l[m] * alpha + sum;   // this lane's share of the row sum
 #pragma unroll
         for (int i = 0; i < D / 16; i++) o[m][i] *= alpha;
@@ -289,17 +278,19 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
   }
 }
 
-// One block per row: the parts of its unit, if a cut goes through it, weighted by their sums.  A wavefront finds the weights, then
-// 256 / (D / 4) threads per column vector share the parts.
-template <typename T, int D, int STEP>
+// The parts of the units that a cut goes through, weighted by their sums.  A block takes R rows of a row tile (a divisor of it), with D / 4 threads on a
+// row: all of the threads share a row's parts, in turn for each row, or where the parts are few every group of threads has a row.
+constexpr int JOIN_ROWS = 8, JOIN_FEW = 16;
+template <typename T, int D, int STEP, int R>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p, const PagedCache cache, int most_blocks) {
-  constexpr int C4 = D / 4, GROUPS = 256 / C4;
-  __shared__ float weight[BLOCKS];
+  constexpr int C4 = D / 4, GROUPS = 256 / C4, U = 4;
   __shared__ f32x4 red[GROUPS][C4];
+  __shared__ float2 red_ml[GROUPS];
   const int tid = threadIdx.x, lane = tid & 63;
-  // blockIdx.x: (sequence, row of all rows of a kv head, kv head)
-  const int all_rows = p.n * p.group, hk = blockIdx.x % p.Hkv, row = blockIdx.x / p.Hkv % all_rows, s = blockIdx.x / p.Hkv / all_rows;
-  const int rt = row / p.tile, r = row - rt * p.tile, entry = s * p.row_tiles + rt;
+  // blockIdx.x: (sequence, R rows of all rows of a kv head, kv head)
+  const int all_rows = p.n * p.group, row_blocks = (all_rows + R - 1) / R;
+  const int hk = blockIdx.x % p.Hkv, row0 = blockIdx.x / p.Hkv % row_blocks * R, s = blockIdx.x / p.Hkv / row_blocks;
+  const int rt = row0 / p.tile, entry = s * p.row_tiles + rt;
   PagedWalk<STEP> walk(p, cache, lane);
   int before = 0, steps = 0;
   do {
@@ -313,70 +304,111 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   if (parts == 1) return;
   // part k is in slot 2 (b0 + k), but for the first where that block's range begins with another unit
   const int first_slot = 2 * b0 + (first > cuts.at(b0));
-  auto slot = [&](int k) { return ((int64_t)(k == 0 ? first_slot : 2 * (b0 + k))) * p.tile + r; };
-  const int i = row / p.group, h = hk * p.group + row - i * p.group;
-  if (tid < 64) {
-    float m = -INFINITY, l = 0.f;
-    for (int k = lane; k < parts; k += 64) {
-      const float2 ml = p.part_ml[slot(k)];
-      const float now = fmaxf(m, ml.x), ref = now == -INFINITY ? 0.f : now;
-      l = l * ody_exp2(m - ref) + ml.y * ody_exp2(ml.x - ref), m = now;
-    }
-    float top = m;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float ref = top == -INFINITY ? 0.f : top;
-    l *= ody_exp2(m - ref);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int k = lane; k < parts; k += 64) weight[k] = ody_exp2(p.part_ml[slot(k)].x - ref) * inv;
-    if (lane == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + i] = l == 0.f ? -INFINITY : (top + __log2f(l)) * ODY_LN2;
-  }
   const int d4 = tid % C4, g = tid / C4;
-  const float* src = p.part + 4 * d4;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  __syncthreads();
-#pragma unroll 4
-  for (int k = g; k < parts; k += GROUPS) acc += weight[k] * *reinterpret_cast<const f32x4*>(src + slot(k) * D);
-  red[g][d4] = acc;
-  __syncthreads();
-  if (g != 0) return;
+  auto write = [&](int row, float m, float l, f32x4 acc) {
+    const int i = row / p.group, h = hk * p.group + row - i * p.group;
+    typedef T out4 __attribute__((ext_vector_type(4)));
+    acc *= l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<out4*>(static_cast<T*>(p.out) + s * p.so.b + i * p.so.l + h * p.so.h + 4 * d4) = out4{(T)acc[0], (T)acc[1], (T)acc[2], (T)acc[3]};
+    if (d4 == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + i] = l == 0.f ? -INFINITY : (m + __log2f(l)) * ODY_LN2;
+  };
+  // parts from .. in steps of `by`, U at a time
+  auto sum = [&](int row, int from, int by, float& m, float& l, f32x4& acc) {
+    const int r = row - rt * p.tile;
+    m = -INFINITY, l = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = from; k < parts; k += U * by) {
+      float2 ml[U];
+      f32x4 o[U];
 #pragma unroll
-  for (int k = 1; k < GROUPS; k++) acc += red[k][d4];
-  typedef T out4 __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<out4*>(static_cast<T*>(p.out) + s * p.so.b + i * p.so.l + h * p.so.h + 4 * d4) = out4{(T)acc[0], (T)acc[1], (T)acc[2], (T)acc[3]};
+      for (int u = 0; u < U; u++) {
+        const int part = min(k + u * by, parts - 1);
+        const int64_t at = (int64_t)(part == 0 ? first_slot : 2 * (b0 + part)) * p.tile + r;
+        ml[u] = p.part_ml[at];
+        o[u] = *reinterpret_cast<const f32x4*>(p.part + at * D + 4 * d4);
+      }
+      float now = m;
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (u == 0 || k + u * by < parts) now = fmaxf(now, ml[u].x);
+      const float ref = now == -INFINITY ? 0.f : now, old = ody_exp2(m - ref);
+      m = now, l *= old, acc *= old;
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (u == 0 || k + u * by < parts) {
+          const float w = ody_exp2(ml[u].x - ref);
+          l += ml[u].y * w, acc += o[u] * w;
+        }
+    }
+  };
+  float m, l;
+  f32x4 acc;
+  if (R > 1 && parts <= JOIN_FEW) {
+    for (int row = row0 + g; row < min(row0 + R, all_rows); row += GROUPS) {
+      sum(row, 0, 1, m, l, acc);
+      write(row, m, l, acc);
+    }
+    return;
+  }
+  for (int row = row0; row < min(row0 + R, all_rows); row++) {
+    sum(row, g, GROUPS, m, l, acc);
+    red[g][d4] = acc;
+    if (d4 == 0) red_ml[g] = make_float2(m, l);
+    __syncthreads();
+    if (g == 0) {
+      m = -INFINITY, l = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < GROUPS; k++) m = fmaxf(m, red_ml[k].x);
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int k = 0; k < GROUPS; k++) {
+        const float w = ody_exp2(red_ml[k].x - ref);
+        l += red_ml[k].y * w, acc += red[k][d4] * w;
+      }
+      write(row, m, l, acc);
+    }
+    if (R > 1) __syncthreads();
+  }
 }
 
-// Row tiles of 16, 32 or 64.
-int row_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-int step_keys(int dtype) { return WAVES * (dtype == ODY_BF16 ? 32 : 16); }
+// Row tiles of 16, 32 or 64 here, the rest in bf16 by the kernel of many rows.
 struct Plan {
-  int tile, row_tiles, blocks;
+  int tile, row_tiles, step, blocks;
   bool joined;          // a cut may go through a unit
   bool fits;            // the steps can be counted
   size_t part_bytes, ml_bytes;
 };
 Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype) {
   const int64_t rows = (int64_t)n * group;
-  const int tile = row_tile(rows), row_tiles = (int)((rows + tile - 1) / tile);
-  const int64_t steps = std::max((int64_t)1, (most_keys + step_keys(dtype) - 1) / step_keys(dtype));   // of a unit, at most
-  const int blocks = (int)std::min((double)BLOCKS, (double)S * row_tiles * Hkv * steps);
+  const bool chunk = rows > 64 && dtype == ODY_BF16;
+  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : chunk ? PAGED_CHUNK_ROWS : 64, row_tiles = (int)((rows + tile - 1) / tile);
+  const int step = chunk ? PAGED_CHUNK_KEYS : WAVES * (dtype == ODY_BF16 ? 32 : 16);
+  const int64_t steps = std::max((int64_t)1, (most_keys + step - 1) / step);   // of a unit, at most
+  const double all = (double)S * row_tiles * Hkv * steps;
+  const int blocks = (int)std::min((double)BLOCKS, all);
   const bool joined = steps > 1;
   const size_t parts = joined ? (size_t)blocks * 2 * tile : 0;
-  return Plan{tile, row_tiles, blocks, joined, (double)S * row_tiles * Hkv * steps < 2147483648.0, parts * D * sizeof(float), parts * sizeof(float2)};
+  return Plan{tile, row_tiles, step, blocks, joined, all < 2147483648.0, parts * D * sizeof(float), parts * sizeof(float2)};
 }
 
+template <typename T, int D, int STEP, int R>
+int join(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
+  if (!pl.joined) return ODY_OK;
+  const int row_blocks = (p.n * p.group + R - 1) / R;
+  ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, R>), dim3((unsigned)(p.S * row_blocks * p.Hkv)), dim3(256), 0, p, c, pl.blocks);
+  return ody_check_launch("paged_join");
+}
 template <typename T, int D, int NT>
 int launch(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
   ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
-  int rc = ody_check_launch("paged_attn");
-  if (rc || !pl.joined) return rc;
-  ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, WAVES * Tile<T, D>::KEYS>), dim3((unsigned)(p.S * p.n * p.Hq)), dim3(256), 0, p, c, pl.blocks);
-  return ody_check_launch("paged_join");
+  const int rc = ody_check_launch("paged_attn");
+  return rc ? rc : join<T, D, WAVES * Tile<T, D>::KEYS, NT == 4 ? JOIN_ROWS : 1>(p, c, pl, st);
 }
 template <typename T, int D>
 int by_rows(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
+  if (pl.tile == PAGED_CHUNK_ROWS) {
+    const int rc = ody_launch_paged_chunk(p, D, c, pl.blocks, st);
+    return rc ? rc : join<bf16, D, PAGED_CHUNK_KEYS, JOIN_ROWS>(p, c, pl, st);
+  }
   return pl.tile == 16 ? launch<T, D, 1>(p, c, pl, st) : pl.tile == 32 ? launch<T, D, 2>(p, c, pl, st) : launch<T, D, 4>(p, c, pl, st);
 }
 template <typename T>
@@ -409,7 +441,9 @@ extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_
               ODY_ERR_WORKSPACE, "ody_paged_attn: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", pl.part_bytes + pl.ml_bytes,
               workspace_bytes);
   float* part = static_cast<float*>(workspace);
-  const PagedAttnParams p{q, out, lse, {sq_s, sq_n, sq_h}, {so_s, so_n, so_h}, S, n, Hq, Hkv, Hq / Hkv, scale * ODY_LOG2E, pl.row_tiles, pl.tile,
+  const PagedAttnParams p{q, out, lse, {sq_s, sq_n, sq_h}, {so_s, so_n, so_h}, S, n, Hq, Hkv, Hq / Hkv,
+                          scale == 0.f ? 1.f : std::fabs(scale) * ODY_LOG2E, scale == 0.f ? 0u : ~0u,
+                          scale < 0.f ? (dtype == ODY_BF16 ? 0x80008000u : 0x80000000u) : 0u, pl.row_tiles, pl.tile,
                           part, reinterpret_cast<float2*>(static_cast<char*>(workspace) + pl.part_bytes)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == ODY_BF16 ? by_head_dim<bf16>(p, D, c, pl, st) : by_head_dim<float>(p, D, c, pl, st);
