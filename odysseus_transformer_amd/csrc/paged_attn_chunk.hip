@@ -2,30 +2,34 @@
 // times the tokens).
 //
 // Bound by the matrix cores and, as much, by the vector work of the softmax between the two products.  A block of four wavefronts takes 128 rows of one
-// (sequence, kv head), 32 a wavefront, and streams the keys in tiles of 64 through LDS, two buffers, the loads a tile ahead and the page numbers
-// two.  Both products are computed transposed, so that a row's maximum, sum and rescaling belong to one lane (and the one 32 lanes away):
+// (sequence, kv head), 32 a wavefront, and streams the keys in tiles of 64, which direct loads bring to LDS a tile ahead (the page numbers two).  Both
+// products are computed transposed, so that a row's maximum, sum and rescaling belong to one lane and the one 32 lanes away:
 //
 //      S^T (keys x rows) = K Q^T        A: K rows from LDS      B: this lane's query row, in registers
 //      O^T (D x rows) += V^T P^T        B: P^T as the accumulators of S^T hold it      A: V^T by transposing LDS reads
 //
-// on v_mfma_f32_32x32x16_bf16 (lane = 32 g + i: A row i / B column i, k = 8 g .. 8 g + 7; accumulator column i, rows 8 (r / 4) + 4 g + r % 4).
+// on v_mfma_f32_32x32x16_bf16, tiles laid out and read as attn_rowtile.h has it.
 #include <cmath>
+#include <type_traits>
+#include "attn_rowtile.h"
 #include "paged.h"
 
 namespace {
 
-constexpr int KEYS = PAGED_CHUNK_KEYS, ROWS = PAGED_CHUNK_ROWS;
+using namespace rowtile;
+
+constexpr int KEYS = PAGED_CHUNK_KEYS, BLOCK_ROWS = PAGED_CHUNK_ROWS, WAVES = 4;
+static_assert(KEYS == ROWS && BLOCK_ROWS == 32 * WAVES, "a tile of keys, 32 rows a wavefront");
+
+__device__ const bf16x8 no_key[16] = {};   // the row that a key without a page, or behind the last one, is read from
 
 template <int D>
-__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnParams p, const PagedCache cache) {
-  constexpr int KP = D + 8;     // pitches: 16-byte reads of 16 rows, and transposing reads of 4 rows x 32 columns, hit every bank alike
-  constexpr int VP = D + 32;
-  constexpr int KS = D / 16, DT = D / 32;
-  constexpr int CPR = D / 8, RPL = 256 / CPR, LOADS = KEYS / RPL;   // 16-byte chunks of a row, rows of one load of the block
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
-  bf16* Ks = reinterpret_cast<bf16*>(smem_raw);            // [2][KEYS][KP]
-  bf16* Vs = Ks + 2 * KEYS * KP;                           // [2][KEYS][VP]
-  __shared__ __attribute__((aligned(8))) unsigned char paged[2][KEYS / 8];   // the tile's groups of 8 keys that have a page
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedAttnParams p, const PagedCache cache) {
+  constexpr int KS = D / 16, DT = D / 32, TILE = KEYS * D, STAGE = 2 * TILE;         // elements
+  constexpr int LANES = D / 8, PER = 64 / LANES, STEP = PER * WAVES, LOADS = KEYS / STEP;   // of a direct load: lanes on a row, rows; of a tile
+  static_assert(STEP % 16 == 0, "swz of the rows of the other loads");
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  bf16* stages = reinterpret_cast<bf16*>(smem);   // [2][K tile | V tile]
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 5, i = lane & 31;
   PagedWalk<KEYS> walk(p, cache, lane);
@@ -34,14 +38,50 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnPara
   if (block >= cuts.blocks) return;
   const int begin = cuts.at(block), end = cuts.at(block + 1);
   int pos = begin, hk, step, steps, entry = walk.find(pos, hk, step, steps);
+  const int lrow = PER * wave + lane / LANES, lcol = 8 * ((lane % LANES) ^ swz<D>(lrow));   // of this lane in the first direct load
+  const float c2 = p.scale_log2e;
+  Readers<D> rd;
+  rd.init(stages, g, i);
 
   while (pos < end) {
-    const int s = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * ROWS;
-    const int rows = min(ROWS, p.n * p.group - row0), length = paged_length(cache, s);
-    const int keys = paged_keys(p, cache, length, rt), steps_here = min(steps - step, end - pos);
+    const int s = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * BLOCK_ROWS;
+    const int rows = min(BLOCK_ROWS, p.n * p.group - row0), length = paged_length(cache, s);
+    const int keys = paged_keys(p, cache, length, rt), steps_here = min(steps - step, end - pos), tiles = keys > 0 ? steps_here : 0;
     const bf16* kp = static_cast<const bf16*>(cache.k) + hk * cache.sk.h;
     const bf16* vp = static_cast<const bf16*>(cache.v) + hk * cache.sv.h;
     const int* table = cache.table + s * cache.table_stride;
+
+    // ---- pages: of the rows that this lane loads, and of the tile's group lane % 8 of 8 keys
+    struct Pages { int of[LOADS], group; };
+    auto lookup = [&](int t) {
+      Pages pg;
+      const int n0 = (step + t) * KEYS;
+#pragma unroll
+      for (int j = 0; j < LOADS; j++) pg.of[j] = table[min(n0 + lrow + STEP * j, keys - 1) >> cache.shift];
+      pg.group = table[min(n0 + 8 * (lane & 7), keys - 1) >> cache.shift];
+      return pg;
+    };
+    auto load = [&](int t, const Pages& pg) {
+      bf16* stage = stages + (t & 1) * STAGE;
+#pragma unroll
+      for (int j = 0; j < LOADS; j++) {
+        const int key = (step + t) * KEYS + lrow + STEP * j, row = key & ((1 << cache.shift) - 1);
+        const bool have = key < keys && (unsigned)pg.of[j] < (unsigned)cache.pages;
+        const bf16* none = reinterpret_cast<const bf16*>(no_key) + lcol;
+        const bf16* ks = kp + pg.of[j] * cache.sk.p + row * cache.sk.r + lcol;
+        const bf16* vs = vp + pg.of[j] * cache.sv.p + row * cache.sv.r + lcol;
+        __builtin_amdgcn_global_load_lds((global_ptr)(have ? ks : none), (lds_ptr)(stage + (WAVES * j + wave) * 512), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((global_ptr)(have ? vs : none), (lds_ptr)(stage + TILE + (WAVES * j + wave) * 512), 16, 0, 0);
+      }
+    };
+    Pages next;
+    int group_page = 0;
+    if (tiles > 0) {
+      next = lookup(0);
+      load(0, next);
+      group_page = next.group;
+      next = lookup(1);
+    }
 
     // ---- this lane's row: token ri, query head h
     const int r = row0 + min(32 * wave + i, rows - 1), ri = r / p.group, h = hk * p.group + r - ri * p.group;
@@ -57,145 +97,88 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnPara
     const int seen = 32 * wave < rows ? __builtin_amdgcn_readfirstlane(min(keys - 1, length - p.n + (row0 + last_row) / p.group)) : -1;
 
     f32x16 o[DT];
-    float m = -INFINITY, l = 0.f;
+    clear(o);
+    float ref = -INFINITY, l4[4] = {0.f, 0.f, 0.f, 0.f};
+    auto tile = [&](int n0, unsigned have) {
+      f32x16 x[2];
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++)
+      for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) o[dt][e] = 0.f;
-
-    // ---- loads: row tid / CPR + RPL j of a tile, 16 bytes at column 8 (tid % CPR)
-    const int lr = tid / CPR, lc = tid % CPR * 8;
-    int pg[LOADS];
-    bf16x8 kr[LOADS], vr[LOADS];
-    unsigned has;   // bit j: row j's page is one
-    auto lookup = [&](int t) {
+        for (int kt = 0; kt < 2; kt++) x[kt] = mfma32(row_frag(rd, 32 * kt, ks), qf[ks], ks == 0 ? f32x16{0} : x[kt]);
+      if (n0 + KEYS - 1 > safe || have != 0xff) {
 #pragma unroll
-      for (int j = 0; j < LOADS; j++) pg[j] = table[max(0, min((step + t) * KEYS + lr + RPL * j, keys - 1)) >> cache.shift];
-    };
-    auto load = [&](int t) {
-      has = 0;
+        for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-      for (int j = 0; j < LOADS; j++) {
-        const int key = (step + t) * KEYS + lr + RPL * j, row = key & ((1 << cache.shift) - 1);
-        const bool ok = (unsigned)pg[j] < (unsigned)cache.pages;
-        has |= (unsigned)ok << j;
-        if (ok && key < keys) {
-          kr[j] = *reinterpret_cast<const bf16x8*>(kp + pg[j] * cache.sk.p + row * cache.sk.r + lc);
-          vr[j] = *reinterpret_cast<const bf16x8*>(vp + pg[j] * cache.sv.p + row * cache.sv.r + lc);
-        } else {
-          kr[j] = vr[j] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+          for (int e = 0; e < 16; e++)
+            if (n0 + 32 * kt + acc_row(e, g) > lim || (have >> (4 * kt + (e >> 2)) & 1) == 0) x[kt][e] = -INFINITY;
+      }
+      float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+      for (int e = 1; e < 16; e++) top = fmaxf(top, fmaxf(x[0][e], x[1][e]));
+      top = half_swap_max(top) * c2;
+      if (__builtin_amdgcn_ballot_w64(top > ref) != 0) {   // somebody's maximum has grown
+        const float now = fmaxf(ref, top), alpha = now == -INFINITY ? 1.f : ody_exp2(ref - now);
+        ref = now;
+#pragma unroll
+        for (int e = 0; e < 4; e++) l4[e] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[dt][e] *= alpha;
+      }
+      const float minus = ref == -INFINITY ? 0.f : -ref;
+      auto half = [&](auto which) {
+        constexpr int kt = decltype(which)::value;
+        bf16x8 pb[2], vf[2];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const float w = ody_exp2(fmaf(x[kt][e], c2, minus));
+          l4[e & 3] += w;
+          pb[e >> 3][e & 7] = (bf16)w;
         }
-      }
-    };
-    auto store = [&](int buf) {
+        auto product = [&](auto slice) {   // 16 keys, 64 columns
+          constexpr int ss = decltype(slice)::value & 1, hf = decltype(slice)::value >> 1;
+          tr_frags<ROWS + 32 * kt + 16 * ss, hf>(vf, rd);
 #pragma unroll
-      for (int j = 0; j < LOADS; j++) {
-        *reinterpret_cast<bf16x8*>(Ks + (buf * KEYS + lr + RPL * j) * KP + lc) = kr[j];
-        *reinterpret_cast<bf16x8*>(Vs + (buf * KEYS + lr + RPL * j) * VP + lc) = vr[j];
-        if (lc == 0 && (lr + RPL * j) % 8 == 0) paged[buf][(lr + RPL * j) / 8] = has >> j & 1;
-      }
+          for (int dt = 0; dt < 2; dt++) o[2 * hf + dt] = mfma32(vf[dt], pb[ss], o[2 * hf + dt]);
+        };
+        product(std::integral_constant<int, 0>{});
+        if constexpr (D == 128) product(std::integral_constant<int, 2>{});
+        product(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) product(std::integral_constant<int, 3>{});
+      };
+      half(std::integral_constant<int, 0>{});
+      half(std::integral_constant<int, 1>{});
     };
-    const int tiles = keys > 0 ? steps_here : 0;
-    if (tiles > 0) {
-      lookup(0);
-      load(0);
-      lookup(1);
-      store(0);
-    }
-    __syncthreads();
-
-    const int tr_row = (i & 15) >> 2, tr_col = 16 * (i >> 4) + 4 * (i & 3);   // of a transposing read, within 16 lanes
     for (int t = 0; t < tiles; t++) {
-      const int buf = t & 1, n0 = (step + t) * KEYS;
+      const unsigned have = (unsigned)__builtin_amdgcn_ballot_w64((unsigned)group_page < (unsigned)cache.pages) & 0xff;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();   // the tile has landed, and everyone is done with the one before
       if (t + 1 < tiles) {
-        load(t + 1);
-        lookup(t + 2);
+        load(t + 1, next);
+        group_page = next.group;
+        next = lookup(t + 2);
       }
-      if (n0 <= seen) {
-        const bf16* Kb = Ks + buf * KEYS * KP;
-        const bf16* Vb = Vs + buf * KEYS * VP;
-        f32x16 x[2];
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-#pragma unroll
-          for (int e = 0; e < 16; e++) x[kt][e] = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < KS; ks++) x[kt] = mfma32(*reinterpret_cast<const bf16x8*>(Kb + (32 * kt + i) * KP + 16 * ks + 8 * g), qf[ks], x[kt]);
-        }
-        const uint64_t have = *reinterpret_cast<const uint64_t*>(paged[buf]);
-        if (n0 + KEYS - 1 > safe || !__all(have == 0x0101010101010101ull)) {
-#pragma unroll
-          for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-              const int group = 4 * kt + (e >> 2);
-              if (n0 + 8 * group + 4 * g + (e & 3) > lim || (have >> (8 * group) & 1) == 0) x[kt][e] = -INFINITY;
-            }
-        }
-        float top = x[0][0];
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) top = fmaxf(top, x[kt][e]);
-        top = fmaxf(top, xor32(top)) * p.scale_log2e;
-        const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
-        if (!__all(now == m)) {   // somebody's maximum has grown
-          const float alpha = ody_exp2(m - ref);
-          l *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[dt][e] *= alpha;
-        }
-        m = now;
-        bf16x8 pb[2][2];
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const float w = ody_exp2(fmaf(x[kt][e], p.scale_log2e, -ref));
-            l += w;
-            pb[kt][e / 8][e % 8] = (bf16)w;
-          }
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-          for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int ss = 0; ss < 2; ss++) {
-              const bf16* va = Vb + (32 * kt + 16 * ss + 4 * g + tr_row) * VP + 32 * dt + tr_col;
-              o[dt] = mfma32(concat4(lds_read_tr16(va), lds_read_tr16(va + 8 * VP)), pb[kt][ss], o[dt]);
-            }
-      }
-      if (t + 1 < tiles) store(buf ^ 1);
-      __syncthreads();
+      const int n0 = (step + t) * KEYS;
+      if (n0 <= seen) tile(n0, have);
+      rd.move(t & 1 ? -(int)(STAGE * sizeof(bf16)) : (int)(STAGE * sizeof(bf16)));
     }
+    if (tiles & 1) rd.move(-(int)(STAGE * sizeof(bf16)));
+    __syncthreads();   // everyone is done with the stages
 
-    // ---- o[dt][4 a + e] of this lane's row: column 32 dt + 8 a + 4 g + e
-    const float sum = l + xor32(l);
-    const bool whole = steps_here == steps;
+    const float sum = half_swap_sum((l4[0] + l4[1]) + (l4[2] + l4[3]));
     if (32 * wave + i < rows) {
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        bf16* dst = static_cast<bf16*>(p.out) + s * p.so.b + ri * p.so.l + h * p.so.h + 4 * g;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-          for (int a = 0; a < 4; a++) {
-            bf16x4 w;
-#pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = (bf16)(o[dt][4 * a + e] * inv);
-            *reinterpret_cast<bf16x4*>(dst + 32 * dt + 8 * a) = w;
-          }
-        if (g == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + ri] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * ODY_LN2;
+      if (steps_here == steps) {
+        store_row(static_cast<bf16*>(p.out) + s * p.so.b + ri * p.so.l + h * p.so.h, o, sum == 0.f ? 0.f : 1.f / sum, g);
+        if (g == 0) p.lse[((int64_t)s * p.Hq + h) * p.n + ri] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * ODY_LN2;
       } else {
-        const int64_t at = (int64_t)(2 * block + (pos > begin)) * ROWS + 32 * wave + i;
+        const int64_t at = (int64_t)(2 * block + (pos > begin)) * BLOCK_ROWS + 32 * wave + i;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
           for (int a = 0; a < 4; a++)
             *reinterpret_cast<f32x4*>(p.part + at * D + 32 * dt + 8 * a + 4 * g) = f32x4{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
-        if (g == 0) p.part_ml[at] = make_float2(m, sum);
+        if (g == 0) p.part_ml[at] = make_float2(ref, sum);
       }
     }
     pos += steps_here;
@@ -206,9 +189,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(const PagedAttnPara
 
 template <int D>
 int launch(const PagedAttnParams& p, const PagedCache& c, int blocks, hipStream_t st) {
-  constexpr size_t smem = (size_t)2 * KEYS * ((D + 8) + (D + 32)) * sizeof(bf16);
+  constexpr size_t smem = (size_t)4 * KEYS * D * sizeof(bf16);
   if (int rc = ody_allow_dynamic_lds(reinterpret_cast<const void*>(&paged_chunk_kernel<D>), smem, "ody_paged_attn")) return rc;
-  ODY_LAUNCH("paged_chunk", st, (paged_chunk_kernel<D>), dim3(blocks), dim3(256), smem, p, c);
+  ODY_LAUNCH("paged_chunk", st, (paged_chunk_kernel<D>), dim3(blocks), dim3(64 * WAVES), smem, p, c);
   return ody_check_launch("paged_chunk");
 }
 
