@@ -39,6 +39,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
   const int begin = cuts.at(block), end = cuts.at(block + 1);
   int pos = begin, hk, step, steps, entry = walk.find(pos, hk, step, steps);
   const int lrow = PER * wave + lane / LANES, lcol = 8 * ((lane % LANES) ^ swz<D>(lrow));   // of this lane in the first direct load
+  const int64_t lk = lane / LANES * cache.sk.r + lcol, lv = lane / LANES * cache.sv.r + lcol;
   const float c2 = p.scale_log2e;
   Readers<D> rd;
   rd.init(stages, g, i);
@@ -51,35 +52,32 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
     const bf16* vp = static_cast<const bf16*>(cache.v) + hk * cache.sv.h;
     const int* table = cache.table + s * cache.table_stride;
 
-    // ---- pages: of the rows that this lane loads, and of the tile's group lane % 8 of 8 keys
-    struct Pages { int of[LOADS], group; };
-    auto lookup = [&](int t) {
-      Pages pg;
-      const int n0 = (step + t) * KEYS;
-#pragma unroll
-      for (int j = 0; j < LOADS; j++) pg.of[j] = table[min(n0 + lrow + STEP * j, keys - 1) >> cache.shift];
-      pg.group = table[min(n0 + 8 * (lane & 7), keys - 1) >> cache.shift];
-      return pg;
-    };
-    auto load = [&](int t, const Pages& pg) {
+    // ---- lane n % 8 holds the page of the tile's n-th group of 8 keys; the rows of a direct load are in one of them
+    auto lookup = [&](int t) { return table[min((step + t) * KEYS + 8 * (lane & 7), keys - 1) >> cache.shift]; };
+    auto load = [&](int t, int pages, unsigned have) {
       bf16* stage = stages + (t & 1) * STAGE;
 #pragma unroll
       for (int j = 0; j < LOADS; j++) {
-        const int key = (step + t) * KEYS + lrow + STEP * j, row = key & ((1 << cache.shift) - 1);
-        const bool have = key < keys && (unsigned)pg.of[j] < (unsigned)cache.pages;
-        const bf16* none = reinterpret_cast<const bf16*>(no_key) + lcol;
-        const bf16* ks = kp + pg.of[j] * cache.sk.p + row * cache.sk.r + lcol;
-        const bf16* vs = vp + pg.of[j] * cache.sv.p + row * cache.sv.r + lcol;
-        __builtin_amdgcn_global_load_lds((global_ptr)(have ? ks : none), (lds_ptr)(stage + (WAVES * j + wave) * 512), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((global_ptr)(have ? vs : none), (lds_ptr)(stage + TILE + (WAVES * j + wave) * 512), 16, 0, 0);
+        const int first = STEP * j + PER * wave, key = (step + t) * KEYS + first, row = key & ((1 << cache.shift) - 1);
+        const int page = __builtin_amdgcn_readlane(pages, first / 8);
+        const bf16* ks = kp + page * cache.sk.p + row * cache.sk.r + lk;
+        const bf16* vs = vp + page * cache.sv.p + row * cache.sv.r + lv;
+        if (key + PER > keys || (have >> (first / 8) & 1) == 0) {
+          const bool none = key + lane / LANES >= keys || (have >> (first / 8) & 1) == 0;
+          const bf16* zero = reinterpret_cast<const bf16*>(no_key) + lcol;
+          ks = none ? zero : ks, vs = none ? zero : vs;
+        }
+        __builtin_amdgcn_global_load_lds((global_ptr)ks, (lds_ptr)(stage + (WAVES * j + wave) * 512), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((global_ptr)vs, (lds_ptr)(stage + TILE + (WAVES * j + wave) * 512), 16, 0, 0);
       }
     };
-    Pages next;
-    int group_page = 0;
+    auto have_pages = [&](int pages) { return (unsigned)__builtin_amdgcn_ballot_w64((unsigned)pages < (unsigned)cache.pages) & 0xff; };
+    int next = 0;
+    unsigned have = 0;
     if (tiles > 0) {
       next = lookup(0);
-      load(0, next);
-      group_page = next.group;
+      have = have_pages(next);
+      load(0, next, have);
       next = lookup(1);
     }
 
@@ -151,16 +149,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
       half(std::integral_constant<int, 1>{});
     };
     for (int t = 0; t < tiles; t++) {
-      const unsigned have = (unsigned)__builtin_amdgcn_ballot_w64((unsigned)group_page < (unsigned)cache.pages) & 0xff;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();   // the tile has landed, and everyone is done with the one before
+      const unsigned now = have;
       if (t + 1 < tiles) {
-        load(t + 1, next);
-        group_page = next.group;
+        have = have_pages(next);
+        load(t + 1, next, have);
         next = lookup(t + 2);
       }
       const int n0 = (step + t) * KEYS;
-      if (n0 <= seen) tile(n0, have);
+      if (n0 <= seen) tile(n0, now);
       rd.move(t & 1 ? -(int)(STAGE * sizeof(bf16)) : (int)(STAGE * sizeof(bf16)));
     }
     if (tiles & 1) rd.move(-(int)(STAGE * sizeof(bf16)));
