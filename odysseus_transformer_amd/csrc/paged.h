@@ -14,6 +14,9 @@ struct PagedCache {
   PageStrides sk, sv;
   int64_t table_stride;
   int pages, shift, width;
+  unsigned k_page, k_row, v_page, v_row;   // bytes from page to page and from row to row (paged_check: rows of a page lie within 4 GiB, as pages' starts do)
+  PagedCache(void* k_, void* v_, const int* table_, const int* lengths_, PageStrides sk_, PageStrides sv_, int64_t table_stride_, int pages_, int page_size,
+             int width_, int dtype);
 };
 
 struct PagedAttnParams {
@@ -44,7 +47,7 @@ int ody_launch_paged_chunk(const PagedAttnParams& p, int D, const PagedCache& c,
 
 #ifdef __HIPCC__
 // ---- Division of the work.  A unit is a row tile of one (sequence, kv head); its work is a row of steps of STEP keys, up to the last key
-// that its last row sees, one at least.  All steps of all units, in the order (sequence, row tile, kv head, step), are cut into gridDim.x
+// that its last row sees, one at least.  All steps of all units, in the order (kv head, sequence, row tile, step), are cut into gridDim.x
 // ranges of equal length (to a step), so that blocks finish together whatever the lengths are; a unit that a cut goes through has its
 // results joined by a second kernel.  Fewer steps than blocks: a step each, for as many as there are.  Every block finds its range by itself from the lengths on the device: a captured graph replays with
 // the lengths of that time, and there is no plan to be kept.
@@ -71,6 +74,13 @@ __device__ __forceinline__ int paged_wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);   // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);
   return x;
+}
+
+// The range that a block takes, of `blocks`: blocks of one XCD, which share its L2, take ranges in a row, so that row tiles of one (sequence, kv head) meet
+// there.  Behind the last range: none.
+__device__ __forceinline__ int paged_range(int block, int blocks) {
+  const int each = (blocks + 7) / 8, range = (block & 7) * each + (block >> 3);
+  return block >> 3 < each ? range : blocks;
 }
 
 // Where the cuts are: `total` steps (below 2^31, which the host checks) over as many of the blocks as have one.
@@ -108,17 +118,18 @@ struct PagedWalk {
     while (next()) {}
     return before + all();
   }
-  // The pair that step `pos` of all kv heads is one of, its steps, and which kv head's and which of them it is.
-  __device__ __forceinline__ int find(int pos, int& hk, int& step, int& steps) {
+  // The pair that step `pos` of all kv heads is one of, `total` of each; its steps, and which kv head's and which of them it is.
+  __device__ __forceinline__ int find(int pos, int total, int& hk, int& step, int& steps) {
+    hk = (int)((unsigned)pos / (unsigned)total);
+    pos -= hk * total;
     if (at != 0) {
       at = before = 0;
       chunk();
     }
-    while ((before + all()) * p.Hkv <= pos && next()) {}
-    const int k = __popcll(__ballot((before + sums) * p.Hkv <= pos));
+    while (before + all() <= pos && next()) {}
+    const int k = __popcll(__ballot(before + sums <= pos));
     steps = __builtin_amdgcn_readlane(mine, k);
-    const int into = pos - (before + __builtin_amdgcn_readlane(sums, k) - steps) * p.Hkv;
-    hk = (int)((unsigned)into / (unsigned)steps), step = into - hk * steps;
+    step = pos - (before + __builtin_amdgcn_readlane(sums, k) - steps);
     return at + k;
   }
 };

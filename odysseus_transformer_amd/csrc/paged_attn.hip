@@ -105,11 +105,12 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
   __shared__ float sm[WAVES][16 * NT], sl[WAVES][16 * NT];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q = lane >> 4;
   PagedWalk<STEP> walk(p, cache, lane);
-  const PagedCuts cuts(walk.total() * p.Hkv, gridDim.x);
-  const int block = blockIdx.x;
+  const int each = walk.total();   // steps of a kv head
+  const PagedCuts cuts(each * p.Hkv, gridDim.x);
+  const int block = paged_range(blockIdx.x, cuts.blocks);
   if (block >= cuts.blocks) return;
   const int begin = cuts.at(block), end = cuts.at(block + 1);
-  int pos = begin, hk, step, steps, entry = walk.find(pos, hk, step, steps);
+  int pos = begin, hk, step, steps, entry = walk.find(pos, each, hk, step, steps);
 
   while (pos < end) {
     const int s = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * p.tile;
@@ -274,7 +275,10 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
 
     pos += steps_here;
     step = 0;
-    if (++hk == p.Hkv && pos < end) hk = 0, steps = paged_steps<STEP>(p, cache, ++entry);
+    if (pos < end) {
+      if (++entry == walk.entries) entry = 0, hk++;
+      steps = paged_steps<STEP>(p, cache, entry);
+    }
   }
 }
 
@@ -300,7 +304,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     }
   } while (walk.next());
   const PagedCuts cuts((walk.before + walk.all()) * p.Hkv, most_blocks);
-  const int first = before * p.Hkv + hk * steps, b0 = cuts.block_of(first), b1 = cuts.block_of(first + steps - 1), parts = b1 - b0 + 1;
+  const int first = hk * (walk.before + walk.all()) + before, b0 = cuts.block_of(first), b1 = cuts.block_of(first + steps - 1), parts = b1 - b0 + 1;
   if (parts == 1) return;
   // part k is in slot 2 (b0 + k), but for the first where that block's range begins with another unit
   const int first_slot = 2 * b0 + (first > cuts.at(b0));
@@ -384,7 +388,7 @@ Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype)
   const int step = chunk ? PAGED_CHUNK_KEYS : WAVES * (dtype == ODY_BF16 ? 32 : 16);
   const int64_t steps = std::max((int64_t)1, (most_keys + step - 1) / step);   // of a unit, at most
   const double all = (double)S * row_tiles * Hkv * steps;
-  const int blocks = (int)std::min((double)BLOCKS, all);
+  const int blocks = (int)std::min((double)BLOCKS, std::ceil(all / 8) * 8);   // a multiple of 8: paged_range
   const bool joined = steps > 1;
   const size_t parts = joined ? (size_t)blocks * 2 * tile : 0;
   return Plan{tile, row_tiles, step, blocks, joined, all < 2147483648.0, parts * D * sizeof(float), parts * sizeof(float2)};
@@ -429,8 +433,8 @@ extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_
                               int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
                               int64_t so_s, int64_t so_n, int64_t so_h, int pages, int page_size, int table_width, int64_t table_stride,
                               float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  const PagedCache c{const_cast<void*>(k_pages), const_cast<void*>(v_pages), page_table, lengths, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h},
-                     table_stride, pages, paged_shift(page_size), table_width};
+  const PagedCache c(const_cast<void*>(k_pages), const_cast<void*>(v_pages), page_table, lengths, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride,
+                     pages, page_size, table_width, dtype);
   if (int rc = paged_check("ody_paged_attn", S, n, Hq, Hkv, D, dtype, c, page_size)) return rc;
   ODY_REQUIRE(q && out && lse, ODY_ERR_NULL, "ody_paged_attn: q, out or lse is NULL");
   ODY_REQUIRE(paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype) && paged_rows_aligned(out, so_s, so_n, so_h, dtype), ODY_ERR_MISALIGNED,
