@@ -43,6 +43,11 @@ struct PagedAttnParams {
 
 // The kernel of many rows (paged_attn_chunk.hip): rows of a tile, keys of a step
 constexpr int PAGED_CHUNK_ROWS = 128, PAGED_CHUNK_KEYS = 64;
+
+// Blocks for so many steps.  A range that ends inside a unit writes 128 rows in fp32 (as many bytes as two steps read) and starts with a latency of five: two
+// blocks a compute unit where they have 16 steps each, else at most one, of 8 at least.  Us with 4 / 8 / 16 steps at least, 32 heads on 8 behind 8192 keys:
+// 32 tokens 31.5 / 26.8 / 34.5 (and 36 with one), 128 tokens 50 / 55 / 46, 512 tokens 100.5 / 98.6 / 99.5.
+__device__ __forceinline__ int paged_chunk_blocks(int steps, int most) { return steps >= 16 * most ? most : steps < 16 ? 1 : steps / 8 < most / 2 ? steps / 8 : most / 2; }
 int ody_launch_paged_chunk(const PagedAttnParams& p, int D, const PagedCache& c, int blocks, hipStream_t st);
 
 #ifdef __HIPCC__
@@ -59,12 +64,6 @@ __device__ __forceinline__ int paged_keys(const PagedAttnParams& p, const PagedC
   const int last = p.row_tiles == 1 ? p.n - 1 : last_row / p.group;
   return max(0, min(c.width << c.shift, length - p.n + last + 1));
 }
-template <int STEP>
-__device__ __forceinline__ int paged_steps(const PagedAttnParams& p, const PagedCache& c, int e) {
-  const int s = p.row_tiles == 1 ? e : e / p.row_tiles, keys = paged_keys(p, c, paged_length(c, s), e - s * p.row_tiles);
-  return max(1, (keys - 1) / STEP + 1);
-}
-
 // Inclusive sums over the lanes of a wavefront, within rows of 16 lanes and then from row to row.
 __device__ __forceinline__ int paged_wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1, 2, 4, 8
@@ -83,28 +82,37 @@ __device__ __forceinline__ int paged_range(int block, int blocks) {
   return block >> 3 < each ? range : blocks;
 }
 
-// Where the cuts are: `total` steps (below 2^31, which the host checks) over as many of the blocks as have one.
+// Where the cuts are: `total` steps (below 2^31, which the host checks) over as many of the blocks as there are steps for; the ranges that are a step longer lie evenly
+// among the others.
 struct PagedCuts {
-  int total, blocks, base, more;   // the first `more` blocks have base + 1 steps, the others base
+  int total, blocks, base, more;
   __device__ __forceinline__ PagedCuts(int steps, int most_blocks) : total(steps), blocks(min(most_blocks, steps)) {
     base = (unsigned)total / (unsigned)blocks, more = total - base * blocks;
   }
-  __device__ __forceinline__ int at(int block) const { return block * base + min(block, more); }
-  __device__ __forceinline__ int block_of(int step) const {
-    const int heavy = more * (base + 1);
-    return step < heavy ? (int)((unsigned)step / (unsigned)(base + 1)) : more + (int)((unsigned)(step - heavy) / (unsigned)base);
+  __device__ __forceinline__ int at(int range) const { return range * base + (int)((unsigned)(range * more) / (unsigned)blocks); }
+  __device__ __forceinline__ int range_of(int step) const {
+    int r = min(blocks - 1, (int)((float)step * (float)blocks / (float)total));   // at most one off
+    if (at(r) > step) r--;
+    if (at(r + 1) <= step) r++;
+    return r;
   }
 };
 
-// One walk over the (sequence, row tile) pairs by a wavefront: a chunk of 64 of them, their steps and the sums so far.
+// A walk over the (sequence, row tile) pairs by a wavefront, a chunk of 64 of them at a time: a lane has the length of its pair's sequence, the pair's
+// steps and the sum of steps so far.
 template <int STEP>
 struct PagedWalk {
   const PagedAttnParams& p;
   const PagedCache& c;
-  int lane, entries, at = 0, before = 0, mine = 0, sums = 0;   // sums: inclusive, of this chunk
+  int lane, entries, at = 0, before = 0, length = 0, mine = 0, sums = 0;   // sums: inclusive, of this chunk
   __device__ __forceinline__ PagedWalk(const PagedAttnParams& p_, const PagedCache& c_, int lane_) : p(p_), c(c_), lane(lane_), entries(p_.S * p_.row_tiles) { chunk(); }
   __device__ __forceinline__ void chunk() {
-    mine = at + lane < entries ? paged_steps<STEP>(p, c, at + lane) : 0;
+    mine = 0;
+    if (at + lane < entries) {
+      const int e = at + lane, s = p.row_tiles == 1 ? e : e / p.row_tiles;
+      length = paged_length(c, s);
+      mine = max(1, (paged_keys(p, c, length, e - s * p.row_tiles) - 1) / STEP + 1);
+    }
     sums = paged_wave_scan(mine);
   }
   __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(sums, 63); }
@@ -118,19 +126,44 @@ struct PagedWalk {
     while (next()) {}
     return before + all();
   }
-  // The pair that step `pos` of all kv heads is one of, `total` of each; its steps, and which kv head's and which of them it is.
-  __device__ __forceinline__ int find(int pos, int total, int& hk, int& step, int& steps) {
-    hk = (int)((unsigned)pos / (unsigned)total);
-    pos -= hk * total;
-    if (at != 0) {
-      at = before = 0;
-      chunk();
+  __device__ __forceinline__ void rewind() {
+    if (at == 0) return;
+    at = before = 0;
+    chunk();
+  }
+};
+
+// A place in the order of all steps: kv head, pair (sequence, row tile), step of it.
+template <int STEP>
+struct PagedPlace {
+  int hk, entry, s, rt, length, steps, step;
+  // that of step `pos`, `each` of every kv head
+  __device__ __forceinline__ PagedPlace(PagedWalk<STEP>& w, int pos, int each) {
+    hk = (int)((unsigned)pos / (unsigned)each);
+    pos -= hk * each;
+    w.rewind();
+    while (w.before + w.all() <= pos && w.next()) {}
+    entry = w.at + __popcll(__ballot(w.before + w.sums <= pos));
+    take(w);
+    step = pos - (w.before + __builtin_amdgcn_readlane(w.sums, entry - w.at) - steps);
+  }
+  // the first step of the next unit
+  __device__ __forceinline__ void next_unit(PagedWalk<STEP>& w) {
+    if (++entry == w.entries) {
+      entry = 0, hk++;
+      w.rewind();
+    } else if (entry == w.at + 64) {
+      w.next();
     }
-    while (before + all() <= pos && next()) {}
-    const int k = __popcll(__ballot(before + sums <= pos));
-    steps = __builtin_amdgcn_readlane(mine, k);
-    step = pos - (before + __builtin_amdgcn_readlane(sums, k) - steps);
-    return at + k;
+    take(w);
+    step = 0;
+  }
+
+ private:
+  __device__ __forceinline__ void take(const PagedWalk<STEP>& w) {
+    const int k = entry - w.at;
+    steps = __builtin_amdgcn_readlane(w.mine, k), length = __builtin_amdgcn_readlane(w.length, k);
+    s = w.p.row_tiles == 1 ? entry : entry / w.p.row_tiles, rt = entry - s * w.p.row_tiles;
   }
 };
 #endif

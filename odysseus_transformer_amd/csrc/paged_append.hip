@@ -16,76 +16,88 @@ struct AppendParams {
 
 template <typename T> __device__ __forceinline__ float rounded(float x) { return (float)(T)x; }
 
-// A block takes TOKENS tokens: their angles go to LDS, then consecutive threads take consecutive vectors of a head, x[j] together
-// with x[j + D / 2].  A token before place 0 is none: its queries become 0, nothing else is written.
-template <typename T, int D, int TOKENS, bool ROTATE>
+// A block takes a token: consecutive threads take consecutive vectors of a head, x[j] together with x[j + D / 2].  Bound by memory, or for few tokens by
+// latencies: a thread's first vectors are under way while the block evaluates the token's angles, which go to LDS (64 tokens of 48 heads 3.8 -> 3.2 us,
+// launch included).  Results leave without taking cache room (3001 tokens of 48 heads 15.5 -> 12.7 us), and operands that the last-level cache cannot hold
+// beside them are read past it (STREAM; 4 x 4096 tokens of 96 heads 141 -> 135 us, 5.0 TB/s; 3001 of 48 12.7 -> 14.3).  A token before place 0 is none: its
+// queries become 0, nothing else is written.
+template <typename T, int D, bool ROTATE, bool STREAM>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p, const PagedCache cache) {
   constexpr int N = Vec16B<T>::N, HALF = D / 2, VECS = HALF / N;
   typedef typename Vec16B<T>::type vec;
-  __shared__ __attribute__((aligned(16))) float cs[TOKENS][HALF], sn[TOKENS][HALF];
-  const int64_t first = (int64_t)blockIdx.x * TOKENS, all = (int64_t)p.S * p.n;
-  const int mine = (int)min((int64_t)TOKENS, all - first);
+  typedef unsigned raw __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) float cs[HALF], sn[HALF];
+  const int token = blockIdx.x, s = token / p.n, i = token - s * p.n, tid = threadIdx.x;
+  const int h0 = ROTATE ? 0 : p.Hq, items = (p.Hq + 2 * p.Hkv - h0) * VECS;   // pairs of vectors
+  const T* x = static_cast<const T*>(p.x) + s * p.sx.b + i * p.sx.l + h0 * p.sx.h;
+  auto load = [&](int v, vec& a, vec& b) {
+    const T* src = x + v / VECS * p.sx.h + v % VECS * N;
+    if (STREAM) {
+      a = __builtin_bit_cast(vec, __builtin_nontemporal_load(reinterpret_cast<const raw*>(src)));
+      b = __builtin_bit_cast(vec, __builtin_nontemporal_load(reinterpret_cast<const raw*>(src + HALF)));
+    } else {
+      a = *reinterpret_cast<const vec*>(src);
+      b = *reinterpret_cast<const vec*>(src + HALF);
+    }
+  };
+  vec a, b;
+  if (tid < items) load(tid, a, b);
+  const int place = max(cache.lengths[s], 0) - p.n + i;
+  // where the token's keys and values go
+  int page = -1;
+  if (place >= 0 && place >> cache.shift < cache.width) page = cache.table[s * cache.table_stride + (place >> cache.shift)];
+  const bool paged = (unsigned)page < (unsigned)cache.pages;
+  const int row = place & ((1 << cache.shift) - 1);
   if (ROTATE) {
-    for (int e = threadIdx.x; e < mine * HALF; e += 256) {
-      const int t = e / HALF, j = e % HALF, s = (int)((first + t) / p.n), i = (int)((first + t) % p.n);
-      const float pos = p.pos ? (float)p.pos[first + t] : (float)(max(cache.lengths[s], 0) - p.n + i);
-      const float th = pos * p.inv_freq[j];
-      cs[t][j] = rounded<T>(cosf(th));   // rounded to the values' type before use, as ody_rope has them
-      sn[t][j] = rounded<T>(sinf(th));
+    if (tid < HALF) {
+      const float pos = p.pos ? (float)p.pos[token] : (float)place, th = pos * p.inv_freq[tid];
+      cs[tid] = rounded<T>(cosf(th));   // rounded to the values' type before use, as ody_rope has them
+      sn[tid] = rounded<T>(sinf(th));
     }
     __syncthreads();
   }
-  const int h0 = ROTATE ? 0 : p.Hq, heads = p.Hq + 2 * p.Hkv - h0;
-  for (int v = threadIdx.x; v < mine * heads * VECS; v += 256) {
-    const int j = v % VECS * N, h = h0 + v / VECS % heads, t = v / (VECS * heads);
-    const int s = (int)((first + t) / p.n), i = (int)((first + t) % p.n);
-    const int place = max(cache.lengths[s], 0) - p.n + i;
-    const T* src = static_cast<const T*>(p.x) + s * p.sx.b + i * p.sx.l + h * p.sx.h + j;
+  for (int v = tid; v < items; v += 256) {
+    const int j = v % VECS * N, h = h0 + v / VECS;
+    if (v != tid) load(v, a, b);
     T* dst;
     if (h < p.Hq) {
       dst = static_cast<T*>(p.q) + s * p.sq.b + i * p.sq.l + h * p.sq.h + j;
-      if (place < 0) {
-        const vec zero = {};
-        *reinterpret_cast<vec*>(dst) = zero;
-        *reinterpret_cast<vec*>(dst + HALF) = zero;
-        continue;
-      }
+      if (place < 0) a = b = vec{};
     } else {
-      if (place < 0 || place >> cache.shift >= cache.width) continue;
-      const int page = cache.table[s * cache.table_stride + (place >> cache.shift)], row = place & ((1 << cache.shift) - 1);
-      if (page < 0 || page >= cache.pages) continue;
+      if (!paged) continue;
       const bool key = h < p.Hq + p.Hkv;
-      const int hk = h - p.Hq - (key ? 0 : p.Hkv);
       const PageStrides& st = key ? cache.sk : cache.sv;
-      dst = static_cast<T*>(key ? cache.k : cache.v) + page * st.p + row * st.r + hk * st.h + j;
+      dst = static_cast<T*>(key ? cache.k : cache.v) + page * st.p + row * st.r + (h - p.Hq - (key ? 0 : p.Hkv)) * st.h + j;
     }
-    vec a = *reinterpret_cast<const vec*>(src), b = *reinterpret_cast<const vec*>(src + HALF);
     if (ROTATE && h < p.Hq + p.Hkv) {
       vec a1, b1;
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        const float c = cs[t][j + e], sine = sn[t][j + e], x1 = (float)a[e], x2 = (float)b[e];
+        const float c = cs[j + e], sine = sn[j + e], x1 = (float)a[e], x2 = (float)b[e];
         a1[e] = (T)(x1 * c - x2 * sine);
         b1[e] = (T)(x2 * c + x1 * sine);
       }
       a = a1, b = b1;
     }
-    *reinterpret_cast<vec*>(dst) = a;
-    *reinterpret_cast<vec*>(dst + HALF) = b;
+    __builtin_nontemporal_store(__builtin_bit_cast(raw, a), reinterpret_cast<raw*>(dst));
+    __builtin_nontemporal_store(__builtin_bit_cast(raw, b), reinterpret_cast<raw*>(dst + HALF));
   }
 }
 
-template <typename T, int D, int TOKENS>
+template <typename T, int D>
 int launch(const AppendParams& p, const PagedCache& cache, hipStream_t st) {
-  const int64_t all = (int64_t)p.S * p.n;
-  const dim3 grid((unsigned)((all + TOKENS - 1) / TOKENS));
-  if (p.q) ODY_LAUNCH("paged_append", st, (paged_append_kernel<T, D, TOKENS, true>), grid, dim3(256), 0, p, cache);
-  else ODY_LAUNCH("paged_append", st, (paged_append_kernel<T, D, TOKENS, false>), grid, dim3(256), 0, p, cache);
+  const dim3 grid((unsigned)(p.S * p.n));
+  const bool stream = (double)2 * p.S * p.n * (p.Hq + 2 * p.Hkv) * D * sizeof(T) > (double)((size_t)192 << 20);
+#define LAUNCH(R, ST) ODY_LAUNCH("paged_append", st, (paged_append_kernel<T, D, R, ST>), grid, dim3(256), 0, p, cache)
+  if (p.q) {
+    if (stream) LAUNCH(true, true);
+    else LAUNCH(true, false);
+  } else {
+    if (stream) LAUNCH(false, true);
+    else LAUNCH(false, false);
+  }
+#undef LAUNCH
   return ody_check_launch("paged_append");
-}
-template <typename T>
-int by_head_dim(const AppendParams& p, int D, const PagedCache& cache, hipStream_t st) {
-  return D == 64 ? launch<T, 64, 1>(p, cache, st) : launch<T, 128, 1>(p, cache, st);
 }
 
 }  // namespace
@@ -130,5 +142,6 @@ extern "C" int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v
               "ody_paged_append: qkv and q need 16-byte aligned pointers and strides");
   const AppendParams p{qkv, q, position_ids, inv_freq, {sx_s, sx_n, sx_h}, {sq_s, sq_n, sq_h}, S, n, Hq, Hkv};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == ODY_BF16 ? by_head_dim<bf16>(p, D, c, st) : by_head_dim<float>(p, D, c, st);
+  if (dtype == ODY_BF16) return D == 64 ? launch<bf16, 64>(p, c, st) : launch<bf16, 128>(p, c, st);
+  return D == 64 ? launch<float, 64>(p, c, st) : launch<float, 128>(p, c, st);
 }

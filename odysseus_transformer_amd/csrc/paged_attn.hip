@@ -10,7 +10,8 @@
 // row c of a K operand stands for is chosen so that a lane's scores are those of GK keys in a row, tile + GK q ..: its P is then the B operand for the very
 // keys whose V rows this lane loads.  V rows are loaded GK at a time with 16 lanes on a row; component i of the vectors is row c of operand i, which
 // stands for column c * DV + i of V, so the transposition is bytes exchanged within a lane (bf16) or nothing at all (fp32).
-// Loads run one tile ahead of the products, the page numbers two.  A group of GK keys lies within a page: two table entries a lane and tile.
+// With 16 rows of 128 columns a wavefront has two tiles in registers, one under way while the products read the other; with more rows, or half the columns,
+// a tile's K goes out when the products have read that of the one before, and so does its V.  A group of GK keys lies within a page: two table entries a lane and tile.
 #include <algorithm>
 #include <cmath>
 #include "paged.h"
@@ -25,50 +26,43 @@ template <int D> struct Tile<bf16, D> {
   typedef bf16x8 kvec;
   typedef bf16 vvec __attribute__((ext_vector_type(DV)));
   // K vector j of a lane: operand row c stands for key 8 (c / 4) + 4 (j / (D / 32)) + c % 4
-  __device__ static int key_row(int c, int j) { return 4 * (j / (D / 32)) + (c & 3); }
-  __device__ static int key_col(int q, int j) { return 32 * (j % (D / 32)) + 8 * q; }
+  __device__ static constexpr int key_row(int j) { return 4 * (j / (D / 32)); }
+  __device__ static constexpr int key_col(int q, int j) { return 32 * (j % (D / 32)) + 8 * q; }
 };
 template <int D> struct Tile<float, D> {
   static constexpr int KEYS = 16, GK = 4, KV = D / 16, DV = D / 16;
   typedef f32x4 kvec;
   typedef float vvec __attribute__((ext_vector_type(DV)));
-  __device__ static int key_row(int c, int) { return c & 3; }
-  __device__ static int key_col(int q, int j) { return 16 * j + 4 * q; }
-};
-
-template <typename T, int D>
-struct Loaded {   // one tile of keys
-  typename Tile<T, D>::kvec k[Tile<T, D>::KV];
-  typename Tile<T, D>::vvec v[Tile<T, D>::GK];
-  bool page;      // the lane's keys, tile + GK q .., have one
+  __device__ static constexpr int key_row(int) { return 0; }
+  __device__ static constexpr int key_col(int q, int j) { return 16 * j + 4 * q; }
 };
 
 // scores of the lane's GK keys against column c's query row
 template <int D>
-__device__ __forceinline__ void scores(const Loaded<bf16, D>& t, const bf16x8 (&qf)[D / 32], float (&x)[8]) {
+__device__ __forceinline__ void scores(const bf16x8 (&k)[D / 16], const bf16x8 (&qf)[D / 32], float (&x)[8]) {
 #pragma unroll
   for (int st = 0; st < 2; st++) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < D / 32; ks++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t.k[st * (D / 32) + ks], qf[ks], s, 0, 0, 0);
+    for (int ks = 0; ks < D / 32; ks++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st * (D / 32) + ks], qf[ks], s, 0, 0, 0);
 #pragma unroll
     for (int r = 0; r < 4; r++) x[4 * st + r] = s[r];
   }
 }
 template <int D>
-__device__ __forceinline__ void scores(const Loaded<float, D>& t, const f32x4 (&qf)[D / 16], float (&x)[4]) {
+__device__ __forceinline__ void scores(const f32x4 (&k)[D / 16], const f32x4 (&qf)[D / 16], float (&x)[4]) {
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < D / 16; j++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[j][e], qf[j][e], s, 0, 0, 0);
+    for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][e], qf[j][e], s, 0, 0, 0);
 #pragma unroll
   for (int r = 0; r < 4; r++) x[r] = s[r];
 }
 
 // o[i], row c: column c * DV + i of the result
 template <int D, int NT>
-__device__ __forceinline__ void values(const Loaded<bf16, D>& t, const float (&w)[NT][8], f32x4 (&o)[NT][D / 16]) {
+__device__ __forceinline__ void values(const typename Tile<bf16, D>::vvec (&rows)[8], const float (&w)[NT][8], f32x4 (&o)[NT][D / 16]) {
   bf16x8 pb[NT];
 #pragma unroll
   for (int m = 0; m < NT; m++)
@@ -76,7 +70,7 @@ __device__ __forceinline__ void values(const Loaded<bf16, D>& t, const float (&w
     for (int e = 0; e < 8; e++) pb[m][e] = (bf16)w[m][e];
   unsigned v[8][D / 32];
 #pragma unroll
-  for (int j = 0; j < 8; j++) __builtin_memcpy(v[j], &t.v[j], sizeof(v[j]));
+  for (int j = 0; j < 8; j++) __builtin_memcpy(v[j], &rows[j], sizeof(v[j]));
 #pragma unroll
   for (int i = 0; i < D / 16; i++) {
     i32x4 a;
@@ -88,19 +82,20 @@ __device__ __forceinline__ void values(const Loaded<bf16, D>& t, const float (&w
   }
 }
 template <int D, int NT>
-__device__ __forceinline__ void values(const Loaded<float, D>& t, const float (&w)[NT][4], f32x4 (&o)[NT][D / 16]) {
+__device__ __forceinline__ void values(const typename Tile<float, D>::vvec (&rows)[4], const float (&w)[NT][4], f32x4 (&o)[NT][D / 16]) {
 #pragma unroll
   for (int r = 0; r < 4; r++)
 #pragma unroll
     for (int i = 0; i < D / 16; i++)
 #pragma unroll
-      for (int m = 0; m < NT; m++) o[m][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.v[r][i], w[m][r], o[m][i], 0, 0, 0);
+      for (int m = 0; m < NT; m++) o[m][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows[r][i], w[m][r], o[m][i], 0, 0, 0);
 }
 
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel(const PagedAttnParams p, const PagedCache cache) {
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAttnParams p, const PagedCache cache) {
   typedef Tile<T, D> G;
   constexpr int STEP = WAVES * G::KEYS, GK = G::GK, OP = D + 4;
+  constexpr bool TWO = NT == 1 && D == 128;   // tiles in registers
   __shared__ __attribute__((aligned(16))) float Os[WAVES][16][OP];
   __shared__ float sm[WAVES][16 * NT], sl[WAVES][16 * NT];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q = lane >> 4;
@@ -110,14 +105,16 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
   const int block = paged_range(blockIdx.x, cuts.blocks);
   if (block >= cuts.blocks) return;
   const int begin = cuts.at(block), end = cuts.at(block + 1);
-  int pos = begin, hk, step, steps, entry = walk.find(pos, each, hk, step, steps);
+  int pos = begin;
+  const unsigned of_lane_k = (c & 3) * cache.k_row + G::key_col(q, 0) * sizeof(T), of_lane_v = c * G::DV * sizeof(T);
+  PagedPlace<STEP> at(walk, pos, each);
 
   while (pos < end) {
-    const int s = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * p.tile;
-    const int rows = min(p.tile, p.n * p.group - row0), length = paged_length(cache, s);
+    const int s = at.s, rt = at.rt, hk = at.hk, length = at.length, step = at.step, steps = at.steps, row0 = rt * p.tile;
+    const int rows = min(p.tile, p.n * p.group - row0);
     const int keys = paged_keys(p, cache, length, rt), steps_here = min(steps - step, end - pos);
-    const T* kp = static_cast<const T*>(cache.k) + hk * cache.sk.h;
-    const T* vp = static_cast<const T*>(cache.v) + hk * cache.sv.h;
+    const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(cache.k) + hk * cache.sk.h) + of_lane_k;
+    const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(cache.v) + hk * cache.sv.h) + of_lane_v;
     const int* table = cache.table + s * cache.table_stride;
     const int in_page = (1 << cache.shift) - 1, last_group = max(keys - 1, 0) & -GK;
 
@@ -152,30 +149,41 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
       const int base = key0 + min(t, tiles - 1) * STEP;
       return Pages{table[min(base + GK * (c >> 2), last_group) >> cache.shift], table[min(base + GK * q, last_group) >> cache.shift]};
     };
-    auto load = [&](Loaded<T, D>& t, int at, const Pages& pg) {
-      const int base = key0 + at * STEP, gk = min(base + GK * (c >> 2), last_group), gv = min(base + GK * q, last_group);
-      t.page = (unsigned)pg.v < (unsigned)cache.pages;
-      const T* kr = kp + ((unsigned)pg.k < (unsigned)cache.pages ? pg.k : 0) * cache.sk.p + (gk & in_page) * cache.sk.r;
-      const T* vr = vp + (t.page ? pg.v : 0) * cache.sv.p + (gv & in_page) * cache.sv.r + c * G::DV;
-#pragma unroll
-      for (int j = 0; j < G::KV; j++) t.k[j] = *reinterpret_cast<const typename G::kvec*>(kr + G::key_row(c, j) * cache.sk.r + G::key_col(q, j));
-#pragma unroll
-      for (int j = 0; j < GK; j++) t.v[j] = *reinterpret_cast<const typename G::vvec*>(vr + j * cache.sv.r);
+    struct Loaded {   // a tile's rows
+      typename G::kvec k[G::KV];
+      typename G::vvec v[GK];
+      bool page;      // the lane's keys, tile + GK q .., have one
     };
-    auto compute = [&](Loaded<T, D>& t, int at) {
-      const int base = key0 + at * STEP, first = base + GK * q;   // the lane's keys
+    auto load_k = [&](Loaded& to, int t, const Pages& pg) __attribute__((always_inline)) {
+      const int gk = min(key0 + t * STEP + GK * (c >> 2), last_group);
+      const char* src = kp + (uint64_t)((unsigned)pg.k < (unsigned)cache.pages ? pg.k : 0) * cache.k_page + (unsigned)(gk & in_page) * cache.k_row;
+#pragma unroll
+      for (int j = 0; j < G::KV; j++)
+        to.k[j] = *reinterpret_cast<const typename G::kvec*>(src + G::key_row(j) * (uint64_t)cache.k_row + G::key_col(0, j) * sizeof(T));
+    };
+    auto load_v = [&](Loaded& to, int t, const Pages& pg) __attribute__((always_inline)) {
+      const int gv = min(key0 + t * STEP + GK * q, last_group);
+      to.page = (unsigned)pg.v < (unsigned)cache.pages;
+      const char* src = vp + (uint64_t)(to.page ? pg.v : 0) * cache.v_page + (unsigned)(gv & in_page) * cache.v_row;
+#pragma unroll
+      for (int j = 0; j < GK; j++) to.v[j] = *reinterpret_cast<const typename G::vvec*>(src + j * (uint64_t)cache.v_row);
+    };
+    // the products with tile t; `k_read` is called when those with its K have been formed
+    auto compute = [&](Loaded& x, int t, auto k_read) __attribute__((always_inline)) {
+      const int base = key0 + t * STEP, first = base + GK * q;   // the lane's keys
       float w[NT][GK];
 #pragma unroll
-      for (int m = 0; m < NT; m++) scores<D>(t, qf[m], w[m]);
+      for (int m = 0; m < NT; m++) scores<D>(x.k, qf[m], w[m]);
+      k_read();
       // keys that a row does not see, that no token has, that have no page: neither their scores nor their values count, whatever lies there
-      if (base + G::KEYS - 1 > safe || !__all(t.page)) {
-        const int most = t.page ? keys - 1 : -1;
+      if (base + G::KEYS - 1 > safe || !__all(x.page)) {
+        const int most = x.page ? keys - 1 : -1;
 #pragma unroll
         for (int e = 0; e < GK; e++) {
 #pragma unroll
           for (int m = 0; m < NT; m++)
             if (first + e > min(lim[m], most)) w[m][e] = -INFINITY;
-          if (first + e > most) t.v[e] = typename G::vvec{};
+          if (first + e > most) x.v[e] = typename G::vvec{};
         }
       }
 #pragma unroll
@@ -194,30 +202,40 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
 #pragma unroll
         for (int i = 0; i < D / 16; i++) o[m][i] *= alpha;
       }
-      values<D, NT>(t, w, o);
+      values<D, NT>(x.v, w, o);
     };
-    if (NT == 4) {   // two tiles do not fit the registers beside 64 rows
-      Loaded<T, D> a;
-      for (int t = 0; t < tiles; t++) {
-        load(a, t, lookup(t));
-        compute(a, t);
-      }
-    } else if (tiles > 0) {
-      Loaded<T, D> a, b;
-      load(a, 0, lookup(0));
-      Pages next = lookup(1);
-      for (int t = 0; t < tiles; t += 2) {
-        if (t + 1 < tiles) {
-          load(b, t + 1, next);
-          next = lookup(t + 2);
+    if (tiles > 0) {
+      Pages now = lookup(0), next = lookup(1);
+      Loaded x;
+      load_k(x, 0, now);
+      load_v(x, 0, now);
+      if constexpr (TWO) {
+        Loaded y;
+        auto nothing = [] {};
+        for (int t = 0; t < tiles; t += 2) {
+          if (t + 1 < tiles) {
+            load_k(y, t + 1, next);
+            load_v(y, t + 1, next);
+            next = lookup(t + 2);
+          }
+          compute(x, t, nothing);
+          if (t + 1 >= tiles) break;
+          if (t + 2 < tiles) {
+            load_k(x, t + 2, next);
+            load_v(x, t + 2, next);
+            next = lookup(t + 3);
+          }
+          compute(y, t + 1, nothing);
         }
-        compute(a, t);
-        if (t + 1 >= tiles) break;
-        if (t + 2 < tiles) {
-          load(a, t + 2, next);
-          next = lookup(t + 3);
+      } else {
+        now = next, next = lookup(2);
+        for (int t = 0; t < tiles; t++) {
+          compute(x, t, [&]() __attribute__((always_inline)) { if (t + 1 < tiles) load_k(x, t + 1, now); });
+          if (t + 1 < tiles) {
+            load_v(x, t + 1, now);
+            now = next, next = lookup(t + 3);
+          }
         }
-        compute(b, t + 1);
       }
     }
 
@@ -274,11 +292,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 2 : 1) void paged_attn_kernel
     }
 
     pos += steps_here;
-    step = 0;
-    if (pos < end) {
-      if (++entry == walk.entries) entry = 0, hk++;
-      steps = paged_steps<STEP>(p, cache, entry);
-    }
+    if (pos < end) at.next_unit(walk);
   }
 }
 
@@ -303,8 +317,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
       before = walk.before + __builtin_amdgcn_readlane(walk.sums, entry - walk.at) - steps;
     }
   } while (walk.next());
-  const PagedCuts cuts((walk.before + walk.all()) * p.Hkv, most_blocks);
-  const int first = hk * (walk.before + walk.all()) + before, b0 = cuts.block_of(first), b1 = cuts.block_of(first + steps - 1), parts = b1 - b0 + 1;
+  const int all_steps = (walk.before + walk.all()) * p.Hkv;
+  const PagedCuts cuts(all_steps, p.tile == PAGED_CHUNK_ROWS ? paged_chunk_blocks(all_steps, most_blocks) : most_blocks);
+  const int first = hk * (walk.before + walk.all()) + before, b0 = cuts.range_of(first), b1 = cuts.range_of(first + steps - 1), parts = b1 - b0 + 1;
   if (parts == 1) return;
   // part k is in slot 2 (b0 + k), but for the first where that block's range begins with another unit
   const int first_slot = 2 * b0 + (first > cuts.at(b0));
@@ -374,7 +389,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   }
 }
 
-// Row tiles of 16, 32 or 64 here, the rest in bf16 by the kernel of many rows.
+// Row tiles of 16 or 32 here, more rows in bf16 by the kernel of many rows.
 struct Plan {
   int tile, row_tiles, step, blocks;
   bool joined;          // a cut may go through a unit
@@ -384,7 +399,7 @@ struct Plan {
 Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype) {
   const int64_t rows = (int64_t)n * group;
   const bool chunk = rows > 64 && dtype == ODY_BF16;
-  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : chunk ? PAGED_CHUNK_ROWS : 64, row_tiles = (int)((rows + tile - 1) / tile);
+  const int tile = rows <= 16 ? 16 : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);
   const int step = chunk ? PAGED_CHUNK_KEYS : WAVES * (dtype == ODY_BF16 ? 32 : 16);
   const int64_t steps = std::max((int64_t)1, (most_keys + step - 1) / step);   // of a unit, at most
   const double all = (double)S * row_tiles * Hkv * steps;
@@ -405,7 +420,7 @@ template <typename T, int D, int NT>
 int launch(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
   ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
   const int rc = ody_check_launch("paged_attn");
-  return rc ? rc : join<T, D, WAVES * Tile<T, D>::KEYS, NT == 4 ? JOIN_ROWS : 1>(p, c, pl, st);
+  return rc ? rc : join<T, D, WAVES * Tile<T, D>::KEYS, 1>(p, c, pl, st);
 }
 template <typename T, int D>
 int by_rows(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
@@ -413,7 +428,7 @@ int by_rows(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipSt
     const int rc = ody_launch_paged_chunk(p, D, c, pl.blocks, st);
     return rc ? rc : join<bf16, D, PAGED_CHUNK_KEYS, JOIN_ROWS>(p, c, pl, st);
   }
-  return pl.tile == 16 ? launch<T, D, 1>(p, c, pl, st) : pl.tile == 32 ? launch<T, D, 2>(p, c, pl, st) : launch<T, D, 4>(p, c, pl, st);
+  return pl.tile == 16 ? launch<T, D, 1>(p, c, pl, st) : launch<T, D, 2>(p, c, pl, st);
 }
 template <typename T>
 int by_head_dim(const PagedAttnParams& p, int D, const PagedCache& c, const Plan& pl, hipStream_t st) {

@@ -60,11 +60,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 5, i = lane & 31;
   PagedWalk<KEYS> walk(p, cache, lane);
   const int each = walk.total();   // steps of a kv head
-  const PagedCuts cuts(each * p.Hkv, gridDim.x);
+  const PagedCuts cuts(each * p.Hkv, paged_chunk_blocks(each * p.Hkv, gridDim.x));
   const int block = paged_range(blockIdx.x, cuts.blocks);
   if (block >= cuts.blocks) return;
   const int begin = cuts.at(block), end = cuts.at(block + 1);
-  int pos = begin, hk, step, steps, entry = walk.find(pos, each, hk, step, steps);
+  int pos = begin;
+  PagedPlace<KEYS> at(walk, pos, each);
   const int lcol = 8 * ((lane % LANES) ^ swz<D>(PER * wave + lane / LANES));   // of this lane in its direct loads
   const unsigned lk = lane / LANES * cache.k_row + 2 * lcol, lv = lane / LANES * cache.v_row + 2 * lcol;   // bytes
   const float c2 = p.scale_log2e;
@@ -72,8 +73,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
   rd.init(reinterpret_cast<const bf16*>(smem), g, i);
 
   while (pos < end) {
-    const int s = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - s * p.row_tiles, row0 = rt * BLOCK_ROWS;
-    const int rows = min(BLOCK_ROWS, p.n * p.group - row0), length = paged_length(cache, s);
+    const int s = at.s, rt = at.rt, hk = at.hk, length = at.length, step = at.step, steps = at.steps, row0 = rt * BLOCK_ROWS;
+    const int rows = min(BLOCK_ROWS, p.n * p.group - row0);
     const int keys = paged_keys(p, cache, length, rt), steps_here = min(steps - step, end - pos), tiles = keys > 0 ? steps_here : 0;
     const int key0 = KEYS * step;
     const char* kp = reinterpret_cast<const char*>(static_cast<const bf16*>(cache.k) + hk * cache.sk.h);
@@ -283,11 +284,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
       }
     }
     pos += steps_here;
-    step = 0;
-    if (pos < end) {
-      if (++entry == walk.entries) entry = 0, hk++;
-      steps = paged_steps<KEYS>(p, cache, entry);
-    }
+    if (pos < end) at.next_unit(walk);
   }
 }
 
