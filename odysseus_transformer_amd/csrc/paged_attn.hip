@@ -91,7 +91,16 @@ __device__ __forceinline__ void values(const typename Tile<float, D>::vvec (&row
       for (int m = 0; m < NT; m++) o[m][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows[r][i], w[m][r], o[m][i], 0, 0, 0);
 }
 
-template <typename T, int D, int NT>
+template <bool STREAM, typename V>
+__device__ __forceinline__ V load_vector(const char* p) {
+  typedef unsigned raw __attribute__((ext_vector_type(sizeof(V) / 4)));
+  if constexpr (STREAM) return __builtin_bit_cast(V, __builtin_nontemporal_load(reinterpret_cast<const raw*>(p)));
+  else return *reinterpret_cast<const V*>(p);
+}
+
+// STREAM: keys that one row tile reads, in rows of whole cache lines, take no cache room (16 x 4001 keys of 32 heads 130 -> 124 us, 131072 of 8 heads 103 -> 100;
+// in rows of 64 columns, of which a load takes half a line, 16.6 -> 17.7).
+template <typename T, int D, int NT, bool STREAM>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAttnParams p, const PagedCache cache) {
   typedef Tile<T, D> G;
   constexpr int STEP = WAVES * G::KEYS, GK = G::GK, OP = D + 4;
@@ -159,14 +168,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAt
       const char* src = kp + (uint64_t)((unsigned)pg.k < (unsigned)cache.pages ? pg.k : 0) * cache.k_page + (unsigned)(gk & in_page) * cache.k_row;
 #pragma unroll
       for (int j = 0; j < G::KV; j++)
-        to.k[j] = *reinterpret_cast<const typename G::kvec*>(src + G::key_row(j) * (uint64_t)cache.k_row + G::key_col(0, j) * sizeof(T));
+        to.k[j] = load_vector<STREAM, typename G::kvec>(src + G::key_row(j) * (uint64_t)cache.k_row + G::key_col(0, j) * sizeof(T));
     };
     auto load_v = [&](Loaded& to, int t, const Pages& pg) __attribute__((always_inline)) {
       const int gv = min(key0 + t * STEP + GK * q, last_group);
       to.page = (unsigned)pg.v < (unsigned)cache.pages;
       const char* src = vp + (uint64_t)(to.page ? pg.v : 0) * cache.v_page + (unsigned)(gv & in_page) * cache.v_row;
 #pragma unroll
-      for (int j = 0; j < GK; j++) to.v[j] = *reinterpret_cast<const typename G::vvec*>(src + j * (uint64_t)cache.v_row);
+      for (int j = 0; j < GK; j++) to.v[j] = load_vector<STREAM, typename G::vvec>(src + j * (uint64_t)cache.v_row);
     };
     // the products with tile t; `k_read` is called when those with its K have been formed
     auto compute = [&](Loaded& x, int t, auto k_read) __attribute__((always_inline)) {
@@ -418,7 +427,8 @@ int join(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStrea
 }
 template <typename T, int D, int NT>
 int launch(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
-  ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
+  if (D == 128 && pl.row_tiles == 1) ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT, D == 128>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
+  else ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT, false>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
   const int rc = ody_check_launch("paged_attn");
   return rc ? rc : join<T, D, WAVES * Tile<T, D>::KEYS, 1>(p, c, pl, st);
 }
