@@ -400,8 +400,9 @@ int ody_attn_bwd_dropout(const void* q, const void* k, const void* v, const void
  *                   Sequences may share pages that none of them appends to.
  * lengths           (S) int32: tokens of a sequence WITH the n new ones; below 0 as 0.  Device memory, as the table is: a captured graph
  *                   replays with what they hold then.
- * New token i sits at place lengths - n + i.  Where that is negative there is no token (shorter sequences of a batch are padded on the left;
- * length 0 is a sequence that takes no part).  A place behind the table's last column has no page.
+ * new_tokens        (S) int32, or NULL: of the n new tokens a sequence has the last new_tokens (NULL: all; 0: it takes no part).
+ * New token i sits at place lengths - n + i.  Where that is negative, or i < n - new_tokens, there is no token: sequences with fewer than n are padded on
+ * the left.  A place behind the table's last column has no page.
  *
  * ody_paged_append  qkv (S, n, Hq + 2 Hkv, D), the packed projection, strides sx_*.  q != NULL: queries and keys are rotated as ody_rope
  *                   rotates them, by position_ids (S, n) int64, contiguous, or with NULL by their places, and inv_freq (D / 2) fp32; the queries go to q
@@ -413,12 +414,12 @@ int ody_attn_bwd_dropout(const void* q, const void* k, const void* v, const void
  * D in {64, 128}; bf16 and fp32; pointers and strides of qkv, q, out and the pages on 16 bytes.
  */
 int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v_pages, const int* page_table, const int* lengths,
-                     const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,
+                     const int* new_tokens, const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,
                      int64_t sx_s, int64_t sx_n, int64_t sx_h, int64_t sq_s, int64_t sq_n, int64_t sq_h,
                      int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
                      int pages, int page_size, int table_width, int64_t table_stride, int dtype, void* stream);
 size_t ody_paged_attn_workspace_bytes(int S, int n, int Hq, int Hkv, int D, int page_size, int table_width, int dtype);
-int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* lengths, void* out, float* lse,
+int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* lengths, const int* new_tokens, void* out, float* lse,
                    int S, int n, int Hq, int Hkv, int D, int64_t sq_s, int64_t sq_n, int64_t sq_h,
                    int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
                    int64_t so_s, int64_t so_n, int64_t so_h, int pages, int page_size, int table_width, int64_t table_stride,

@@ -61,9 +61,9 @@ SIGNATURES = {
     "ody_norm_linear_swiglu_h": (_i, [_p, _p, _f, _p, _p] + [_i] * 3 + [_i64] * 3 + [_i, _p]),
     "ody_attn_bwd_rope": (_i, [_p] * 9 + [_i] * 6 + [_i64] * 24 + [_f, _i, _i, _i, _p, _sz, _p, _p, _p]),
     "ody_attn_fwd_dropout": (_i, [_p] * 5 + [_i] * 6 + [_i64] * 12 + [_f, _i, _i, _p, _sz, _p, _f, _u64]),
-    "ody_paged_append": (_i, [_p] * 8 + [_i] * 5 + [_i64] * 12 + [_i] * 3 + [_i64, _i, _p]),
+    "ody_paged_append": (_i, [_p] * 9 + [_i] * 5 + [_i64] * 12 + [_i] * 3 + [_i64, _i, _p]),
     "ody_paged_attn_workspace_bytes": (_sz, [_i] * 8),
-    "ody_paged_attn": (_i, [_p] * 7 + [_i] * 5 + [_i64] * 12 + [_i] * 3 + [_i64, _f, _i, _p, _sz, _p]),
+    "ody_paged_attn": (_i, [_p] * 8 + [_i] * 5 + [_i64] * 12 + [_i] * 3 + [_i64, _f, _i, _p, _sz, _p]),
     "ody_attn_bwd_dropout": (_i, [_p] * 9 + [_i] * 6 + [_i64] * 24 + [_f, _i, _i, _i, _p, _sz, _p, _f, _u64]),
 }
 

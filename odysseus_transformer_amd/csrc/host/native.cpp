@@ -551,23 +551,30 @@ PyObject* norm_linear_swiglu_h(Call c) {
 // waits for a gradient.
 struct Paged {
   const at::Tensor &k, &v, &table, &lengths;
-  Paged(Call& c, Py_ssize_t i, const at::Tensor& x) : k(c.heads(i, &x)), v(c.heads(i + 1, &x)), table(c.any(i + 2)), lengths(c.any(i + 3)) {
+  const int* fresh;
+  Paged(Call& c, Py_ssize_t i, Py_ssize_t new_tokens, const at::Tensor& x)
+      : k(c.heads(i, &x)), v(c.heads(i + 1, &x)), table(c.any(i + 2)), lengths(c.any(i + 3)), fresh(nullptr) {
     need(k.sizes() == v.sizes() && k.size(3) == x.size(3));
     need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == x.size(0) && table.stride(1) == 1 && table.size(1) < INT32_MAX);
     need(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.is_contiguous() && lengths.size(0) == x.size(0));
+    if (!c.none(new_tokens)) {
+      const at::Tensor& t = c.any(new_tokens);
+      need(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.size(0) == x.size(0));
+      fresh = t.data_ptr<int>();
+    }
     need(!at::GradMode::is_enabled() || !(x.requires_grad() || k.requires_grad() || v.requires_grad()));
   }
   int pages() const { return (int)k.size(0); }
   int page_size() const { return (int)k.size(1); }
   int columns() const { return (int)table.size(1); }
 };
-#define PAGED_TABLE(c) (c).table.data_ptr<int>(), (c).lengths.data_ptr<int>()
+#define PAGED_TABLE(c) (c).table.data_ptr<int>(), (c).lengths.data_ptr<int>(), (c).fresh
 #define PAGED_SHAPE(c) (c).pages(), (c).page_size(), (c).columns(), (c).table.stride(0)
 
-// (qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids or None, inv_freq or None: no rotation) -> q
+// (qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids or None, inv_freq or None: no rotation, new_tokens or None) -> q
 PyObject* paged_append(Call c) {
   const at::Tensor& x = c.heads(0, nullptr);
-  const Paged pg(c, 2, x);
+  const Paged pg(c, 2, 8, x);
   const int64_t Hq = c.whole(1), S = x.size(0), n = x.size(1), D = x.size(3), Hkv = pg.k.size(2);
   need(Hq > 0 && x.size(2) == Hq + 2 * Hkv);
   if (c.none(7)) {
@@ -587,10 +594,10 @@ PyObject* paged_append(Call c) {
   return wrap(q);
 }
 
-// (q, k_pages, v_pages, page_table, lengths, scale) -> (out, lse)
+// (q, k_pages, v_pages, page_table, lengths, scale, new_tokens or None) -> (out, lse)
 PyObject* paged_attn(Call c) {
   const at::Tensor& q = c.heads(0, nullptr);
-  const Paged pg(c, 1, q);
+  const Paged pg(c, 1, 6, q);
   const int S = q.size(0), n = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = pg.k.size(2);
   const float scale = (float)c.real(5);
   at::Tensor out = make({S, n, Hq, D}, q), lse = make_f32({S, Hq, n}, q);
@@ -650,7 +657,7 @@ PyMethodDef methods[] = {
     METHOD(rmsnorm_fwd, 3), METHOD(rmsnorm_bwd, 5), METHOD(gemm, 3), METHOD(linear_residual, 3), METHOD(linear_rope, 5), METHOD(linear_swiglu, 2),
     METHOD(linear_swiglu_h, 2), METHOD(linear_dgrad_swiglu, 3), METHOD(attn_fwd, 5), METHOD(attn_bwd, 13), METHOD(flash, 5), METHOD(rope, 6), METHOD(rope_table, 5),
     METHOD(norm_linear_rope, 8), METHOD(norm_linear_swiglu_h, 4),
-    METHOD(paged_append, 8), METHOD(paged_attn, 6),
+    METHOD(paged_append, 9), METHOD(paged_attn, 7),
     METHOD(current_stream, 0), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_odysseus_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -11,11 +11,12 @@ struct PagedCache {
   void* v;
   const int* table;     // (S, width): page of rows [c << shift, (c + 1) << shift) of a sequence; outside [0, pages): none
   const int* lengths;   // (S): tokens of the sequence, the new ones included
+  const int* fresh;     // (S): how many of the n new ones it has, the last ones; null: all
   PageStrides sk, sv;
   int64_t table_stride;
   int pages, shift, width;
   unsigned k_page, k_row, v_page, v_row;   // bytes from page to page and from row to row (paged_check: rows of a page lie within 4 GiB, as pages' starts do)
-  PagedCache(void* k_, void* v_, const int* table_, const int* lengths_, PageStrides sk_, PageStrides sv_, int64_t table_stride_, int pages_, int page_size,
+  PagedCache(void* k_, void* v_, const int* table_, const int* lengths_, const int* fresh_, PageStrides sk_, PageStrides sv_, int64_t table_stride_, int pages_, int page_size,
              int width_, int dtype);
 };
 
@@ -58,11 +59,13 @@ int ody_launch_paged_chunk(const PagedAttnParams& p, int D, const PagedCache& c,
 // the lengths of that time, and there is no plan to be kept.
 // Tokens of a sequence; less than nothing is nothing.
 __device__ __forceinline__ int paged_length(const PagedCache& c, int s) { return max(0, c.lengths[s]); }
-// Keys that the last row of a row tile sees: places behind the table's last column have no page (the host checks width << shift < 2^31).
-__device__ __forceinline__ int paged_keys(const PagedAttnParams& p, const PagedCache& c, int length, int rt) {
+// New tokens of sequence s, of n.
+__device__ __forceinline__ int paged_fresh(const PagedCache& c, int s, int n) { return c.fresh ? max(0, min(c.fresh[s], n)) : n; }
+// Keys that the last row of a row tile sees, none if it has no token: places behind the table's last column have no page (the host checks width << shift < 2^31).
+__device__ __forceinline__ int paged_keys(const PagedAttnParams& p, const PagedCache& c, int length, int fresh, int rt) {
   const int last_row = min((rt + 1) * p.tile, p.n * p.group) - 1;   // rows are below 2^31, and so is a row tile more
   const int last = p.row_tiles == 1 ? p.n - 1 : last_row / p.group;
-  return max(0, min(c.width << c.shift, length - p.n + last + 1));
+  return last < p.n - fresh ? 0 : max(0, min(c.width << c.shift, length - p.n + last + 1));
 }
 // Inclusive sums over the lanes of a wavefront, within rows of 16 lanes and then from row to row.
 __device__ __forceinline__ int paged_wave_scan(int x) {
@@ -104,14 +107,14 @@ template <int STEP>
 struct PagedWalk {
   const PagedAttnParams& p;
   const PagedCache& c;
-  int lane, entries, at = 0, before = 0, length = 0, mine = 0, sums = 0;   // sums: inclusive, of this chunk
+  int lane, entries, at = 0, before = 0, length = 0, fresh = 0, mine = 0, sums = 0;   // sums: inclusive, of this chunk
   __device__ __forceinline__ PagedWalk(const PagedAttnParams& p_, const PagedCache& c_, int lane_) : p(p_), c(c_), lane(lane_), entries(p_.S * p_.row_tiles) { chunk(); }
   __device__ __forceinline__ void chunk() {
     mine = 0;
     if (at + lane < entries) {
       const int e = at + lane, s = p.row_tiles == 1 ? e : e / p.row_tiles;
-      length = paged_length(c, s);
-      mine = max(1, (paged_keys(p, c, length, e - s * p.row_tiles) - 1) / STEP + 1);
+      length = paged_length(c, s), fresh = paged_fresh(c, s, p.n);
+      mine = max(1, (paged_keys(p, c, length, fresh, e - s * p.row_tiles) - 1) / STEP + 1);
     }
     sums = paged_wave_scan(mine);
   }
@@ -136,7 +139,7 @@ struct PagedWalk {
 // A place in the order of all steps: kv head, pair (sequence, row tile), step of it.
 template <int STEP>
 struct PagedPlace {
-  int hk, entry, s, rt, length, steps, step;
+  int hk, entry, s, rt, length, fresh, steps, step;
   // that of step `pos`, `each` of every kv head
   __device__ __forceinline__ PagedPlace(PagedWalk<STEP>& w, int pos, int each) {
     hk = (int)((unsigned)pos / (unsigned)each);
@@ -162,7 +165,7 @@ struct PagedPlace {
  private:
   __device__ __forceinline__ void take(const PagedWalk<STEP>& w) {
     const int k = entry - w.at;
-    steps = __builtin_amdgcn_readlane(w.mine, k), length = __builtin_amdgcn_readlane(w.length, k);
+    steps = __builtin_amdgcn_readlane(w.mine, k), length = __builtin_amdgcn_readlane(w.length, k), fresh = __builtin_amdgcn_readlane(w.fresh, k);
     s = w.p.row_tiles == 1 ? entry : entry / w.p.row_tiles, rt = entry - s * w.p.row_tiles;
   }
 };

@@ -19,7 +19,7 @@ template <typename T> __device__ __forceinline__ float rounded(float x) { return
 // A block takes a token: consecutive threads take consecutive vectors of a head, x[j] together with x[j + D / 2].  Bound by memory, or for few tokens by
 // latencies: a thread's first vectors are under way while the block evaluates the token's angles, which go to LDS (64 tokens of 48 heads 3.8 -> 3.2 us,
 // launch included).  Results leave without taking cache room (3001 tokens of 48 heads 15.5 -> 12.7 us), and operands that the last-level cache cannot hold
-// beside them are read past it (STREAM; 4 x 4096 tokens of 96 heads 141 -> 135 us, 5.0 TB/s; 3001 of 48 12.7 -> 14.3).  A token before place 0 is none: its
+// beside them are read past it (STREAM; 4 x 4096 tokens of 96 heads 141 -> 135 us, 5.0 TB/s; 3001 of 48 12.7 -> 14.3).  A token that is none: its
 // queries become 0, nothing else is written.
 template <typename T, int D, bool ROTATE, bool STREAM>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p, const PagedCache cache) {
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendParams p,
   };
   vec a, b;
   if (tid < items) load(tid, a, b);
-  const int place = max(cache.lengths[s], 0) - p.n + i;
+  const int place = i < p.n - paged_fresh(cache, s, p.n) ? -1 : max(cache.lengths[s], 0) - p.n + i;
   // where the token's keys and values go
   int page = -1;
   if (place >= 0 && place >> cache.shift < cache.width) page = cache.table[s * cache.table_stride + (place >> cache.shift)];
@@ -102,9 +102,9 @@ int launch(const AppendParams& p, const PagedCache& cache, hipStream_t st) {
 
 }  // namespace
 
-PagedCache::PagedCache(void* k_, void* v_, const int* table_, const int* lengths_, PageStrides sk_, PageStrides sv_, int64_t table_stride_, int pages_,
+PagedCache::PagedCache(void* k_, void* v_, const int* table_, const int* lengths_, const int* fresh_, PageStrides sk_, PageStrides sv_, int64_t table_stride_, int pages_,
                        int page_size, int width_, int dtype)
-    : k(k_), v(v_), table(table_), lengths(lengths_), sk(sk_), sv(sv_), table_stride(table_stride_), pages(pages_), shift(paged_shift(page_size)),
+    : k(k_), v(v_), table(table_), lengths(lengths_), fresh(fresh_), sk(sk_), sv(sv_), table_stride(table_stride_), pages(pages_), shift(paged_shift(page_size)),
       width(width_) {
   const int64_t bytes = dtype == ODY_BF16 ? 2 : 4;
   k_page = (unsigned)(bytes * sk.p), k_row = (unsigned)(bytes * sk.r), v_page = (unsigned)(bytes * sv.p), v_row = (unsigned)(bytes * sv.r);
@@ -131,11 +131,11 @@ int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype
 }
 
 extern "C" int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v_pages, const int* page_table, const int* lengths,
-                                const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,
+                                const int* new_tokens, const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,
                                 int64_t sx_s, int64_t sx_n, int64_t sx_h, int64_t sq_s, int64_t sq_n, int64_t sq_h,
                                 int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
                                 int pages, int page_size, int table_width, int64_t table_stride, int dtype, void* stream) {
-  const PagedCache c(k_pages, v_pages, page_table, lengths, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride, pages, page_size, table_width, dtype);
+  const PagedCache c(k_pages, v_pages, page_table, lengths, new_tokens, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride, pages, page_size, table_width, dtype);
   if (int rc = paged_check("ody_paged_append", S, n, Hq, Hkv, D, dtype, c, page_size)) return rc;
   ODY_REQUIRE(qkv && (q == nullptr || inv_freq), ODY_ERR_NULL, "ody_paged_append: qkv, or inv_freq of a rotation, is NULL");
   ODY_REQUIRE(paged_rows_aligned(qkv, sx_s, sx_n, sx_h, dtype) && (q == nullptr || paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype)), ODY_ERR_MISALIGNED,

@@ -121,7 +121,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAt
   while (pos < end) {
     const int s = at.s, rt = at.rt, hk = at.hk, length = at.length, step = at.step, steps = at.steps, row0 = rt * p.tile;
     const int rows = min(p.tile, p.n * p.group - row0);
-    const int keys = paged_keys(p, cache, length, rt), steps_here = min(steps - step, end - pos);
+    const int none = p.n - at.fresh;   // the first tokens, which are none
+    const int keys = paged_keys(p, cache, length, at.fresh, rt), steps_here = min(steps - step, end - pos);
     const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(cache.k) + hk * cache.sk.h) + of_lane_k;
     const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(cache.v) + hk * cache.sv.h) + of_lane_v;
     const int* table = cache.table + s * cache.table_stride;
@@ -137,9 +138,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAt
       const T* qp = static_cast<const T*>(p.q) + s * p.sq.b + i * p.sq.l + h * p.sq.h;
 #pragma unroll
       for (int j = 0; j < (int)(D * sizeof(T) / 64); j++) qf[m][j] = p.signed_query(*reinterpret_cast<const typename G::kvec*>(qp + G::key_col(q, j)));
-      lim[m] = min(keys - 1, length - p.n + i);
+      lim[m] = i < none ? -1 : min(keys - 1, length - p.n + i);
     }
-    safe = min(safe, length - p.n + row0 / p.group);
+    safe = row0 / p.group < none ? -1 : min(safe, length - p.n + row0 / p.group);
 
     f32x4 o[NT][D / 16];
     float mx[NT], l[NT];
@@ -427,8 +428,9 @@ int join(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStrea
 }
 template <typename T, int D, int NT>
 int launch(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
-  if (D == 128 && pl.row_tiles == 1) ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT, D == 128>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
-  else ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT, false>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
+  constexpr bool LINES = D == 128;   // a tile of 16 rows is the only one
+  if (NT == 1 || (LINES && pl.row_tiles == 1)) ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT, LINES>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
+  else ODY_LAUNCH("paged_attn", st, (paged_attn_kernel<T, D, NT, NT == 1 && LINES>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c);
   const int rc = ody_check_launch("paged_attn");
   return rc ? rc : join<T, D, WAVES * Tile<T, D>::KEYS, 1>(p, c, pl, st);
 }
@@ -453,12 +455,12 @@ extern "C" size_t ody_paged_attn_workspace_bytes(int S, int n, int Hq, int Hkv, 
   return pl.part_bytes + pl.ml_bytes;
 }
 
-extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* lengths, void* out,
+extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* lengths, const int* new_tokens, void* out,
                               float* lse, int S, int n, int Hq, int Hkv, int D, int64_t sq_s, int64_t sq_n, int64_t sq_h,
                               int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
                               int64_t so_s, int64_t so_n, int64_t so_h, int pages, int page_size, int table_width, int64_t table_stride,
                               float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  const PagedCache c(const_cast<void*>(k_pages), const_cast<void*>(v_pages), page_table, lengths, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride,
+  const PagedCache c(const_cast<void*>(k_pages), const_cast<void*>(v_pages), page_table, lengths, new_tokens, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride,
                      pages, page_size, table_width, dtype);
   if (int rc = paged_check("ody_paged_attn", S, n, Hq, Hkv, D, dtype, c, page_size)) return rc;
   ODY_REQUIRE(q && out && lse, ODY_ERR_NULL, "ody_paged_attn: q, out or lse is NULL");

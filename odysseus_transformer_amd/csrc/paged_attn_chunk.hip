@@ -75,7 +75,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
   while (pos < end) {
     const int s = at.s, rt = at.rt, hk = at.hk, length = at.length, step = at.step, steps = at.steps, row0 = rt * BLOCK_ROWS;
     const int rows = min(BLOCK_ROWS, p.n * p.group - row0);
-    const int keys = paged_keys(p, cache, length, rt), steps_here = min(steps - step, end - pos), tiles = keys > 0 ? steps_here : 0;
+    const int none = p.n - at.fresh;   // the first tokens, which are none
+    const int keys = paged_keys(p, cache, length, at.fresh, rt), steps_here = min(steps - step, end - pos), tiles = keys > 0 ? steps_here : 0;
     const int key0 = KEYS * step;
     const char* kp = reinterpret_cast<const char*>(static_cast<const bf16*>(cache.k) + hk * cache.sk.h);
     const char* vp = reinterpret_cast<const char*>(static_cast<const bf16*>(cache.v) + hk * cache.sv.h);
@@ -126,8 +127,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) qf[ks] = p.signed_query(*reinterpret_cast<const bf16x8*>(qp + 16 * ks));
     }
-    const int lim = min(keys - 1, length - p.n + ri);   // last key that it sees
-    const int safe = __builtin_amdgcn_readfirstlane(min(keys - 1, length - p.n + (row0 + min(32 * wave, rows - 1)) / p.group));   // ... that all of the wavefront's see
+    const int lim = ri < none ? -1 : min(keys - 1, length - p.n + ri);   // last key that it sees
+    const int first_token = (row0 + min(32 * wave, rows - 1)) / p.group;
+    const int safe = __builtin_amdgcn_readfirstlane(first_token < none ? -1 : min(keys - 1, length - p.n + first_token));   // ... that all of the wavefront's see
 
     f32x16 o[DT];
     clear(o);

@@ -461,9 +461,9 @@ class _PartialResults:
 
 
 # --------------------------------------------------------------------------- key / value cache in pages
-def _check_paged(who: str, x, k_pages, v_pages, page_table, lengths) -> None:
+def _check_paged(who: str, x, k_pages, v_pages, page_table, lengths, new_tokens) -> None:
     """What the kernels of a paged cache cannot see: types, devices and shapes that fit `x` (S, n, heads, D), and that nobody waits for a gradient."""
-    _need_gpu(x, k_pages, v_pages, page_table, lengths)
+    _need_gpu(x, k_pages, v_pages, page_table, lengths, new_tokens)
     _dt(x)
     if x.dim() != 4 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != x.shape[3]:
         raise ValueError(f"{who}: (S, n, heads, D) tokens and (pages, page_size, kv heads, D) pages expected, got {tuple(x.shape)}, {tuple(k_pages.shape)} "
@@ -476,21 +476,23 @@ def _check_paged(who: str, x, k_pages, v_pages, page_table, lengths) -> None:
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != S or page_table.stride(1) != 1 or page_table.device != x.device:
         raise ValueError(f"{who}: page_table must be an int32 ({S}, columns) tensor on {x.device} with unit column stride, got {tuple(page_table.shape)} "
                          f"{page_table.dtype} stride {page_table.stride()} on {page_table.device}")
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (S,) or not lengths.is_contiguous() or lengths.device != x.device:
-        raise ValueError(f"{who}: lengths must be a contiguous int32 ({S},) tensor on {x.device}, got {tuple(lengths.shape)} {lengths.dtype} on {lengths.device}")
+    for name, t in (("lengths", lengths), ("new_tokens", new_tokens)):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (S,) or not t.is_contiguous() or t.device != x.device):
+            raise ValueError(f"{who}: {name} must be a contiguous int32 ({S},) tensor on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError(f"{who} has no backward: a cache is for inference, call it under torch.no_grad() or on detached tensors")
 
 
 def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, position_ids=None, base: float = 10000.0, inv_freq=None,
-                  rotate: bool = True):
+                  rotate: bool = True, new_tokens=None):
     """New tokens into a cache in pages: qkv (S, n, Hq + 2 Hkv, D), the packed projection, of which the keys and values of every sequence go to
     their rows of k_pages / v_pages (pages, page_size, Hkv, D).  Returns the queries (S, n, Hq, D).
 
     page_table (S, columns) int32: the pages of a sequence in order; an entry outside [0, pages) is none.  lengths (S) int32: the tokens of
-    each sequence WITH the new ones, of which the last n are these: token i has place lengths - n + i, and where that is negative it is padding
-    (shorter sequences are padded on the left, length 0 takes no part): its queries become 0 and nothing is written.  page_size is a
-    power of two from 8 on; any strides that are multiples of 16 bytes.
+    each sequence WITH the new ones, of which the last n are these: token i has place lengths - n + i.  Where that is negative it is padding, and
+    so are the first n - new_tokens[s] of a sequence with fewer than n, if new_tokens (S) int32 is given (padding on the left; 0: the sequence takes no
+    part): the queries of padding become 0 and nothing is written.  page_size is a power of two from 8 on; any strides that are multiples of 16
+    bytes, pages and the rows of a page less than 4 GiB apart.  No two sequences may append to one row.
 
     rotate: queries and keys are rotated as rope_ rotates them, by position_ids -- (S, n), or (n) for all -- or by the tokens' places; the
     queries are a new tensor.  rotate=False: they have been rotated already (linear_rope, norm_linear_rope); the result is a view of qkv."""
@@ -499,13 +501,13 @@ def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, posi
     if qkv.is_cuda:
         if inv_freq is None and rotate:
             inv_freq = rope_inv_freq(qkv.shape[-1], base, qkv.device)
-        plain = native.paged_append(qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids, inv_freq if rotate else None)
+        plain = native.paged_append(qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids, inv_freq if rotate else None, new_tokens)
         if plain is not None:
             return plain
     if qkv.is_cuda and qkv.device.index != torch.cuda.current_device():
         with torch.cuda.device(qkv.device):
-            return paged_append_(qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids, base, inv_freq, rotate)
-    _check_paged("paged_append_", qkv, k_pages, v_pages, page_table, lengths)
+            return paged_append_(qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids, base, inv_freq, rotate, new_tokens)
+    _check_paged("paged_append_", qkv, k_pages, v_pages, page_table, lengths, new_tokens)
     S, n, heads, D = qkv.shape
     Hkv = k_pages.shape[2]
     if n_heads <= 0 or heads != n_heads + 2 * Hkv:
@@ -518,24 +520,26 @@ def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, posi
     if rotate and position_ids is not None:
         position_ids = position_ids.to(torch.int64).expand(S, n).contiguous()
     _lib.call("ody_paged_append", qkv.data_ptr(), q.data_ptr() if rotate else 0, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-              lengths.data_ptr(), position_ids.data_ptr() if rotate and position_ids is not None else 0, inv_freq.data_ptr() if rotate else 0,
+              lengths.data_ptr(), 0 if new_tokens is None else new_tokens.data_ptr(),
+              position_ids.data_ptr() if rotate and position_ids is not None else 0, inv_freq.data_ptr() if rotate else 0,
               S, n, n_heads, Hkv, D, *_blhd(qkv, "qkv"), *_blhd(q, "q"), *_blhd(k_pages, "k_pages"), *_blhd(v_pages, "v_pages"),
               k_pages.shape[0], k_pages.shape[1], page_table.shape[1], page_table.stride(0), _dt(qkv), _stream())
     return q
 
 
-def paged_attn(q, k_pages, v_pages, page_table, lengths, scale: Optional[float] = None):
+def paged_attn(q, k_pages, v_pages, page_table, lengths, scale: Optional[float] = None, new_tokens=None):
     """Attention of the n newest tokens of every sequence, q (S, n, Hq, D), over a cache in pages that holds them already (paged_append_, which
     says what the arguments are): a token sees the places up to its own.  -> out (S, n, Hq, D), lse (S, Hq, n) fp32, 0 and -inf for a
     token that sees none."""
     if q.is_cuda:
-        plain = native.paged_attn(q, k_pages, v_pages, page_table, lengths, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale)
+        plain = native.paged_attn(q, k_pages, v_pages, page_table, lengths, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale,
+                                  new_tokens)
         if plain is not None:
             return plain
     if q.is_cuda and q.device.index != torch.cuda.current_device():
         with torch.cuda.device(q.device):
-            return paged_attn(q, k_pages, v_pages, page_table, lengths, scale)
-    _check_paged("paged_attn", q, k_pages, v_pages, page_table, lengths)
+            return paged_attn(q, k_pages, v_pages, page_table, lengths, scale, new_tokens)
+    _check_paged("paged_attn", q, k_pages, v_pages, page_table, lengths, new_tokens)
     S, n, Hq, D = q.shape
     Hkv = k_pages.shape[2]
     out = torch.empty((S, n, Hq, D), dtype=q.dtype, device=q.device)
@@ -545,8 +549,9 @@ def paged_attn(q, k_pages, v_pages, page_table, lengths, scale: Optional[float] 
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     ws_bytes = _lib.load().ody_paged_attn_workspace_bytes(S, n, Hq, Hkv, D, k_pages.shape[1], page_table.shape[1], _dt(q))
     ws = _own_scratch(ws_bytes, "paged_attn_workspace", q.device) if ws_bytes else None
-    _lib.call("ody_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-              lse.data_ptr(), S, n, Hq, Hkv, D, *_blhd(q, "q"), *_blhd(k_pages, "k_pages"), *_blhd(v_pages, "v_pages"), *_blhd(out, "out"),
+    _lib.call("ody_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+              0 if new_tokens is None else new_tokens.data_ptr(), out.data_ptr(), lse.data_ptr(), S, n, Hq, Hkv, D,
+              *_blhd(q, "q"), *_blhd(k_pages, "k_pages"), *_blhd(v_pages, "v_pages"), *_blhd(out, "out"),
               k_pages.shape[0], k_pages.shape[1], page_table.shape[1], page_table.stride(0), scale, _dt(q), ws.data_ptr() if ws is not None else 0,
               ws_bytes, _stream())
     return out, lse

@@ -37,6 +37,13 @@ def page_of(c, s, place):
     return (p, place % c["page"]) if 0 <= p < c["k"].shape[0] else None
 
 
+def first_token(c, s, n):
+    """The first of a sequence's n rows that is a token, n if none is: c["new"], where it is there, numbers them."""
+    length = max(int(c["lengths"][s]), 0)
+    new = n if c.get("new") is None else min(max(int(c["new"][s]), 0), n)
+    return max(n - new, min(n - length, n))
+
+
 def append(c, Hq, inv_freq=None, positions=None):
     """-> q, k_pages, v_pages in float64 (copies), and for each an array of |a cos| + |b sin|, the scale of the products in it."""
     x = c["qkv"]
@@ -48,7 +55,7 @@ def append(c, Hq, inv_freq=None, positions=None):
     for s in range(S):
         for i in range(n):
             place = max(int(c["lengths"][s]), 0) - n + i
-            if place < 0:
+            if i < first_token(c, s, n):
                 continue
             new = x[s, i].double()
             mag = new.abs()
@@ -87,7 +94,7 @@ def attend(c, scale=None):
         j = torch.tensor(places)
         for i in range(n):
             seen = j <= length - n + i
-            if not seen.any():
+            if not seen.any() or i < first_token(c, s, n):
                 continue
             for h in range(Hq):
                 kk, vv = K[seen, h * Hkv // Hq], V[seen, h * Hkv // Hq]

@@ -22,7 +22,7 @@ def _inv_freq(D, base=10000.0):
 
 def _check_attn(c, g, scale=None):
     from odysseus_transformer_amd import ops
-    out, lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"], scale=scale)
+    out, lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"], scale=scale, new_tokens=g.get("new"))
     torch.cuda.synchronize()
     o, s, mean, dots = ref.attend(c, scale)
     tol_o, tol_s = ref.attend_bounds(c, o, s, mean, dots)
@@ -44,7 +44,7 @@ def _check_append(c, g, Hq, positions=None, rotate=True):
     qkv = g["qkv"].clone()
     got = ops.paged_append_(g["qkv"], Hq, g["k"], g["v"], g["table"], g["lengths"],
                             position_ids=None if positions is None else positions.to(g["qkv"].device),
-                            inv_freq=f.to(g["qkv"].device) if rotate else None, rotate=rotate)
+                            inv_freq=f.to(g["qkv"].device) if rotate else None, rotate=rotate, new_tokens=g.get("new"))
     torch.cuda.synchronize()
     assert torch.equal(g["qkv"], qkv), "the projection was written to"
     assert torch.equal(g["v"].cpu(), v.to(dtype)), "values"
@@ -160,6 +160,74 @@ def test_attn_scale_and_strided_queries(dev):
     c["q"] = c["qkv"][:, :, :4]
     g["q"] = g["qkv"][:, :, :4]                                   # a slice of the packed projection
     _check_attn(c, g)
+
+
+NEW = [
+    # lengths, new tokens, n, Hq, Hkv, D, page, dtype
+    ([40, 300, 7, 90], [1, 1, 0, 1], 1, 8, 2, 128, 16, BF16),
+    ([40, 300, 7, 90, 3], [5, 0, 2, 9, -1], 5, 4, 2, 64, 8, BF16),               # more than n, fewer than none
+    ([150, 300, 100, 20], [64, 1, 0, 20], 64, 4, 1, 128, 32, BF16),              # tiles of a sequence without a token in front
+    ([700, 150, 131, 60, 200], [130, 3, 0, 60, 129], 130, 4, 2, 128, 64, BF16),
+    ([270, 90, 200], [1, 80, 66], 80, 2, 1, 64, 16, BF16),
+    ([40, 300, 7, 90], [1, 0, 1, 0], 1, 4, 2, 64, 16, F32),
+    ([90, 200, 33], [33, 2, 0], 33, 4, 1, 128, 8, F32),
+    ([50, 60], [0, 0], 3, 4, 2, 128, 16, BF16),                                  # nobody
+    ([500, 60], [0, 0], 100, 4, 2, 128, 16, BF16),
+]
+
+
+@pytest.mark.parametrize("case", NEW, ids=lambda c: "n%d_H%d_%d_D%d_p%d_%s" % (*c[2:7], str(c[7])[-4:]))
+def test_sequences_with_fewer_new_tokens(case, dev):
+    lengths, new, n, Hq, Hkv, D, page, dtype = case
+    print(f"new {case}", flush=True)
+    c = ref.make(lengths, n, Hq, Hkv, D, page, dtype, seed=n + D)
+    c["new"] = torch.tensor(new, dtype=torch.int32)
+    g = _to(c, dev)
+    _check_attn(c, g)
+    _check_append(c, g, Hq)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[64], [65, 1], [128, 63], [192, 191], [321, 448, 64], [130 + 64 * 9]], ids=str)
+def test_chunks_of_few_tiles(D, lengths, dev):
+    """As many tiles of keys as a loop with several of them in flight can begin and end with, n from one row more than the few-rows kernel takes."""
+    for n in (65, 128, 200):
+        c = ref.make(lengths, n, 2, 1, D, 8, BF16, seed=sum(lengths) + n)
+        _check_attn(c, _to(c, dev))
+
+
+@pytest.mark.parametrize("rows", [33, 47, 48, 49, 64, 65])
+def test_rows_around_the_tiles(rows, dev):
+    c = ref.make([500, 90, 33], rows, 2, 2, 128, 16, BF16, seed=rows)
+    _check_attn(c, _to(c, dev))
+
+
+@pytest.mark.parametrize("column", [0, 1, 5, 9, 10])
+def test_chunks_with_a_page_missing(column, dev):
+    """Tiles before and behind a missing page, which leaves holes in front of the newest tokens, under them, and at the start."""
+    c = ref.make([352], 130, 4, 2, 128, 32, BF16, seed=column)
+    c["table"][0, column] = -7
+    _check_attn(c, _to(c, dev))
+
+
+def test_both_host_paths_agree(dev, monkeypatch):
+    from odysseus_transformer_amd import ops
+    c = ref.make([300, 40, 9], 3, 8, 2, 128, 16, BF16, seed=14)
+    c["new"] = torch.tensor([3, 1, 0], dtype=torch.int32)
+    res = []
+    for native in (True, False):
+        if not native:
+            for name in ("paged_append", "paged_attn"):
+                monkeypatch.setattr(ops.native, name, lambda *a: None)
+        g = _to(c, dev)
+        q = ops.paged_append_(g["qkv"], 8, g["k"], g["v"], g["table"], g["lengths"], new_tokens=g["new"])
+        own = ops.paged_append_(g["qkv"], 8, g["k"], g["v"], g["table"], g["lengths"], position_ids=torch.arange(3, device=dev), base=500.0)
+        held = ops.paged_append_(g["qkv"], 8, g["k"], g["v"], g["table"], g["lengths"], rotate=False, new_tokens=g["new"])
+        assert held.data_ptr() == g["qkv"].data_ptr()
+        res.append((q, own, held, g["k"], g["v"], *ops.paged_attn(q, g["k"], g["v"], g["table"], g["lengths"], new_tokens=g["new"]),
+                    *ops.paged_attn(q, g["k"], g["v"], g["table"], g["lengths"], 0.3)))
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
 
 
 def test_unowned_rows_are_neither_read_nor_written(dev):
