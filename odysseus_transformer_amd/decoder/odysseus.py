@@ -27,6 +27,7 @@ from ..parallel_state import get_model_parallel_rank, get_model_parallel_world_s
 from ..utils.allgather import allgather_bsz1
 from ..utils.linear_tpsp import ColumnParallelLinear, ColumnParallelLinearAG, RowParallelLinearRS
 from ..utils.linear_zero3 import LinearZeRO3
+from ..utils.paged_cache import PagedKVCache
 
 
 def _rope_theta(config) -> float:
@@ -141,6 +142,8 @@ class LlamaFlashAttention2TPSP(nn.Module):
                 "make sure to use `sdpa` in the mean time, and open an issue at "
                 "https://github.com/huggingface/transformers")
         bsz, local_q_len, _ = hidden_states.size()
+        if isinstance(past_key_value, PagedKVCache):
+            return self._forward_paged(hidden_states, past_key_value, attention_mask, kwargs.get("input_norm"), kwargs.get("residual"))
         assert bsz == 1, f"bsz: {bsz}"
         # the training path: no padding and nothing in the cache yet.  A padding mask or earlier cache content takes
         # the general path below, as decoder/odysseus.py:215-263 hands both on to the host's flash-attention call.
@@ -198,8 +201,9 @@ class LlamaFlashAttention2TPSP(nn.Module):
                     self._update_cache(past_key_value, k.detach(), v.detach(), q_len, cache_position)
                 attn_output = ops.flash_attn_func(q, k, v, 0.0, softmax_scale=scale, causal=True)
 
-        attn_output = attn_output.reshape(bsz, q_len, nh * D)
-        residual = kwargs.get("residual")
+        return self._output(attn_output.reshape(bsz, q_len, nh * D), kwargs.get("residual"), past_key_value)
+
+    def _output(self, attn_output, residual, past_key_value):
         if residual is not None and self._can_fuse_residual(residual, attn_output):
             # the caller's skip connection rides in the output projection's epilogue
             attn_output = ops.run_function(ops.LinearResidualFunc, attn_output, self.o_proj.weight, residual)
@@ -210,6 +214,52 @@ class LlamaFlashAttention2TPSP(nn.Module):
         if self.return_arity == 2:
             return attn_output, None
         return attn_output, None, past_key_value
+
+    def _forward_paged(self, hidden_states, cache: PagedKVCache, attention_mask, norm, residual):
+        """The new tokens of all sequences of a cache in pages, hidden_states (cache.max_sequences, n, hidden) behind cache.begin(): the cache takes
+        the place of decoder/odysseus.py:215-263, and its positions that of position_ids.  Inference on one rank."""
+        S, n, _ = hidden_states.shape
+        nh, nkv, D = self.n_local_heads, self.n_local_kv_heads, self.head_dim
+        if get_model_parallel_world_size() != 1:
+            raise NotImplementedError("a cache in pages holds whole sequences: one rank")
+        if attention_mask is not None:
+            raise ValueError("a cache in pages knows the padding of its batch (PagedKVCache.begin); attention_mask must be None")
+        if self.training and self.attention_dropout != 0.0:
+            raise ValueError("attention dropout over a cache in pages: call eval() first")
+        if cache.position_ids is None or tuple(cache.position_ids.shape) != (S, n):
+            raise ValueError(f"hidden_states are {tuple(hidden_states.shape)}, but the cache's step is for "
+                             f"{None if cache.position_ids is None else tuple(cache.position_ids.shape)} tokens: PagedKVCache.begin() comes before it")
+        scale = 1.0 / math.sqrt(D)
+        k_pages, v_pages = cache.layer(self.layer_idx or 0)
+        where = (k_pages, v_pages, cache.page_table, cache.lengths)
+        # nothing but these tokens, as many of every sequence: the rows that the cache would be read back from are at hand.  (A captured step is
+        # replayed for steps of which that may not be so.)
+        fresh = cache.fresh and not (hidden_states.is_cuda and torch.cuda.is_current_stream_capturing())
+        rotated = True   # by the projection
+        if norm is not None and not (self.pack_weight and self._can_fuse_rope(hidden_states)):
+            hidden_states, norm = norm(hidden_states), None
+        x = hidden_states.reshape(1, S * n, -1)   # the projections take one sequence
+        if norm is not None:
+            qkv = ops.norm_linear_rope(x[0], norm.weight, norm.variance_epsilon, self.qkv_proj.weight, nh + nkv, D, cache.position_ids.view(-1),
+                                       self.rope_theta)
+        elif fresh and self.pack_weight and self._can_fuse_rope(x):
+            qkv = ops.run_function(ops.LinearRoPEFunc, x, self.qkv_proj.weight, nh + nkv, D, cache.position_ids.view(-1), self.rope_theta)
+        else:
+            if self.pack_weight:
+                qkv = self.qkv_proj(x)
+            else:
+                qkv = torch.cat((self.q_proj(x), self.k_proj(x), self.v_proj(x)), dim=-1)
+            rotated = fresh
+            if rotated:
+                qkv = ops.apply_rope_packed(qkv.view(S, n, nh + 2 * nkv, D), nh + nkv, cache.position_ids, self.rope_theta)
+        qkv = qkv.view(S, n, nh + 2 * nkv, D)
+        q = ops.paged_append_(qkv, nh, *where, base=self.rope_theta, rotate=not rotated, new_tokens=cache.new_tokens)
+        if fresh:
+            attn_output = ops.flash_attn_func(q, qkv[:, :, nh:nh + nkv], qkv[:, :, nh + nkv:], 0.0, softmax_scale=scale, causal=True)
+        else:
+            attn_output = ops.paged_attn(q, *where, scale=scale, new_tokens=cache.new_tokens)[0]
+        y = self._output(attn_output.reshape(1, S * n, nh * D), None if residual is None else residual.reshape(x.shape), cache)
+        return (y[0].view(hidden_states.shape), *y[1:])
 
     def _can_fuse_rope(self, hidden_states) -> bool:
         """The fused node stands for gather(x) W^T followed by the rotation, which is what the packed projection
@@ -303,7 +353,10 @@ class LlamaMLPZeRO(nn.Module):
             x = input_norm(x)
         if fusable and self.fuse_elementwise:
             return ops.run_function(ops.SwiGLUMLPResidualFunc, x, w1, w2, residual)
-        y = self.down_proj(ops.swiglu(self.gate_up_proj(x)))
+        shape = x.shape
+        if x.dim() == 3 and get_model_parallel_world_size() == 1:   # the projections take one sequence; a batch comes with a cache in pages
+            x = x.reshape(1, -1, shape[-1])
+        y = self.down_proj(ops.swiglu(self.gate_up_proj(x))).view(*shape[:-1], -1)
         return y if residual is None else residual + y
 
 

@@ -462,3 +462,243 @@ def test_refusals(dev):
         ops.paged_attn(c["q"].clone().requires_grad_(True), *args())
     with pytest.raises(RuntimeError):
         ops.paged_attn(c["q"].cpu(), *args())
+
+
+# ---------------------------------------------------------------- the cache under the attention module and the decoder layer
+def _config(d, Hq, Hkv, D, inter=512):
+    import types
+    return types.SimpleNamespace(hidden_size=d, num_attention_heads=Hq, num_key_value_heads=Hkv, head_dim=D, intermediate_size=inter, hidden_act="silu",
+                                 attention_dropout=0.0, rms_norm_eps=1e-6, rope_theta=10000.0, pretraining_tp=1)
+
+
+def _layer(dtype, D, dev, **kw):
+    from odysseus_transformer_amd.decoder.odysseus import OdysseusDecoderLayer
+    torch.manual_seed(3)
+    layer = OdysseusDecoderLayer(_config(256, 4, 2, D), **kw).to(dtype).to(dev).eval()
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.copy_(torch.randn(p.shape, dtype=torch.float32).to(p) * 0.05 if p.dim() > 1 else 1 + 0.1 * torch.randn(p.shape, dtype=torch.float32).to(p))
+    return layer
+
+
+def _cache(dtype, D, dev, **kw):
+    from odysseus_transformer_amd.utils.paged_cache import PagedKVCache
+    c = PagedKVCache(**{**dict(num_layers=1, num_pages=40, max_sequences=3, max_length=200, n_kv_heads=2, head_dim=D, page_size=16, dtype=dtype, device=dev), **kw})
+    for t in c.layer(0):
+        t.fill_(float("nan"))                                     # nothing that was not written may be read
+    return c
+
+
+def _whole(layer, x):
+    """The layer over a whole sequence at once, in float32 on the CPU, by the formulas."""
+    import odysseus_oracle as o
+    a, m = layer.self_attn, layer.mlp
+    f = lambda t: t.detach().float().cpu()  # noqa: E731
+    norm = lambda h, w: h * torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-6) * f(w)  # noqa: E731
+    w = f(a.qkv_proj.weight) if a.pack_weight else torch.cat([f(t.weight) for t in (a.q_proj, a.k_proj, a.v_proj)])
+    x = f(x)
+    n = norm(x, layer.input_layernorm.weight)
+    h = x + torch.cat([o.attention_block(r[None], w, f(a.o_proj.weight), a.num_heads, a.num_key_value_heads, a.head_dim)[0] for r in n])
+    n = norm(h, layer.post_attention_layernorm.weight)
+    gate, up = (n @ f(m.gate_up_proj.weight).t()).chunk(2, -1)
+    return h + (torch.nn.functional.silu(gate) * up) @ f(m.down_proj.weight).t()
+
+
+def _tol(dtype, steps=12):
+    """Relative to a row's norm: so many roundings to the type on the way, half a step each, and sums of up to 512 products on both sides."""
+    return steps * torch.finfo(dtype).eps / 2 + 1024 * 2 ** -24
+
+
+@pytest.mark.parametrize("dtype,D,kw", [(BF16, 128, {}), (BF16, 64, {}), (BF16, 128, dict(fused=False)), (F32, 64, {})], ids=["bf16_128", "bf16_64", "plain", "f32"])
+def test_decoder_layer_over_a_cache_in_pages(dtype, D, kw, dev):
+    """Prompts of different lengths, single tokens, a step for some only, proposed tokens that are taken back, a sequence that ends and one that begins in
+    its place: every row is the one that the layer gives for the whole sequence at once."""
+    layer, cache = _layer(dtype, D, dev, **kw), _cache(dtype, D, dev)
+    g = torch.Generator().manual_seed(5)
+    rows = [torch.randn(1, 200, 256, generator=g).to(dtype) for _ in range(4)]
+    want = [_whole(layer, r) for r in rows]
+    row_of, at = [0, 1, 2], [0, 0, 0]
+
+    def step(new):
+        n = cache.begin(new)
+        x = torch.zeros(3, n, 256, dtype=dtype)
+        for s, t in enumerate(new):
+            x[s, n - t:] = rows[row_of[s]][0, at[s]:at[s] + t]
+        with torch.no_grad():
+            y = layer(x.to(dev), past_key_values=cache)
+        for s, t in enumerate(new):
+            r, e = want[row_of[s]][0, at[s]:at[s] + t], y[s, n - t:].float().cpu()
+            assert y[s, n - t:].isfinite().all()
+            assert (e - r).norm() <= _tol(dtype) * r.norm(), f"step {new}, sequence {s}: {(e - r).norm() / r.norm():.2e}"
+            at[s] += t
+        assert y.isfinite().all()
+
+    step([70, 9, 33])
+    for _ in range(3):
+        step([1, 1, 1])
+    step([1, 0, 1])
+    step([0, 20, 1])
+    step([66, 5, 2])
+    at[0] -= 40
+    cache.truncate(0, at[0])
+    step([40, 1, 1])
+    cache.free(1)
+    row_of[1], at[1] = 3, 0
+    step([1, 50, 0])
+    step([1, 1, 1])
+
+
+def test_equal_prompts_into_an_empty_cache(dev):
+    """Where a cache holds nothing else, attention reads the tokens at hand: what it holds afterwards serves the next steps."""
+    for dtype, D in ((BF16, 128), (BF16, 64), (F32, 128)):
+        layer = _layer(dtype, D, dev)
+        x = torch.randn(3, 61, 256, generator=torch.Generator().manual_seed(6)).to(dtype).to(dev)
+        a, b = _cache(dtype, D, dev), _cache(dtype, D, dev)
+        want = _whole(layer, x)
+        with torch.no_grad():
+            a.begin([60, 60, 60])
+            b.begin([60, 60, 60])
+            assert a.fresh and b.fresh
+            b.fresh = False
+            ya, yb = layer(x[:, :60], past_key_values=a), layer(x[:, :60], past_key_values=b)
+            for y in (ya, yb):
+                assert (y.float().cpu() - want[:, :60]).norm() <= _tol(dtype) * want[:, :60].norm()
+            for c in (a, b):
+                c.begin(1)
+                y = layer(x[:, 60:], past_key_values=c)
+                assert (y.float().cpu() - want[:, 60:]).norm() <= _tol(dtype) * want[:, 60:].norm()
+
+
+def test_unpacked_projections_and_a_lone_sequence(dev):
+    from odysseus_transformer_amd.decoder.odysseus import LlamaFlashAttention2TPSP
+    import odysseus_oracle as o
+    for D in (64, 128):
+        torch.manual_seed(4)
+        m = LlamaFlashAttention2TPSP(_config(256, 4, 2, D), 0, pack_weight=False).to(BF16).to(dev).eval()
+        f = lambda t: t.weight.detach().float().cpu()  # noqa: E731
+        x = torch.randn(1, 44, 256).to(BF16)
+        want = o.attention_block(x.float(), torch.cat((f(m.q_proj), f(m.k_proj), f(m.v_proj))), f(m.o_proj), 4, 2, D)[0]
+        cache, at = _cache(BF16, D, dev, max_sequences=1), 0
+        for n in (40, 1, 3):
+            cache.begin([n])
+            with torch.no_grad():
+                y, _, c = m(x[:, at:at + n].to(dev), past_key_value=cache)
+            assert c is cache
+            r = want[:, at:at + n]
+            assert (y.float().cpu() - r).norm() <= _tol(BF16, 8) * r.norm()
+            at += n
+
+
+def test_captured_step_of_a_layer_is_replayed_behind_begin(dev):
+    """A decoding step as a graph: begin() rewrites what it reads.  Three and four sequences: norms in the products' prologues and apart."""
+    for S in (3, 6):
+        layer = _layer(BF16, 128, dev)
+        caches = [_cache(BF16, 128, dev, max_sequences=S, num_pages=80) for _ in range(2)]
+        x = torch.randn(S, 60, 256, generator=torch.Generator().manual_seed(8)).to(BF16).to(dev)
+        first = [20, 3, 31, 1, 8, 16][:S]
+        for c in caches:
+            n = c.begin(first)
+            with torch.no_grad():
+                layer(x[:, :n], past_key_values=c)
+        static = torch.zeros(S, 1, 256, dtype=BF16, device=dev)
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        caches[0].begin(1)
+        with torch.no_grad():
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                layer(static, past_key_values=caches[0])
+            torch.cuda.current_stream().wait_stream(side)
+            with torch.cuda.graph(graph):
+                y = layer(static, past_key_values=caches[0])
+        for s in range(S):
+            caches[0].truncate(s, first[s])                       # the rehearsal's token
+        for t in range(6):
+            new = [1] * S if t != 3 else [1, 0] + [1] * (S - 2)
+            static.copy_(x[:, 40 + t:41 + t])
+            caches[0].begin(new)
+            graph.replay()
+            got = y.clone()
+            caches[1].begin(new)
+            with torch.no_grad():
+                want = layer(static, past_key_values=caches[1])
+            live = torch.tensor(new, device=dev) > 0
+            assert torch.equal(got[live], want[live]), f"step {t}"
+        # a step into an empty cache, captured: not one that a later replay may take for the first
+        cache = _cache(BF16, 128, dev, max_sequences=S, num_pages=80)
+        one, y1 = torch.cuda.CUDAGraph(), None
+        cache.begin([1] * S)
+        assert cache.fresh
+        with torch.no_grad(), torch.cuda.graph(one):
+            y1 = layer(static, past_key_values=cache)
+        for s in range(S):
+            cache.truncate(s, 0)
+            caches[1].free(s)
+        for t in range(3):
+            static.copy_(x[:, t:t + 1])
+            for c in (cache, caches[1]):
+                c.begin([1] * S)
+            one.replay()
+            with torch.no_grad():
+                want = layer(static, past_key_values=caches[1])
+            err = (y1.float() - want.float()).norm() / want.float().norm()
+            assert err <= _tol(BF16, 24), f"step {t}: {err:.2e}"    # the eager one's first step reads the tokens at hand
+
+
+def test_module_refuses_gradients_through_the_cache(dev):
+    layer, cache = _layer(BF16, 64, dev), _cache(BF16, 64, dev)
+    cache.begin([3, 3, 0])
+    x = torch.zeros(3, 3, 256, dtype=BF16, device=dev)
+    with pytest.raises(RuntimeError, match="backward"):
+        layer(x, past_key_values=cache)                           # the weights want gradients
+    with torch.no_grad():
+        layer(x, past_key_values=cache)
+        with pytest.raises(ValueError, match="bfloat16|float32"):
+            layer(x, past_key_values=_begun(_cache(F32, 64, dev)))
+
+
+def _begun(cache):
+    cache.begin([3, 3, 0])
+    return cache
+
+
+@pytest.mark.parametrize("fuse_layers", [False, True], ids=["modules_swapped", "layers_swapped"])
+def test_host_model_decodes_with_a_cache_in_pages(fuse_layers, dev):
+    """A patched host model: prompts of different lengths, then greedy tokens, against the oracle's layers over each sequence alone."""
+    transformers = pytest.importorskip("transformers")
+    import odysseus_oracle as o
+    from odysseus_transformer_amd.decoder.odysseus import apply_odysseus_attn_patch_llama
+    cfg = transformers.LlamaConfig(hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                                   vocab_size=300, max_position_embeddings=512, rms_norm_eps=1e-6)
+    torch.manual_seed(9)
+    model = transformers.LlamaForCausalLM(cfg).float()
+    apply_odysseus_attn_patch_llama(model, fuse_layers=fuse_layers)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.copy_(torch.randn(p.shape) * 0.05 if p.dim() > 1 else 1 + 0.1 * torch.randn(p.shape))
+    model = model.eval().to(dev)
+    sd = {k: v.float().cpu() for k, v in model.state_dict().items()}
+
+    def alone(seq):
+        h = sd["model.embed_tokens.weight"][torch.tensor([seq])]
+        for i in range(2):
+            at = f"model.layers.{i}."
+            h = o.decoder_layer_fwd(h, {name: sd[at + key] for name, key in (
+                ("ln1", "input_layernorm.weight"), ("w_qkv", "self_attn.qkv_proj.weight"), ("w_o", "self_attn.o_proj.weight"),
+                ("ln2", "post_attention_layernorm.weight"), ("w_gate_up", "mlp.gate_up_proj.weight"), ("w_down", "mlp.down_proj.weight"))}, 4, 2, 64)
+        return o.linear_fwd(o.rmsnorm(h, sd["model.norm.weight"]), sd["lm_head.weight"])[0, -1]
+
+    seqs = [torch.randint(0, 300, (n,), generator=torch.Generator().manual_seed(n)).tolist() for n in (40, 13, 27)]
+    cache = _cache(F32, 64, dev, num_layers=2)
+    for t in cache.layer(1):
+        t.fill_(float("nan"))
+    n = cache.begin([len(q) for q in seqs])
+    ids = torch.tensor([[0] * (n - len(q)) + q for q in seqs], device=dev)
+    for _ in range(6):
+        with torch.no_grad():
+            logits = model(ids, past_key_values=cache, use_cache=True).logits[:, -1].cpu()
+        for s, q in enumerate(seqs):
+            want = alone(q)
+            assert (logits[s] - want).norm() <= 2 * _tol(F32) * want.norm(), s    # two layers
+            q.append(int(want.argmax()))
+        cache.begin(1)
+        ids = torch.tensor([q[-1:] for q in seqs], device=dev)
