@@ -42,13 +42,29 @@ struct PagedAttnParams {
 #endif
 };
 
-// The kernel of many rows (paged_attn_chunk.hip): rows of a tile, keys of a step
-constexpr int PAGED_CHUNK_ROWS = 128, PAGED_CHUNK_KEYS = 64;
+// The kernels of many rows (paged_attn_chunk.hip, paged_attn_wide.hip): rows of a tile, keys of a step
+constexpr int PAGED_CHUNK_ROWS = 128, PAGED_WIDE_ROWS = 256, PAGED_CHUNK_KEYS = 64;
 
-// Blocks for so many steps.  A range that ends inside a unit writes 128 rows in fp32 (as many bytes as two steps read) and starts with a latency of five: two
-// blocks a compute unit where they have 16 steps each, else at most one, of 8 at least.  Us with 4 / 8 / 16 steps at least, 32 heads on 8 behind 8192 keys:
-// 32 tokens 31.5 / 26.8 / 34.5 (and 36 with one), 128 tokens 50 / 55 / 46, 512 tokens 100.5 / 98.6 / 99.5.
-__device__ __forceinline__ int paged_chunk_blocks(int steps, int most) { return steps >= 16 * most ? most : steps < 16 ? 1 : steps / 8 < most / 2 ? steps / 8 : most / 2; }
+// What a unit costs the kernels of many rows besides its steps, in steps: the latencies in front of the first products, queries in and results out.  It counts as
+// so many steps at the unit's start, of which nothing comes.  (0 / 2 / 4 / 6 / 8: a prompt of 4096 tokens, 32 heads on 8, 253 / 232 / 204 / 187 / 188 us; 512
+// tokens behind 8192 keys 95 / 95 / 90 / 87 / 88.)
+constexpr int PAGED_EXTRA = 6;
+__host__ __device__ constexpr int paged_extra(int tile) { return tile >= PAGED_CHUNK_ROWS ? PAGED_EXTRA : 0; }
+#ifdef __HIPCC__
+// Ranges that so many steps are cut into, one for a block, of which there are `most`.  With many rows four steps each at least (4 / 6 / 8 / 16, 17 tokens of 32
+// heads on 8 behind 2000 keys: 19.5 / 21.6 / 24.7 / 31 us, behind 8192 25.3 / 26.3 / 27.5 / 36); 128 rows two blocks a compute unit only with 16 steps each
+// (512 tokens behind 8192 keys 96 us, 111 with one block; 17 behind 32768 with two blocks of 8 steps 52, with one 48).  A multiple of the units, where
+// they are few: no range has parts of two of them if they are alike (17 tokens behind 8192 keys 33 -> 28 us).
+__device__ __forceinline__ int paged_blocks(const PagedAttnParams& p, int steps, int most) {
+  int blocks = most;
+  if (p.tile >= PAGED_CHUNK_ROWS && !(p.tile == PAGED_CHUNK_ROWS && steps >= 16 * most))
+    blocks = max(1, min(p.tile == PAGED_CHUNK_ROWS ? most / 2 : most, steps / 4));
+  const int units = p.S * p.row_tiles * p.Hkv;
+  if (4 * units <= blocks) blocks -= blocks % units;
+  return blocks;
+}
+#endif
+int ody_launch_paged_wide(const PagedAttnParams& p, const PagedCache& c, int blocks, hipStream_t st);
 int ody_launch_paged_chunk(const PagedAttnParams& p, int D, const PagedCache& c, int blocks, hipStream_t st);
 
 #ifdef __HIPCC__
@@ -114,7 +130,7 @@ struct PagedWalk {
     if (at + lane < entries) {
       const int e = at + lane, s = p.row_tiles == 1 ? e : e / p.row_tiles;
       length = paged_length(c, s), fresh = paged_fresh(c, s, p.n);
-      mine = max(1, (paged_keys(p, c, length, fresh, e - s * p.row_tiles) - 1) / STEP + 1);
+      mine = max(1, (paged_keys(p, c, length, fresh, e - s * p.row_tiles) - 1) / STEP + 1) + paged_extra(p.tile);
     }
     sums = paged_wave_scan(mine);
   }

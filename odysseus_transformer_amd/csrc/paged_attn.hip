@@ -10,15 +10,20 @@
 // row c of a K operand stands for is chosen so that a lane's scores are those of GK keys in a row, tile + GK q ..: its P is then the B operand for the very
 // keys whose V rows this lane loads.  V rows are loaded GK at a time with 16 lanes on a row; component i of the vectors is row c of operand i, which
 // stands for column c * DV + i of V, so the transposition is bytes exchanged within a lane (bf16) or nothing at all (fp32).
-// With 16 rows of 128 columns a wavefront has two tiles in registers, one under way while the products read the other; with more rows, or half the columns,
-// a tile's K goes out when the products have read that of the one before, and so does its V.  A group of GK keys lies within a page: two table entries a lane and tile.
+// A tile's K goes out when the products have read that of the one before, and so does its V (two tiles in registers, the one under way while the products read
+// the other: the same times to 1 %).  A group of GK keys lies within a page: two table entries a lane and tile.
+//
+// Measured, bf16, heads of 128, results joined: 64 sequences of up to 8192 keys, 32 heads on 8, 199 us (5.4 TB/s of K and V; a copy runs at 5.1, a sum at 6.0 to
+// 6.3); 16 of 4001, 32 heads, 124 us (5.5); one of 131072 100 us (5.4), of 8192 13.6, of 100 5.1, where launches and the chain length, table, keys, join are all.
 #include <algorithm>
 #include <cmath>
 #include "paged.h"
 
 namespace {
 
-constexpr int WAVES = 4, BLOCKS = 512;   // two blocks on each of 256 compute units
+// Two blocks on each of 256 compute units.  256 / 512 / 1024: 64 sequences of up to 8192 keys 218 / 202 / 203 us, one of 8192 13.7 / 14.0 / 14.0, chunks of
+// 512 tokens behind 8192 (paged_attn_chunk.hip) 110 / 106 / 130.
+constexpr int WAVES = 4, BLOCKS = 512;
 
 template <typename T, int D> struct Tile;
 template <int D> struct Tile<bf16, D> {
@@ -104,13 +109,12 @@ template <typename T, int D, int NT, bool STREAM>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAttnParams p, const PagedCache cache) {
   typedef Tile<T, D> G;
   constexpr int STEP = WAVES * G::KEYS, GK = G::GK, OP = D + 4;
-  constexpr bool TWO = NT == 1 && D == 128;   // tiles in registers
   __shared__ __attribute__((aligned(16))) float Os[WAVES][16][OP];
   __shared__ float sm[WAVES][16 * NT], sl[WAVES][16 * NT];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q = lane >> 4;
   PagedWalk<STEP> walk(p, cache, lane);
   const int each = walk.total();   // steps of a kv head
-  const PagedCuts cuts(each * p.Hkv, gridDim.x);
+  const PagedCuts cuts(each * p.Hkv, paged_blocks(p, each * p.Hkv, gridDim.x));
   const int block = paged_range(blockIdx.x, cuts.blocks);
   if (block >= cuts.blocks) return;
   const int begin = cuts.at(block), end = cuts.at(block + 1);
@@ -219,32 +223,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAt
       Loaded x;
       load_k(x, 0, now);
       load_v(x, 0, now);
-      if constexpr (TWO) {
-        Loaded y;
-        auto nothing = [] {};
-        for (int t = 0; t < tiles; t += 2) {
-          if (t + 1 < tiles) {
-            load_k(y, t + 1, next);
-            load_v(y, t + 1, next);
-            next = lookup(t + 2);
-          }
-          compute(x, t, nothing);
-          if (t + 1 >= tiles) break;
-          if (t + 2 < tiles) {
-            load_k(x, t + 2, next);
-            load_v(x, t + 2, next);
-            next = lookup(t + 3);
-          }
-          compute(y, t + 1, nothing);
-        }
-      } else {
-        now = next, next = lookup(2);
-        for (int t = 0; t < tiles; t++) {
-          compute(x, t, [&]() __attribute__((always_inline)) { if (t + 1 < tiles) load_k(x, t + 1, now); });
-          if (t + 1 < tiles) {
-            load_v(x, t + 1, now);
-            now = next, next = lookup(t + 3);
-          }
+      now = next, next = lookup(2);
+      for (int t = 0; t < tiles; t++) {
+        compute(x, t, [&]() __attribute__((always_inline)) { if (t + 1 < tiles) load_k(x, t + 1, now); });
+        if (t + 1 < tiles) {
+          load_v(x, t + 1, now);
+          now = next, next = lookup(t + 3);
         }
       }
     }
@@ -307,29 +291,42 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAt
 }
 
 // The parts of the units that a cut goes through, weighted by their sums.  A block takes R rows of a row tile (a divisor of it), with D / 4 threads on a
-// row: all of the threads share a row's parts, in turn for each row, or where the parts are few every group of threads has a row.
-constexpr int JOIN_ROWS = 8, JOIN_FEW = 16;
-template <typename T, int D, int STEP, int R>
+// row: groups of them share the parts of a lone row, of several each has its own.  (512 tokens behind 8192 keys, four or five parts a row: 106 us in all with 8
+// rows a block, 131 with one; 17 tokens behind 16000 keys, more than 16 parts: 31 us, 36 with the parts of 8 rows shared in turn.)
+// BY_CUTS: a row tile for each cut, which is the first one through its unit or does nothing, and not one for each unit, of which there are more (2048 units of 256
+// rows and 128 keys: 272 -> 161 us).
+constexpr int JOIN_ROWS = 8;
+template <typename T, int D, int STEP, int R, bool BY_CUTS>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p, const PagedCache cache, int most_blocks) {
   constexpr int C4 = D / 4, GROUPS = 256 / C4, U = 4;
   __shared__ f32x4 red[GROUPS][C4];
   __shared__ float2 red_ml[GROUPS];
   const int tid = threadIdx.x, lane = tid & 63;
-  // blockIdx.x: (sequence, R rows of all rows of a kv head, kv head)
-  const int all_rows = p.n * p.group, row_blocks = (all_rows + R - 1) / R;
-  const int hk = blockIdx.x % p.Hkv, row0 = blockIdx.x / p.Hkv % row_blocks * R, s = blockIdx.x / p.Hkv / row_blocks;
-  const int rt = row0 / p.tile, entry = s * p.row_tiles + rt;
+  const int all_rows = p.n * p.group, extra = paged_extra(p.tile);
   PagedWalk<STEP> walk(p, cache, lane);
-  int before = 0, steps = 0;
-  do {
-    if (entry >= walk.at && entry < walk.at + 64) {
-      steps = __builtin_amdgcn_readlane(walk.mine, entry - walk.at);
-      before = walk.before + __builtin_amdgcn_readlane(walk.sums, entry - walk.at) - steps;
-    }
-  } while (walk.next());
-  const int all_steps = (walk.before + walk.all()) * p.Hkv;
-  const PagedCuts cuts(all_steps, p.tile == PAGED_CHUNK_ROWS ? paged_chunk_blocks(all_steps, most_blocks) : most_blocks);
-  const int first = hk * (walk.before + walk.all()) + before, b0 = cuts.range_of(first), b1 = cuts.range_of(first + steps - 1), parts = b1 - b0 + 1;
+  const int each = walk.total();
+  const PagedCuts cuts(each * p.Hkv, paged_blocks(p, each * p.Hkv, most_blocks));
+  int hk, s, rt, row0, first, steps, b0;   // the unit's place; the block's first row, of all rows of the kv head; the unit's first step, how many; the range that begins with its keys
+  if (BY_CUTS) {   // blockIdx.x: (cut, R rows of a row tile)
+    const int row_blocks = (min(p.tile, all_rows) + R - 1) / R, cut = 1 + blockIdx.x / row_blocks;
+    if (cut >= cuts.blocks) return;
+    PagedPlace<STEP> at(walk, cuts.at(cut), each);
+    hk = at.hk, s = at.s, rt = at.rt, steps = at.steps, first = cuts.at(cut) - at.step, b0 = cut - 1;
+    row0 = rt * p.tile + blockIdx.x % row_blocks * R;
+    // between two units, or not between steps; not the first cut through this unit; rows that are none
+    if (at.step <= extra || cuts.at(b0) > first + extra || row0 >= all_rows) return;
+  } else {         // (sequence, R rows of a kv head, kv head)
+    const int row_blocks = (all_rows + R - 1) / R;
+    hk = blockIdx.x % p.Hkv, row0 = blockIdx.x / p.Hkv % row_blocks * R, s = blockIdx.x / p.Hkv / row_blocks;
+    rt = row0 / p.tile;
+    const int entry = s * p.row_tiles + rt;
+    walk.rewind();
+    while (entry >= walk.at + 64) walk.next();
+    steps = __builtin_amdgcn_readlane(walk.mine, entry - walk.at);
+    first = hk * each + walk.before + __builtin_amdgcn_readlane(walk.sums, entry - walk.at) - steps;
+    b0 = cuts.range_of(first + extra);
+  }
+  const int b1 = cuts.range_of(first + steps - 1), parts = b1 - b0 + 1;
   if (parts == 1) return;
   // part k is in slot 2 (b0 + k), but for the first where that block's range begins with another unit
   const int first_slot = 2 * b0 + (first > cuts.at(b0));
@@ -371,49 +368,53 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   };
   float m, l;
   f32x4 acc;
-  if (R > 1 && parts <= JOIN_FEW) {
+  if (R > 1) {
     for (int row = row0 + g; row < min(row0 + R, all_rows); row += GROUPS) {
       sum(row, 0, 1, m, l, acc);
       write(row, m, l, acc);
     }
     return;
   }
-  for (int row = row0; row < min(row0 + R, all_rows); row++) {
-    sum(row, g, GROUPS, m, l, acc);
-    red[g][d4] = acc;
-    if (d4 == 0) red_ml[g] = make_float2(m, l);
-    __syncthreads();
-    if (g == 0) {
-      m = -INFINITY, l = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  sum(row0, g, GROUPS, m, l, acc);
+  red[g][d4] = acc;
+  if (d4 == 0) red_ml[g] = make_float2(m, l);
+  __syncthreads();
+  if (g == 0) {
+    m = -INFINITY, l = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < GROUPS; k++) m = fmaxf(m, red_ml[k].x);
-      const float ref = m == -INFINITY ? 0.f : m;
+    for (int k = 0; k < GROUPS; k++) m = fmaxf(m, red_ml[k].x);
+    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int k = 0; k < GROUPS; k++) {
-        const float w = ody_exp2(red_ml[k].x - ref);
-        l += red_ml[k].y * w, acc += red[k][d4] * w;
-      }
-      write(row, m, l, acc);
+    for (int k = 0; k < GROUPS; k++) {
+      const float w = ody_exp2(red_ml[k].x - ref);
+      l += red_ml[k].y * w, acc += red[k][d4] * w;
     }
-    if (R > 1) __syncthreads();
+    write(row0, m, l, acc);
   }
 }
 
-// Row tiles of 16 or 32 here, more rows in bf16 by the kernel of many rows.
+// Row tiles of 16 or 32 here; more than 64 rows in bf16 by the kernels of many rows.  32 tokens of 4 heads a kv head behind 131072 keys: 206 us in tiles of 32, 145
+// by paged_attn_chunk.hip; at 17 to 64 tokens behind 8192 both take 25 to 30.  Tiles of 64 here would not fit the registers.
+// paged_attn_wide.hip for heads of 128 where 64 units and more keep its 256 blocks busy (2000 keys, 32 heads on 8: 128 tokens 34 us, 28 in tiles of 128, 512 tokens
+// 44 and 46; 2048 tokens behind 8192 keys 312 and 354), pages hold a tile of keys, so that its address is one, and its tiles cover at most an eighth more rows than
+// tiles of 128 would (257 rows of each of 32 heads behind 8192 keys: 91 us in two of 256, 78 in three).
 struct Plan {
   int tile, row_tiles, step, blocks;
   bool joined;          // a cut may go through a unit
   bool fits;            // the steps can be counted
   size_t part_bytes, ml_bytes;
 };
-Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype) {
+Plan plan(int S, int n, int group, int Hkv, int D, int page_size, int width, int dtype) {
+  const int64_t most_keys = (int64_t)page_size * width;
   const int64_t rows = (int64_t)n * group;
   const bool chunk = rows > 64 && dtype == ODY_BF16;
-  const int tile = rows <= 16 ? 16 : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);
+  const int64_t wide_tiles = (rows + PAGED_WIDE_ROWS - 1) / PAGED_WIDE_ROWS, chunk_tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
+  const bool wide = chunk && D == 128 && page_size >= PAGED_CHUNK_KEYS && (double)S * wide_tiles * Hkv >= 64 && 14 * wide_tiles <= 8 * chunk_tiles;
+  const int tile = rows <= 16 ? 16 : wide ? PAGED_WIDE_ROWS : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);
   const int step = chunk ? PAGED_CHUNK_KEYS : WAVES * (dtype == ODY_BF16 ? 32 : 16);
   const int64_t steps = std::max((int64_t)1, (most_keys + step - 1) / step);   // of a unit, at most
-  const double all = (double)S * row_tiles * Hkv * steps;
-  const int blocks = (int)std::min((double)BLOCKS, std::ceil(all / 8) * 8);   // a multiple of 8: paged_range
+  const double all = (double)S * row_tiles * Hkv * (steps + paged_extra(tile));
+  const int blocks = (int)std::min((double)(wide ? BLOCKS / 2 : BLOCKS), std::ceil(all / 8) * 8);   // a multiple of 8: paged_range
   const bool joined = steps > 1;
   const size_t parts = joined ? (size_t)blocks * 2 * tile : 0;
   return Plan{tile, row_tiles, step, blocks, joined, all < 2147483648.0, parts * D * sizeof(float), parts * sizeof(float2)};
@@ -422,8 +423,12 @@ Plan plan(int S, int n, int group, int Hkv, int D, int64_t most_keys, int dtype)
 template <typename T, int D, int STEP, int R>
 int join(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
   if (!pl.joined) return ODY_OK;
-  const int row_blocks = (p.n * p.group + R - 1) / R;
-  ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, R>), dim3((unsigned)(p.S * row_blocks * p.Hkv)), dim3(256), 0, p, c, pl.blocks);
+  const int64_t rows = (int64_t)p.n * p.group, units = (int64_t)p.S * p.row_tiles * p.Hkv;
+  if (units >= pl.blocks)
+    ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, R, true>), dim3((unsigned)((pl.blocks - 1) * ((std::min(rows, (int64_t)pl.tile) + R - 1) / R))),
+               dim3(256), 0, p, c, pl.blocks);
+  else
+    ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, R, false>), dim3((unsigned)(p.S * ((rows + R - 1) / R) * p.Hkv)), dim3(256), 0, p, c, pl.blocks);
   return ody_check_launch("paged_join");
 }
 template <typename T, int D, int NT>
@@ -436,8 +441,8 @@ int launch(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStr
 }
 template <typename T, int D>
 int by_rows(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
-  if (pl.tile == PAGED_CHUNK_ROWS) {
-    const int rc = ody_launch_paged_chunk(p, D, c, pl.blocks, st);
+  if (pl.tile >= PAGED_CHUNK_ROWS) {
+    const int rc = pl.tile == PAGED_WIDE_ROWS ? ody_launch_paged_wide(p, c, pl.blocks, st) : ody_launch_paged_chunk(p, D, c, pl.blocks, st);
     return rc ? rc : join<bf16, D, PAGED_CHUNK_KEYS, JOIN_ROWS>(p, c, pl, st);
   }
   return pl.tile == 16 ? launch<T, D, 1>(p, c, pl, st) : launch<T, D, 2>(p, c, pl, st);
@@ -451,7 +456,7 @@ int by_head_dim(const PagedAttnParams& p, int D, const PagedCache& c, const Plan
 
 extern "C" size_t ody_paged_attn_workspace_bytes(int S, int n, int Hq, int Hkv, int D, int page_size, int table_width, int dtype) {
   if (S <= 0 || n <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || page_size <= 0 || table_width <= 0) return 0;   // the call refuses these
-  const Plan pl = plan(S, n, Hq / Hkv, Hkv, D, (int64_t)page_size * table_width, dtype);
+  const Plan pl = plan(S, n, Hq / Hkv, Hkv, D, page_size, table_width, dtype);
   return pl.part_bytes + pl.ml_bytes;
 }
 
@@ -466,7 +471,7 @@ extern "C" int ody_paged_attn(const void* q, const void* k_pages, const void* v_
   ODY_REQUIRE(q && out && lse, ODY_ERR_NULL, "ody_paged_attn: q, out or lse is NULL");
   ODY_REQUIRE(paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype) && paged_rows_aligned(out, so_s, so_n, so_h, dtype), ODY_ERR_MISALIGNED,
               "ody_paged_attn: q and out need 16-byte aligned pointers and strides");
-  const Plan pl = plan(S, n, Hq / Hkv, Hkv, D, (int64_t)page_size * table_width, dtype);
+  const Plan pl = plan(S, n, Hq / Hkv, Hkv, D, page_size, table_width, dtype);
   ODY_REQUIRE(pl.fits, ODY_ERR_BAD_SHAPE, "ody_paged_attn: 2^31 tiles of keys and more, by the table's width");
   ODY_REQUIRE(pl.part_bytes == 0 || (workspace && workspace_bytes >= pl.part_bytes + pl.ml_bytes && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
               ODY_ERR_WORKSPACE, "ody_paged_attn: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", pl.part_bytes + pl.ml_bytes,

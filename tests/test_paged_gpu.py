@@ -196,6 +196,67 @@ def test_chunks_of_few_tiles(D, lengths, dev):
         _check_attn(c, _to(c, dev))
 
 
+@pytest.mark.parametrize("lengths", [[64], [65, 1], [128, 63], [192, 191], [256, 255], [321, 448, 64], [383], [577, 900], [1500]], ids=str)
+def test_long_chunks_of_few_tiles(lengths, dev):
+    """Pages of a tile of keys and more, tokens of one and of several tiles of 256 rows."""
+    for n, Hq, page in ((129, 1, 64), (256, 2, 128), (70, 4, 64)):
+        c = ref.make(lengths, n, Hq, 1, 128, page, BF16, seed=sum(lengths) + n)
+        _check_attn(c, _to(c, dev))
+
+
+@pytest.mark.parametrize("column", [0, 1, 4, 5, 8, 9, 10, 11])
+def test_long_chunks_with_a_page_missing(column, dev):
+    for new in (None, 150):
+        c = ref.make([760, 90], 200, 4, 2, 128, 64, BF16, seed=column)
+        c["table"][0, column] = 2 ** 31 - 1 if column % 2 else -1
+        c["new"] = None if new is None else torch.tensor([new, 80], dtype=torch.int32)
+        _check_attn(c, _to(c, dev))
+
+
+def test_long_chunks_whose_scores_grow(dev):
+    """The largest score of a row in every one of its tiles above those before it, by more and by less than a reference may lag behind."""
+    for step in (0.5, 3.0, 40.0):
+        c = ref.make([700], 140, 2, 1, 128, 64, BF16, seed=2)
+        q = c["q"][0, 0, 0].float()
+        for j in range(700):
+            at = ref.page_of(c, 0, j)
+            c["k"][at[0], at[1], 0] = (q * (step * (j // 32) / 20 * 11.3 / (q @ q).item() + 0.02 * torch.randn(128, generator=torch.Generator().manual_seed(j)))).to(BF16)
+        c["q"][0, :, :] = q.to(BF16) * torch.linspace(-1, 1, 280).reshape(140, 2, 1).to(BF16)
+        _check_attn(c, _to(c, dev))
+
+
+def _sampled(c, g, rows, dev):
+    """_check_attn for some rows (s, i, h) of a call that is too large for all of them."""
+    from odysseus_transformer_amd import ops
+    out, lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"])
+    out, lse = out.double().cpu(), lse.double().cpu()
+    n, Hq, Hkv, page = c["q"].shape[1], c["q"].shape[2], c["k"].shape[2], c["page"]
+    for s, i, h in rows:
+        places = torch.arange(int(c["lengths"][s]) - n + i + 1)
+        at = c["table"][s, places // page].long(), places % page
+        one = dict(c, q=c["q"][s:s + 1, i:i + 1, h:h + 1], lengths=torch.tensor([len(places)]))
+        K, V = c["k"][at[0], at[1], h * Hkv // Hq].double(), c["v"][at[0], at[1], h * Hkv // Hq].double()
+        q = one["q"][0, 0, 0].double()
+        x = K @ q / math.sqrt(len(q))
+        p = torch.softmax(x, 0)
+        o, m, z = (p @ V)[None, None, None], (p @ V.abs())[None, None, None], torch.logsumexp(x, 0)[None, None, None]
+        tol_o, tol_s = ref.attend_bounds(one, o, z, m, ((K.abs() @ q.abs()).max() / math.sqrt(len(q)))[None, None, None])
+        assert ((out[s, i, h] - o[0, 0, 0]).abs() <= tol_o[0, 0, 0]).all(), (s, i, h)
+        assert (lse[s, h, i] - z[0, 0, 0]).abs() <= tol_s[0, 0, 0], (s, i, h)
+
+
+@pytest.mark.parametrize("case", [([33000], 512, 32, 8, 64), ([33000], 512, 32, 8, 16), ([9000, 17000, 300], 300, 16, 8, 128),
+                                  ([64 + 9 * i for i in range(70)], 64, 32, 8, 64), ([64 + 9 * i for i in range(70)], 64, 32, 8, 16),
+                                  ([900 - 5 * i for i in range(170)], 1, 16, 4, 16)], ids=lambda c: "S%d_max%d_n%d_H%d_%d_p%d" % (len(c[0]), max(c[0]), *c[1:]))
+def test_many_keys_and_many_sequences(case, dev):
+    """More tiles for a block than pages are looked up at once; more units than blocks, each cut at most once."""
+    lengths, n, Hq, Hkv, page = case
+    c = ref.make(lengths, n, Hq, Hkv, 128, page, BF16, seed=n)
+    g = torch.Generator().manual_seed(1)
+    rows = [(int(torch.randint(len(lengths), (1,), generator=g)), int(torch.randint(n, (1,), generator=g)), int(torch.randint(Hq, (1,), generator=g))) for _ in range(30)]
+    _sampled(c, _to(c, dev), rows + [(0, 0, 0), (0, n - 1, Hq - 1)], dev)
+
+
 @pytest.mark.parametrize("rows", [33, 47, 48, 49, 64, 65])
 def test_rows_around_the_tiles(rows, dev):
     c = ref.make([500, 90, 33], rows, 2, 2, 128, 16, BF16, seed=rows)
