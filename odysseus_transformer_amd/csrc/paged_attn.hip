@@ -290,31 +290,31 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAt
   }
 }
 
-// The parts of the units that a cut goes through, weighted by their sums.  A block takes R rows of a row tile (a divisor of it), with D / 4 threads on a
-// row: groups of them share the parts of a lone row, of several each has its own.  (512 tokens behind 8192 keys, four or five parts a row: 106 us in all with 8
-// rows a block, 131 with one; 17 tokens behind 16000 keys, more than 16 parts: 31 us, 36 with the parts of 8 rows shared in turn.)
-// BY_CUTS: a row tile for each cut, which is the first one through its unit or does nothing, and not one for each unit, of which there are more (2048 units of 256
-// rows and 128 keys: 272 -> 161 us).
+// The parts of the units that a cut goes through, weighted by their sums, with D / 4 threads on a row: the parts of a lone row are read by all threads of a block, of
+// several each is a group's of them.
+// BY_CUTS, where those are fewer blocks: a block takes JOIN_ROWS rows of a row tile (which are a divisor of it) at a cut, and the cuts through a unit
+// share its rows.  Else it takes R rows of a unit.  (8 tokens of 256 sequences of up to 1000 keys, 32 heads on 8: 158 us in all, 191 with a block for each row of
+// each unit; 512 tokens of one behind 8192 keys by cuts 103, by units 91, 131 with R = 1; 17 behind 16000, more than 16 parts, 31, 36 with all threads on the
+// rows in turn.)
 constexpr int JOIN_ROWS = 8;
 template <typename T, int D, int STEP, int R, bool BY_CUTS>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p, const PagedCache cache, int most_blocks) {
   constexpr int C4 = D / 4, GROUPS = 256 / C4, U = 4;
+  static_assert(GROUPS >= R, "a group of threads for each of a block's rows");
   __shared__ f32x4 red[GROUPS][C4];
   __shared__ float2 red_ml[GROUPS];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int all_rows = p.n * p.group, extra = paged_extra(p.tile);
+  const int tid = threadIdx.x, lane = tid & 63, all_rows = p.n * p.group, extra = paged_extra(p.tile);
   PagedWalk<STEP> walk(p, cache, lane);
   const int each = walk.total();
   const PagedCuts cuts(each * p.Hkv, paged_blocks(p, each * p.Hkv, most_blocks));
-  int hk, s, rt, row0, first, steps, b0;   // the unit's place; the block's first row, of all rows of the kv head; the unit's first step, how many; the range that begins with its keys
+  // the unit's place, its first step, how many it has; the block's rows are row0 + mine, row0 + mine + through .. of the kv head's, R of them for through = 1
+  int hk, s, rt, row0, first, steps, mine = 0, through = 1;
   if (BY_CUTS) {   // blockIdx.x: (cut, R rows of a row tile)
     const int row_blocks = (min(p.tile, all_rows) + R - 1) / R, cut = 1 + blockIdx.x / row_blocks;
     if (cut >= cuts.blocks) return;
-    PagedPlace<STEP> at(walk, cuts.at(cut), each);
-    hk = at.hk, s = at.s, rt = at.rt, steps = at.steps, first = cuts.at(cut) - at.step, b0 = cut - 1;
-    row0 = rt * p.tile + blockIdx.x % row_blocks * R;
-    // between two units, or not between steps; not the first cut through this unit; rows that are none
-    if (at.step <= extra || cuts.at(b0) > first + extra || row0 >= all_rows) return;
+    const PagedPlace<STEP> at(walk, cuts.at(cut), each);
+    if (at.step <= extra) return;   // between two units, or in what one costs besides its steps
+    hk = at.hk, s = at.s, rt = at.rt, steps = at.steps, first = cuts.at(cut) - at.step, row0 = rt * p.tile + blockIdx.x % row_blocks * R, mine = cut;
   } else {         // (sequence, R rows of a kv head, kv head)
     const int row_blocks = (all_rows + R - 1) / R;
     hk = blockIdx.x % p.Hkv, row0 = blockIdx.x / p.Hkv % row_blocks * R, s = blockIdx.x / p.Hkv / row_blocks;
@@ -324,10 +324,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     while (entry >= walk.at + 64) walk.next();
     steps = __builtin_amdgcn_readlane(walk.mine, entry - walk.at);
     first = hk * each + walk.before + __builtin_amdgcn_readlane(walk.sums, entry - walk.at) - steps;
-    b0 = cuts.range_of(first + extra);
   }
-  const int b1 = cuts.range_of(first + steps - 1), parts = b1 - b0 + 1;
+  const int b0 = cuts.range_of(first + extra), b1 = cuts.range_of(first + steps - 1), parts = b1 - b0 + 1;   // ranges with keys of the unit
   if (parts == 1) return;
+  if (BY_CUTS) mine -= b0 + 1, through = parts - 1;
   // part k is in slot 2 (b0 + k), but for the first where that block's range begins with another unit
   const int first_slot = 2 * b0 + (first > cuts.at(b0));
   const int d4 = tid % C4, g = tid / C4;
@@ -368,14 +368,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   };
   float m, l;
   f32x4 acc;
-  if (R > 1) {
-    for (int row = row0 + g; row < min(row0 + R, all_rows); row += GROUPS) {
+  if (through < R) {
+    const int row = row0 + mine + through * g;
+    if (mine + through * g < R && row < all_rows) {
       sum(row, 0, 1, m, l, acc);
       write(row, m, l, acc);
     }
     return;
   }
-  sum(row0, g, GROUPS, m, l, acc);
+  const int row = row0 + mine;
+  if (mine >= R || row >= all_rows) return;
+  sum(row, g, GROUPS, m, l, acc);
   red[g][d4] = acc;
   if (d4 == 0) red_ml[g] = make_float2(m, l);
   __syncthreads();
@@ -389,7 +392,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
       const float w = ody_exp2(red_ml[k].x - ref);
       l += red_ml[k].y * w, acc += red[k][d4] * w;
     }
-    write(row0, m, l, acc);
+    write(row, m, l, acc);
   }
 }
 
@@ -423,12 +426,10 @@ Plan plan(int S, int n, int group, int Hkv, int D, int page_size, int width, int
 template <typename T, int D, int STEP, int R>
 int join(const PagedAttnParams& p, const PagedCache& c, const Plan& pl, hipStream_t st) {
   if (!pl.joined) return ODY_OK;
-  const int64_t rows = (int64_t)p.n * p.group, units = (int64_t)p.S * p.row_tiles * p.Hkv;
-  if (units >= pl.blocks)
-    ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, R, true>), dim3((unsigned)((pl.blocks - 1) * ((std::min(rows, (int64_t)pl.tile) + R - 1) / R))),
-               dim3(256), 0, p, c, pl.blocks);
-  else
-    ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, R, false>), dim3((unsigned)(p.S * ((rows + R - 1) / R) * p.Hkv)), dim3(256), 0, p, c, pl.blocks);
+  const int64_t rows = (int64_t)p.n * p.group, by_units = p.S * ((rows + R - 1) / R) * p.Hkv,
+                by_cuts = (pl.blocks - 1) * ((std::min(rows, (int64_t)pl.tile) + JOIN_ROWS - 1) / JOIN_ROWS);
+  if (by_cuts < by_units) ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, JOIN_ROWS, true>), dim3((unsigned)by_cuts), dim3(256), 0, p, c, pl.blocks);
+  else ODY_LAUNCH("paged_join", st, (paged_join_kernel<T, D, STEP, R, false>), dim3((unsigned)by_units), dim3(256), 0, p, c, pl.blocks);
   return ody_check_launch("paged_join");
 }
 template <typename T, int D, int NT>
