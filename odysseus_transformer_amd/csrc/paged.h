@@ -118,20 +118,22 @@ struct PagedCuts {
 };
 
 // A walk over the (sequence, row tile) pairs by a wavefront, a chunk of 64 of them at a time: a lane has the length of its pair's sequence, the pair's
-// steps and the sum of steps so far.
+// steps and the sum of steps so far.  Where there are more pairs, total() first sums up 64 equal shares of them, a lane each, whose loads do not wait for one another,
+// and find() starts with the share that a step is in (1024 sequences of 100 keys, 8 kv heads: 112 -> 106 us).
 template <int STEP>
 struct PagedWalk {
   const PagedAttnParams& p;
   const PagedCache& c;
   int lane, entries, at = 0, before = 0, length = 0, fresh = 0, mine = 0, sums = 0;   // sums: inclusive, of this chunk
+  int share = 1, share_mine = 0, share_sums = 0;
   __device__ __forceinline__ PagedWalk(const PagedAttnParams& p_, const PagedCache& c_, int lane_) : p(p_), c(c_), lane(lane_), entries(p_.S * p_.row_tiles) { chunk(); }
+  __device__ __forceinline__ int steps_of(int e, int& len, int& new_) const {
+    const int s = p.row_tiles == 1 ? e : e / p.row_tiles;
+    len = paged_length(c, s), new_ = paged_fresh(c, s, p.n);
+    return max(1, (paged_keys(p, c, len, new_, e - s * p.row_tiles) - 1) / STEP + 1) + paged_extra(p.tile);
+  }
   __device__ __forceinline__ void chunk() {
-    mine = 0;
-    if (at + lane < entries) {
-      const int e = at + lane, s = p.row_tiles == 1 ? e : e / p.row_tiles;
-      length = paged_length(c, s), fresh = paged_fresh(c, s, p.n);
-      mine = max(1, (paged_keys(p, c, length, fresh, e - s * p.row_tiles) - 1) / STEP + 1) + paged_extra(p.tile);
-    }
+    mine = at + lane < entries ? steps_of(at + lane, length, fresh) : 0;
     sums = paged_wave_scan(mine);
   }
   __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(sums, 63); }
@@ -141,9 +143,30 @@ struct PagedWalk {
     chunk();
     return true;
   }
-  __device__ __forceinline__ int total() {   // of one kv head; ends on the last chunk
-    while (next()) {}
-    return before + all();
+  __device__ __forceinline__ int total() {   // of one kv head
+    if (entries <= 64) return all();
+    share = (entries + 63) / 64;
+    const int end = min(entries, (lane + 1) * share);
+#pragma unroll 8
+    for (int e = lane * share; e < end; e++) {
+      int len, new_;
+      share_mine += steps_of(e, len, new_);
+    }
+    share_sums = paged_wave_scan(share_mine);
+    return __builtin_amdgcn_readlane(share_sums, 63);
+  }
+  __device__ __forceinline__ void start(int k) {   // with share k
+    at = k * share, before = __builtin_amdgcn_readlane(share_sums, k) - __builtin_amdgcn_readlane(share_mine, k);
+    chunk();
+  }
+  // behind total(): the chunk that step `pos` is in, or pair `entry`
+  __device__ __forceinline__ void find(int pos) {
+    if (entries > 64) start(__popcll(__ballot(share_sums <= pos)));
+    while (before + all() <= pos && next()) {}
+  }
+  __device__ __forceinline__ void find_entry(int entry) {
+    if (entries > 64) start(entry / share);
+    while (entry >= at + 64) next();
   }
   __device__ __forceinline__ void rewind() {
     if (at == 0) return;
@@ -160,8 +183,7 @@ struct PagedPlace {
   __device__ __forceinline__ PagedPlace(PagedWalk<STEP>& w, int pos, int each) {
     hk = (int)((unsigned)pos / (unsigned)each);
     pos -= hk * each;
-    w.rewind();
-    while (w.before + w.all() <= pos && w.next()) {}
+    w.find(pos);
     entry = w.at + __popcll(__ballot(w.before + w.sums <= pos));
     take(w);
     step = pos - (w.before + __builtin_amdgcn_readlane(w.sums, entry - w.at) - steps);

@@ -320,8 +320,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
     hk = blockIdx.x % p.Hkv, row0 = blockIdx.x / p.Hkv % row_blocks * R, s = blockIdx.x / p.Hkv / row_blocks;
     rt = row0 / p.tile;
     const int entry = s * p.row_tiles + rt;
-    walk.rewind();
-    while (entry >= walk.at + 64) walk.next();
+    walk.find_entry(entry);
     steps = __builtin_amdgcn_readlane(walk.mine, entry - walk.at);
     first = hk * each + walk.before + __builtin_amdgcn_readlane(walk.sums, entry - walk.at) - steps;
   }
