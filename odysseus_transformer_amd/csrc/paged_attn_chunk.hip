@@ -38,6 +38,9 @@ __device__ const bf16x8 no_key[16] = {};   // the row that a key without a page,
 __device__ __forceinline__ void direct_load(const char* from, unsigned to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
+__device__ __forceinline__ void direct_load(const char* from, unsigned of_lane, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(of_lane), "s"(from) : "memory");
+}
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -96,12 +99,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
       const int first = key0 + KEYS * t + PER * wave + STEP * j, in_page = (1 << cache.shift) - 1;
       const int at = (STEP * j + PER * wave) / 8, page = __builtin_amdgcn_readlane(pages, at);
       const char* row = base + (uint64_t)(unsigned)page * of_page + (unsigned)(first & in_page) * of_row;
-      const char* src = row + of_lane;
-      if constexpr (!decltype(plain)::value) {
+      const unsigned to = place + (WAVES * j + wave) * 1024;
+      if constexpr (decltype(plain)::value) {
+        direct_load(row, of_lane, to);
+      } else {
         const bool none = first + lane / LANES >= keys || (have >> at & 1) == 0;
-        src = none ? reinterpret_cast<const char*>(no_key) + 2 * lcol : src;
+        unsigned l = of_lane;
+        asm volatile("" : "+v"(l));   // 64 bits of it here, and not from turn to turn: the loops have no register to spare
+        direct_load(none ? reinterpret_cast<const char*>(no_key) + 2 * lcol : row + l, to);
       }
-      direct_load(src, place + (WAVES * j + wave) * 1024);
     };
     auto load_k = [&](auto plain, int j, int t, int pages, unsigned have) __attribute__((always_inline)) { load(plain, j, t, pages, have, kp, cache.k_page, cache.k_row, lk, places + (t & 1) * 2 * TILE); };
     auto load_v = [&](auto plain, int j, int t, int pages, unsigned have) __attribute__((always_inline)) { load(plain, j, t, pages, have, vp, cache.v_page, cache.v_row, lv, places + (2 + (t & 1)) * 2 * TILE); };
