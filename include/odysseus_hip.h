@@ -411,7 +411,9 @@ int ody_attn_bwd_dropout(const void* q, const void* k, const void* v, const void
  * ody_paged_attn    out (S, n, Hq, D) and lse (S, Hq, n), contiguous fp32, of q (S, n, Hq, D): token i sees the places up to its own that have a
  *                   page, as ody_attn_fwd's causal mask with Lk = lengths has it; 0 and -inf where that is none.  Query head h reads kv head
  *                   h / (Hq / Hkv).  workspace: ody_paged_attn_workspace_bytes(...) bytes, 256-byte aligned, of no value before or after.
- * D in {64, 128}; bf16 and fp32; pointers and strides of qkv, q, out and the pages on 16 bytes.
+ * D in {64, 128}; bf16 and fp32; pointers and strides of qkv, q, out and the pages on 16 bytes; pages, and the rows of a page, less than 4 GiB apart
+ * (ODY_ERR_UNSUPPORTED).  Values that a row does not see count as 0 times themselves where another row of its tile sees them: a NaN of a later new token may
+ * reach an earlier one's row.  What no token owns is never read into a result.
  */
 int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v_pages, const int* page_table, const int* lengths,
                      const int* new_tokens, const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,

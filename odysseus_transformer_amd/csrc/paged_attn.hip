@@ -10,6 +10,7 @@
 // row c of a K operand stands for is chosen so that a lane's scores are those of GK keys in a row, tile + GK q ..: its P is then the B operand for the very
 // keys whose V rows this lane loads.  V rows are loaded GK at a time with 16 lanes on a row; component i of the vectors is row c of operand i, which
 // stands for column c * DV + i of V, so the transposition is bytes exchanged within a lane (bf16) or nothing at all (fp32).
+// In bf16 P is rounded for its product, as V is stored, and summed up in fp32 unrounded, as in the attention over contiguous keys: half a step of each weight.
 // A tile's K goes out when the products have read that of the one before, and so does its V (two tiles in registers, the one under way while the products read
 // the other: the same times to 1 %).  A group of GK keys lies within a page: two table entries a lane and tile.
 //

@@ -1,8 +1,8 @@
 // Attention of long chunks over a key / value cache in pages, bf16, heads of 128: row tiles of 256, of which paged_attn_chunk.hip takes 128.
 //
 // The same two products, transposed, over the same tiles of 64 keys as there.  Here one block has a compute unit and a wavefront a SIMD with all of its registers:
-// 64 rows each, as two halves that share every fragment read from LDS, whose reads limit the kernel of 128 rows (a transposing read has half the rate of
-// others).  A turn of the loop forms O^T of tile t and S^T of tile t + 1 in four phases of 16 products, and under each product one element of P, of the half
+// 64 rows each, as two halves that share every fragment read from LDS and every scalar instruction, of which the kernel of 128 rows has twice as many.  A
+// turn of the loop forms O^T of tile t and S^T of tile t + 1 in four phases of 16 products, and under each product one element of P, of the half
 // tile whose scores are complete and whose turn as an operand is next:
 //
 //      S^T(t + 1), first 32 keys      P(t), second 32 keys, rows 0 .. 31

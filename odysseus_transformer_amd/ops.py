@@ -530,7 +530,7 @@ def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, posi
 def paged_attn(q, k_pages, v_pages, page_table, lengths, scale: Optional[float] = None, new_tokens=None):
     """Attention of the n newest tokens of every sequence, q (S, n, Hq, D), over a cache in pages that holds them already (paged_append_, which
     says what the arguments are): a token sees the places up to its own.  -> out (S, n, Hq, D), lse (S, Hq, n) fp32, 0 and -inf for a
-    token that sees none."""
+    token that sees none.  (A NaN or infinite value of a later new token may reach the rows of earlier ones of its sequence.)"""
     if q.is_cuda:
         plain = native.paged_attn(q, k_pages, v_pages, page_table, lengths, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale,
                                   new_tokens)
