@@ -13,7 +13,8 @@ take it as their `past_key_value(s)`:
         y = layer(x1, past_key_values=cache)      # x1 (8, 1, hidden)
 
 `page_table`, `lengths`, `new_tokens` and `position_ids` are device tensors that stay where they are and are rewritten by begin(): a step
-that was captured into a graph is replayed after it.  begin() works on the host, once a step for all layers, and belongs outside of captures.
+that was captured into a graph is replayed after it.  begin() works on the host, once a step for all layers, on the stream that runs the steps; it
+refuses to be captured itself, as free() and truncate() do.
 """
 from __future__ import annotations
 
@@ -57,6 +58,7 @@ class PagedKVCache:
         the others out -- or, for one number, of every sequence that holds some.  Returns n, the most of them; the step's inputs are
         (max_sequences, n, ...), shorter ones padded on the left.  Nothing changes if there are not enough pages (MemoryError) or a
         sequence would outgrow max_length (ValueError)."""
+        self._not_captured()
         if not hasattr(tokens, "__iter__"):
             new = [int(tokens) if length else 0 for length in self._length]
         else:
@@ -98,7 +100,9 @@ class PagedKVCache:
         self.truncate(sequence, 0)
 
     def truncate(self, sequence: int, length: int) -> None:
-        """Takes back tokens behind the first `length` of a sequence (proposed ones that were not accepted), and the pages that they leave empty."""
+        """Takes back tokens behind the first `length` of a sequence (proposed ones that were not accepted), after their step, and the pages that they
+        leave empty."""
+        self._not_captured()
         if not 0 <= sequence < self.max_sequences:
             raise ValueError(f"sequence {sequence} of {self.max_sequences}")
         if not 0 <= length <= self._length[sequence]:
@@ -108,8 +112,12 @@ class PagedKVCache:
             self.page_table[sequence, keep:] = -1
             self._free.extend(reversed(owned[keep:]))
             del owned[keep:]
-        self._length[sequence], self._new[sequence] = length, 0
+        self._length[sequence], self._new[sequence], self.fresh = length, 0, False
         self._write_counts()
+
+    def _not_captured(self) -> None:
+        if self.page_table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKVCache: the book-keeping of a step belongs in front of its replay, not into a captured graph")
 
     def _pages_for(self, length: int) -> int:
         return (length + self.page_size - 1) // self.page_size

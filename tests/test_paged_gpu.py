@@ -717,6 +717,21 @@ def test_module_refuses_gradients_through_the_cache(dev):
             layer(x, past_key_values=_begun(_cache(F32, 64, dev)))
 
 
+def test_book_keeping_is_not_captured(dev):
+    cache = _cache(BF16, 64, dev)
+    cache.begin([5, 3])
+    before = cache.page_table.clone(), cache.sequence_lengths(), cache.free_pages()
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device=dev)
+    with torch.cuda.graph(graph):
+        y = x + 1
+        for call in (lambda: cache.begin(1), lambda: cache.truncate(0, 2), lambda: cache.free(1)):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    graph.replay()
+    assert (y == 1).all() and torch.equal(cache.page_table, before[0]) and cache.sequence_lengths() == before[1] and cache.free_pages() == before[2]
+    cache.begin(1)
+
+
 def _begun(cache):
     cache.begin([3, 3, 0])
     return cache
