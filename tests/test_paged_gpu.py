@@ -247,7 +247,8 @@ def _sampled(c, g, rows, dev):
 
 @pytest.mark.parametrize("case", [([33000], 512, 32, 8, 64), ([33000], 512, 32, 8, 16), ([9000, 17000, 300], 300, 16, 8, 128),
                                   ([64 + 9 * i for i in range(70)], 64, 32, 8, 64), ([64 + 9 * i for i in range(70)], 64, 32, 8, 16),
-                                  ([900 - 5 * i for i in range(170)], 1, 16, 4, 16)], ids=lambda c: "S%d_max%d_n%d_H%d_%d_p%d" % (len(c[0]), max(c[0]), *c[1:]))
+                                  ([900 - 5 * i for i in range(170)], 1, 16, 4, 16), ([64 + 9 * i for i in range(70)], 10, 16, 4, 16),
+                                  ([64 + 9 * i for i in range(20)], 40, 8, 8, 64)], ids=lambda c: "S%d_max%d_n%d_H%d_%d_p%d" % (len(c[0]), max(c[0]), *c[1:]))
 def test_many_keys_and_many_sequences(case, dev):
     """More tiles for a block than pages are looked up at once; more units than blocks, each cut at most once."""
     lengths, n, Hq, Hkv, page = case
