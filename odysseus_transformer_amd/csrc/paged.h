@@ -51,10 +51,10 @@ constexpr int PAGED_CHUNK_ROWS = 128, PAGED_WIDE_ROWS = 256, PAGED_CHUNK_KEYS = 
 constexpr int PAGED_EXTRA = 6;
 __host__ __device__ constexpr int paged_extra(int tile) { return tile >= PAGED_CHUNK_ROWS ? PAGED_EXTRA : 0; }
 #ifdef __HIPCC__
-// Ranges that so many steps are cut into, one for a block, of which there are `most`.  With many rows four steps each at least (4 / 6 / 8 / 16, 17 tokens of 32
-// heads on 8 behind 2000 keys: 19.5 / 21.6 / 24.7 / 31 us, behind 8192 25.3 / 26.3 / 27.5 / 36); 128 rows two blocks a compute unit only with 16 steps each
-// (512 tokens behind 8192 keys 96 us, 111 with one block; 17 behind 32768 with two blocks of 8 steps 52, with one 48).  A multiple of the units, where
-// they are few: no range has parts of two of them if they are alike (17 tokens behind 8192 keys 33 -> 28 us).
+// Ranges that so many steps are cut into, one for a block, of which there are `most`.  With many rows four steps each at least (4 / 8 / 16, 32 heads on 8 behind 2000
+// keys: 48 tokens 21 / 26 / 32 us, 128 tokens 26 / 28 / 34); 128 rows two blocks a compute unit only with 16 steps each (512 tokens behind 8192 keys 96 us, 111
+// with one block; 17 behind 32768 with two blocks of 8 steps 52, with one 48).  A multiple of the units, where they are few: no range has parts of two of them if
+// they are alike (3 sequences of 5000 keys, 40 heads on 10: 24.2 -> 22.6 us).
 __device__ __forceinline__ int paged_blocks(const PagedAttnParams& p, int steps, int most) {
   int blocks = most;
   if (p.tile >= PAGED_CHUNK_ROWS && !(p.tile == PAGED_CHUNK_ROWS && steps >= 16 * most))

@@ -396,10 +396,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   }
 }
 
-// Row tiles of 16 or 32 here; more than 64 rows in bf16 by the kernels of many rows.  32 tokens of 4 heads a kv head behind 131072 keys: 206 us in tiles of 32, 145
-// by paged_attn_chunk.hip; at 17 to 64 tokens behind 8192 both take 25 to 30.  33 to 64 rows, which read everything twice here, go there where 128 (sequence, kv head)
-// pairs and more share the chip's reads (10 tokens of 32 heads on 8: 64 sequences of up to 8192 keys 371 us here, 254 there, 64 of up to 1000 63 and 54; 8 of
-// 4000 39 and 41, one of 2000 13 and 19).  Tiles of 64 here would not fit the registers.
+// Row tiles of 16 or 32 here (64 would not fit the registers); many rows in bf16 by the kernels for them: from 129 on, from 65 on but for few (sequence, kv head)
+// pairs and few keys, where more, shorter ranges win (32 heads on 8: 17 tokens behind 500 / 2000 / 8192 / 32768 keys 13.6 / 15.1 / 25.2 / 47 us here, 17.6 / 19.6 / 26.4
+// / 43 there; of 4 sequences 20 / 28 / 51 and 18 / 25 / 41), and from 33 on where there are many, which would be read from memory twice here (10 tokens each of 64
+// sequences of up to 8192 keys 371 us here, 254 there, of up to 1000 63 and 54; 8 of 4000 39 and 41, one of 2000 13 and 19).
 // paged_attn_wide.hip for heads of 128 where 64 units and more keep its 256 blocks busy (2000 keys, 32 heads on 8: 128 tokens 34 us, 28 in tiles of 128, 512 tokens
 // 44 and 46; 2048 tokens behind 8192 keys 312 and 354), pages hold a tile of keys, so that its address is one, and its tiles cover at most an eighth more rows than
 // tiles of 128 would (257 rows of each of 32 heads behind 8192 keys: 91 us in two of 256, 78 in three).
@@ -412,7 +412,8 @@ struct Plan {
 Plan plan(int S, int n, int group, int Hkv, int D, int page_size, int width, int dtype) {
   const int64_t most_keys = (int64_t)page_size * width;
   const int64_t rows = (int64_t)n * group;
-  const bool chunk = dtype == ODY_BF16 && (rows > 64 || (rows > 32 && (double)S * Hkv >= 128));
+  const double pairs = (double)S * Hkv;
+  const bool chunk = dtype == ODY_BF16 && (rows > 128 || (rows > 64 ? pairs >= 16 || most_keys > 16384 : rows > 32 && pairs >= 128));
   const int64_t wide_tiles = (rows + PAGED_WIDE_ROWS - 1) / PAGED_WIDE_ROWS, chunk_tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
   const bool wide = chunk && D == 128 && page_size >= PAGED_CHUNK_KEYS && (double)S * wide_tiles * Hkv >= 64 && 14 * wide_tiles <= 8 * chunk_tiles;
   const int tile = rows <= 16 ? 16 : wide ? PAGED_WIDE_ROWS : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);

@@ -1,5 +1,5 @@
-// Attention of many new tokens over a key / value cache in pages, bf16: a chunk of a prompt, more than 64 rows of a kv head (its query heads
-// times the tokens).
+// Attention of many new tokens over a key / value cache in pages, bf16: a chunk of a prompt, or many rows of a kv head (its query heads times the
+// tokens) by a few tokens of many sequences; the rule is in paged_attn.hip.
 //
 // Bound by the matrix cores and, as much, by the vector work of the softmax between the two products.  A block of four wavefronts takes 128 rows of one
 // (sequence, kv head), 32 a wavefront, and walks over the keys in tiles of 64, two halves each.  Both products are computed transposed, so that a row's
@@ -14,7 +14,7 @@
 //
 // P is rounded to bf16 for its product and summed up in fp32 unrounded, as in the attention over contiguous keys.
 //
-// Measured, 32 heads on 8 of 128 in pages of 16: 17 tokens behind 2000 keys 20 us, 512 behind 8192 97, 2048 behind 8192 354 (870 TFLOP/s); heads of 64, 512 behind
+// Measured, 32 heads on 8 of 128 in pages of 16: 128 tokens behind 2000 keys 26 us, 512 behind 8192 97, 2048 behind 8192 354 (870 TFLOP/s); heads of 64, 512 behind
 // 8191, 65 (540).
 #include <cmath>
 #include <type_traits>
