@@ -401,8 +401,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
 // / 43 there; of 4 sequences 20 / 28 / 51 and 18 / 25 / 41), and from 33 on where there are many, which would be read from memory twice here (10 tokens each of 64
 // sequences of up to 8192 keys 371 us here, 254 there, of up to 1000 63 and 54; 8 of 4000 39 and 41, one of 2000 13 and 19).
 // paged_attn_wide.hip for heads of 128 where 64 units and more keep its 256 blocks busy (2000 keys, 32 heads on 8: 128 tokens 34 us, 28 in tiles of 128, 512 tokens
-// 44 and 46; 2048 tokens behind 8192 keys 312 and 354), pages hold a tile of keys, so that its address is one, and its tiles cover at most an eighth more rows than
-// tiles of 128 would (257 rows of each of 32 heads behind 8192 keys: 91 us in two of 256, 78 in three).
+// 44 and 46; 2048 tokens behind 8192 keys 312 and 354, in pages of 16 346 and 357; 300 each of 64 sequences of up to 3000 keys, pages of 16, 637 and 774) and its tiles
+// cover at most an eighth more rows than tiles of 128 would (257 rows of each of 32 heads behind 8192 keys: 91 us in two of 256, 78 in three).
 struct Plan {
   int tile, row_tiles, step, blocks;
   bool joined;          // a cut may go through a unit
@@ -415,7 +415,7 @@ Plan plan(int S, int n, int group, int Hkv, int D, int page_size, int width, int
   const double pairs = (double)S * Hkv;
   const bool chunk = dtype == ODY_BF16 && (rows > 128 || (rows > 64 ? pairs >= 16 || most_keys > 16384 : rows > 32 && pairs >= 128));
   const int64_t wide_tiles = (rows + PAGED_WIDE_ROWS - 1) / PAGED_WIDE_ROWS, chunk_tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
-  const bool wide = chunk && D == 128 && page_size >= PAGED_CHUNK_KEYS && (double)S * wide_tiles * Hkv >= 64 && 14 * wide_tiles <= 8 * chunk_tiles;
+  const bool wide = chunk && D == 128 && (double)S * wide_tiles * Hkv >= 64 && 14 * wide_tiles <= 8 * chunk_tiles;
   const int tile = rows <= 16 ? 16 : wide ? PAGED_WIDE_ROWS : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);
   const int step = chunk ? PAGED_CHUNK_KEYS : WAVES * (dtype == ODY_BF16 ? 32 : 16);
   const int64_t steps = std::max((int64_t)1, (most_keys + step - 1) / step);   // of a unit, at most

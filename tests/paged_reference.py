@@ -85,13 +85,13 @@ def attend(c, scale=None):
     mean, dots = torch.zeros_like(out), torch.zeros(S, Hq, n, dtype=torch.float64)
     for s in range(S):
         length = max(int(c["lengths"][s]), 0)
-        places = [j for j in range(length) if page_of(c, s, j) is not None]
-        if not places:
+        j = torch.arange(min(length, c["table"].shape[1] * c["page"]))
+        pages = c["table"][s, j // c["page"]].long()
+        with_page = (pages >= 0) & (pages < c["k"].shape[0])
+        j, pages = j[with_page], pages[with_page]
+        if not len(j):
             continue
-        at = [page_of(c, s, j) for j in places]
-        pages, rows = torch.tensor([a[0] for a in at]), torch.tensor([a[1] for a in at])
-        K, V = c["k"][pages, rows].double(), c["v"][pages, rows].double()        # (keys, Hkv, D)
-        j = torch.tensor(places)
+        K, V = c["k"][pages, j % c["page"]].double(), c["v"][pages, j % c["page"]].double()        # (keys, Hkv, D)
         for i in range(n):
             seen = j <= length - n + i
             if not seen.any() or i < first_token(c, s, n):

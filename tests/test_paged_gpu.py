@@ -225,24 +225,60 @@ def test_long_chunks_whose_scores_grow(dev):
         _check_attn(c, _to(c, dev))
 
 
-def _sampled(c, g, rows, dev):
-    """_check_attn for some rows (s, i, h) of a call that is too large for all of them."""
+def _sampled(c, g, count, seed):
+    """_check_attn for some rows of a call that is too large for all of them, the first and the last one of each sequence's among them."""
     from odysseus_transformer_amd import ops
-    out, lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"])
+    out, lse = ops.paged_attn(g["q"], g["k"], g["v"], g["table"], g["lengths"], new_tokens=g.get("new"))
     out, lse = out.double().cpu(), lse.double().cpu()
-    n, Hq, Hkv, page = c["q"].shape[1], c["q"].shape[2], c["k"].shape[2], c["page"]
+    S, n, Hq = c["q"].shape[:3]
+    Hkv = c["k"].shape[2]
+    r = torch.Generator().manual_seed(seed)
+    draw = lambda most: int(torch.randint(most, (1,), generator=r))  # noqa: E731
+    rows = [(draw(S), draw(n), draw(Hq)) for _ in range(count)] + [(s, i, draw(Hq)) for s in range(min(S, 12)) for i in (0, n - 1)]
     for s, i, h in rows:
-        places = torch.arange(int(c["lengths"][s]) - n + i + 1)
-        at = c["table"][s, places // page].long(), places % page
-        one = dict(c, q=c["q"][s:s + 1, i:i + 1, h:h + 1], lengths=torch.tensor([len(places)]))
-        K, V = c["k"][at[0], at[1], h * Hkv // Hq].double(), c["v"][at[0], at[1], h * Hkv // Hq].double()
-        q = one["q"][0, 0, 0].double()
-        x = K @ q / math.sqrt(len(q))
-        p = torch.softmax(x, 0)
-        o, m, z = (p @ V)[None, None, None], (p @ V.abs())[None, None, None], torch.logsumexp(x, 0)[None, None, None]
-        tol_o, tol_s = ref.attend_bounds(one, o, z, m, ((K.abs() @ q.abs()).max() / math.sqrt(len(q)))[None, None, None])
+        kv = h * Hkv // Hq
+        one = dict(c, q=c["q"][s:s + 1, i:i + 1, h:h + 1], k=c["k"][:, :, kv:kv + 1], v=c["v"][:, :, kv:kv + 1], table=c["table"][s:s + 1],
+                   lengths=c["lengths"][s:s + 1] - n + i + 1, new=torch.tensor([int(i >= ref.first_token(c, s, n))]))
+        o, z, mean, dots = ref.attend(one)
+        tol_o, tol_s = ref.attend_bounds(one, o, z, mean, dots)
+        if z.item() == -math.inf:
+            assert lse[s, h, i] == -math.inf and (out[s, i, h] == 0).all(), (s, i, h)
+            continue
         assert ((out[s, i, h] - o[0, 0, 0]).abs() <= tol_o[0, 0, 0]).all(), (s, i, h)
         assert (lse[s, h, i] - z[0, 0, 0]).abs() <= tol_s[0, 0, 0], (s, i, h)
+
+
+# as many sequences and kv heads as tiles of 256 rows are taken for
+WIDE = [([64, 65, 128, 63, 192, 191, 256, 255], 200), ([321, 448, 200, 383, 577, 900, 260, 1500], 200), ([130] * 8, 250), ([700, 300, 257, 256, 1, 90, 0, 40], 256),
+        ([33, 513, 769, 1025, 1281, 640, 704, 832], 512)]
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 256])
+@pytest.mark.parametrize("lengths,n", WIDE, ids=lambda x: str(x) if isinstance(x, int) else "max%d" % max(x))
+def test_tiles_of_256_rows(lengths, n, page, dev):
+    """Ranges of one tile of keys to many, tokens and sequences that are not there, a page missing before, under and behind plain tiles."""
+    for new, holes in ((False, False), (True, False), (False, True)):
+        c = ref.make(lengths, n, 16 if n == 512 else 8, 8, 128, page, BF16, seed=n + page)
+        if new:
+            c["new"] = torch.tensor([n, n // 2, 1, 0, n, 7, n, n - 1], dtype=torch.int32)
+        if holes:
+            for s, column in ((0, 0), (1, 3), (1, 200 // page), (5, 640 // page), (7, 1)):
+                c["table"][s, min(column, c["table"].shape[1] - 1)] = -1 if s % 2 else 2 ** 31 - 1
+        _sampled(c, _to(c, dev), 40, page)
+
+
+def test_tiles_of_256_rows_whose_scores_grow(dev):
+    """The largest score of a row in every one of its tiles above those before it, by more and by less than a reference may lag behind."""
+    for step in (0.5, 3.0, 40.0):
+        c = ref.make([700] * 8, 200, 8, 8, 128, 64, BF16, seed=2)
+        q = c["q"][0, 0, 0].float()
+        for s in range(8):
+            j = torch.arange(700)
+            noise = torch.randn(700, 128, generator=torch.Generator().manual_seed(s)) * 0.02
+            k = (q * (step * (j // 32) / 20 * 11.3 / (q @ q).item())[:, None] + noise).to(BF16)
+            c["k"][c["table"][s, j // 64].long(), j % 64] = k[:, None]
+        c["q"][:] = q.to(BF16) * torch.linspace(-1, 1, 8 * 200 * 8).reshape(8, 200, 8, 1).to(BF16)
+        _sampled(c, _to(c, dev), 60, 1)
 
 
 @pytest.mark.parametrize("case", [([33000], 512, 32, 8, 64), ([33000], 512, 32, 8, 16), ([9000, 17000, 300], 300, 16, 8, 128),
@@ -253,9 +289,7 @@ def test_many_keys_and_many_sequences(case, dev):
     """More tiles for a block than pages are looked up at once; more units than blocks, each cut at most once."""
     lengths, n, Hq, Hkv, page = case
     c = ref.make(lengths, n, Hq, Hkv, 128, page, BF16, seed=n)
-    g = torch.Generator().manual_seed(1)
-    rows = [(int(torch.randint(len(lengths), (1,), generator=g)), int(torch.randint(n, (1,), generator=g)), int(torch.randint(Hq, (1,), generator=g))) for _ in range(30)]
-    _sampled(c, _to(c, dev), rows + [(0, 0, 0), (0, n - 1, Hq - 1)], dev)
+    _sampled(c, _to(c, dev), 30, 1)
 
 
 @pytest.mark.parametrize("rows", [33, 47, 48, 49, 64, 65])
