@@ -248,17 +248,18 @@ def _sampled(c, g, count, seed):
         assert (lse[s, h, i] - z[0, 0, 0]).abs() <= tol_s[0, 0, 0], (s, i, h)
 
 
-# as many sequences and kv heads as tiles of 256 rows are taken for
+# as many sequences and kv heads as tiles of 256 rows are taken for (heads of 64 in tiles of 128)
 WIDE = [([64, 65, 128, 63, 192, 191, 256, 255], 200), ([321, 448, 200, 383, 577, 900, 260, 1500], 200), ([130] * 8, 250), ([700, 300, 257, 256, 1, 90, 0, 40], 256),
         ([33, 513, 769, 1025, 1281, 640, 704, 832], 512)]
 
 
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("page", [8, 16, 32, 64, 256])
 @pytest.mark.parametrize("lengths,n", WIDE, ids=lambda x: str(x) if isinstance(x, int) else "max%d" % max(x))
-def test_tiles_of_256_rows(lengths, n, page, dev):
+def test_tiles_of_256_rows(lengths, n, page, D, dev):
     """Ranges of one tile of keys to many, tokens and sequences that are not there, a page missing before, under and behind plain tiles."""
     for new, holes in ((False, False), (True, False), (False, True)):
-        c = ref.make(lengths, n, 16 if n == 512 else 8, 8, 128, page, BF16, seed=n + page)
+        c = ref.make(lengths, n, 16 if n == 512 else 8, 8, D, page, BF16, seed=n + page)
         if new:
             c["new"] = torch.tensor([n, n // 2, 1, 0, n, 7, n, n - 1], dtype=torch.int32)
         if holes:
@@ -267,14 +268,15 @@ def test_tiles_of_256_rows(lengths, n, page, dev):
         _sampled(c, _to(c, dev), 40, page)
 
 
-def test_tiles_of_256_rows_whose_scores_grow(dev):
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_of_256_rows_whose_scores_grow(D, dev):
     """The largest score of a row in every one of its tiles above those before it, by more and by less than a reference may lag behind."""
     for step in (0.5, 3.0, 40.0):
-        c = ref.make([700] * 8, 200, 8, 8, 128, 64, BF16, seed=2)
+        c = ref.make([700] * 8, 200, 8, 8, D, 64, BF16, seed=2)
         q = c["q"][0, 0, 0].float()
         for s in range(8):
             j = torch.arange(700)
-            noise = torch.randn(700, 128, generator=torch.Generator().manual_seed(s)) * 0.02
+            noise = torch.randn(700, D, generator=torch.Generator().manual_seed(s)) * 0.02
             k = (q * (step * (j // 32) / 20 * 11.3 / (q @ q).item())[:, None] + noise).to(BF16)
             c["k"][c["table"][s, j // 64].long(), j % 64] = k[:, None]
         c["q"][:] = q.to(BF16) * torch.linspace(-1, 1, 8 * 200 * 8).reshape(8, 200, 8, 1).to(BF16)
