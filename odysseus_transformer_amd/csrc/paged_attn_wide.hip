@@ -15,7 +15,7 @@
 // are rescaled at once, O one half tile later.
 //
 // Measured against tiles of 128 rows, 32 heads on 8: 2048 tokens behind 8192 keys 354 -> 312 us (990 TFLOP/s; the kernel without a cache, attn_fwd_pipe.hip, 1 220 to
-// 1 320), 512 behind 32768 301 -> 265 (1 030), 512 behind 8191 97 -> 87, of which the join takes 10.  The matrix cores are busy half of the time.  Of a turn's
+// 1 320), 512 behind 32768 301 -> 258 (1 060), 512 behind 8191 97 -> 87, of which the join takes 10.  The matrix cores are busy half of the time.  Of a turn's
 // 4 090 cycles the loads cost 9 %, the exponentials 5, the LDS reads of K and of V 2 each, sums 3, maxima and the references 2 (left out in turn); nothing of it alone.
 #include <cmath>
 #include "attn_rowtile.h"
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_wide_kernel(const PagedAt
       };
       // The reads that may be under way: those of a phase's second half, of fragments that are one read each (K) or two (V)
       constexpr int LGKM_4 = 0xc47f, LGKM_8 = 0xc87f;
-      auto s_phase = [&](auto plain, int kt, int of, int e0, int q) INLINE {   // S of half tile kt; elements e0 .. of P of half tile `of`; quarter q of the loads
+      auto s_phase = [&](int kt, int of, int e0) INLINE {   // S of half tile kt; elements e0 .. of P of half tile `of`
 #pragma unroll
         for (int n = 0; n < 8; n++)
 #pragma unroll
@@ -298,15 +298,15 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_wide_kernel(const PagedAt
             if (n == 0) score_new(y[kt][qt], fr[n], qf[qt][n]);
             else score_onto(y[kt][qt], fr[n], qf[qt][n]);
             FENCE();
-            if (n == 2 && qt == 0) load_k(plain, q);
-            if (n == 5 && qt == 0) load_v(plain, q);
             if (qt == 1) fr[n] = vfrag(kt, n);
             weight(of, e0 + 2 * n + qt);
             FENCE();
           }
       };
-      // O with half tile kt; ...; the largest scores of half tile kt (of the next tile), which s_phase formed; what `under` has for the n-th pair of products
-      auto pv_phase = [&](auto plain, int kt, int of, int e0, int q, auto under) INLINE {
+      // O with half tile kt; ...; the largest scores of half tile kt (of the next tile), which s_phase formed; what `under` has for the n-th pair of products.  The
+      // direct loads go out here, where half as many LDS reads do: three quarters of a tile's with half tile 0, the first of the next one's with half tile 1
+      // (pages of 16: 343 -> 328 us than with one in each phase, 512 tokens behind 32488 keys 267 -> 258).
+      auto pv_phase = [&](auto plain, int kt, int of, int e0, auto under) INLINE {
 #pragma unroll
         for (int n = 0; n < 8; n++)
 #pragma unroll
@@ -316,8 +316,10 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_wide_kernel(const PagedAt
             o[qt][n & 3] = mfma32(fr[n], pb[kt][qt][n >> 2], o[qt][n & 3]);
             FENCE();
             if (qt == 0) under(n);
-            if (n == 2 && qt == 0) load_k(plain, q);
-            if (n == 5 && qt == 0) load_v(plain, q);
+            if (qt == 0 && kt == 0 && n >= 1 && n <= 3) load_k(plain, n);
+            if (qt == 0 && kt == 0 && n >= 4 && n <= 6) load_v(plain, n - 3);
+            if (qt == 0 && kt == 1 && n == 2) load_k(plain, 0);
+            if (qt == 0 && kt == 1 && n == 5) load_v(plain, 0);
             if (qt == 1) fr[n] = kfrag(kt ^ 1, n);
             weight(of, e0 + 2 * n + qt);
             if (n >= 2 && n < 6) {   // two registers of each half's scores (complete three products behind s_phase)
@@ -368,16 +370,16 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_wide_kernel(const PagedAt
       // turn t.  PLAIN: all rows see all of tile t + 1, and tiles t + 2 .. t + 4 are whole
       auto turn = [&](auto plain, int t) INLINE {
         const int n0 = key0 + KEYS * (t + 1);
-        s_phase(plain, 0, 1, 0, 1);
-        pv_phase(plain, 0, 1, 16, 2, [](int) {});
+        s_phase(0, 1, 0);
+        pv_phase(plain, 0, 1, 16, [](int) {});
         decide(plain, 0, n0, have[0] & 15);
-        s_phase(plain, 1, 0, 0, 3);
-        // K of t + 2 and V of t + 1 have landed (behind them the 8 loads of the tiles after); everyone is done with K of t + 1 and V of t - 1
+        // K of t + 2 and V of t + 1 have landed (behind them the 8 loads of the tiles after); everyone is done with K of t and V of t - 1
         wait_loads<8>();
         barrier();
+        s_phase(1, 0, 0);
         if ((t & (PAGE_TILES - 1)) == PAGE_TILES - 2) direct_load_dword(entry(t / PAGE_TILES + 2), page_place + (t / PAGE_TILES & 1) * 256);
         const unsigned ok = have[0] >> 4;
-        pv_phase(plain, 1, 0, 16, 0, [&](int n) INLINE {
+        pv_phase(plain, 1, 0, 16, [&](int n) INLINE {
           if (n == 0) {
             to_slot(krow, t + 1, t + 2);
             const int before = sk.pages;
