@@ -112,6 +112,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(const PagedAt
   constexpr int STEP = WAVES * G::KEYS, GK = G::GK, OP = D + 4;
   __shared__ __attribute__((aligned(16))) float Os[WAVES][16][OP];
   __shared__ float sm[WAVES][16 * NT], sl[WAVES][16 * NT];
+  paged_arguments(p, cache);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q = lane >> 4;
   PagedWalk<STEP> walk(p, cache, lane);
   const int each = walk.total();   // steps of a kv head
@@ -304,6 +305,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   static_assert(GROUPS >= R, "a group of threads for each of a block's rows");
   __shared__ f32x4 red[GROUPS][C4];
   __shared__ float2 red_ml[GROUPS];
+  paged_arguments(p, cache);
   const int tid = threadIdx.x, lane = tid & 63, all_rows = p.n * p.group, extra = paged_extra(p.tile);
   PagedWalk<STEP> walk(p, cache, lane);
   const int each = walk.total();
