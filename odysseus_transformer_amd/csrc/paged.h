@@ -78,7 +78,8 @@ __device__ __forceinline__ int paged_length(const PagedCache& c, int s) { return
 // New tokens of sequence s, of n.
 __device__ __forceinline__ int paged_fresh(const PagedCache& c, int s, int n) { return c.fresh ? max(0, min(c.fresh[s], n)) : n; }
 // The arguments' cache lines at once, in front of everything: one after the other, where they are first needed, they are a latency each
-// (8 heads, groups of 4, D=128: one sequence of 8 192 tokens 14.2 -> 14.0 us, three of 2 048 in fp32 13.3 -> 13.0; n=5, D=64: 17.2 -> 16.9).
+// (one sequence of 8 192 tokens, 32 heads on 8, D=128: 14.2 -> 14.0 us; three of 500 to 2 048 in fp32, 8 heads, D=64: 13.3 -> 13.0;
+// five new tokens of eight of 700 to 5 000, 16 heads on 4, D=64: 17.2 -> 16.9).
 __device__ __forceinline__ void paged_arguments(const PagedAttnParams& p, const PagedCache& c) {
   asm volatile("" ::"s"(p.q), "s"(p.S), "s"(c.k), "s"(c.width), "s"((int)gridDim.x));
 }
