@@ -402,7 +402,7 @@ int ody_attn_bwd_dropout(const void* q, const void* k, const void* v, const void
  *                   replays with what they hold then.
  * new_tokens        (S) int32, or NULL: of the n new tokens a sequence has the last new_tokens (NULL: all; 0: it takes no part).
  * New token i sits at place lengths - n + i.  Where that is negative, or i < n - new_tokens, there is no token: sequences with fewer than n are padded on
- * the left.  A place behind the table's last column has no page.
+ * the left.  A place behind the table's last column has no page.  A table has at most 2^31 - 4096 places (table_width * page_size; ODY_ERR_BAD_SHAPE).
  *
  * ody_paged_append  qkv (S, n, Hq + 2 Hkv, D), the packed projection, strides sx_*.  q != NULL: queries and keys are rotated as ody_rope
  *                   rotates them, by position_ids (S, n) int64, contiguous, or with NULL by their places, and inv_freq (D / 2) fp32; the queries go to q

@@ -45,6 +45,11 @@ struct PagedAttnParams {
 // The kernels of many rows (paged_attn_chunk.hip, paged_attn_wide.hip): rows of a tile, keys of a step
 constexpr int PAGED_CHUNK_ROWS = 128, PAGED_WIDE_ROWS = 256, PAGED_CHUNK_KEYS = 64;
 
+// How far the kernels count past a sequence's last key, in 32 bits, before they cut off what is behind it: the places of tiles whose page numbers go out ahead
+// (paged_attn_wide.hip: 64 groups of 8 keys at a time, at most 1 080 past a key; paged_attn_chunk.hip: four tiles, 248) and a tile's or a step's end.  A table may hold
+// 2^31 less so many places.
+constexpr int PAGED_AHEAD = 4096;
+
 // What a unit costs the kernels of many rows besides its steps, in steps: the latencies in front of the first products, queries in and results out.  It counts as
 // so many steps at the unit's start, of which nothing comes.  (0 / 2 / 4 / 6 / 8: a prompt of 4096 tokens, 32 heads on 8, 253 / 232 / 204 / 187 / 188 us; 512
 // tokens behind 8192 keys 95 / 95 / 90 / 87 / 88.)
@@ -83,7 +88,7 @@ __device__ __forceinline__ int paged_fresh(const PagedCache& c, int s, int n) { 
 __device__ __forceinline__ void paged_arguments(const PagedAttnParams& p, const PagedCache& c) {
   asm volatile("" ::"s"(p.q), "s"(p.S), "s"(c.k), "s"(c.width), "s"((int)gridDim.x));
 }
-// Keys that the last row of a row tile sees, none if it has no token: places behind the table's last column have no page (the host checks width << shift < 2^31).
+// Keys that the last row of a row tile sees, none if it has no token: places behind the table's last column have no page (the host checks width << shift <= 2^31 - PAGED_AHEAD).
 __device__ __forceinline__ int paged_keys(const PagedAttnParams& p, const PagedCache& c, int length, int fresh, int rt) {
   const int last_row = min((rt + 1) * p.tile, p.n * p.group) - 1;   // rows are below 2^31, and so is a row tile more
   const int last = p.row_tiles == 1 ? p.n - 1 : last_row / p.group;
