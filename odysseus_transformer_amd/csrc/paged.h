@@ -90,7 +90,7 @@ __device__ __forceinline__ void paged_arguments(const PagedAttnParams& p, const 
 }
 // Keys that the last row of a row tile sees, none if it has no token: places behind the table's last column have no page (the host checks width << shift <= 2^31 - PAGED_AHEAD).
 __device__ __forceinline__ int paged_keys(const PagedAttnParams& p, const PagedCache& c, int length, int fresh, int rt) {
-  const int last_row = min((rt + 1) * p.tile, p.n * p.group) - 1;   // rows are below 2^31, and so is a row tile more
+  const int last_row = min((rt + 1) * p.tile, p.n * p.group) - 1;   // rows, and a row tile more, are below 2^31 (paged_check)
   const int last = p.row_tiles == 1 ? p.n - 1 : last_row / p.group;
   return last < p.n - fresh ? 0 : max(0, min(c.width << c.shift, length - p.n + last + 1));
 }

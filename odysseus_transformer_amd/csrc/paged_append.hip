@@ -120,7 +120,10 @@ int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype
   ODY_REQUIRE(page_size >= 8 && (page_size & (page_size - 1)) == 0, ODY_ERR_UNSUPPORTED, "%s: page_size %d: a power of two from 8 on", who, page_size);
   ODY_REQUIRE((int64_t)c.width * page_size <= ((int64_t)1 << 31) - PAGED_AHEAD, ODY_ERR_BAD_SHAPE, "%s: a table of more than 2^31 - %d places (%d columns, pages of %d)",
               who, PAGED_AHEAD, c.width, page_size);
-  ODY_REQUIRE((int64_t)S * n * (Hq + 2 * (int64_t)Hkv) < (int64_t)1 << 31, ODY_ERR_BAD_SHAPE, "%s: 2^31 heads of all new tokens and more", who);
+  // rows are counted in 32 bits, up to the end of the last row tile, and vectors of a token up to the end of a block's turn; the product itself may be beyond 64
+  const int64_t heads = Hq + 2 * (int64_t)Hkv;
+  ODY_REQUIRE(heads < ((int64_t)1 << 31) / 16 - 256 && (double)S * n * heads < (double)(((int64_t)1 << 31) - PAGED_WIDE_ROWS), ODY_ERR_BAD_SHAPE,
+              "%s: %lld heads of a token, or heads of all new tokens together, are too many", who, (long long)heads);
   const int64_t bytes = dtype == ODY_BF16 ? 2 : 4, most = (int64_t)1 << 32;
   for (const PageStrides& s : {c.sk, c.sv})
     ODY_REQUIRE(s.p >= 0 && s.r >= 0 && s.p < most / bytes && s.r < most / bytes / page_size, ODY_ERR_UNSUPPORTED,

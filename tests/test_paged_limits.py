@@ -27,3 +27,14 @@ def test_room_behind_the_last_column(name, page):
     assert _code(name, page=page, width=most) == -3
     assert _code(name, page=page, width=most + 1) == -1
     assert _code(name, page=page, width=2 ** 31 // page - 1) == (-3 if most == 2 ** 31 // page - 1 else -1)
+
+
+@pytest.mark.parametrize("name", ["ody_paged_append", "ody_paged_attn"])
+def test_new_tokens_and_heads(name):
+    """Rows, and vectors of a token, are counted in 32 bits; the products that the check forms fit 64 whatever the sizes are."""
+    top = 2 ** 31 - 1
+    for sizes in (dict(S=top, n=top, Hq=2, Hkv=1), dict(S=top, n=top, Hq=top, Hkv=1), dict(S=top, n=3, Hq=top, Hkv=top), dict(S=1 << 29, n=1, Hq=2, Hkv=1),
+                  dict(n=1 << 29, Hq=2, Hkv=1), dict(n=2 ** 31 // 6, Hq=4, Hkv=1), dict(Hq=2 ** 27, Hkv=1), dict(Hq=top, Hkv=1), dict(Hq=2 ** 30, Hkv=2 ** 30)):
+        assert _code(name, **sizes) == -1, sizes
+    for sizes in (dict(S=1 << 28, n=1, Hq=4, Hkv=1), dict(n=2 ** 31 // 6 - 64, Hq=4, Hkv=1), dict(Hq=2 ** 26, Hkv=1)):
+        assert _code(name, **sizes) == -3, sizes
