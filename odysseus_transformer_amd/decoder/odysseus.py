@@ -229,6 +229,8 @@ class LlamaFlashAttention2TPSP(nn.Module):
         if cache.position_ids is None or tuple(cache.position_ids.shape) != (S, n):
             raise ValueError(f"hidden_states are {tuple(hidden_states.shape)}, but the cache's step is for "
                              f"{None if cache.position_ids is None else tuple(cache.position_ids.shape)} tokens: PagedKVCache.begin() comes before it")
+        if self.layer_idx is None and cache.num_layers > 1:
+            raise ValueError(f"a cache in pages of {cache.num_layers} layers, but this module does not know which one it is: give it a layer_idx")
         scale = 1.0 / math.sqrt(D)
         k_pages, v_pages = cache.layer(self.layer_idx or 0)
         where = (k_pages, v_pages, cache.page_table, cache.lengths)

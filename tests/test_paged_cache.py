@@ -149,3 +149,18 @@ def test_entry_points_refuse_without_a_gpu():
         ops.paged_append_(x, 4, x, x, x, x, position_ids=torch.zeros(2, 1), rotate=False)
     with pytest.raises(RuntimeError, match="HIP device"):
         ops.paged_attn(x, x, x, x, x)
+
+
+def test_a_layer_without_an_index_over_a_cache_of_several():
+    """Modules that do not say which layer they are would share one layer's pages, and overwrite each other's keys."""
+    m, c = _module().eval(), _cache(dtype=torch.float32)
+    c.begin([5, 5, 5])
+    x = torch.zeros(3, 5, 128)
+    m.layer_idx = None
+    with pytest.raises(ValueError, match="layer_idx"), torch.no_grad():
+        m(x, past_key_values=c)
+    one = _cache(dtype=torch.float32, num_layers=1)
+    one.begin([5, 5, 5])
+    m.layer_idx = None
+    with pytest.raises(RuntimeError, match="HIP device"), torch.no_grad():   # a lone layer needs none
+        m(x, past_key_values=one)
