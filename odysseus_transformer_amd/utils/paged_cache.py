@@ -44,7 +44,7 @@ class PagedKVCache:
         self.page_table = torch.full((max_sequences, self._columns), -1, dtype=torch.int32, device=device)
         self._counts = torch.zeros((2, max_sequences), dtype=torch.int32, device=device)
         self.lengths, self.new_tokens = self._counts[0], self._counts[1]
-        self.position_ids = None                                   # (max_sequences, n) int64 of the present step, 0 for padding
+        self.position_ids = None                                   # (max_sequences, n) int64 of the present step, 0 for padding; None: there is none
         self._positions = torch.zeros(max_sequences * max_length, dtype=torch.int64, device=device)
         self._owned: List[List[int]] = [[] for _ in range(max_sequences)]
         self._free = list(range(num_pages - 1, -1, -1))
@@ -101,7 +101,7 @@ class PagedKVCache:
 
     def truncate(self, sequence: int, length: int) -> None:
         """Takes back tokens behind the first `length` of a sequence (proposed ones that were not accepted), after their step, and the pages that they
-        leave empty."""
+        leave empty.  The step is over then: begin() comes before the next one."""
         self._not_captured()
         if not 0 <= sequence < self.max_sequences:
             raise ValueError(f"sequence {sequence} of {self.max_sequences}")
@@ -112,6 +112,8 @@ class PagedKVCache:
             self.page_table[sequence, keep:] = -1
             self._free.extend(reversed(owned[keep:]))
             del owned[keep:]
+        if length and self._new[sequence]:
+            self.position_ids = None   # modules ask for it; the storage stays
         self._length[sequence], self._new[sequence], self.fresh = length, 0, False
         self._write_counts()
 

@@ -164,3 +164,33 @@ def test_a_layer_without_an_index_over_a_cache_of_several():
     m.layer_idx = None
     with pytest.raises(RuntimeError, match="HIP device"), torch.no_grad():   # a lone layer needs none
         m(x, past_key_values=one)
+
+
+def test_no_step_behind_truncate():
+    """A sequence whose new tokens were taken back has none: a step that runs before the next begin() would leave it out without a word."""
+    m, x = _module().eval(), torch.zeros(3, 1, 128)
+
+    def run(c):
+        with torch.no_grad():
+            m(x, past_key_values=c)
+    for length in (5, 6):
+        c = _cache(dtype=torch.float32)
+        c.begin([5, 5, 5])
+        c.begin(1)
+        at = c.position_ids.data_ptr()
+        c.truncate(1, length)
+        with pytest.raises(ValueError, match="begin"):
+            run(c)
+        c.begin(1)
+        assert c.position_ids.data_ptr() == at               # a captured step reads them again
+        with pytest.raises(RuntimeError, match="HIP device"):
+            run(c)
+    # a sequence that ends in front of a step takes no part in it, nor does one that takes none lose any
+    c = _cache(dtype=torch.float32)
+    c.begin([5, 5, 5])
+    c.begin([1, 1, 0])
+    c.free(0)
+    c.truncate(2, 3)
+    assert c.lengths.tolist() == [0, 6, 0] and c.new_tokens.tolist() == [0, 1, 0]
+    with pytest.raises(RuntimeError, match="HIP device"):
+        run(c)
