@@ -355,10 +355,7 @@ class LlamaMLPZeRO(nn.Module):
             x = input_norm(x)
         if fusable and self.fuse_elementwise:
             return ops.run_function(ops.SwiGLUMLPResidualFunc, x, w1, w2, residual)
-        shape = x.shape
-        if x.dim() == 3 and get_model_parallel_world_size() == 1:   # the projections take one sequence; a batch comes with a cache in pages
-            x = x.reshape(1, -1, shape[-1])
-        y = self.down_proj(ops.swiglu(self.gate_up_proj(x))).view(*shape[:-1], -1)
+        y = self.down_proj(ops.swiglu(self.gate_up_proj(x)))
         return y if residual is None else residual + y
 
 

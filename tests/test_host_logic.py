@@ -834,3 +834,20 @@ def test_merge_parts_of_the_header_and_of_the_ring():
     from odysseus_transformer_amd import ops
     header = (Path(__file__).resolve().parents[1] / "include" / "odysseus_hip.h").read_text()
     assert ops._PartialResults.MOST == int(re.search(r"#define ODY_MERGE_PARTS (\d+)", header).group(1))
+
+
+def test_mlp_hands_its_projections_the_batch_as_it_is(monkeypatch):
+    """Hooks on a projection see (batch, tokens, features), whatever the batch is."""
+    from odysseus_transformer_amd import ops
+    from odysseus_transformer_amd.decoder.odysseus import LlamaMLPZeRO
+    mlp = LlamaMLPZeRO(types.SimpleNamespace(hidden_size=8, intermediate_size=16))
+    mlp.gate_up_proj, mlp.down_proj = torch.nn.Linear(8, 32, bias=False), torch.nn.Linear(16, 8, bias=False)
+    monkeypatch.setattr(ops, "swiglu", lambda gu: torch.nn.functional.silu(gu.chunk(2, -1)[0]) * gu.chunk(2, -1)[1])
+    seen = []
+    for m in (mlp.gate_up_proj, mlp.down_proj):
+        m.register_forward_hook(lambda mod, args, out: seen.append((tuple(args[0].shape), tuple(out.shape))))
+    for shape in ((1, 5, 8), (3, 5, 8), (4, 8)):
+        seen.clear()
+        x = torch.randn(shape)
+        y = mlp(x)
+        assert y.shape == x.shape and seen == [(shape, (*shape[:-1], 32)), ((*shape[:-1], 16), shape)]
