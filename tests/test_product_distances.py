@@ -75,3 +75,33 @@ def test_wait_states_around_products_by_hand(source, tmp_path):
                     other, those, hand = code[k]
                     assert not (hand and other.startswith("v_mfma") and set().union(*map(_registers, those[1:])) & result), f"{name}: {other} {those} {waited} behind {op} {operands}"
     assert products > 50
+
+
+def _assembly(source, folder):
+    from odysseus_transformer_amd import build
+    out = folder / f"{source}.s"
+    subprocess.run([build._hipcc(), *build.HIPCC_FLAGS, "-I", str(build.INCLUDE), "-S", "--cuda-device-only", str(build.CSRC / f"{source}.hip"), "-o", str(out)],
+                   check=True, capture_output=True, timeout=300)
+    return out.read_text()
+
+
+def test_wait_states_around_products_of_tiles_of_256_rows(tmp_path):
+    test_wait_states_around_products_by_hand("paged_attn_wide", tmp_path)
+
+
+# what reads or writes m0 without naming it
+M0 = re.compile(r"s_(movrel|set_gpr_idx|sendmsg|ttracedata)|v_(movrel|interp)|ds_(gws|ordered|\w+_addtid)|global_load_lds|buffer_load\w*_lds")
+
+
+@pytest.mark.parametrize("source", ["paged_attn_chunk", "paged_attn_wide"])
+def test_m0_belongs_to_the_direct_loads(source, tmp_path):
+    """Direct loads written as assembly set m0, which no such statement can name as overwritten (it is a reserved register).  So nothing else of these
+    kernels may use it: a value that the compiler kept there would be lost."""
+    loads = 0
+    for name, code, _ in _kernels(_assembly(source, tmp_path)):
+        for op, operands, by_hand in code:
+            if by_hand:
+                loads += op.startswith("global_load_lds")
+            else:
+                assert not M0.match(op) and not any(re.search(r"\bm0\b|\blds$", o) for o in operands), f"{name}: {op} {operands}"
+    assert loads >= 20
