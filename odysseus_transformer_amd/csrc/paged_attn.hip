@@ -14,8 +14,9 @@
 // A tile's K goes out when the products have read that of the one before, and so does its V (two tiles in registers, the one under way while the products read
 // the other: the same times to 1 %).  A group of GK keys lies within a page: two table entries a lane and tile.
 //
-// Measured, bf16, heads of 128, results joined: 64 sequences of up to 8192 keys, 32 heads on 8, 199 us (5.4 TB/s of K and V; a copy runs at 5.1, a sum at 6.0 to
-// 6.3); 16 of 4001, 32 heads, 124 us (5.5); one of 131072 100 us (5.4), of 8192 13.6, of 100 5.1, where launches and the chain length, table, keys, join are all.
+// Measured, bf16, heads of 128, results joined: 64 sequences of up to 8192 keys, 32 heads on 8, in rows of all heads 196 to 200 us (5.4 TB/s of K and V; a copy runs
+// at 5.1, a sum at 6.0 to 6.3), with heads outside of rows 171 to 177 (6.1); 16 of 4001, 32 heads, 125 us (5.5); one of 131072 100 us (5.4), of 8192 13.5, where launches
+// and the chain length, table, keys, join are all.  One of 100 5.4 under a table of one step, 7.4 under a wider one, for which the join is launched too.
 #include <algorithm>
 #include <cmath>
 #include "paged.h"
@@ -398,13 +399,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   }
 }
 
+// The host knows no lengths: `keys` below are the places of the table (17 tokens of one sequence behind 500 keys, 32 heads on 8: 12.6 us under a table for at most 16384
+// keys, 16.2 under a wider one).
 // Row tiles of 16 or 32 here (64 would not fit the registers); many rows in bf16 by the kernels for them: from 129 on, from 65 on but for few (sequence, kv head)
 // pairs and few keys, where more, shorter ranges win (32 heads on 8: 17 tokens behind 500 / 2000 / 8192 / 32768 keys 13.6 / 15.1 / 25.2 / 47 us here, 17.6 / 19.6 / 26.4
 // / 43 there; of 4 sequences 20 / 28 / 51 and 18 / 25 / 41), and from 33 on where there are many, which would be read from memory twice here (10 tokens each of 64
 // sequences of up to 8192 keys 371 us here, 254 there, of up to 1000 63 and 54; 8 of 4000 39 and 41, one of 2000 13 and 19).
-// paged_attn_wide.hip for heads of 128 where 64 units and more keep its 256 blocks busy (2000 keys, 32 heads on 8: 128 tokens 34 us, 28 in tiles of 128, 512 tokens
-// 44 and 46; 2048 tokens behind 8192 keys 312 and 354, in pages of 16 346 and 357; 300 each of 64 sequences of up to 3000 keys, pages of 16, 637 and 774) and its tiles
-// cover at most an eighth more rows than tiles of 128 would (257 rows of each of 32 heads behind 8192 keys: 91 us in two of 256, 78 in three).
+// paged_attn_wide.hip for heads of 128 where 64 units and more keep its 256 blocks busy (2000 keys, 32 heads on 8: 128 tokens, which are 16 units, 34 us, 28 in tiles of
+// 128, 512 tokens, 64 units, 44 and 46; between them, and with few units of many keys, the two have not been timed against each other; 2048 tokens behind 8192 keys 312
+// and 354, in pages of 16 328 and 357; 300 each of 64 sequences of up to 3000 keys, pages of 16, 637 and 774) and its tiles
+// cover at most a seventh more rows than tiles of 128 would (257 rows of each of 32 heads behind 8192 keys: 91 us in two of 256, 78 in three).
 struct Plan {
   int tile, row_tiles, step, blocks;
   bool joined;          // a cut may go through a unit

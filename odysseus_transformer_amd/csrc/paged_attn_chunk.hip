@@ -14,8 +14,9 @@
 //
 // P is rounded to bf16 for its product and summed up in fp32 unrounded, as in the attention over contiguous keys.
 //
-// Measured, 32 heads on 8 of 128 in pages of 16: 128 tokens behind 2000 keys 26 us, 512 behind 8192 97, 2048 behind 8192 354 (870 TFLOP/s); heads of 64, 512 behind
-// 8191, 65 (540).
+// Measured with the join, 32 heads on 8 of 128 in pages of 16: 128 tokens behind 2000 keys 25 us, 256 behind 8192 58 (590 TFLOP/s), behind 32768 158 (870); heads of 64,
+// 512 behind 8191, 61 (580), 2048 behind 8192 222 (700).  Heads of 128 take 156 bytes of scratch memory: the loop of plain turns has none of it, a turn that is not plain
+// reloads 20 registers, for which it waits until the direct loads in front of them have landed too.
 #include <cmath>
 #include <type_traits>
 #include "attn_rowtile.h"
@@ -36,7 +37,7 @@ __device__ const bf16x8 no_key[16] = {};   // the row that a key without a page,
 
 // A direct load, 16 bytes a lane, to LDS address `to` on.  As assembly, for behind the builtin the compiler makes transposing reads wait for it (they could
 // read what it writes, as far as it knows); the waits that there have to be stand in the loop.  It has no result that the compiler could use too early,
-// and nothing else in these kernels uses m0.
+// and nothing else in these kernels uses m0 (a reserved register, which cannot be named as overwritten; a test looks through the generated code).
 __device__ __forceinline__ void direct_load(const char* from, unsigned to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(const PagedA
       } else {
         const bool none = first + lane / LANES >= keys || (have >> at & 1) == 0;
         unsigned l = of_lane;
-        asm volatile("" : "+v"(l));   // 64 bits of it here, and not from turn to turn: the loops have no register to spare
+        asm volatile("" : "+v"(l));   // 64 bits of it here, and not from turn to turn: the loops have no register to spare (that of plain turns went to scratch memory)
         direct_load(none ? reinterpret_cast<const char*>(no_key) + 2 * lcol : row + l, to);
       }
     };

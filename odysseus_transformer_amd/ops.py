@@ -492,7 +492,7 @@ def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, posi
     each sequence WITH the new ones, of which the last n are these: token i has place lengths - n + i.  Where that is negative it is padding, and
     so are the first n - new_tokens[s] of a sequence with fewer than n, if new_tokens (S) int32 is given (padding on the left; 0: the sequence takes no
     part): the queries of padding become 0 and nothing is written.  page_size is a power of two from 8 on; any strides that are multiples of 16
-    bytes, pages and the rows of a page less than 4 GiB apart.  No two sequences may append to one row.
+    bytes, pages and the rows of a page less than 4 GiB apart.  No two new tokens may have one row.
 
     rotate: queries and keys are rotated as rope_ rotates them, by position_ids -- (S, n), or (n) for all -- or by the tokens' places; the
     queries are a new tensor.  rotate=False: they have been rotated already (linear_rope, norm_linear_rope); the result is a view of qkv."""
