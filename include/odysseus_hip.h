@@ -407,7 +407,8 @@ int ody_attn_bwd_dropout(const void* q, const void* k, const void* v, const void
  * ody_paged_append  qkv (S, n, Hq + 2 Hkv, D), the packed projection, strides sx_*.  q != NULL: queries and keys are rotated as ody_rope
  *                   rotates them, by position_ids (S, n) int64, contiguous, or with NULL by their places, and inv_freq (D / 2) fp32; the queries go to q
  *                   (S, n, Hq, D), strides sq_*, 0 where there is no token.  q == NULL: nothing is rotated.  Keys and values go to
- *                   their pages.  Rows of pages that no new token has keep what they hold.  No two new tokens may have one row.
+ *                   their pages.  Rows of pages that no new token has keep what they hold.  No two new tokens may have one row.  Fewer than
+ *                   2^24 tokens a call (S * n).
  * ody_paged_attn    out (S, n, Hq, D) and lse (S, Hq, n), contiguous fp32, of q (S, n, Hq, D): token i sees the places up to its own that have a
  *                   page, as ody_attn_fwd's causal mask with Lk = lengths has it; 0 and -inf where that is none.  Query head h reads kv head
  *                   h / (Hq / Hkv).  workspace: ody_paged_attn_workspace_bytes(...) bytes, 256-byte aligned, of no value before or after.

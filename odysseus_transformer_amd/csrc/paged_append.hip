@@ -141,6 +141,7 @@ extern "C" int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v
                                 int pages, int page_size, int table_width, int64_t table_stride, int dtype, void* stream) {
   const PagedCache c(k_pages, v_pages, page_table, lengths, new_tokens, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride, pages, page_size, table_width, dtype);
   if (int rc = paged_check("ody_paged_append", S, n, Hq, Hkv, D, dtype, c, page_size)) return rc;
+  ODY_REQUIRE((int64_t)S * n < (int64_t)1 << 24, ODY_ERR_BAD_SHAPE, "ody_paged_append: 2^24 new tokens and more (a block of 256 threads each)");
   ODY_REQUIRE(qkv && (q == nullptr || inv_freq), ODY_ERR_NULL, "ody_paged_append: qkv, or inv_freq of a rotation, is NULL");
   ODY_REQUIRE(paged_rows_aligned(qkv, sx_s, sx_n, sx_h, dtype) && (q == nullptr || paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype)), ODY_ERR_MISALIGNED,
               "ody_paged_append: qkv and q need 16-byte aligned pointers and strides");

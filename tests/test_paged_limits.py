@@ -38,3 +38,11 @@ def test_new_tokens_and_heads(name):
         assert _code(name, **sizes) == -1, sizes
     for sizes in (dict(S=1 << 28, n=1, Hq=4, Hkv=1), dict(n=2 ** 31 // 6 - 64, Hq=4, Hkv=1), dict(Hq=2 ** 26, Hkv=1)):
         assert _code(name, **sizes) == -3, sizes
+
+
+def test_tokens_of_one_launch():
+    """A block of 256 threads for a token, and fewer than 2^32 threads in a launch: refused by name, and before anything is launched."""
+    for S, n, code in ((1 << 14, 1 << 10, -1), (1 << 24, 1, -1), (1 << 12, (1 << 12) - 1, -3)):
+        with pytest.raises(_lib.OdysseusHipError) as e:   # -3: the projection is misaligned
+            _lib.call("ody_paged_append", Q, Q, Q, Q, Q, Q, 0, 0, Q, S, n, 2, 1, 64, 256, 256, 60, 128, 128, 64, 2048, 64, 64, 2048, 64, 64, 4, 16, 3, 3, 0, 0)
+        assert e.value.code == code, (S, n)
