@@ -428,6 +428,38 @@ int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, cons
                    int64_t so_s, int64_t so_n, int64_t so_h, int pages, int page_size, int table_width, int64_t table_stride,
                    float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- a cache in pages that holds its values in 8 bits -----------------------
+ * As above, with pages of e4m3 values (1 byte; no infinities, 448 the largest) and a power of two for each block of tokens and head: the value at a place is
+ * its e4m3 value times 2^(byte - 127).
+ * k_scales, v_scales  (pages, page_size / block, Hkv) bytes, strides s*z_p (page), s*z_b (block of a page), s*z_h (head).  block: a power of two from 8 to 64,
+ *                     at most page_size.
+ * ody_paged_append_q8 as ody_paged_append.  2^e of a block and head: the least with e >= -126 and max |x| <= 448 * 2^e over the finite values of its tokens there; with
+ *                     earlier tokens in the block at least what it was.  Values x 2^-e are rounded to the nearest e4m3 value, half way to the even one; one that is
+ *                     not finite becomes NaN.  Rotated keys are rounded to 32 bits in between and not to `dtype`.  Where earlier tokens are in a block whose e rises, their
+ *                     rows are rounded to the new one (exact, but for values below 2^-6 of the scale).  Fewer than 2^24 tokens and 2^23 blocks of them a call.
+ * ody_paged_read_q8   k, v (S, places, Hkv, D) of `dtype`, contiguous: the values of places 0 .. places - 1, exactly; 0 behind a sequence's length and where there
+ *                     is no page.  S < 65536, places * Hkv < 2^31.
+ * ody_paged_attn_q8   as ody_paged_attn, q and out of `dtype`; values are converted to it, exactly, in front of the products.
+ * Pages and their strides on 16 bytes, pages and the rows of a page less than 4 GiB apart, as above; scales need no alignment.
+ */
+int ody_paged_append_q8(const void* qkv, void* q, void* k_pages, void* v_pages, uint8_t* k_scales, uint8_t* v_scales, const int* page_table,
+                        const int* lengths, const int* new_tokens, const int64_t* position_ids, const float* inv_freq, int S, int n, int Hq, int Hkv, int D,
+                        int64_t sx_s, int64_t sx_n, int64_t sx_h, int64_t sq_s, int64_t sq_n, int64_t sq_h,
+                        int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
+                        int64_t skz_p, int64_t skz_b, int64_t skz_h, int64_t svz_p, int64_t svz_b, int64_t svz_h,
+                        int pages, int page_size, int block, int table_width, int64_t table_stride, int dtype, void* stream);
+int ody_paged_read_q8(const void* k_pages, const void* v_pages, const uint8_t* k_scales, const uint8_t* v_scales, const int* page_table, const int* lengths,
+                      void* k, void* v, int S, int places, int Hkv, int D, int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
+                      int64_t skz_p, int64_t skz_b, int64_t skz_h, int64_t svz_p, int64_t svz_b, int64_t svz_h,
+                      int pages, int page_size, int block, int table_width, int64_t table_stride, int dtype, void* stream);
+size_t ody_paged_attn_q8_workspace_bytes(int S, int n, int Hq, int Hkv, int D, int page_size, int table_width, int dtype);
+int ody_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_scales, const uint8_t* v_scales, const int* page_table,
+                      const int* lengths, const int* new_tokens, void* out, float* lse, int S, int n, int Hq, int Hkv, int D,
+                      int64_t sq_s, int64_t sq_n, int64_t sq_h, int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
+                      int64_t skz_p, int64_t skz_b, int64_t skz_h, int64_t svz_p, int64_t svz_b, int64_t svz_h,
+                      int64_t so_s, int64_t so_n, int64_t so_h, int pages, int page_size, int block, int table_width, int64_t table_stride,
+                      float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- optimizer ------------------------------------------------------------
  * One step of torch.optim.AdamW (the optimizer of the reference's training loop, train.py:170,216) on one
  * tensor of n elements, in one pass instead of the host framework's seven element-wise passes:

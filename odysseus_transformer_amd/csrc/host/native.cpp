@@ -39,7 +39,8 @@ namespace {
   X(ody_linear_rope_ws) X(ody_linear_swiglu) X(ody_linear_swiglu_h_fused) X(ody_linear_swiglu_h)                                  \
   X(ody_linear_dgrad_swiglu_workspace_bytes) X(ody_linear_dgrad_swiglu) X(ody_attn_fwd_workspace_bytes) X(ody_attn_fwd)           \
   X(ody_attn_bwd_workspace_bytes) X(ody_attn_bwd) X(ody_attn_bwd_rope) X(ody_rope) X(ody_rope_table)           \
-  X(ody_norm_linear_rope) X(ody_norm_linear_swiglu_h) X(ody_paged_append) X(ody_paged_attn) X(ody_paged_attn_workspace_bytes)
+  X(ody_norm_linear_rope) X(ody_norm_linear_swiglu_h) X(ody_paged_append) X(ody_paged_attn) X(ody_paged_attn_workspace_bytes) \
+  X(ody_paged_append_q8) X(ody_paged_read_q8) X(ody_paged_attn_q8) X(ody_paged_attn_q8_workspace_bytes)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -554,15 +555,21 @@ struct Paged {
   const int* fresh;
   Paged(Call& c, Py_ssize_t i, Py_ssize_t new_tokens, const at::Tensor& x)
       : k(c.heads(i, &x)), v(c.heads(i + 1, &x)), table(c.any(i + 2)), lengths(c.any(i + 3)), fresh(nullptr) {
-    need(k.sizes() == v.sizes() && k.size(3) == x.size(3));
-    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == x.size(0) && table.stride(1) == 1 && table.size(1) < INT32_MAX);
-    need(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.is_contiguous() && lengths.size(0) == x.size(0));
-    if (!c.none(new_tokens)) {
+    need(k.size(3) == x.size(3));
+    check(c, new_tokens, x.size(0), x.requires_grad());
+  }
+  Paged(Call& c, const at::Tensor& k_, const at::Tensor& v_, Py_ssize_t i) : k(k_), v(v_), table(c.any(i)), lengths(c.any(i + 1)), fresh(nullptr) {}
+  // new_tokens below 0: there is no such argument
+  void check(Call& c, Py_ssize_t new_tokens, int64_t S, bool gradient) {
+    need(k.sizes() == v.sizes());
+    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == S && table.stride(1) == 1 && table.size(1) < INT32_MAX);
+    need(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.is_contiguous() && lengths.size(0) == S);
+    if (new_tokens >= 0 && !c.none(new_tokens)) {
       const at::Tensor& t = c.any(new_tokens);
-      need(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.size(0) == x.size(0));
+      need(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.size(0) == S);
       fresh = t.data_ptr<int>();
     }
-    need(!at::GradMode::is_enabled() || !(x.requires_grad() || k.requires_grad() || v.requires_grad()));
+    need(!at::GradMode::is_enabled() || !(gradient || k.requires_grad() || v.requires_grad()));
   }
   int pages() const { return (int)k.size(0); }
   int page_size() const { return (int)k.size(1); }
@@ -570,6 +577,79 @@ struct Paged {
 };
 #define PAGED_TABLE(c) (c).table.data_ptr<int>(), (c).lengths.data_ptr<int>(), (c).fresh
 #define PAGED_SHAPE(c) (c).pages(), (c).page_size(), (c).columns(), (c).table.stride(0)
+
+// A cache in 8 bits: arguments i .. i + 5 are k_pages, v_pages, k_scales, v_scales, page_table, lengths.
+const at::Tensor& bytes_of(Call& c, Py_ssize_t i, at::ScalarType type, int64_t dims) {
+  const at::Tensor& t = c.any(i);
+  need(t.scalar_type() == type && t.dim() == dims && (dims == 3 || t.stride(3) == 1));
+  for (int64_t d = 0; d < dims; d++) need(t.size(d) < INT32_MAX);
+  return t;
+}
+struct PagedQ8 : Paged {
+  const at::Tensor &kz, &vz;
+  PagedQ8(Call& c, Py_ssize_t i)
+      : Paged(c, bytes_of(c, i, at::kFloat8_e4m3fn, 4), bytes_of(c, i + 1, at::kFloat8_e4m3fn, 4), i + 4), kz(bytes_of(c, i + 2, at::kFloat8_e8m0fnu, 3)),
+        vz(bytes_of(c, i + 3, at::kFloat8_e8m0fnu, 3)) {
+    need(kz.sizes() == vz.sizes() && kz.size(0) == k.size(0) && kz.size(2) == k.size(2) && kz.size(1) > 0 && k.size(1) % kz.size(1) == 0);
+  }
+  int block() const { return page_size() / (int)kz.size(1); }
+};
+#define PAGED_Q8(c) (c).k.data_ptr(), (c).v.data_ptr(), (uint8_t*)(c).kz.data_ptr(), (uint8_t*)(c).vz.data_ptr()
+#define PAGED_Q8_STRIDES(c) STRIDES((c).k), STRIDES((c).v), STRIDES((c).kz), STRIDES((c).vz)
+#define PAGED_Q8_SHAPE(c) (c).pages(), (c).page_size(), (c).block(), (c).columns(), (c).table.stride(0)
+
+// (qkv, n_heads, k_pages, v_pages, k_scales, v_scales, page_table, lengths, position_ids or None, inv_freq or None: no rotation, new_tokens or None) -> q
+PyObject* paged_append_q8(Call c) {
+  const at::Tensor& x = c.heads(0, nullptr);
+  PagedQ8 pg(c, 2);
+  const int64_t Hq = c.whole(1), S = x.size(0), n = x.size(1), D = x.size(3), Hkv = pg.k.size(2);
+  pg.check(c, 10, S, x.requires_grad());
+  need(Hq > 0 && x.size(2) == Hq + 2 * Hkv && pg.k.size(3) == D && x.numel() > 0);
+  if (c.none(9)) {
+    need(c.none(8));
+    at::Tensor q = x.narrow(2, 0, Hq);
+    CALL(ody_paged_append_q8, x.data_ptr(), nullptr, PAGED_Q8(pg), PAGED_TABLE(pg), nullptr, nullptr, (int)S, (int)n, (int)Hq, (int)Hkv, (int)D, STRIDES(x), STRIDES(q),
+         PAGED_Q8_STRIDES(pg), PAGED_Q8_SHAPE(pg), dt(x), (void*)c.stream);
+    return wrap(q);
+  }
+  if (!c.none(8)) need(c.any(8).dim() == 2 && c.any(8).size(0) == S);
+  const int64_t* pos = positions(c, 8, S * n);
+  const at::Tensor& f = frequencies(c, 9, D);
+  need(f.dim() == 1);
+  at::Tensor q = make({S, n, Hq, D}, x);
+  CALL(ody_paged_append_q8, x.data_ptr(), q.data_ptr(), PAGED_Q8(pg), PAGED_TABLE(pg), pos, f.data_ptr<float>(), (int)S, (int)n, (int)Hq, (int)Hkv, (int)D, STRIDES(x),
+       STRIDES(q), PAGED_Q8_STRIDES(pg), PAGED_Q8_SHAPE(pg), dt(x), (void*)c.stream);
+  return wrap(q);
+}
+
+// (k_pages, v_pages, k_scales, v_scales, page_table, lengths, places, whether in fp32) -> (k, v)
+PyObject* paged_read_q8(Call c) {
+  PagedQ8 pg(c, 0);
+  const int64_t places = c.whole(6), S = pg.table.dim() == 2 ? pg.table.size(0) : 0, Hkv = pg.k.size(2), D = pg.k.size(3);
+  pg.check(c, -1, S, false);
+  need(places > 0 && places < INT32_MAX && S > 0 && pg.k.numel() > 0);
+  const bool f32 = c.flag(7);
+  const auto options = pg.k.options().dtype(f32 ? at::kFloat : at::kBFloat16).requires_grad(false);
+  at::Tensor k = at::empty({S, places, Hkv, D}, options), v = at::empty({S, places, Hkv, D}, options);
+  CALL(ody_paged_read_q8, PAGED_Q8(pg), pg.table.data_ptr<int>(), pg.lengths.data_ptr<int>(), k.data_ptr(), v.data_ptr(), (int)S, (int)places, (int)Hkv, (int)D,
+       PAGED_Q8_STRIDES(pg), PAGED_Q8_SHAPE(pg), dt(k), (void*)c.stream);
+  return tuple(k, v);
+}
+
+// (q, k_pages, v_pages, k_scales, v_scales, page_table, lengths, scale, new_tokens or None) -> (out, lse)
+PyObject* paged_attn_q8(Call c) {
+  const at::Tensor& q = c.heads(0, nullptr);
+  PagedQ8 pg(c, 1);
+  const int S = q.size(0), n = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = pg.k.size(2);
+  pg.check(c, 8, S, q.requires_grad());
+  need(pg.k.size(3) == D && q.numel() > 0);
+  const float scale = (float)c.real(7);
+  at::Tensor out = make({S, n, Hq, D}, q), lse = make_f32({S, Hq, n}, q);
+  Scratch ws(lib.ody_paged_attn_q8_workspace_bytes(S, n, Hq, Hkv, D, pg.page_size(), pg.columns(), dt(q)), "paged_attn_workspace", q, own_scratch_fn);
+  CALL(ody_paged_attn_q8, q.data_ptr(), PAGED_Q8(pg), PAGED_TABLE(pg), out.data_ptr(), lse.data_ptr<float>(), S, n, Hq, Hkv, D, STRIDES(q), PAGED_Q8_STRIDES(pg),
+       STRIDES(out), PAGED_Q8_SHAPE(pg), scale, dt(q), ws.ptr(), ws.bytes, (void*)c.stream);
+  return tuple(out, lse);
+}
 
 // (qkv, n_heads, k_pages, v_pages, page_table, lengths, position_ids or None, inv_freq or None: no rotation, new_tokens or None) -> q
 PyObject* paged_append(Call c) {
@@ -657,7 +737,7 @@ PyMethodDef methods[] = {
     METHOD(rmsnorm_fwd, 3), METHOD(rmsnorm_bwd, 5), METHOD(gemm, 3), METHOD(linear_residual, 3), METHOD(linear_rope, 5), METHOD(linear_swiglu, 2),
     METHOD(linear_swiglu_h, 2), METHOD(linear_dgrad_swiglu, 3), METHOD(attn_fwd, 5), METHOD(attn_bwd, 13), METHOD(flash, 5), METHOD(rope, 6), METHOD(rope_table, 5),
     METHOD(norm_linear_rope, 8), METHOD(norm_linear_swiglu_h, 4),
-    METHOD(paged_append, 9), METHOD(paged_attn, 7),
+    METHOD(paged_append, 9), METHOD(paged_attn, 7), METHOD(paged_append_q8, 11), METHOD(paged_read_q8, 8), METHOD(paged_attn_q8, 9),
     METHOD(current_stream, 0), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_odysseus_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

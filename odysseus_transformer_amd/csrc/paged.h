@@ -17,7 +17,7 @@ struct PagedCache {
   int pages, shift, width;
   unsigned k_page, k_row, v_page, v_row;   // bytes from page to page and from row to row (paged_check: rows of a page lie within 4 GiB, as pages' starts do)
   PagedCache(void* k_, void* v_, const int* table_, const int* lengths_, const int* fresh_, PageStrides sk_, PageStrides sv_, int64_t table_stride_, int pages_, int page_size,
-             int width_, int dtype);
+             int width_, int value_bytes);
 };
 
 struct PagedAttnParams {
@@ -220,10 +220,12 @@ struct PagedPlace {
 };
 #endif
 
-// Host side: the checks that both entry points share.
-int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype, const PagedCache& c, int page_size);
-static inline bool paged_rows_aligned(const void* ptr, int64_t a, int64_t b, int64_t c, int dtype) {
-  const int q = dtype == ODY_BF16 ? 8 : 4;
+// Host side: the checks that the entry points share.
+static inline int paged_bytes(int dtype) { return dtype == ODY_BF16 ? 2 : 4; }
+// value_bytes: of a cached key's or value's component
+int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype, int value_bytes, const PagedCache& c, int page_size);
+static inline bool paged_rows_aligned(const void* ptr, int64_t a, int64_t b, int64_t c, int bytes) {
+  const int q = 16 / bytes;
   return ody_aligned16(ptr) && a % q == 0 && b % q == 0 && c % q == 0;
 }
 static inline int paged_shift(int page_size) { return page_size > 0 ? __builtin_ctz((unsigned)page_size) : 0; }

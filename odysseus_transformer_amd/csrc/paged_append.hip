@@ -103,14 +103,14 @@ int launch(const AppendParams& p, const PagedCache& cache, hipStream_t st) {
 }  // namespace
 
 PagedCache::PagedCache(void* k_, void* v_, const int* table_, const int* lengths_, const int* fresh_, PageStrides sk_, PageStrides sv_, int64_t table_stride_, int pages_,
-                       int page_size, int width_, int dtype)
+                       int page_size, int width_, int value_bytes)
     : k(k_), v(v_), table(table_), lengths(lengths_), fresh(fresh_), sk(sk_), sv(sv_), table_stride(table_stride_), pages(pages_), shift(paged_shift(page_size)),
       width(width_) {
-  const int64_t bytes = dtype == ODY_BF16 ? 2 : 4;
+  const int64_t bytes = value_bytes;
   k_page = (unsigned)(bytes * sk.p), k_row = (unsigned)(bytes * sk.r), v_page = (unsigned)(bytes * sv.p), v_row = (unsigned)(bytes * sv.r);
 }
 
-int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype, const PagedCache& c, int page_size) {
+int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype, int value_bytes, const PagedCache& c, int page_size) {
   ODY_REQUIRE(c.k && c.v && c.table && c.lengths, ODY_ERR_NULL, "%s: k_pages, v_pages, page_table or lengths is NULL", who);
   ODY_REQUIRE(S > 0 && n > 0 && Hq > 0 && Hkv > 0 && c.pages > 0 && c.width > 0, ODY_ERR_BAD_SHAPE,
               "%s: sizes must be positive (S=%d n=%d Hq=%d Hkv=%d pages=%d table_width=%d)", who, S, n, Hq, Hkv, c.pages, c.width);
@@ -124,12 +124,12 @@ int paged_check(const char* who, int S, int n, int Hq, int Hkv, int D, int dtype
   const int64_t heads = Hq + 2 * (int64_t)Hkv;
   ODY_REQUIRE(heads < ((int64_t)1 << 31) / 16 - 256 && (double)S * n * heads < (double)(((int64_t)1 << 31) - PAGED_WIDE_ROWS), ODY_ERR_BAD_SHAPE,
               "%s: %lld heads of a token, or heads of all new tokens together, are too many", who, (long long)heads);
-  const int64_t bytes = dtype == ODY_BF16 ? 2 : 4, most = (int64_t)1 << 32;
+  const int64_t bytes = value_bytes, most = (int64_t)1 << 32;
   for (const PageStrides& s : {c.sk, c.sv})
     ODY_REQUIRE(s.p >= 0 && s.r >= 0 && s.p < most / bytes && s.r < most / bytes / page_size, ODY_ERR_UNSUPPORTED,
                 "%s: pages, or the rows of a page, lie 4 GiB and more apart", who);
   ODY_REQUIRE(c.table_stride >= c.width || S == 1, ODY_ERR_BAD_SHAPE, "%s: rows of the page table overlap", who);
-  ODY_REQUIRE(paged_rows_aligned(c.k, c.sk.p, c.sk.r, c.sk.h, dtype) && paged_rows_aligned(c.v, c.sv.p, c.sv.r, c.sv.h, dtype), ODY_ERR_MISALIGNED,
+  ODY_REQUIRE(paged_rows_aligned(c.k, c.sk.p, c.sk.r, c.sk.h, value_bytes) && paged_rows_aligned(c.v, c.sv.p, c.sv.r, c.sv.h, value_bytes), ODY_ERR_MISALIGNED,
               "%s: k_pages and v_pages need 16-byte aligned pointers and strides", who);
   return ODY_OK;
 }
@@ -139,11 +139,11 @@ extern "C" int ody_paged_append(const void* qkv, void* q, void* k_pages, void* v
                                 int64_t sx_s, int64_t sx_n, int64_t sx_h, int64_t sq_s, int64_t sq_n, int64_t sq_h,
                                 int64_t sk_p, int64_t sk_r, int64_t sk_h, int64_t sv_p, int64_t sv_r, int64_t sv_h,
                                 int pages, int page_size, int table_width, int64_t table_stride, int dtype, void* stream) {
-  const PagedCache c(k_pages, v_pages, page_table, lengths, new_tokens, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride, pages, page_size, table_width, dtype);
-  if (int rc = paged_check("ody_paged_append", S, n, Hq, Hkv, D, dtype, c, page_size)) return rc;
+  const PagedCache c(k_pages, v_pages, page_table, lengths, new_tokens, {sk_p, sk_r, sk_h}, {sv_p, sv_r, sv_h}, table_stride, pages, page_size, table_width, paged_bytes(dtype));
+  if (int rc = paged_check("ody_paged_append", S, n, Hq, Hkv, D, dtype, paged_bytes(dtype), c, page_size)) return rc;
   ODY_REQUIRE((int64_t)S * n < (int64_t)1 << 24, ODY_ERR_BAD_SHAPE, "ody_paged_append: 2^24 new tokens and more (a block of 256 threads each)");
   ODY_REQUIRE(qkv && (q == nullptr || inv_freq), ODY_ERR_NULL, "ody_paged_append: qkv, or inv_freq of a rotation, is NULL");
-  ODY_REQUIRE(paged_rows_aligned(qkv, sx_s, sx_n, sx_h, dtype) && (q == nullptr || paged_rows_aligned(q, sq_s, sq_n, sq_h, dtype)), ODY_ERR_MISALIGNED,
+  ODY_REQUIRE(paged_rows_aligned(qkv, sx_s, sx_n, sx_h, paged_bytes(dtype)) && (q == nullptr || paged_rows_aligned(q, sq_s, sq_n, sq_h, paged_bytes(dtype))), ODY_ERR_MISALIGNED,
               "ody_paged_append: qkv and q need 16-byte aligned pointers and strides");
   const AppendParams p{qkv, q, position_ids, inv_freq, {sx_s, sx_n, sx_h}, {sq_s, sq_n, sq_h}, S, n, Hq, Hkv};
   hipStream_t st = static_cast<hipStream_t>(stream);

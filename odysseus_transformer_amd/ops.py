@@ -461,17 +461,21 @@ class _PartialResults:
 
 
 # --------------------------------------------------------------------------- key / value cache in pages
-def _check_paged(who: str, x, k_pages, v_pages, page_table, lengths, new_tokens) -> None:
-    """What the kernels of a paged cache cannot see: types, devices and shapes that fit `x` (S, n, heads, D), and that nobody waits for a gradient."""
+def _check_paged(who: str, x, k_pages, v_pages, page_table, lengths, new_tokens, scales=None) -> None:
+    """What the kernels of a paged cache cannot see: types, devices and shapes that fit `x` (S, n, heads, D), and that nobody waits for a gradient.
+    scales: of a cache in 8 bits."""
     _need_gpu(x, k_pages, v_pages, page_table, lengths, new_tokens)
     _dt(x)
+    dtype = x.dtype if scales is None else torch.float8_e4m3fn
     if x.dim() != 4 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != x.shape[3]:
         raise ValueError(f"{who}: (S, n, heads, D) tokens and (pages, page_size, kv heads, D) pages expected, got {tuple(x.shape)}, {tuple(k_pages.shape)} "
                          f"and {tuple(v_pages.shape)}")
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype != x.dtype or t.device != x.device:
-            raise ValueError(f"{who}: {name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
+        if t.dtype != dtype or t.device != x.device:
+            raise ValueError(f"{who}: {name} must be {dtype} on {x.device}, got {t.dtype} on {t.device}")
         _blhd(t, name)
+    if scales is not None:
+        _check_scales(who, k_pages, *scales)
     S = x.shape[0]
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != S or page_table.stride(1) != 1 or page_table.device != x.device:
         raise ValueError(f"{who}: page_table must be an int32 ({S}, columns) tensor on {x.device} with unit column stride, got {tuple(page_table.shape)} "
@@ -481,6 +485,17 @@ def _check_paged(who: str, x, k_pages, v_pages, page_table, lengths, new_tokens)
             raise ValueError(f"{who}: {name} must be a contiguous int32 ({S},) tensor on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError(f"{who} has no backward: a cache is for inference, call it under torch.no_grad() or on detached tensors")
+
+
+def _check_scales(who: str, k_pages, k_scales, v_scales) -> None:
+    """The scales of a cache in 8 bits, one for each block of tokens of a page and head."""
+    _need_gpu(k_scales, v_scales)
+    pages, page_size, Hkv, _ = k_pages.shape
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if t.dtype != torch.float8_e8m0fnu or t.device != k_pages.device:
+            raise ValueError(f"{who}: {name} must be {torch.float8_e8m0fnu} on {k_pages.device}, got {t.dtype} on {t.device}")
+        if t.dim() != 3 or t.shape != k_scales.shape or t.shape[0] != pages or t.shape[2] != Hkv or t.shape[1] == 0 or page_size % t.shape[1]:
+            raise ValueError(f"{who}: {name} must be ({pages}, blocks of a page, {Hkv}) for pages of {page_size}, got {tuple(t.shape)}")
 
 
 def paged_append_(qkv, n_heads: int, k_pages, v_pages, page_table, lengths, position_ids=None, base: float = 10000.0, inv_freq=None,
@@ -554,6 +569,99 @@ def paged_attn(q, k_pages, v_pages, page_table, lengths, scale: Optional[float] 
               *_blhd(q, "q"), *_blhd(k_pages, "k_pages"), *_blhd(v_pages, "v_pages"), *_blhd(out, "out"),
               k_pages.shape[0], k_pages.shape[1], page_table.shape[1], page_table.stride(0), scale, _dt(q), ws.data_ptr() if ws is not None else 0,
               ws_bytes, _stream())
+    return out, lse
+
+
+def paged_append_q8_(qkv, n_heads: int, k_pages, v_pages, k_scales, v_scales, page_table, lengths, position_ids=None, base: float = 10000.0,
+                     inv_freq=None, rotate: bool = True, new_tokens=None):
+    """paged_append_ into a cache that holds its values in 8 bits: k_pages, v_pages (pages, page_size, Hkv, D) float8_e4m3fn, k_scales, v_scales (pages,
+    page_size / block, Hkv) float8_e8m0fnu with any strides, one power of two for each block of tokens and head; block a power of two from 8 to 64.
+
+    A block's scale is the least power of two, from 2^-126 on, that takes the largest finite value of its tokens to 448 at most, and at least what it was
+    where the block holds earlier tokens: those are rounded to the new one if it rises, by a power of two, so that only values below 2^-6 of it change.
+    (Tokens that are taken back later leave the scale that they needed.)  Rotated keys are rounded once, to the nearest of the eight bits; a value that is
+    not finite becomes NaN.  Queries are as paged_append_ returns them, in qkv's type."""
+    if not rotate and position_ids is not None:
+        raise ValueError("paged_append_q8_: positions are for a rotation")
+    if qkv.is_cuda:
+        if inv_freq is None and rotate:
+            inv_freq = rope_inv_freq(qkv.shape[-1], base, qkv.device)
+        plain = native.paged_append_q8(qkv, n_heads, k_pages, v_pages, k_scales, v_scales, page_table, lengths, position_ids, inv_freq if rotate else None, new_tokens)
+        if plain is not None:
+            return plain
+    if qkv.is_cuda and qkv.device.index != torch.cuda.current_device():
+        with torch.cuda.device(qkv.device):
+            return paged_append_q8_(qkv, n_heads, k_pages, v_pages, k_scales, v_scales, page_table, lengths, position_ids, base, inv_freq, rotate, new_tokens)
+    _check_paged("paged_append_q8_", qkv, k_pages, v_pages, page_table, lengths, new_tokens, (k_scales, v_scales))
+    S, n, heads, D = qkv.shape
+    Hkv = k_pages.shape[2]
+    if n_heads <= 0 or heads != n_heads + 2 * Hkv:
+        raise ValueError(f"paged_append_q8_: {heads} heads are not {n_heads} query heads and {Hkv} heads of keys and of values")
+    if rotate:
+        check_rope_args(qkv, heads, position_ids, inv_freq)
+    q = torch.empty((S, n, n_heads, D), dtype=qkv.dtype, device=qkv.device) if rotate else qkv[:, :, :n_heads]
+    if qkv.numel() == 0:
+        return q
+    if rotate and position_ids is not None:
+        position_ids = position_ids.to(torch.int64).expand(S, n).contiguous()
+    _lib.call("ody_paged_append_q8", qkv.data_ptr(), q.data_ptr() if rotate else 0, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
+              v_scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), 0 if new_tokens is None else new_tokens.data_ptr(),
+              position_ids.data_ptr() if rotate and position_ids is not None else 0, inv_freq.data_ptr() if rotate else 0,
+              S, n, n_heads, Hkv, D, *_blhd(qkv, "qkv"), *_blhd(q, "q"), *_blhd(k_pages, "k_pages"), *_blhd(v_pages, "v_pages"),
+              *k_scales.stride(), *v_scales.stride(), k_pages.shape[0], k_pages.shape[1], k_pages.shape[1] // k_scales.shape[1], page_table.shape[1],
+              page_table.stride(0), _dt(qkv), _stream())
+    return q
+
+
+def paged_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, lengths, places: int, dtype=torch.bfloat16):
+    """What a cache in 8 bits holds (paged_append_q8_ says what the arguments are): -> k, v (S, places, Hkv, D) of `dtype` (bfloat16 or float32, exactly), the
+    values of each sequence's places 0 .. places - 1, 0 behind its length and where it has no page."""
+    if k_pages.is_cuda:
+        plain = native.paged_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, lengths, places, dtype == torch.float32) \
+            if dtype in (torch.bfloat16, torch.float32) else None
+        if plain is not None:
+            return plain
+    if k_pages.is_cuda and k_pages.device.index != torch.cuda.current_device():
+        with torch.cuda.device(k_pages.device):
+            return paged_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, lengths, places, dtype)
+    if places < 0 or page_table.dim() != 2 or k_pages.dim() != 4:
+        raise ValueError(f"paged_read_q8: (S, columns) pages and at least 0 places expected, got {tuple(page_table.shape)} and {places}")
+    S, (_, _, Hkv, D) = page_table.shape[0], k_pages.shape
+    k, v = torch.empty((2, S, places, Hkv, D), dtype=dtype, device=k_pages.device)
+    _check_paged("paged_read_q8", k, k_pages, v_pages, page_table, lengths, None, (k_scales, v_scales))
+    if k.numel() == 0:
+        return k, v
+    _lib.call("ody_paged_read_q8", k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+              k.data_ptr(), v.data_ptr(), S, places, Hkv, D, *_blhd(k_pages, "k_pages"), *_blhd(v_pages, "v_pages"), *k_scales.stride(), *v_scales.stride(),
+              k_pages.shape[0], k_pages.shape[1], k_pages.shape[1] // k_scales.shape[1], page_table.shape[1], page_table.stride(0), _dt(k), _stream())
+    return k, v
+
+
+def paged_attn_q8(q, k_pages, v_pages, k_scales, v_scales, page_table, lengths, scale: Optional[float] = None, new_tokens=None):
+    """paged_attn over a cache in 8 bits (paged_append_q8_ says what the arguments are); out has the queries' type."""
+    if q.is_cuda:
+        plain = native.paged_attn_q8(q, k_pages, v_pages, k_scales, v_scales, page_table, lengths, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale,
+                                     new_tokens)
+        if plain is not None:
+            return plain
+    if q.is_cuda and q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return paged_attn_q8(q, k_pages, v_pages, k_scales, v_scales, page_table, lengths, scale, new_tokens)
+    _check_paged("paged_attn_q8", q, k_pages, v_pages, page_table, lengths, new_tokens, (k_scales, v_scales))
+    S, n, Hq, D = q.shape
+    Hkv = k_pages.shape[2]
+    out = torch.empty((S, n, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((S, Hq, n), dtype=torch.float32, device=q.device)
+    if q.numel() == 0:
+        return out, lse
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    ws_bytes = _lib.load().ody_paged_attn_q8_workspace_bytes(S, n, Hq, Hkv, D, k_pages.shape[1], page_table.shape[1], _dt(q))
+    ws = _own_scratch(ws_bytes, "paged_attn_workspace", q.device) if ws_bytes else None
+    _lib.call("ody_paged_attn_q8", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(),
+              lengths.data_ptr(), 0 if new_tokens is None else new_tokens.data_ptr(), out.data_ptr(), lse.data_ptr(), S, n, Hq, Hkv, D,
+              *_blhd(q, "q"), *_blhd(k_pages, "k_pages"), *_blhd(v_pages, "v_pages"), *k_scales.stride(), *v_scales.stride(), *_blhd(out, "out"),
+              k_pages.shape[0], k_pages.shape[1], k_pages.shape[1] // k_scales.shape[1], page_table.shape[1], page_table.stride(0), scale, _dt(q),
+              ws.data_ptr() if ws is not None else 0, ws_bytes, _stream())
     return out, lse
 
 
