@@ -460,6 +460,21 @@ int ody_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, c
                       int64_t so_s, int64_t so_n, int64_t so_h, int pages, int page_size, int block, int table_width, int64_t table_stride,
                       float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- sampling --------------------------------------------------------------
+ * ody_sample  a token of each of `rows` rows of `vocab` logits (bf16 or fp32, rows row_stride elements apart), and its log-probability among what is kept, by a given
+ *             random number u (rows) from [0, 1).  The order of a row's tokens is by falling logits, the lower index first among equals; weights are exp((x - max) / temperature).
+ *             The first token is kept always; others while they are among the first top_k (0 or less: all), the weights before them sum up to less than top_p times those
+ *             of all that top_k keeps (1 or more: all), and their own is at least min_p (0 or less: all).  tokens (rows): the first in the order with which the
+ *             weights kept so far sum up to more than u times all that are kept; logprobs (rows): the logarithm of its share of those.  temperature 0, below 0 or NaN:
+ *             the first, with logprob 0.  NaN logits count as -inf; +inf ones are equals with all of the weight; a row of nothing but -inf gives -1 and -inf.
+ *             temperature, top_k, top_p, min_p: (rows) each, or NULL: the number for all.  Sums are of whole multiples of 2^(log2(vocab) - 62) or less, rounded up: the same
+ *             for any order of summation.  rows < 2^22, vocab <= 2^21 - 4; logits aligned to their size.
+ *             Reads 16-byte pieces that hold at least one logit of the row.
+ */
+int ody_sample(const void* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+               float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int rows, int vocab,
+               int64_t row_stride, int dtype, void* stream);
+
 /* ---- optimizer ------------------------------------------------------------
  * One step of torch.optim.AdamW (the optimizer of the reference's training loop, train.py:170,216) on one
  * tensor of n elements, in one pass instead of the host framework's seven element-wise passes:

@@ -40,7 +40,7 @@ namespace {
   X(ody_linear_dgrad_swiglu_workspace_bytes) X(ody_linear_dgrad_swiglu) X(ody_attn_fwd_workspace_bytes) X(ody_attn_fwd)           \
   X(ody_attn_bwd_workspace_bytes) X(ody_attn_bwd) X(ody_attn_bwd_rope) X(ody_rope) X(ody_rope_table)           \
   X(ody_norm_linear_rope) X(ody_norm_linear_swiglu_h) X(ody_paged_append) X(ody_paged_attn) X(ody_paged_attn_workspace_bytes) \
-  X(ody_paged_append_q8) X(ody_paged_read_q8) X(ody_paged_attn_q8) X(ody_paged_attn_q8_workspace_bytes)
+  X(ody_paged_append_q8) X(ody_paged_read_q8) X(ody_paged_attn_q8) X(ody_paged_attn_q8_workspace_bytes) X(ody_sample)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -687,6 +687,34 @@ PyObject* paged_attn(Call c) {
   return tuple(out, lse);
 }
 
+// (logits, u, temperature, top_k, top_p, min_p), of the last four numbers or tensors -> (tokens, logprobs)
+PyObject* sample(Call c) {
+  const at::Tensor& x = c.matrix(0, nullptr);
+  const int64_t rows = x.size(0), vocab = x.size(1);
+  need(rows > 0 && vocab > 0 && (rows == 1 || x.stride(0) >= vocab) && !(at::GradMode::is_enabled() && x.requires_grad()));
+  auto each = [&](Py_ssize_t i, at::ScalarType type) -> const void* {
+    const at::Tensor& t = c.any(i);
+    need(t.scalar_type() == type && t.dim() == 1 && t.size(0) == rows && t.is_contiguous());
+    return t.data_ptr();
+  };
+  const float* u = (const float*)each(1, at::kFloat);
+  const float* of_rows[4] = {};
+  double of_all[4] = {};
+  const double most[4] = {HUGE_VAL, INT32_MAX, 1.0, 1.0};
+  for (int k = 0; k < 4; k++) {
+    if (THPVariable_Check(c.args[2 + k])) {
+      of_rows[k] = (const float*)each(2 + k, k == 1 ? at::kInt : at::kFloat);
+    } else {
+      of_all[k] = k == 1 ? (double)c.whole(2 + k) : c.real(2 + k);
+      need(of_all[k] >= 0 && of_all[k] <= most[k]);
+    }
+  }
+  at::Tensor tokens = at::empty({rows}, x.options().dtype(at::kLong).requires_grad(false)), logprobs = make_f32({rows}, x);
+  CALL(ody_sample, x.data_ptr(), u, of_rows[0], (const int*)of_rows[1], of_rows[2], of_rows[3], (float)of_all[0], (int)of_all[1], (float)of_all[2], (float)of_all[3],
+       tokens.data_ptr<int64_t>(), logprobs.data_ptr<float>(), (int)rows, (int)vocab, x.stride(0), dt(x), (void*)c.stream);
+  return tuple(tokens, logprobs);
+}
+
 // the raw stream that the ops above launch on
 PyObject* current_stream(Call) {
   return PyLong_FromVoidPtr((void*)c10::hip::getCurrentHIPStream(c10::hip::current_device()).stream());
@@ -737,7 +765,7 @@ PyMethodDef methods[] = {
     METHOD(rmsnorm_fwd, 3), METHOD(rmsnorm_bwd, 5), METHOD(gemm, 3), METHOD(linear_residual, 3), METHOD(linear_rope, 5), METHOD(linear_swiglu, 2),
     METHOD(linear_swiglu_h, 2), METHOD(linear_dgrad_swiglu, 3), METHOD(attn_fwd, 5), METHOD(attn_bwd, 13), METHOD(flash, 5), METHOD(rope, 6), METHOD(rope_table, 5),
     METHOD(norm_linear_rope, 8), METHOD(norm_linear_swiglu_h, 4),
-    METHOD(paged_append, 9), METHOD(paged_attn, 7), METHOD(paged_append_q8, 11), METHOD(paged_read_q8, 8), METHOD(paged_attn_q8, 9),
+    METHOD(paged_append, 9), METHOD(paged_attn, 7), METHOD(paged_append_q8, 11), METHOD(paged_read_q8, 8), METHOD(paged_attn_q8, 9), METHOD(sample, 6),
     METHOD(current_stream, 0), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_odysseus_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -673,6 +673,58 @@ def _own_scratch(nbytes: int, name: str, device) -> torch.Tensor:
     return scratch(nbytes, name, device)
 
 
+# --------------------------------------------------------------------------- the next token
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A token of each row of logits (rows, vocab), bfloat16 or float32, rows any distance apart, and its log-probability, by random numbers u (rows) float32
+    from [0, 1) -> tokens (rows) int64, logprobs (rows) float32.
+
+    The order of a row's tokens is by falling logits, the lower index first among equals; weights are exp((logit - largest) / temperature).  The first is kept
+    always, the others while they are among the first top_k (0: all), the weights before them sum up to less than top_p of all that top_k keeps (1: all) and
+    their own is at least min_p (0: all).  The token is the first with which the weights kept so far exceed u of all that are kept; its log-probability is
+    that of its share.  Temperature 0 is the first token, of log-probability 0.
+
+    Each setting is a number, or a tensor (rows) on the device with one of each row: float32, top_k int32.  A row that is nothing but -inf gives token -1 and
+    log-probability -inf; NaN counts as -inf, and tokens of +inf share all of the weight.  Equal inputs give equal results, whatever the batch around them."""
+    if not torch.is_tensor(u):
+        raise TypeError(f"sample: u must be a tensor of random numbers, got {type(u).__name__}")
+    if logits.is_cuda:
+        plain = native.sample(logits, u, temperature, top_k, top_p, min_p)
+        if plain is not None:
+            return plain
+    if logits.is_cuda and logits.device.index != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return sample(logits, u, temperature, top_k, top_p, min_p)
+    _need_gpu(logits, u)
+    dt = _dt(logits)
+    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"sample: (rows, vocab) logits with unit column stride expected, got {tuple(logits.shape)} stride {logits.stride()}")
+    rows, vocab = logits.shape
+    if rows > 1 and logits.stride(0) < vocab:
+        raise ValueError(f"sample: rows of logits overlap (stride {logits.stride()})")
+    pointers, numbers = [], []
+    for name, v, dtype, least, most in (("u", u, torch.float32, 0, 0), ("temperature", temperature, torch.float32, 0.0, math.inf),
+                                        ("top_k", top_k, torch.int32, 0, 2 ** 31 - 1), ("top_p", top_p, torch.float32, 0.0, 1.0),
+                                        ("min_p", min_p, torch.float32, 0.0, 1.0)):
+        if torch.is_tensor(v):
+            _need_gpu(v)
+            if v.dtype != dtype or tuple(v.shape) != (rows,) or not v.is_contiguous() or v.device != logits.device:
+                raise ValueError(f"sample: {name} must be a contiguous {dtype} ({rows},) tensor on {logits.device}, got {tuple(v.shape)} {v.dtype} on {v.device}")
+            pointers.append(v.data_ptr())
+            numbers.append(0)
+        else:
+            if not least <= v <= most:
+                raise ValueError(f"sample: {name} must be from {least} to {most}, got {v}")
+            pointers.append(0)
+            numbers.append(int(v) if name == "top_k" else float(v))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise RuntimeError("sample has no backward: call it under torch.no_grad() or on detached logits")
+    tokens = torch.empty((rows,), dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+    if rows:
+        _lib.call("ody_sample", logits.data_ptr(), *pointers, *numbers[1:], tokens.data_ptr(), logprobs.data_ptr(), rows, vocab, logits.stride(0), dt, _stream())
+    return tokens, logprobs
+
+
 # --------------------------------------------------------------------------- linears
 def _rowmajor2d(t: torch.Tensor, name: str) -> int:
     if t.dim() != 2 or t.stride(1) != 1:
