@@ -74,8 +74,10 @@ __global__ __launch_bounds__(256) void paged_append_q8_kernel(const AppendParams
     for (int k = tid; k < tokens * HALF; k += 256) {
       const int t = k / HALF, j = k % HALF;
       const float at = p.pos ? (float)p.pos[(int64_t)s * p.n + i0 + t] : (float)(first + i0 + t), th = at * p.inv_freq[j];
-      cs[t][j] = rounded<T>(cosf(th));   // rounded to the values' type before use, as ody_rope has them
-      sn[t][j] = rounded<T>(sinf(th));
+      // rounded to the values' type before use, as ody_rope has them; from 64 bits, for a key on a border of its eight bits would show which way a cosine went
+      double sine, cosine;
+      sincos((double)th, &sine, &cosine);
+      cs[t][j] = rounded<T>((float)cosine), sn[t][j] = rounded<T>((float)sine);
     }
   }
 
