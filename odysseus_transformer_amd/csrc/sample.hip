@@ -2,15 +2,20 @@
 //
 // The order of a row's tokens is by falling logits, the lower index first among equals.  Each cut leaves a prefix of that order, and the token is where the sums of the
 // weights exp((x - max) / T) along it pass the random number's share of what is kept: all of it asks for one thing, the first token at which a sum along the order (of
-// tokens, or of weights) reaches a target.  No row is sorted for that.  Sums by buckets of x, 2048 of them, say which bucket the place is in; the bucket's tokens, a few as a
-// rule, are gathered and ordered; a bucket of too many tokens is divided anew, by the bits of x, until it has few or one value.  Where top_k is small, the buckets count tokens, what may be
-// among the first is gathered, and nothing else has a weight formed.
+// tokens, or of weights) reaches a target.  No row is sorted for that:
+//
+//   bf16   There are few values.  Tokens are counted by value -- 8192 of them, 32 octaves of either sign, from the largest that can have a weight down; the few tokens nearer to 0
+//          keep weights of their own -- and a weight is formed for each value and not for each token.
+//   fp32   Sums of the weights by buckets of x, 2048 of them, say which bucket the place is in; the bucket's tokens, a few as a rule, are gathered and ordered.  Where top_k is small the
+//          buckets count tokens, what may be among the first is gathered, and nothing else has a weight formed.
+//
+// What is gathered and too many to be ordered is divided by the bits of x, until it is few or has one value.
 //
 // Weights are whole numbers of 2^-FRAC (FRAC = 62 - log2 of the row's length, 45 for a vocabulary of 128000): sums in any order, by atomics too, are the same.  They are formed in 64 bits, whose
 // vector rate is that of 32 here, as 2^-(n / 1024) 2^(-r / 1024), |r| <= 1 / 2, from a table and a polynomial of the second degree: off by 2^-37 of themselves, so that a place is
 // missed where a random number is as near to a border of its share as that.
 //
-// A block has a row, which stays in its registers where it fits (1024 threads of 16 vectors) and is read again for each pass where not.
+// A block has a row and reads it in three passes or more, the first one from memory and the others from the caches.
 #include <algorithm>
 #include <cmath>
 #include "ody_common.h"
@@ -21,8 +26,8 @@ typedef unsigned long long u64;
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef const u32x4 __attribute__((address_space(1)))* vector_ptr;
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64, BUCKETS = 2048, LIST = 4096, OCTAVE = 1024;
-constexpr int MOST = (1 << 21) - 4;   // tokens of a row: nth_of() counts the matches of 16 wavefronts a turn in 2 * LIST numbers, at most 512 turns of 4 * THREADS tokens
+constexpr int THREADS = 512, WAVES = THREADS / 64, BUCKETS = 2048, LIST = 4096, OCTAVE = 1024, VALUES = 8192;
+constexpr int MOST = (1 << 21) - 4;   // tokens of a row: nth_of() counts the matches in each 64 vectors, of 4 values or 8, in 2 * LIST numbers
 
 struct SampleParams {
   const void* logits;
@@ -65,32 +70,19 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned k) { return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 // A row, in vectors of 16 bytes that hold at least one value of it.  What is not the row's counts as -inf, which has no weight and so is never a result.
-template <typename T, int NV>
+template <typename T>
 struct Row {
-  static constexpr int N = 16 / (int)sizeof(T);
+  static constexpr int N = 16 / (int)sizeof(T), AHEAD = 4;
+  static constexpr unsigned LOWEST = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
   const T* base;      // 16-byte aligned, at most N - 1 values before the row
   int head, vocab, vectors;
   bool infinite;      // the largest logit is +inf: those count as 0, all others as -inf
-  u32x4 held[NV > 0 ? NV : 1];
 
   __device__ __forceinline__ Row(const T* row, int vocab_) : vocab(vocab_), infinite(false) {
     head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     base = row - head;
     vectors = (head + vocab + N - 1) / N;
-    if constexpr (NV > 0) {
-#pragma unroll
-      for (int v = 0; v < NV; v++) {
-        const int at = v * THREADS + (int)threadIdx.x;
-        held[v] = at < vectors ? ((vector_ptr)base)[at] : u32x4{LOWEST, LOWEST, LOWEST, LOWEST};
-      }
-#pragma unroll
-      for (int v = 0; v < NV; v++) {
-        const int at = v * THREADS + (int)threadIdx.x;
-        if (at * N < head || (at + 1) * N > head + vocab) held[v] = without(held[v], at);
-      }
-    }
   }
-  static constexpr unsigned LOWEST = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
   __device__ __forceinline__ u32x4 without(u32x4 raw, int at) const {
     const int first = at * N - head;
 #pragma unroll
@@ -101,11 +93,6 @@ struct Row {
       }
     return raw;
   }
-  __device__ __forceinline__ static float element(const u32x4& raw, int e) {
-    const unsigned word = sizeof(T) == 2 ? raw[e / 2] : raw[e], bits = sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16;
-    return __builtin_bit_cast(float, bits);
-  }
-  __device__ __forceinline__ int index(int v, int e) const { return (v * THREADS + (int)threadIdx.x) * N - head + e; }
   __device__ __forceinline__ static u32x4 infinite_only(u32x4 raw) {
 #pragma unroll
     for (int w = 0; w < 4; w++) {
@@ -115,22 +102,9 @@ struct Row {
     }
     return raw;
   }
-  // the thread's vector of a turn, from memory
-  __device__ __forceinline__ u32x4 read(int v) const {
-    const int at = v * THREADS + (int)threadIdx.x;
-    u32x4 raw = {LOWEST, LOWEST, LOWEST, LOWEST};
-    if (at < vectors) {
-      raw = ((vector_ptr)base)[at];
-      if (at * N < head || (at + 1) * N > head + vocab) raw = without(raw, at);
-      if (infinite) raw = infinite_only(raw);
-    }
-    return raw;
-  }
-  // +inf is the largest: from now on
-  __device__ void only_infinite() {
-    infinite = true;
-#pragma unroll
-    for (int v = 0; v < NV; v++) held[v] = infinite_only(held[v]);
+  __device__ __forceinline__ static float element(const u32x4& raw, int e) {
+    const unsigned word = sizeof(T) == 2 ? raw[e / 2] : raw[e], bits = sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16;
+    return __builtin_bit_cast(float, bits);
   }
   // Element e, which no constant is.
   __device__ __forceinline__ static float any_element(const u32x4& raw, int e) {
@@ -138,52 +112,93 @@ struct Row {
     const unsigned word = at == 0 ? raw[0] : at == 1 ? raw[1] : at == 2 ? raw[2] : raw[3], bits = sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16;
     return __builtin_bit_cast(float, bits);
   }
+  __device__ __forceinline__ int index(int at, int e) const { return at * N - head + e; }
+  // What vector `at`, which was read, holds of the row.
+  __device__ __forceinline__ u32x4 of_row(u32x4 raw, int at) const {
+    if (at * N < head || (at + 1) * N > head + vocab) raw = without(raw, at);   // the first and the last one, and those behind
+    if (infinite) raw = infinite_only(raw);
+    return raw;
+  }
+  __device__ __forceinline__ u32x4 read(int at) const { return of_row(((vector_ptr)base)[min(at, vectors - 1)], at); }
+  // f(vector, its number) for each of a thread's vectors, AHEAD of them under way.  Threads without one in the last turn have what is nowhere in the row.
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    const int tid = threadIdx.x, turns = (vectors + THREADS - 1) / THREADS, last = min(tid, vectors - 1 - (turns - 1) * THREADS);
+    auto load = [&](int turn) __attribute__((always_inline)) { return ((vector_ptr)base + min(turn, turns - 1) * THREADS)[turn < turns - 1 ? tid : last]; };
+    u32x4 next[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) next[k] = load(k);
+    for (int turn = 0; turn < turns; turn += AHEAD) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; k++) {
+        if (turn + k >= turns) break;
+        u32x4 raw = next[k];
+        next[k] = load(turn + k + AHEAD);
+        const int at = (turn + k) * THREADS + tid;
+        if (turn + k == 0 || turn + k == turns - 1 || infinite) raw = of_row(raw, at);
+        f(raw, at);
+      }
+    }
+  }
+  // f(x, vector, element) for each value
+  template <typename F> __device__ __forceinline__ void all(F f) const {
+    each([&](const u32x4& raw, int at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < N; e++) f(element(raw, e), at, e);
+    });
+  }
   // f(x, index) for every x for which keep(x) holds, which are few
-  template <typename K, typename F> __device__ __forceinline__ void matches(K keep, F f) {
-    auto vector = [&](const u32x4& raw, int v) __attribute__((always_inline)) {
+  template <typename K, typename F> __device__ __forceinline__ void matches(K keep, F f) const {
+    each([&](const u32x4& raw, int at) __attribute__((always_inline)) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < N; e++) any |= keep(element(raw, e));
+      if (!any) return;
       unsigned mask = 0;
 #pragma unroll
       for (int e = 0; e < N; e++) mask |= keep(element(raw, e)) ? 1u << e : 0u;
       while (mask) {
         const int e = __ffs(mask) - 1;
         mask &= mask - 1;
-        int t = threadIdx.x;
-        asm volatile("" : "+v"(t));   // the index here, and not of all elements in front of it
-        f(any_element(raw, e), (v * THREADS + t) * N - head + e);
+        f(any_element(raw, e), index(at, e));
       }
-    };
-    if constexpr (NV > 0) {
+    });
+  }
+  // ---- bf16
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ u16x2 lower(u16x2 a, u16x2 b) { return __builtin_elementwise_min(a, b); }
+  // count[] by value, VALUES / 2 - 1 - d or VALUES / 2 + d for the bits base + d of the positive or the negative value.  Others, NaN among them, are not counted: bits below the base, of which
+  // `least` tells, positive ones beyond, of which `most` tells, and negative ones beyond.
+  __device__ __forceinline__ void count_values(unsigned* count, unsigned base, unsigned& least, int& most) const {
+    const u16x2 from = {(unsigned short)base, (unsigned short)base};
+    u16x2 l = {0xffff, 0xffff};
+    i16x2 g = {-0x8000, -0x8000};
+    each([&](const u32x4& raw, int) __attribute__((always_inline)) {
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        asm volatile("" : "+v"(held[v]));
-        vector(held[v], v);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int w = 0; w < 4; w++) {
+        const unsigned word = raw[w];
+        const i16x2 both = __builtin_bit_cast(i16x2, word);
+        const u16x2 size = __builtin_bit_cast(u16x2, word & 0x7fff7fffu), sign = __builtin_bit_cast(u16x2, both >> 15);
+        const u16x2 d = size - from, place = (u16x2){VALUES / 2 - 1, VALUES / 2 - 1} - (d ^ sign);
+        l = lower(l, size), g = __builtin_elementwise_max(g, both);
+        if (d[0] < VALUES / 2) atomicAdd(&count[place[0]], 1u);
+        if (d[1] < VALUES / 2) atomicAdd(&count[place[1]], 1u);
       }
-    } else {
-      for (int v = 0; v * THREADS < vectors; v++) vector(read(v), v);
-    }
+    });
+    least = min(l[0], l[1]), most = max(g[0], g[1]);
   }
-  // f(x, turn, element): index(turn, element) is the token's
-  template <typename F> __device__ __forceinline__ void turn(int v, F f) const {
-    const u32x4 raw = read(v);
+  // f(x, index) of every x with these bits, of which there are few
+  template <typename F> __device__ __forceinline__ void equals(unsigned bits, F f) const {
+    const unsigned both = bits << 16 | bits;
+    each([&](const u32x4& raw, int at) __attribute__((always_inline)) {
+      u16x2 l = {1, 1};
 #pragma unroll
-    for (int e = 0; e < N; e++) f(element(raw, e), v, e);
-  }
-  template <typename F> __device__ __forceinline__ void again(F f) const {   // for the seldom passes, whose code would be as long as the row
-    for (int v = 0; v * THREADS < vectors; v++) turn(v, f);
-  }
-  template <typename F> __device__ __forceinline__ void all(F f) {
-    if constexpr (NV > 0) {
+      for (int w = 0; w < 4; w++) l = lower(l, __builtin_bit_cast(u16x2, raw[w] ^ both));
+      if (l[0] && l[1]) return;
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        asm volatile("" : "+v"(held[v]));   // what one pass makes of a value is not kept for the next one: there are no registers for that
-#pragma unroll
-        for (int e = 0; e < N; e++) f(element(held[v], e), v, e);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-      again(f);
-    }
+      for (int e = 0; e < N; e++)
+        if ((e & 1 ? raw[e / 2] >> 16 : raw[e / 2] & 0xffff) == bits) f(element(raw, e), index(at, e));
+    });
   }
 };
 
@@ -235,38 +250,39 @@ __device__ __forceinline__ u64 read_lane(u64 x, int lane) {
 struct Shared {
   double table[OCTAVE];
   u64 mass[BUCKETS], finer[BUCKETS];        // of the first division, and of further ones
-  unsigned count[BUCKETS], finer_count[BUCKETS];
+  unsigned count[VALUES], finer_count[BUCKETS];
   u64 list[LIST], ordered[LIST];
   unsigned rank[256];
-  u64 wave[2][WAVES];
+  u64 wave[WAVES];
   float wave_max[WAVES];
-  u64 found[2], least;
-  unsigned words[4];
+  u64 found[2], least, small[2];
+  unsigned words[4], small_tokens;
 };
-static_assert(WAVES == 16, "a row of 16 lanes sums up the wavefronts");
+static_assert(WAVES <= 16, "a row of 16 lanes sums up the wavefronts");
 
-// Exclusive sum over the block; `all`: of all threads.  Calls take turns with `k`.
-__device__ __forceinline__ u64 block_scan(Shared& s, int k, u64 x, u64& all) {
+// Exclusive sum over the block; `all`: of all threads.
+__device__ __forceinline__ u64 block_scan(Shared& s, u64 x, u64& all) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const u64 upto = wave_scan(x);
-  if (lane == 63) s.wave[k][wave] = upto;
+  __syncthreads();   // a sum before this one has been read
+  if (lane == 63) s.wave[wave] = upto;
   __syncthreads();
-  const u64 waves = row_scan(s.wave[k][lane & 15]);
-  all = read_lane(waves, 15);
+  const u64 waves = row_scan(s.wave[lane & (WAVES - 1)]);
+  all = read_lane(waves, WAVES - 1);
   const u64 before = wave ? read_lane(waves, wave - 1) : 0;
   return before + upto - x;
 }
 
-template <typename T, int NV>
+template <typename T>
 struct Sampler {
   Shared& s;
-  Row<T, NV>& row;
+  Row<T>& row;
   Weights w;
 
   // s.list's n entries in rising order to s.ordered.
-  __device__ void order(int n) {
+  __device__ __forceinline__ void order(int n) {
     const int tid = threadIdx.x;
-    if (n <= 256) {   // by the number of smaller ones, which 1024 / 64, 1024 / 128 or 1024 / 256 threads count for each
+    if (n <= 256) {   // by the number of smaller ones, which THREADS / 64, / 128 or / 256 threads count for each
       const int size = n <= 64 ? 64 : n <= 128 ? 128 : 256, i = tid & (size - 1), parts = THREADS / size, part = tid / size, each = (n + parts - 1) / parts;
       if (tid < size) s.rank[tid] = 0;
       __syncthreads();
@@ -297,23 +313,24 @@ struct Sampler {
   }
 
   // Tokens for which keep(x) holds into s.list, as (falling key, index); how many there are, which may be more than fit.
-  template <bool AGAIN, typename F> __device__ __forceinline__ int gather(F keep) {
+  template <typename F> __device__ __forceinline__ int gather(F keep) {
+    return listed([&](auto take) __attribute__((always_inline)) { row.matches(keep, take); });
+  }
+  template <typename F> __device__ __forceinline__ int listed(F walk) {
     __syncthreads();
     if (threadIdx.x == 0) s.words[0] = 0;
     __syncthreads();
-    auto take = [&](float x, int i) __attribute__((always_inline)) {
+    walk([&](float x, int i) __attribute__((always_inline)) {
       const unsigned at = atomicAdd(&s.words[0], 1u);
       if (at < LIST) s.list[at] = (u64)~key_of(x) << 32 | (unsigned)i;
-    };
-    if constexpr (AGAIN) row.again([&](float x, int v, int e) { if (keep(x)) take(x, row.index(v, e)); });
-    else row.matches(keep, take);
+    });
     __syncthreads();
     return (int)s.words[0];
   }
 
   static constexpr int PER = LIST / THREADS;   // entries of the ordered list a thread
   // Sums of the weights up to and with each entry of a thread, `mass` before all of them; without an entry that of the one before.
-  __device__ u64 sums(int n, u64 mass, u64 (&upto)[PER], u64 (&was)[PER]) {
+  __device__ __forceinline__ u64 sums(int n, u64 mass, u64 (&upto)[PER], u64 (&was)[PER]) {
     u64 mine[PER], sum = 0, all;
 #pragma unroll
     for (int k = 0; k < PER; k++) {
@@ -321,18 +338,18 @@ struct Sampler {
       if (i < n) sum += w.of(of_key(~(unsigned)(s.ordered[i] >> 32)));
       mine[k] = sum;
     }
-    const u64 before = mass + block_scan(s, 0, sum, all);
+    const u64 before = mass + block_scan(s, sum, all);
 #pragma unroll
     for (int k = 0; k < PER; k++) upto[k] = before + mine[k], was[k] = k ? upto[k - 1] : before;
     return mass + all;
   }
   // The first of the n ordered entries at which the sum (of tokens, or of weights) behind `before` reaches the target: its entry, and the sum of weights up to and with it.
-  __device__ void reach(int n, bool by_count, u64 target, u64 count, u64 mass, u64& entry, u64& mass_upto) {
+  __device__ __forceinline__ void reach(int n, bool by_count, u64 target, u64 count, u64 mass, u64& entry, u64& mass_upto) {
     u64 upto[PER], was[PER];
     sums(n, mass, upto, was);
     find(n, by_count, target, count, upto, was, entry, mass_upto);
   }
-  __device__ void find(int n, bool by_count, u64 target, u64 count, const u64 (&upto)[PER], const u64 (&was)[PER], u64& entry, u64& mass_upto) {
+  __device__ __forceinline__ void find(int n, bool by_count, u64 target, u64 count, const u64 (&upto)[PER], const u64 (&was)[PER], u64& entry, u64& mass_upto) {
 #pragma unroll
     for (int k = 0; k < PER; k++) {
       const int i = threadIdx.x * PER + k;
@@ -342,91 +359,142 @@ struct Sampler {
     entry = s.found[0], mass_upto = s.found[1];
   }
 
-  // The bucket in which the sum reaches the target; the sums before it are added to `count` and `mass`.
-  __device__ int bucket_of(const u64* masses, const unsigned* counts, bool by_count, bool both, u64 target, u64& count, u64& mass) {
-    constexpr int EACH = BUCKETS / THREADS;
-    const int b0 = threadIdx.x * EACH;
-    u64 sum = 0, tokens = 0, all, c = count;
+  // Where the sum reaches the target among a thread's SLOTS of tokens and weights, `c` and `m` before them: the slot's number, first + k, to all, with the sums before it.
+  template <int SLOTS> __device__ __forceinline__ int slot_of(bool by_count, u64 target, int first, u64 c, u64 m, const unsigned (&tokens)[SLOTS], const u64 (&weights)[SLOTS], u64& count,
+                                                              u64& mass) {
     __syncthreads();
+    u64 weights_here = 0;
+    unsigned tokens_here = 0;
 #pragma unroll
-    for (int k = 0; k < EACH; k++) sum += masses[b0 + k], tokens += counts[b0 + k];
-    u64 m = mass + block_scan(s, 0, sum, all);
-    if (both) c += block_scan(s, 1, tokens, all);
+    for (int k = 0; k < SLOTS; k++) weights_here += weights[k], tokens_here += tokens[k];
+    if (by_count ? c < target && c + tokens_here >= target : m < target && m + weights_here >= target) {
 #pragma unroll
-    for (int k = 0; k < EACH; k++) {
-      const u64 m1 = m + masses[b0 + k], c1 = c + counts[b0 + k];
-      if (by_count ? c < target && c1 >= target : m < target && m1 >= target) s.words[1] = b0 + k, s.found[0] = c, s.found[1] = m;
-      m = m1, c = c1;
+      for (int k = 0; k < SLOTS; k++) {
+        const u64 m1 = m + weights[k], c1 = c + tokens[k];
+        if (by_count ? c < target && c1 >= target : m < target && m1 >= target) s.words[1] = first + k, s.found[0] = c, s.found[1] = m;
+        m = m1, c = c1;
+      }
     }
     __syncthreads();
     count = s.found[0], mass = s.found[1];
     return s.words[1];
   }
+  // ... among buckets, `count` and `mass` before them all
+  __device__ __forceinline__ int bucket_of(const u64* masses, const unsigned* counts, bool by_count, u64 target, u64& count, u64& mass) {
+    constexpr int EACH = BUCKETS / THREADS;
+    u64 weights[EACH], sum = 0, tokens = 0, all;
+    unsigned numbers[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const int b = threadIdx.x * EACH + k;
+      weights[k] = masses ? masses[b] : 0, numbers[k] = counts[b];
+      sum += weights[k], tokens += numbers[k];
+    }
+    const u64 m = masses ? mass + block_scan(s, sum, all) : 0, c = count + block_scan(s, tokens, all);
+    if (by_count && count + all < target) return BUCKETS;   // fewer than that are counted
+    return slot_of<EACH>(by_count, target, threadIdx.x * EACH, c, m, numbers, weights, count, mass);
+  }
 
   // The `nth` (from 1) token with this key, by its index.
-  __device__ int nth_of(unsigned key, unsigned nth) {
-    unsigned* counts = reinterpret_cast<unsigned*>(s.list);   // [turn][wavefront]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, turns = (row.vectors + THREADS - 1) / THREADS;
+  __device__ __forceinline__ int nth_of(unsigned key, unsigned nth) {
+    unsigned* counts = reinterpret_cast<unsigned*>(s.list);   // of each 64 vectors
+    const int lane = threadIdx.x & 63, groups = (row.vectors + 63) / 64;
     __syncthreads();
-    auto matches = [&](int turn, unsigned& mask) {
-      mask = 0;
-      row.turn(turn, [&](float x, int, int e) { if (key_of(x) == key) mask |= 1u << e; });
+    auto matches = [&](int group) {
+      unsigned mask = 0;
+      const int at = group * 64 + lane;
+      const u32x4 raw = row.read(at);
+#pragma unroll
+      for (int e = 0; e < row.N; e++) mask |= key_of(row.element(raw, e)) == key && at < row.vectors ? 1u << e : 0u;
+      return mask;
     };
-    for (int turn = 0; turn < turns; turn++) {
-      unsigned mask;
-      matches(turn, mask);
-      const unsigned upto = (unsigned)wave_scan(__popc(mask));
-      if (lane == 63) counts[turn * WAVES + wave] = upto;
+    for (int group = threadIdx.x / 64; group < groups; group += WAVES) {
+      const unsigned upto = (unsigned)wave_scan(__popc(matches(group)));
+      if (lane == 63) counts[group] = upto;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 64) {   // the first wavefront: the group, and the token in it
       unsigned left = nth;
-      int at = 0;
-      while (at < turns * WAVES - 1 && counts[at] < left) left -= counts[at++];
-      s.words[2] = at, s.words[3] = left;
-    }
-    __syncthreads();
-    const int turn = s.words[2] / WAVES;
-    if (wave == (int)s.words[2] % WAVES) {
-      unsigned mask;
-      matches(turn, mask);
+      int group = 0;
+      for (int g = 0; g < groups; g += 64) {
+        const unsigned mine = g + lane < groups ? counts[g + lane] : 0, upto = (unsigned)wave_scan(mine);
+        const u64 behind = __ballot(upto >= left);
+        if (behind) {
+          const int k = __ffsll(behind) - 1;
+          group = g + k, left -= __builtin_amdgcn_readlane(upto - mine, k);
+          break;
+        }
+        left -= __builtin_amdgcn_readlane(upto, 63);
+      }
+      unsigned mask = matches(group);
       const unsigned mine = __popc(mask), upto = (unsigned)wave_scan(mine);
-      unsigned left = s.words[3];
       if (upto - mine < left && upto >= left) {
         left -= upto - mine;
         while (--left) mask &= mask - 1;
-        s.words[1] = row.index(turn, __ffs(mask) - 1);
+        s.words[1] = row.index(group * 64 + lane, __ffs(mask) - 1);
       }
     }
     __syncthreads();
     return s.words[1];
   }
 
-  // Sum of the weights that are not less than `least`.
-  __device__ u64 heavy(u64 least) {
-    u64 sum = 0, all;
-    row.again([&](float x, int, int) {
-      const u64 wt = w.of(x);
-      if (wt >= least) sum += wt;
-    });
-    block_scan(s, 1, sum, all);
-    return all;
+  // The `nth` (from 1) token with logit x: its entry.
+  __device__ __forceinline__ u64 pick(float x, unsigned nth) {
+    int n;
+    const unsigned bits = __builtin_bit_cast(unsigned, x);
+    if (sizeof(T) == 2 && x != 0.f) n = listed([&](auto take) __attribute__((always_inline)) { row.equals(bits >> 16, take); });
+    else n = gather([&](float y) __attribute__((always_inline)) { return y == x; });
+    if (n <= LIST) {
+      order(n);
+      return s.ordered[nth - 1];
+    }
+    const unsigned key = key_of(x);
+    return (u64)~key << 32 | (unsigned)nth_of(key, nth);
   }
 
-  // Where the sum reaches the target, among the tokens of a bucket, `count` and `mass` before them: the entry (falling key, index), and the weights up to and with it.
-  __device__ void resolve(unsigned bucket, bool by_count, u64 target, u64 count, u64 mass, bool want_index, u64& entry, u64& mass_upto) {
-    const auto in = [&](float x) __attribute__((always_inline)) { return w.bucket(x) == bucket; };
-    int n = gather<false>(in);
+  // The least key for which holds(key), which holds for all from there up to `most`, for it too: 64 of them at once.
+  template <typename F> __device__ __forceinline__ static unsigned least_key(F holds, unsigned least, unsigned most, unsigned guess) {
+    const unsigned lane = threadIdx.x & 63;
+    if (guess > least && guess < most && guess - least > 31 && most - guess > 31) {   // 64 around what it should be
+      const u64 those = __ballot(holds(guess - 32 + lane));
+      if (those >> 63 && !(those & 1)) return guess - 33 + __ffsll(those);
+    }
+    while (most > least) {
+      const unsigned step = (most - least) / 64 + 1, at = least + lane * step;
+      const u64 those = __ballot(at >= most || at < least || holds(at));   // at < least: beyond 32 bits
+      const int k = those ? __ffsll(those) - 1 : 64;
+      if (k < 64) most = min(most, least + k * step);
+      if (k > 0) least += (k - 1) * step + 1;
+      else break;
+    }
+    return most;
+  }
+  // The values of a bucket: from lo to hi.
+  __device__ __forceinline__ void range_of(unsigned bucket, float& lo, float& hi) {
+    const double width = OCTAVE / 64 / w.c;
+    const unsigned top = key_of((float)w.top), bottom = key_of(-INFINITY);
+    auto guess = [&](unsigned b) { return key_of((float)(w.top - ((double)b - 0.5 / (OCTAVE / 64)) * width)); };
+    // the largest of the bucket is one below the least of the buckets in front of it
+    const unsigned first = least_key([&](unsigned k) { return w.bucket(of_key(k)) <= bucket; }, bottom, top, guess(bucket + 1));
+    const unsigned behind = bucket == 0 ? top + 1 : least_key([&](unsigned k) { return w.bucket(of_key(k)) < bucket; }, bottom, top, guess(bucket));
+    lo = of_key(first), hi = of_key(behind - 1);
+  }
+
+  // Where the sum reaches the target, among the tokens with logits from `from` to `to`, `count` and `mass` before them: the entry (falling key, index), and the weights up to and with it.
+  __device__ __forceinline__ void resolve(float from, float to, bool by_count, u64 target, u64 count, u64 mass, bool want_index, u64& entry, u64& mass_upto) {
+    const auto in = [&](float x) __attribute__((always_inline)) { return x >= from && x <= to; };
+    int n = gather(in);
     if (n <= LIST) {
       order(n);
       reach(n, by_count, target, count, mass, entry, mass_upto);
       return;
     }
-    // many: the keys that they lie between, and from there on by those
+    // many: by the bits of their keys, between the least and the largest of them
+    __syncthreads();
     if (threadIdx.x == 0) s.words[2] = ~0u, s.words[3] = 0;
     __syncthreads();
     unsigned lo = ~0u, hi = 0;
-    row.again([&](float x, int, int) {
+    row.all([&](float x, int, int) {
       if (in(x)) lo = min(lo, key_of(x)), hi = max(hi, key_of(x));
     });
     atomicMin(&s.words[2], lo);
@@ -444,17 +512,18 @@ struct Sampler {
       __syncthreads();
       for (int b = threadIdx.x; b < BUCKETS; b += THREADS) s.finer[b] = 0, s.finer_count[b] = 0;
       __syncthreads();
-      row.again([&](float x, int, int) {
+      row.all([&](float x, int, int) {
         const unsigned k = key_of(x);
         if (k >= lo && k <= hi) {
-          atomicAdd(&s.finer[(hi - k) >> shift], w.of(x));
+          if (const u64 wt = w.of(x)) atomicAdd(&s.finer[(hi - k) >> shift], wt);
           atomicAdd(&s.finer_count[(hi - k) >> shift], 1u);
         }
       });
-      const int b = bucket_of(s.finer, s.finer_count, by_count, true, target, count, mass);
+      __syncthreads();
+      const int b = bucket_of(s.finer, s.finer_count, by_count, target, count, mass);
       hi -= (unsigned)b << shift;
       if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1);
-      n = gather<true>([&](float x) { return key_of(x) >= lo && key_of(x) <= hi; });
+      n = gather([&](float x) { return key_of(x) >= lo && key_of(x) <= hi; });
       if (n <= LIST) {
         order(n);
         reach(n, by_count, target, count, mass, entry, mass_upto);
@@ -464,139 +533,291 @@ struct Sampler {
   }
 };
 
-template <typename T, int NV>
+// What a row is sampled by.
+struct Settings {
+  float temperature, top_p, min_p, u;
+  int top_k, frac;
+  bool cut_k, cut_p, cut_m;
+  u64 one, least;   // a weight of 1; the least weight that min_p keeps
+  __device__ __forceinline__ Settings(const SampleParams& p, int r)
+      : temperature(p.temperature ? p.temperature[r] : p.temperature_all), top_p(p.top_p ? p.top_p[r] : p.top_p_all), min_p(p.min_p ? p.min_p[r] : p.min_p_all), u(p.u[r]),
+        top_k(p.top_k ? p.top_k[r] : p.top_k_all), frac(p.frac), cut_k(top_k > 0 && top_k < p.vocab), cut_p(top_p < 1.f), cut_m(min_p > 0.f), one(1ull << p.frac),
+        least(cut_m ? (u64)fmin(ceil((double)min_p * (double)one), 9e18) : 0) {}
+  // the weights with which top_p is reached, of those kept so far, and the random number's
+  __device__ __forceinline__ u64 target_p(u64 kept) const { return max((u64)1, (u64)ceil(fmax((double)top_p, 0.0) * (double)kept)); }
+  __device__ __forceinline__ u64 target_u(u64 kept) const {
+    const double share = (double)u * (double)kept;
+    return share > 0.0 ? min((u64)fmin(share, 9e18) + 1, kept) : (u64)1;
+  }
+  __device__ __forceinline__ Weights weights(float top, const double* table) const {
+    return Weights{OCTAVE * 1.4426950408889634 / (double)temperature, (double)top, __builtin_bit_cast(double, (u64)(1023 + 52 - frac) << 52), top, table};
+  }
+};
+// The least entry's token, or none.
+__device__ __forceinline__ void write_first(const SampleParams& p, int r, bool none, u64 entry) {
+  if (threadIdx.x != 0) return;
+  p.tokens[r] = none ? -1 : (int64_t)(unsigned)entry;
+  p.logprobs[r] = none ? -INFINITY : 0.f;
+}
+__device__ __forceinline__ void write(const SampleParams& p, int r, const Weights& w, u64 entry, double log_kept) {
+  if (threadIdx.x != 0) return;
+  p.tokens[r] = (int64_t)(unsigned)entry;
+  const double log2w = -w.steps(of_key(~(unsigned)(entry >> 32))) / OCTAVE;
+  p.logprobs[r] = (float)((log2w + p.frac) * 0.6931471805599453 - log_kept);
+}
+// The largest of a row, for all threads.
+template <typename T> __device__ __forceinline__ float largest_of(const Row<T>& row, Shared& s) {
+  float x = -INFINITY;
+  row.all([&](float y, int, int) { x = fmaxf(x, y); });   // of a NaN and a number the number
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x = fmaxf(x, __shfl_xor(x, d, 64));
+  if ((threadIdx.x & 63) == 0) s.wave_max[threadIdx.x >> 6] = x;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < WAVES; k++) x = fmaxf(x, s.wave_max[k]);
+  return x;
+}
+__device__ __forceinline__ void fill_table(Shared& s) {
+  for (int j = threadIdx.x; j < OCTAVE; j += THREADS) s.table[j] = POWERS.x[0][j >> 5] * POWERS.x[1][j & 31];
+}
+
+// The window of counted values: bits base .. base + VALUES / 2 - 1 of either sign, below 2^most.
+__device__ __forceinline__ unsigned base_of(int most) { return (unsigned)max(1, (most + 127) * 128 - VALUES / 2); }
+constexpr int USUAL = 7;   // logits below 128: the largest need not be known to count them
+
+__global__ __launch_bounds__(THREADS) void sample_values_kernel(const SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  constexpr int EACH = VALUES / THREADS;   // values of a thread
+  const int r = blockIdx.x, tid = threadIdx.x;
+  Row<bf16> row(static_cast<const bf16*>(p.logits) + r * p.row_stride, p.vocab);
+  const Settings set(p, r);
+  fill_table(s);
+  if (tid == 0) s.small[0] = s.small[1] = 0, s.small_tokens = 0;
+
+  // ---- tokens by value, in a window that may have to be another one once the largest value is known
+  unsigned tokens[EACH + 1], base;   // of a thread's values, and of those next to 0 behind the last positive one
+  bool small;                        // there are such
+  float top = 0.f;
+  Sampler<bf16> a{s, row, {}};
+  int most = USUAL;
+  auto value = [&](int v) { return __builtin_bit_cast(float, v < VALUES / 2 ? (base + (VALUES / 2 - 1 - v)) << 16 : (base + (v - VALUES / 2)) << 16 | 0x80000000u); };
+  for (bool again = false;; again = true) {
+    base = base_of(most);
+    for (int b = tid; b < VALUES; b += THREADS) s.count[b] = 0;
+    if (tid == 0) s.words[0] = VALUES, s.words[1] = s.words[2] = 0;
+    __syncthreads();
+    unsigned least;
+    int greatest;
+    row.count_values(s.count, base, least, greatest);
+    if (__any(least < base)) s.words[1] = 1;
+    if (__any(greatest >= (int)base + VALUES / 2)) s.words[2] = 1;
+    __syncthreads();
+    unsigned first = VALUES;
+#pragma unroll
+    for (int k = EACH - 1; k >= 0; k--) {
+      tokens[k] = s.count[tid * EACH + k];
+      if (tokens[k]) first = tid * EACH + k;
+    }
+    if (again) break;
+    const u64 those = __ballot(first < VALUES);
+    if (those && (tid & 63) == __ffsll(those) - 1) atomicMin(&s.words[0], first);
+    __syncthreads();
+    first = s.words[0];
+    small = s.words[1];
+    const bool beyond = s.words[2];
+    const bool seen = !beyond && (first < VALUES / 2 || (!small && first < VALUES));
+    top = seen ? value(first) : largest_of(row, s);
+    if (top == -INFINITY || !(set.temperature > 0.f)) {   // nothing to choose from, or nothing but the first
+      write_first(p, r, top == -INFINITY, top == -INFINITY ? 0 : a.pick(top, 1));
+      return;
+    }
+    if (top == INFINITY) row.infinite = true, top = 0.f;
+    most = ilogb(fmin((double)fabsf(top) + 36.0 * (double)set.temperature, 0x1p127)) + 1;   // further from 0 there is none that has a weight
+    if (!beyond && !row.infinite && most <= USUAL) break;
+    __syncthreads();
+  }
+  small = s.words[1];
+  a.w = set.weights(top, s.table);
+  if (small) {
+    u64 mass = 0, over = 0;
+    unsigned count = 0;
+    row.matches([&](float x) { return (__builtin_bit_cast(unsigned, x) >> 16 & 0x7fff) < base; }, [&](float x, int) {
+      const u64 wt = a.w.of(x);
+      mass += wt, over += wt >= set.least ? wt : 0, count++;
+    });
+    if (count) {
+      atomicAdd(&s.small[0], mass), atomicAdd(&s.small[1], over);
+      atomicAdd(&s.small_tokens, count);
+    }
+    __syncthreads();
+  }
+  // ---- weights by value
+  u64 weights[EACH + 1], mass_here = 0, tokens_here = 0, over = 0, m, c = 0, all = 0, kept, entry = 0;
+  double log_kept = 0.0;   // of the first wavefront, under what the others do
+  unsigned some = 0;
+#pragma unroll
+  for (int k = 0; k < EACH; k++) some |= tokens[k], weights[k] = 0;
+  if (__any(some != 0))
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const u64 wt = a.w.of(value(tid * EACH + k));
+      weights[k] = wt * tokens[k];
+      mass_here += weights[k], tokens_here += tokens[k], over += wt >= set.least ? weights[k] : 0;
+    }
+  const bool next_to_0 = tid == VALUES / 2 / EACH - 1;
+  tokens[EACH] = next_to_0 ? s.small_tokens : 0, weights[EACH] = next_to_0 ? s.small[0] : 0;
+  mass_here += weights[EACH], tokens_here += tokens[EACH];
+  m = block_scan(s, mass_here, kept);
+  if (set.cut_k) c = block_scan(s, tokens_here, all);
+  if (set.cut_m) {
+    u64 heavy;
+    block_scan(s, over, heavy);
+    over = max(set.one, heavy + s.small[1]);   // the first one at any rate
+  }
+  // ---- the cuts, then the token
+  const unsigned key_small = key_of(__builtin_bit_cast(float, (base - 1) << 16));
+  for (int step = set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
+    if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
+    if (step == 1 && !set.cut_p) continue;
+    if (step == 2) {
+      if (set.cut_m) kept = min(kept, over);
+      if (tid < 64) log_kept = log((double)kept);
+    }
+    const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
+    u64 count = 0, mass = 0, upto;
+    // the slots of a thread are EACH + 1 numbers apart
+    const int slot = a.slot_of<EACH + 1>(step == 0, target, tid * (EACH + 1), c, m, tokens, weights, count, mass);
+    if (slot % (EACH + 1) == EACH) {
+      a.resolve(of_key(~key_small), of_key(key_small), step == 0, target, count, mass, step == 2, entry, upto);
+    } else {
+      const float x = value(slot / (EACH + 1) * EACH + slot % (EACH + 1));
+      const u64 wt = a.w.of(x), nth = step == 0 ? target - count : (target - mass + wt - 1) / wt;
+      upto = mass + nth * wt;
+      if (step == 2) entry = a.pick(x, (unsigned)nth);
+    }
+    if (step < 2) kept = min(kept, upto);
+  }
+  write(p, r, a.w, entry, log_kept);
+}
+
+// ---- fp32
 __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Row<T, NV> row(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
-  const float temperature = p.temperature ? p.temperature[r] : p.temperature_all, top_p = p.top_p ? p.top_p[r] : p.top_p_all,
-              min_p = p.min_p ? p.min_p[r] : p.min_p_all, u = p.u[r];
-  const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
-  s.table[tid] = POWERS.x[0][tid >> 5] * POWERS.x[1][tid & 31];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  Row<float> row(static_cast<const float*>(p.logits) + r * p.row_stride, p.vocab);
+  const Settings set(p, r);
+  fill_table(s);
   for (int b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0, s.count[b] = 0;
-  static_assert(OCTAVE == THREADS, "a thread for each entry");
-
-  float largest = -INFINITY;
-  row.all([&](float x, int, int) { largest = fmaxf(largest, x); });   // of a NaN and a number the number
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, d, 64));
-  if (lane == 0) s.wave_max[wave] = largest;
-  if (tid == 0) s.words[1] = 0x7fffffff, s.least = ~0ull;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < WAVES; k++) largest = fmaxf(largest, s.wave_max[k]);
-  if (largest == -INFINITY || !(temperature > 0.f)) {   // nothing to choose from, or nothing but the first
-    if (largest != -INFINITY) {
-      int at = 0x7fffffff;
-      row.again([&](float x, int v, int e) { if (x == largest) at = min(at, row.index(v, e)); });
-      if (at != 0x7fffffff) atomicMin(&s.words[1], (unsigned)at);
-      __syncthreads();
-    }
-    if (tid == 0) {
-      p.tokens[r] = largest == -INFINITY ? -1 : (int64_t)s.words[1];
-      p.logprobs[r] = largest == -INFINITY ? -INFINITY : 0.f;
-    }
+  float largest = largest_of(row, s);
+  Sampler<float> a{s, row, set.weights(largest, s.table)};
+  if (largest == -INFINITY || !(set.temperature > 0.f)) {   // nothing to choose from, or nothing but the first
+    write_first(p, r, largest == -INFINITY, largest == -INFINITY ? 0 : a.pick(largest, 1));
     return;
   }
   if (largest == INFINITY) {
-    row.only_infinite();
-    largest = 0.f;
+    row.infinite = true;
+    a.w = set.weights(0.f, s.table);
   }
-  Sampler<T, NV> a{s, row, Weights{OCTAVE * 1.4426950408889634 / (double)temperature, (double)largest, __builtin_bit_cast(double, (u64)(1023 + 52 - p.frac) << 52), largest, s.table}};
-  const u64 one = 1ull << p.frac;
-  const bool cut_k = top_k > 0 && top_k < p.vocab, cut_p = top_p < 1.f, cut_m = min_p > 0.f;
-  const u64 least = cut_m ? (u64)fmin(ceil((double)min_p * (double)one), 9e18) : 0;
-  auto target_p = [&](u64 kept) { return max((u64)1, (u64)ceil(fmax((double)top_p, 0.0) * (double)kept)); };
-  auto target_u = [&](u64 kept) {
-    const double share = (double)u * (double)kept;
-    return share > 0.0 ? min((u64)fmin(share, 9e18) + 1, kept) : (u64)1;
-  };
   u64 entry = 0, kept = 0;
-
+  double log_kept = 0.0;   // of the first wavefront, under what the others do
   // ---- few: all that may be among the first top_k into the list
-  bool few = cut_k && top_k <= LIST / 2;
+  bool few = set.cut_k && set.top_k <= LIST / 2;
   if (few) {
-    row.all([&](float x, int, int) { atomicAdd(&s.count[a.w.plain_bucket(x)], 1u); });
+    row.all([&](float x, int, int) {
+      const unsigned b = a.w.plain_bucket(x);
+      if (b < BUCKETS - 1) atomicAdd(&s.count[b], 1u);
+    });
     u64 count = 0, mass = 0;
-    const unsigned last = a.bucket_of(s.mass, s.count, true, true, top_k, count, mass);
-    const int n = a.template gather<false>([&](float x) { return a.w.plain_bucket(x) <= last; });
+    __syncthreads();
+    const int last = a.bucket_of(nullptr, s.count, true, set.top_k, count, mass);
+    int n = LIST + 1;
+    if (last < BUCKETS) n = a.gather([&](float x) { return a.w.plain_bucket(x) <= (unsigned)last; });
     few = n <= LIST;
     if (few) {
       a.order(n);
-      const int k = min(n, top_k);
+      const int k = min(n, set.top_k);
       u64 upto[a.PER], was[a.PER], upto_p;
       kept = a.sums(k, 0, upto, was);
-      if (cut_p) {
-        a.find(k, false, target_p(kept), 0, upto, was, entry, upto_p);
+      if (set.cut_p) {
+        a.find(k, false, set.target_p(kept), 0, upto, was, entry, upto_p);
         kept = min(kept, upto_p);
       }
-      if (cut_m) {   // up to the last one that is heavy enough
-        u64 over = one;
+      if (set.cut_m) {   // up to the last one that is heavy enough
+        u64 over = set.one;
 #pragma unroll
         for (int j = 0; j < a.PER; j++)
-          if (tid * a.PER + j < k && upto[j] - was[j] >= least) over = max(over, upto[j]);
-        __syncthreads();
+          if (tid * a.PER + j < k && upto[j] - was[j] >= set.least) over = max(over, upto[j]);
         if (tid == 0) s.least = 0;
         __syncthreads();
         atomicMax(&s.least, over);
         __syncthreads();
         kept = min(kept, s.least);
       }
+      if (tid < 64) log_kept = log((double)kept);
       __syncthreads();
-      a.find(k, false, target_u(kept), 0, upto, was, entry, upto_p);
+      a.find(k, false, set.target_u(kept), 0, upto, was, entry, upto_p);
     } else {
       __syncthreads();
       for (int b = tid; b < BUCKETS; b += THREADS) s.count[b] = 0;
+      __syncthreads();
     }
   }
-
   // ---- sums of the weights by buckets of all
   if (!few) {
+    u64 over = 0;   // of weights that are not less than min_p
+    if (set.cut_m)
+      row.all([&](float x, int, int) {
+        unsigned b;
+        const u64 wt = a.w.of(x, b);
+        if (wt) atomicAdd(&s.mass[b], wt);
+        over += wt >= set.least ? wt : 0;
+      });
+    else
+      row.all([&](float x, int, int) {
+        unsigned b;
+        if (const u64 wt = a.w.of(x, b)) atomicAdd(&s.mass[b], wt);
+      });
+    if (set.cut_k) row.all([&](float x, int, int) { if (a.w.of(x)) atomicAdd(&s.count[a.w.bucket(x)], 1u); });
     __syncthreads();
-    row.all([&](float x, int, int) {
-      unsigned b;
-      const u64 wt = a.w.of(x, b);
-      atomicAdd(&s.mass[b], wt);
-    });
-    if (cut_k) row.again([&](float x, int, int) { atomicAdd(&s.count[a.w.bucket(x)], 1u); });
-    __syncthreads();
-    u64 sum = 0, over = 0;
-    for (int b = tid; b < BUCKETS; b += THREADS) sum += s.mass[b];
-    block_scan(s, 0, sum, kept);
-    if (cut_m) over = max(one, a.heavy(least));   // the first one at any rate
-    for (int step = cut_k ? 0 : cut_p ? 1 : 2; step < 3; step++) {
-      if (step == 1 && !cut_p) continue;
-      if (step == 2 && cut_m) kept = min(kept, over);
-      const u64 target = step == 0 ? (u64)top_k : step == 1 ? target_p(kept) : target_u(kept);
+    constexpr int EACH = BUCKETS / THREADS;
+    unsigned tokens[EACH];
+    u64 weights[EACH], mass_here = 0, tokens_here = 0, m, c = 0, all = 0, heavy;
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      weights[k] = s.mass[tid * EACH + k], tokens[k] = s.count[tid * EACH + k];
+      mass_here += weights[k], tokens_here += tokens[k];
+    }
+    m = block_scan(s, mass_here, kept);
+    if (set.cut_k) c = block_scan(s, tokens_here, all);
+    if (set.cut_m) {
+      block_scan(s, over, heavy);
+      over = max(set.one, heavy);   // the first one at any rate
+    }
+    for (int step = set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
+      if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
+      if (step == 1 && !set.cut_p) continue;
+      if (step == 2) {
+        if (set.cut_m) kept = min(kept, over);
+        if (tid < 64) log_kept = log((double)kept);
+      }
+      const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
       u64 count = 0, mass = 0, upto;
-      __syncthreads();
-      const unsigned b = a.bucket_of(s.mass, s.count, step == 0, step == 0, target, count, mass);
-      a.resolve(b, step == 0, target, count, mass, step == 2, entry, upto);
+      const unsigned b = a.template slot_of<EACH>(step == 0, target, tid * EACH, c, m, tokens, weights, count, mass);
+      float lo, hi;
+      a.range_of(b, lo, hi);
+      a.resolve(lo, hi, step == 0, target, count, mass, step == 2, entry, upto);
       if (step < 2) kept = min(kept, upto);
     }
   }
-  if (tid == 0) {
-    p.tokens[r] = (int64_t)(unsigned)entry;
-    const double log2w = -a.w.steps(of_key(~(unsigned)(entry >> 32))) / OCTAVE;
-    p.logprobs[r] = (float)((log2w + p.frac) * 0.6931471805599453 - log((double)kept));
-  }
+  write(p, r, a.w, entry, log_kept);
 }
 
-template <typename T, int NV>
-int launch(const SampleParams& p, int rows, hipStream_t st) {
-  if (int rc = ody_allow_dynamic_lds(reinterpret_cast<const void*>(&sample_kernel<T, NV>), sizeof(Shared), "ody_sample")) return rc;
-  ODY_LAUNCH("sample", st, (sample_kernel<T, NV>), dim3((unsigned)rows), dim3(THREADS), sizeof(Shared), p);
+template <typename K> int launch(K kernel, const SampleParams& p, int rows, hipStream_t st) {
+  if (int rc = ody_allow_dynamic_lds(reinterpret_cast<const void*>(kernel), sizeof(Shared), "ody_sample")) return rc;
+  ODY_LAUNCH("sample", st, kernel, dim3((unsigned)rows), dim3(THREADS), sizeof(Shared), p);
   return ody_check_launch("sample");
-}
-template <typename T>
-int by_length(const SampleParams& p, int rows, hipStream_t st) {
-  constexpr int N = 16 / (int)sizeof(T);
-  const int turns = (p.vocab + 2 * N - 2 + THREADS * N - 1) / (THREADS * N);   // however rows are aligned
-  if (turns <= 4) return launch<T, 4>(p, rows, st);
-  if (turns <= 8) return launch<T, 8>(p, rows, st);
-  if (turns <= 16) return launch<T, 16>(p, rows, st);
-  return launch<T, 0>(p, rows, st);
 }
 
 }  // namespace
@@ -614,5 +835,5 @@ extern "C" int ody_sample(const void* logits, const float* u, const float* tempe
   const SampleParams p{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, tokens, logprobs, vocab,
                        std::min(50, 62 - bits)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == ODY_BF16 ? by_length<bf16>(p, rows, st) : by_length<float>(p, rows, st);
+  return dtype == ODY_BF16 ? launch(&sample_values_kernel, p, rows, st) : launch(&sample_kernel, p, rows, st);
 }
