@@ -41,26 +41,6 @@ struct SampleParams {
   int vocab, frac;
 };
 
-// 2^(-j / 32) and 2^(-j / 1024)
-struct Table { double x[2][32]; };
-constexpr Table powers() {
-  Table t{};
-  double root[10] = {}, of = 0.5;   // 2^(-1/2), 2^(-1/4) ..: by Newton's iteration
-  for (int k = 0; k < 10; k++) {
-    double y = of;
-    for (int i = 0; i < 60; i++) y = 0.5 * (y + of / y);
-    root[k] = of = y;
-  }
-  for (int half = 0; half < 2; half++)
-    for (int j = 0; j < 32; j++) {
-      t.x[half][j] = 1.0;
-      for (int k = 0; k < 5; k++)
-        if (j >> (4 - k) & 1) t.x[half][j] *= root[5 * half + k];
-    }
-  return t;
-}
-__device__ const Table POWERS = powers();
-
 // x as a number whose order is that of the logits: -0 as 0, NaN as the lowest
 __device__ __forceinline__ unsigned key_of(float x) {
   x = x == x ? x + 0.f : -INFINITY;
@@ -70,18 +50,30 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned k) { return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 // A row, in vectors of 16 bytes that hold at least one value of it.  What is not the row's counts as -inf, which has no weight and so is never a result.
-template <typename T>
+template <typename T, int NV = 0>
 struct Row {
-  static constexpr int N = 16 / (int)sizeof(T), AHEAD = 4;
+  static constexpr int N = 16 / (int)sizeof(T), AHEAD = 4;   // values of a vector; vectors under way, where they are read for each pass
   static constexpr unsigned LOWEST = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
   const T* base;      // 16-byte aligned, at most N - 1 values before the row
   int head, vocab, vectors;
-  bool infinite;      // the largest logit is +inf: those count as 0, all others as -inf
+  u32x4 held[NV > 0 ? NV : 1];   // NV: the thread's vectors, all of them, read once
 
-  __device__ __forceinline__ Row(const T* row, int vocab_) : vocab(vocab_), infinite(false) {
+  __device__ __forceinline__ Row(const T* row, int vocab_) : vocab(vocab_) {
     head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     base = row - head;
     vectors = (head + vocab + N - 1) / N;
+    if constexpr (NV > 0) {
+      const int tid = threadIdx.x;
+#pragma unroll
+      for (int k = 0; k < NV; k++) held[k] = ((vector_ptr)base)[min(k * THREADS + tid, vectors - 1)];
+      if (tid == 0) held[0] = without(held[0], 0);
+      const u32x4 last = without(((vector_ptr)base)[vectors - 1], vectors - 1), none = {LOWEST, LOWEST, LOWEST, LOWEST};
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        const int at = k * THREADS + tid;
+        if ((k + 1) * THREADS >= vectors) held[k] = at < vectors - 1 ? held[k] : at == vectors - 1 ? last : none;
+      }
+    }
   }
   __device__ __forceinline__ u32x4 without(u32x4 raw, int at) const {
     const int first = at * N - head;
@@ -91,15 +83,6 @@ struct Row {
         if (sizeof(T) == 4) raw[e] = LOWEST;
         else raw[e / 2] = e & 1 ? (raw[e / 2] & 0xffffu) | (LOWEST & 0xffff0000u) : (raw[e / 2] & 0xffff0000u) | (LOWEST & 0xffffu);
       }
-    return raw;
-  }
-  __device__ __forceinline__ static u32x4 infinite_only(u32x4 raw) {
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      const unsigned x = raw[w];
-      if (sizeof(T) == 4) raw[w] = x == 0x7f800000u ? 0u : LOWEST;
-      else raw[w] = ((x & 0xffffu) == 0x7f80u ? 0u : LOWEST & 0xffffu) | ((x & 0xffff0000u) == 0x7f800000u ? 0u : LOWEST & 0xffff0000u);
-    }
     return raw;
   }
   __device__ __forceinline__ static float element(const u32x4& raw, int e) {
@@ -116,12 +99,24 @@ struct Row {
   // What vector `at`, which was read, holds of the row.
   __device__ __forceinline__ u32x4 of_row(u32x4 raw, int at) const {
     if (at * N < head || (at + 1) * N > head + vocab) raw = without(raw, at);   // the first and the last one, and those behind
-    if (infinite) raw = infinite_only(raw);
     return raw;
   }
   __device__ __forceinline__ u32x4 read(int at) const { return of_row(((vector_ptr)base)[min(at, vectors - 1)], at); }
   // f(vector, its number) for each of a thread's vectors, AHEAD of them under way.  Threads without one in the last turn have what is nowhere in the row.
-  template <typename F> __device__ __forceinline__ void each(F f) const {
+  // f(vector, turn) for each of a thread's vectors, which are THREADS apart
+  template <typename F> __device__ __forceinline__ void each(F f) {
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        asm volatile("" : "+v"(held[k]));   // what one pass makes of a vector is not kept for the next one
+        f(held[k], k);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      again([&](const u32x4& raw, int at) __attribute__((always_inline)) { f(raw, at / THREADS); });
+    }
+  }
+  template <typename F> __device__ __forceinline__ void again(F f) const {   // from memory; code of one length for all rows
     const int tid = threadIdx.x, turns = (vectors + THREADS - 1) / THREADS, last = min(tid, vectors - 1 - (turns - 1) * THREADS);
     auto load = [&](int turn) __attribute__((always_inline)) { return ((vector_ptr)base + min(turn, turns - 1) * THREADS)[turn < turns - 1 ? tid : last]; };
     u32x4 next[AHEAD];
@@ -134,21 +129,21 @@ struct Row {
         u32x4 raw = next[k];
         next[k] = load(turn + k + AHEAD);
         const int at = (turn + k) * THREADS + tid;
-        if (turn + k == 0 || turn + k == turns - 1 || infinite) raw = of_row(raw, at);
+        if (turn + k == 0 || turn + k == turns - 1) raw = of_row(raw, at);
         f(raw, at);
       }
     }
   }
   // f(x, vector, element) for each value
   template <typename F> __device__ __forceinline__ void all(F f) const {
-    each([&](const u32x4& raw, int at) __attribute__((always_inline)) {
+    again([&](const u32x4& raw, int at) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < N; e++) f(element(raw, e), at, e);
     });
   }
   // f(x, index) for every x for which keep(x) holds, which are few
   template <typename K, typename F> __device__ __forceinline__ void matches(K keep, F f) const {
-    each([&](const u32x4& raw, int at) __attribute__((always_inline)) {
+    again([&](const u32x4& raw, int at) __attribute__((always_inline)) {
       bool any = false;
 #pragma unroll
       for (int e = 0; e < N; e++) any |= keep(element(raw, e));
@@ -169,7 +164,7 @@ struct Row {
   static __device__ __forceinline__ u16x2 lower(u16x2 a, u16x2 b) { return __builtin_elementwise_min(a, b); }
   // count[] by value, VALUES / 2 - 1 - d or VALUES / 2 + d for the bits base + d of the positive or the negative value.  Others, NaN among them, are not counted: bits below the base, of which
   // `least` tells, positive ones beyond, of which `most` tells, and negative ones beyond.
-  __device__ __forceinline__ void count_values(unsigned* count, unsigned base, unsigned& least, int& most) const {
+  __device__ __forceinline__ void count_values(unsigned* count, unsigned base, unsigned& least, int& most) {
     const u16x2 from = {(unsigned short)base, (unsigned short)base};
     u16x2 l = {0xffff, 0xffff};
     i16x2 g = {-0x8000, -0x8000};
@@ -187,18 +182,35 @@ struct Row {
     });
     least = min(l[0], l[1]), most = max(g[0], g[1]);
   }
-  // f(x, index) of every x with these bits, of which there are few
-  template <typename F> __device__ __forceinline__ void equals(unsigned bits, F f) const {
+  // f(x, index) of every x with these bits, of which there are few: the vectors that have one are read again
+  template <typename F> __device__ __forceinline__ void equals(unsigned bits, F f) {
     const unsigned both = bits << 16 | bits;
-    each([&](const u32x4& raw, int at) __attribute__((always_inline)) {
+    auto one = [&](const u32x4& raw) __attribute__((always_inline)) {
       u16x2 l = {1, 1};
 #pragma unroll
       for (int w = 0; w < 4; w++) l = lower(l, __builtin_bit_cast(u16x2, raw[w] ^ both));
-      if (l[0] && l[1]) return;
+      return l[0] == 0 || l[1] == 0;
+    };
+    auto take = [&](const u32x4& raw, int at) __attribute__((always_inline)) {
+      unsigned mask = 0;
 #pragma unroll
-      for (int e = 0; e < N; e++)
-        if ((e & 1 ? raw[e / 2] >> 16 : raw[e / 2] & 0xffff) == bits) f(element(raw, e), index(at, e));
-    });
+      for (int w = 0; w < 4; w++) mask |= ((raw[w] ^ both) << 16 ? 0u : 1u << 2 * w) | ((raw[w] ^ both) >> 16 ? 0u : 2u << 2 * w);
+      while (mask) {
+        f(__builtin_bit_cast(float, bits << 16), index(at, __ffs(mask) - 1));
+        mask &= mask - 1;
+      }
+    };
+    if constexpr (NV > 0) {
+      unsigned those = 0;
+      each([&](const u32x4& raw, int k) __attribute__((always_inline)) { those |= one(raw) ? 1u << k : 0u; });
+      while (those) {
+        const int at = (__ffs(those) - 1) * THREADS + (int)threadIdx.x;
+        those &= those - 1;
+        take(read(at), at);
+      }
+    } else {
+      again([&](const u32x4& raw, int at) __attribute__((always_inline)) { if (one(raw)) take(raw, at); });
+    }
   }
 };
 
@@ -220,15 +232,25 @@ struct Weights {
   }
   // of a bucket by the value alone: 64 of them for 1
   __device__ __forceinline__ unsigned plain_bucket(float x) const { return (unsigned)fminf((topf - x) * 64.f, (float)(BUCKETS - 1)); }
-  __device__ __forceinline__ u64 of(float x, unsigned& bucket) const {
+  // 2^(-t / OCTAVE), 0 <= t; n: t to the nearest
+  __device__ __forceinline__ double power(double t, unsigned& n) const {
     double r;
-    const unsigned n = nearest(steps(x), r);
-    bucket = bucket_of(n);
+    n = nearest(t, r);
     constexpr double L = -0.6931471805599453 / OCTAVE;
     const double p = fma(fma(L * L / 2, r, L), r, 1.0);
     u64 e = __builtin_bit_cast(u64, table[n % OCTAVE]);
     e = (u64)((unsigned)(e >> 32) - (n / OCTAVE << 20)) << 32 | (unsigned)e;
-    return __builtin_bit_cast(u64, fma(__builtin_bit_cast(double, e), p, magic)) & 0xfffffffffffffull;
+    return __builtin_bit_cast(double, e) * p;
+  }
+  __device__ __forceinline__ u64 whole(double weight) const {
+#pragma clang fp contract(off)   // the same bits wherever it is formed
+    return __builtin_bit_cast(u64, weight + magic) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ u64 of(float x, unsigned& bucket) const {
+    unsigned n;
+    const double weight = power(steps(x), n);
+    bucket = bucket_of(n);
+    return whole(weight);
   }
   __device__ __forceinline__ u64 of(float x) const {
     unsigned b;
@@ -255,7 +277,7 @@ struct Shared {
   unsigned rank[256];
   u64 wave[WAVES];
   float wave_max[WAVES];
-  u64 found[2], least, small[2];
+  u64 found[3], least, small[2];
   unsigned words[4], small_tokens;
 };
 static_assert(WAVES <= 16, "a row of 16 lanes sums up the wavefronts");
@@ -273,10 +295,10 @@ __device__ __forceinline__ u64 block_scan(Shared& s, u64 x, u64& all) {
   return before + upto - x;
 }
 
-template <typename T>
+template <typename T, int NV = 0>
 struct Sampler {
   Shared& s;
-  Row<T>& row;
+  Row<T, NV>& row;
   Weights w;
 
   // s.list's n entries in rising order to s.ordered.
@@ -444,6 +466,10 @@ struct Sampler {
     const unsigned bits = __builtin_bit_cast(unsigned, x);
     if (sizeof(T) == 2 && x != 0.f) n = listed([&](auto take) __attribute__((always_inline)) { row.equals(bits >> 16, take); });
     else n = gather([&](float y) __attribute__((always_inline)) { return y == x; });
+    return nth_listed(n, x, nth);
+  }
+  // ... where the list has the n tokens with it, if they are not too many
+  __device__ __forceinline__ u64 nth_listed(int n, float x, unsigned nth) {
     if (n <= LIST) {
       order(n);
       return s.ordered[nth - 1];
@@ -544,10 +570,16 @@ struct Settings {
         top_k(p.top_k ? p.top_k[r] : p.top_k_all), frac(p.frac), cut_k(top_k > 0 && top_k < p.vocab), cut_p(top_p < 1.f), cut_m(min_p > 0.f), one(1ull << p.frac),
         least(cut_m ? (u64)fmin(ceil((double)min_p * (double)one), 9e18) : 0) {}
   // the weights with which top_p is reached, of those kept so far, and the random number's
-  __device__ __forceinline__ u64 target_p(u64 kept) const { return max((u64)1, (u64)ceil(fmax((double)top_p, 0.0) * (double)kept)); }
-  __device__ __forceinline__ u64 target_u(u64 kept) const {
-    const double share = (double)u * (double)kept;
-    return share > 0.0 ? min((u64)fmin(share, 9e18) + 1, kept) : (u64)1;
+  __device__ __forceinline__ u64 target_p(u64 kept) const {
+    const u64 p64 = part(top_p);
+    return max((u64)1, __umul64hi(p64, kept) + (p64 * kept != 0));
+  }
+  __device__ __forceinline__ u64 target_u(u64 kept) const { return u < 1.f ? min(__umul64hi(part(u), kept) + 1, kept) : kept; }
+  // x 2^64 of a number below 1, without what is below 1; 0 of negative ones and NaN
+  __device__ __forceinline__ static u64 part(float x) {
+    const unsigned bits = __builtin_bit_cast(unsigned, x), mantissa = (bits & 0x7fffff) | 0x800000;
+    const int shift = (int)(bits >> 23) - 127 + 64 - 23;   // at most 40
+    return x > 0.f && shift > -24 ? shift >= 0 ? (u64)mantissa << shift : (u64)mantissa >> -shift : 0;
   }
   __device__ __forceinline__ Weights weights(float top, const double* table) const {
     return Weights{OCTAVE * 1.4426950408889634 / (double)temperature, (double)top, __builtin_bit_cast(double, (u64)(1023 + 52 - frac) << 52), top, table};
@@ -559,14 +591,17 @@ __device__ __forceinline__ void write_first(const SampleParams& p, int r, bool n
   p.tokens[r] = none ? -1 : (int64_t)(unsigned)entry;
   p.logprobs[r] = none ? -INFINITY : 0.f;
 }
-__device__ __forceinline__ void write(const SampleParams& p, int r, const Weights& w, u64 entry, double log_kept) {
+// log2 of the kept weights by 32 bits, y, and what is left of them: kept 2^-y = 1 + d, d of 2^-20 or less.
+__device__ __forceinline__ void write(const SampleParams& p, int r, const Weights& w, u64 entry, u64 kept) {
   if (threadIdx.x != 0) return;
   p.tokens[r] = (int64_t)(unsigned)entry;
-  const double log2w = -w.steps(of_key(~(unsigned)(entry >> 32))) / OCTAVE;
-  p.logprobs[r] = (float)((log2w + p.frac) * 0.6931471805599453 - log_kept);
+  const double y = __log2f((float)kept);
+  unsigned n;
+  const double d = (double)kept * w.power(y * OCTAVE, n) - 1.0, log2w = -w.steps(of_key(~(unsigned)(entry >> 32))) / OCTAVE;
+  p.logprobs[r] = (float)((log2w + p.frac - y) * 0.6931471805599453 - (d - 0.5 * d * d));
 }
 // The largest of a row, for all threads.
-template <typename T> __device__ __forceinline__ float largest_of(const Row<T>& row, Shared& s) {
+template <typename R> __device__ __forceinline__ float largest_of(const R& row, Shared& s) {
   float x = -INFINITY;
   row.all([&](float y, int, int) { x = fmaxf(x, y); });   // of a NaN and a number the number
 #pragma unroll
@@ -577,128 +612,189 @@ template <typename T> __device__ __forceinline__ float largest_of(const Row<T>& 
   for (int k = 0; k < WAVES; k++) x = fmaxf(x, s.wave_max[k]);
   return x;
 }
+// The largest logit is +inf: those are equals with all of the weight.
+template <typename S> __device__ __forceinline__ void sample_infinite(const SampleParams& p, int r, const Settings& set, S& a, Shared& s) {
+  const u64 number = a.gather([&](float x) __attribute__((always_inline)) { return x == INFINITY; });
+  u64 kept = number << set.frac;
+  const auto first_with = [&](u64 sum) { return (sum + set.one - 1) >> set.frac; };
+  if (set.cut_k) kept = min(kept, (u64)set.top_k << set.frac);
+  if (set.cut_p) kept = min(kept, first_with(set.target_p(kept)) << set.frac);
+  if (set.least > set.one) kept = set.one;
+  const u64 entry = a.nth_listed((int)number, INFINITY, (unsigned)first_with(set.target_u(kept)));
+  if (threadIdx.x == 0) p.tokens[r] = (int64_t)(unsigned)entry, p.logprobs[r] = (float)-log((double)(kept >> set.frac));
+}
+// 2^(-j / OCTAVE), by the series of exp around the middle: twelve terms of |x| < 0.35 leave 2^-51.  (Out of memory the table would be the first thing that a block waits for.)
 __device__ __forceinline__ void fill_table(Shared& s) {
-  for (int j = threadIdx.x; j < OCTAVE; j += THREADS) s.table[j] = POWERS.x[0][j >> 5] * POWERS.x[1][j & 31];
+  for (int j = threadIdx.x; j < OCTAVE; j += THREADS) {
+    const double x = (OCTAVE / 2 - j) * (0.6931471805599453 / OCTAVE);
+    double y = 1.0;
+#pragma unroll
+    for (int k = 12; k > 0; k--) y = fma(y * x, 1.0 / k, 1.0);
+    s.table[j] = y * 0.7071067811865476;
+  }
 }
 
-// The window of counted values: bits base .. base + VALUES / 2 - 1 of either sign, below 2^most.
-__device__ __forceinline__ unsigned base_of(int most) { return (unsigned)max(1, (most + 127) * 128 - VALUES / 2); }
+// The window of counted values: bits base .. base + VALUES / 2 - 1 of either sign, below 2^most, a multiple of 128 (of which all have one exponent).
+__device__ __forceinline__ unsigned base_of(int most) { return (unsigned)max(128, (most + 127) * 128 - VALUES / 2); }
 constexpr int USUAL = 7;   // logits below 128: the largest need not be known to count them
 
+template <int NV>
 __global__ __launch_bounds__(THREADS) void sample_values_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
-  constexpr int EACH = VALUES / THREADS;   // values of a thread
+  constexpr int EACH = VALUES / THREADS;   // values of a thread, of one exponent
+  static_assert(128 % EACH == 0, "values of one exponent");
   const int r = blockIdx.x, tid = threadIdx.x;
-  Row<bf16> row(static_cast<const bf16*>(p.logits) + r * p.row_stride, p.vocab);
+  Row<bf16, NV> row(static_cast<const bf16*>(p.logits) + r * p.row_stride, p.vocab);
   const Settings set(p, r);
   fill_table(s);
-  if (tid == 0) s.small[0] = s.small[1] = 0, s.small_tokens = 0;
+  Sampler<bf16, NV> a{s, row, set.weights(0.f, s.table)};
 
   // ---- tokens by value, in a window that may have to be another one once the largest value is known
-  unsigned tokens[EACH + 1], base;   // of a thread's values, and of those next to 0 behind the last positive one
-  bool small;                        // there are such
+  unsigned tokens[EACH], base;   // of a thread's values
   float top = 0.f;
-  Sampler<bf16> a{s, row, {}};
   int most = USUAL;
-  auto value = [&](int v) { return __builtin_bit_cast(float, v < VALUES / 2 ? (base + (VALUES / 2 - 1 - v)) << 16 : (base + (v - VALUES / 2)) << 16 | 0x80000000u); };
   for (bool again = false;; again = true) {
     base = base_of(most);
-    for (int b = tid; b < VALUES; b += THREADS) s.count[b] = 0;
-    if (tid == 0) s.words[0] = VALUES, s.words[1] = s.words[2] = 0;
+    for (int b = tid; b < VALUES / 4; b += THREADS) reinterpret_cast<u32x4*>(s.count)[b] = u32x4{0, 0, 0, 0};
+    if (tid == 0) s.words[0] = ~0u, s.words[1] = 0, s.small[0] = s.small[1] = 0, s.small_tokens = 0;
     __syncthreads();
     unsigned least;
     int greatest;
     row.count_values(s.count, base, least, greatest);
-    if (__any(least < base)) s.words[1] = 1;
-    if (__any(greatest >= (int)base + VALUES / 2)) s.words[2] = 1;
-    __syncthreads();
-    unsigned first = VALUES;
 #pragma unroll
-    for (int k = EACH - 1; k >= 0; k--) {
-      tokens[k] = s.count[tid * EACH + k];
-      if (tokens[k]) first = tid * EACH + k;
+    for (int d = 1; d < 64; d *= 2) least = min(least, (unsigned)__shfl_xor((int)least, d, 64)), greatest = max(greatest, __shfl_xor(greatest, d, 64));
+    if ((tid & 63) == 0) {
+      atomicMin(&s.words[0], least);
+      if (greatest >= 0) atomicMax(&s.words[1], (unsigned)greatest + 1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EACH; k += 4) {
+      const u32x4 four = *reinterpret_cast<const u32x4*>(&s.count[tid * EACH + k]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) tokens[k + e] = four[e];
     }
     if (again) break;
-    const u64 those = __ballot(first < VALUES);
-    if (those && (tid & 63) == __ffsll(those) - 1) atomicMin(&s.words[0], first);
-    __syncthreads();
-    first = s.words[0];
-    small = s.words[1];
-    const bool beyond = s.words[2];
-    const bool seen = !beyond && (first < VALUES / 2 || (!small && first < VALUES));
-    top = seen ? value(first) : largest_of(row, s);
-    if (top == -INFINITY || !(set.temperature > 0.f)) {   // nothing to choose from, or nothing but the first
-      write_first(p, r, top == -INFINITY, top == -INFINITY ? 0 : a.pick(top, 1));
+    const unsigned positive = s.words[1];   // bits of the largest one, and 1
+    top = __builtin_bit_cast(float, (positive - 1) << 16);
+    const bool seen = positive > 0 && positive <= base + VALUES / 2;   // else all are negative, or it is beyond the window: infinite or NaN perhaps
+    if (!seen) top = largest_of(row, s);
+    if (top == -INFINITY) {
+      write_first(p, r, true, 0);
       return;
     }
-    if (top == INFINITY) row.infinite = true, top = 0.f;
-    most = ilogb(fmin((double)fabsf(top) + 36.0 * (double)set.temperature, 0x1p127)) + 1;   // further from 0 there is none that has a weight
-    if (!beyond && !row.infinite && most <= USUAL) break;
+    if (!(set.temperature > 0.f)) break;
+    if (top == INFINITY) {
+      sample_infinite(p, r, set, a, s);
+      return;
+    }
+    // 36 T below the largest there is none that has a weight
+    if (fabsf(top) + 36.f * set.temperature < (float)(1 << USUAL) && (seen || top < 0.f)) break;
+    most = ilogb(fmin((double)fabsf(top) + 36.0 * (double)set.temperature, 0x1p127)) + 1;
     __syncthreads();
   }
-  small = s.words[1];
-  a.w = set.weights(top, s.table);
-  if (small) {
-    u64 mass = 0, over = 0;
-    unsigned count = 0;
-    row.matches([&](float x) { return (__builtin_bit_cast(unsigned, x) >> 16 & 0x7fff) < base; }, [&](float x, int) {
-      const u64 wt = a.w.of(x);
-      mass += wt, over += wt >= set.least ? wt : 0, count++;
-    });
-    if (count) {
-      atomicAdd(&s.small[0], mass), atomicAdd(&s.small[1], over);
-      atomicAdd(&s.small_tokens, count);
+  float x = top;        // the value of the token, and which one of those with it
+  unsigned nth = 1;
+  bool listed = false;   // the token is in `entry`
+  u64 entry = 0, kept = 0;
+  if (set.temperature > 0.f) {
+    a.w.top = top, a.w.topf = top;
+    const bool small = s.words[0] < base;
+    if (small) {   // nearer to 0 than the window
+      u64 mass = 0, over = 0;
+      unsigned count = 0;
+      row.matches([&](float x) { return (__builtin_bit_cast(unsigned, x) >> 16 & 0x7fff) < base; }, [&](float x, int) {
+        const u64 wt = a.w.of(x);
+        mass += wt, over += wt >= set.least ? wt : 0, count++;
+      });
+      if (count) {
+        atomicAdd(&s.small[0], mass), atomicAdd(&s.small[1], over);
+        atomicAdd(&s.small_tokens, count);
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
-  // ---- weights by value
-  u64 weights[EACH + 1], mass_here = 0, tokens_here = 0, over = 0, m, c = 0, all = 0, kept, entry = 0;
-  double log_kept = 0.0;   // of the first wavefront, under what the others do
-  unsigned some = 0;
+    // ---- weights by value: those of a thread are evenly spaced, so that one is a constant times the one before
+    const int v0 = tid * EACH;
+    const bool positive = v0 < VALUES / 2;
+    const unsigned bits = positive ? base + (VALUES / 2 - 1 - v0) : base + (v0 - VALUES / 2);   // of the first one; each has one less, or, among the negative ones, one more
+    const float x0 = __builtin_bit_cast(float, bits << 16 | (positive ? 0u : 0x80000000u));
+    u64 mass_here = 0, m, c = 0, all = 0, over = 0;
+    unsigned tokens_here = 0;
 #pragma unroll
-  for (int k = 0; k < EACH; k++) some |= tokens[k], weights[k] = 0;
-  if (__any(some != 0))
+    for (int k = 0; k < EACH; k++) tokens_here += tokens[k];
+    const int skip = x0 > top ? abs((int)bits - (int)(__builtin_bit_cast(unsigned, top) >> 16 & 0x7fff)) : 0;   // values above the largest: nobody's
+    double first = 0.0, ratio = 0.0;   // of value `skip`; of a step of this exponent
+    if (__any(tokens_here != 0)) {
+      unsigned n;
+      first = a.w.power(a.w.steps(fminf(x0, top)), n);
+      ratio = a.w.power(fmin(__builtin_bit_cast(double, (u64)(1023 - 134 + (bits >> 7)) << 52) * a.w.c, 60.0 * OCTAVE), n);
+      double weight = first;
 #pragma unroll
-    for (int k = 0; k < EACH; k++) {
-      const u64 wt = a.w.of(value(tid * EACH + k));
-      weights[k] = wt * tokens[k];
-      mass_here += weights[k], tokens_here += tokens[k], over += wt >= set.least ? weights[k] : 0;
+      for (int k = 0; k < EACH; k++) {
+        const u64 wt = a.w.whole(weight), sum = wt * tokens[k];
+        mass_here += sum, over += wt >= set.least ? sum : 0;
+        weight *= k < skip ? 1.0 : ratio;
+      }
     }
-  const bool next_to_0 = tid == VALUES / 2 / EACH - 1;
-  tokens[EACH] = next_to_0 ? s.small_tokens : 0, weights[EACH] = next_to_0 ? s.small[0] : 0;
-  mass_here += weights[EACH], tokens_here += tokens[EACH];
-  m = block_scan(s, mass_here, kept);
-  if (set.cut_k) c = block_scan(s, tokens_here, all);
-  if (set.cut_m) {
-    u64 heavy;
-    block_scan(s, over, heavy);
-    over = max(set.one, heavy + s.small[1]);   // the first one at any rate
+    // tokens next to 0 are behind the last positive value's
+    const bool next_to_0 = small && v0 == VALUES / 2 - EACH;
+    m = block_scan(s, mass_here + (next_to_0 ? s.small[0] : 0), kept);
+    if (set.cut_k) c = block_scan(s, tokens_here + (next_to_0 ? s.small_tokens : 0), all);
+    if (set.cut_m) {
+      u64 heavy;
+      block_scan(s, over, heavy);
+      over = max(set.one, heavy + s.small[1]);   // the first one at any rate
+    }
+    // ---- the cuts, then the token
+    for (int step = set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
+      if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
+      if (step == 1 && !set.cut_p) continue;
+      if (step == 2 && set.cut_m) kept = min(kept, over);
+      const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
+      const bool by_count = step == 0;
+      __syncthreads();
+      // found: the value's bits and the number of its token, the weights up to and with that one; or the tokens next to 0, with the sums before them
+      if (by_count ? c < target && c + tokens_here >= target : m < target && m + mass_here >= target) {
+        u64 mass = m, count = c;
+        double weight = first;
+#pragma unroll 1
+        for (int k = 0; k < EACH; k++) {
+          const u64 wt = a.w.whole(weight);
+          const unsigned here = s.count[v0 + k];
+          if (by_count ? count + here >= target : mass + wt * here >= target) {
+            unsigned nth = (unsigned)(target - count);
+            if (!by_count) {   // the least with nth wt >= what is missing
+              const u64 missing = target - mass;
+              nth = max(1u, (unsigned)((double)missing * __builtin_amdgcn_rcp((double)wt)));
+              while (nth * wt < missing) nth++;
+              while ((nth - 1) * wt >= missing) nth--;
+            }
+            s.found[0] = (u64)(positive ? bits - k : (bits + k) | 0x8000u) << 32 | nth, s.found[1] = mass + nth * wt, s.words[1] = 0;
+            break;
+          }
+          mass += wt * here, count += here, weight *= k < skip ? 1.0 : ratio;
+        }
+      } else if (next_to_0 && (by_count ? c + tokens_here < target && c + tokens_here + s.small_tokens >= target : m + mass_here < target && m + mass_here + s.small[0] >= target)) {
+        s.found[0] = c + tokens_here, s.found[1] = m + mass_here, s.words[1] = 1;
+      }
+      __syncthreads();
+      u64 upto = s.found[1];
+      const u64 found = s.found[0];
+      if (s.words[1]) {
+        const unsigned key = key_of(__builtin_bit_cast(float, (base - 1) << 16));
+        a.resolve(of_key(~key), of_key(key), by_count, target, found, s.found[1], step == 2, entry, upto);
+        listed = true;
+      } else {
+        x = __builtin_bit_cast(float, (unsigned)(found >> 32) << 16), nth = (unsigned)found;
+        listed = false;
+      }
+      if (step < 2) kept = min(kept, upto);
+    }
   }
-  // ---- the cuts, then the token
-  const unsigned key_small = key_of(__builtin_bit_cast(float, (base - 1) << 16));
-  for (int step = set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
-    if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
-    if (step == 1 && !set.cut_p) continue;
-    if (step == 2) {
-      if (set.cut_m) kept = min(kept, over);
-      if (tid < 64) log_kept = log((double)kept);
-    }
-    const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
-    u64 count = 0, mass = 0, upto;
-    // the slots of a thread are EACH + 1 numbers apart
-    const int slot = a.slot_of<EACH + 1>(step == 0, target, tid * (EACH + 1), c, m, tokens, weights, count, mass);
-    if (slot % (EACH + 1) == EACH) {
-      a.resolve(of_key(~key_small), of_key(key_small), step == 0, target, count, mass, step == 2, entry, upto);
-    } else {
-      const float x = value(slot / (EACH + 1) * EACH + slot % (EACH + 1));
-      const u64 wt = a.w.of(x), nth = step == 0 ? target - count : (target - mass + wt - 1) / wt;
-      upto = mass + nth * wt;
-      if (step == 2) entry = a.pick(x, (unsigned)nth);
-    }
-    if (step < 2) kept = min(kept, upto);
-  }
-  write(p, r, a.w, entry, log_kept);
+  if (!listed) entry = a.pick(x, nth);
+  if (set.temperature > 0.f) write(p, r, a.w, entry, kept);
+  else write_first(p, r, false, entry);
 }
 
 // ---- fp32
@@ -717,11 +813,10 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
     return;
   }
   if (largest == INFINITY) {
-    row.infinite = true;
-    a.w = set.weights(0.f, s.table);
+    sample_infinite(p, r, set, a, s);
+    return;
   }
   u64 entry = 0, kept = 0;
-  double log_kept = 0.0;   // of the first wavefront, under what the others do
   // ---- few: all that may be among the first top_k into the list
   bool few = set.cut_k && set.top_k <= LIST / 2;
   if (few) {
@@ -755,7 +850,6 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
         __syncthreads();
         kept = min(kept, s.least);
       }
-      if (tid < 64) log_kept = log((double)kept);
       __syncthreads();
       a.find(k, false, set.target_u(kept), 0, upto, was, entry, upto_p);
     } else {
@@ -800,8 +894,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
       if (step == 1 && !set.cut_p) continue;
       if (step == 2) {
         if (set.cut_m) kept = min(kept, over);
-        if (tid < 64) log_kept = log((double)kept);
-      }
+        }
       const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
       u64 count = 0, mass = 0, upto;
       const unsigned b = a.template slot_of<EACH>(step == 0, target, tid * EACH, c, m, tokens, weights, count, mass);
@@ -811,7 +904,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
       if (step < 2) kept = min(kept, upto);
     }
   }
-  write(p, r, a.w, entry, log_kept);
+  write(p, r, a.w, entry, kept);
 }
 
 template <typename K> int launch(K kernel, const SampleParams& p, int rows, hipStream_t st) {
@@ -835,5 +928,8 @@ extern "C" int ody_sample(const void* logits, const float* u, const float* tempe
   const SampleParams p{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, tokens, logprobs, vocab,
                        std::min(50, 62 - bits)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == ODY_BF16 ? launch(&sample_values_kernel, p, rows, st) : launch(&sample_kernel, p, rows, st);
+  if (dtype == ODY_F32) return launch(&sample_kernel, p, rows, st);
+  const int turns = (vocab + 14 + THREADS * 8 - 1) / (THREADS * 8);   // however rows are aligned
+  if (turns <= 8) return launch(&sample_values_kernel<8>, p, rows, st);   // longer rows are counted while they arrive (256 of 128000: 45 us, 51 out of registers)
+  return launch(&sample_values_kernel<0>, p, rows, st);
 }
