@@ -355,8 +355,10 @@ struct Plan {
 Plan plan(int S, int n, int group, int Hkv, int D, int page_size, int width, int dtype) {
   const int64_t most_keys = (int64_t)page_size * width;
   const int64_t rows = (int64_t)n * group;
-  const int tile = rows <= 16 ? 16 : 32, row_tiles = (int)((rows + tile - 1) / tile);
-  const int step = WAVES * subs(tile, D) * (dtype == ODY_BF16 ? 32 : 16);
+  const double pairs = (double)S * Hkv;
+  const bool chunk = dtype == ODY_BF16 && (rows > 128 || (rows > 64 ? pairs >= 16 || most_keys > 16384 : rows > 32 && pairs >= 128));
+  const int tile = rows <= 16 ? 16 : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);
+  const int step = chunk ? PAGED_CHUNK_KEYS : WAVES * subs(tile, D) * (dtype == ODY_BF16 ? 32 : 16);
   const int64_t steps = std::max((int64_t)1, (most_keys + step - 1) / step);   // of a unit, at most
   const double all = (double)S * row_tiles * Hkv * (steps + paged_extra(tile));
   const int blocks = (int)std::min((double)BLOCKS, std::ceil(all / 8) * 8);   // a multiple of 8: paged_range
@@ -372,6 +374,12 @@ int launch(const PagedAttnParams& p, const PagedCache& c, const PagedScales& z, 
   else ODY_LAUNCH("paged_attn_q8", st, (paged_attn_q8_kernel<T, D, NT, NT == 1 && LINES>), dim3(pl.blocks), dim3(64 * WAVES), 0, p, c, z);
   const int rc = ody_check_launch("paged_attn_q8");
   return rc ? rc : paged_join<T, D, WAVES * subs(16 * NT, D) * Sub<T, D>::KEYS, 1>(p, c, pl.joined, pl.blocks, st);
+}
+int many_rows(const PagedAttnParams& p, int D, const PagedCache& c, const PagedScales& z, const Plan& pl, hipStream_t st) {
+  const int rc = ody_launch_paged_chunk_q8(p, D, c, z, pl.blocks, st);
+  if (rc) return rc;
+  return D == 64 ? paged_join<bf16, 64, PAGED_CHUNK_KEYS, PAGED_JOIN_ROWS>(p, c, pl.joined, pl.blocks, st)
+                 : paged_join<bf16, 128, PAGED_CHUNK_KEYS, PAGED_JOIN_ROWS>(p, c, pl.joined, pl.blocks, st);
 }
 template <typename T>
 int by_head_dim(const PagedAttnParams& p, int D, const PagedCache& c, const PagedScales& z, const Plan& pl, hipStream_t st) {
@@ -413,5 +421,6 @@ extern "C" int ody_paged_attn_q8(const void* q, const void* k_pages, const void*
                           scale < 0.f ? (dtype == ODY_BF16 ? 0x80008000u : 0x80000000u) : 0u, pl.row_tiles, pl.tile,
                           part, reinterpret_cast<float2*>(static_cast<char*>(workspace) + pl.part_bytes)};
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (pl.tile >= PAGED_CHUNK_ROWS) return many_rows(p, D, c, z, pl, st);
   return dtype == ODY_BF16 ? by_head_dim<bf16>(p, D, c, z, pl, st) : by_head_dim<float>(p, D, c, z, pl, st);
 }

@@ -580,7 +580,7 @@ def paged_append_q8_(qkv, n_heads: int, k_pages, v_pages, k_scales, v_scales, pa
     A block's scale is the least power of two, from 2^-126 on, that takes the largest finite value of its tokens to 448 at most, and at least what it was
     where the block holds earlier tokens: those are rounded to the new one if it rises, by a power of two, so that only values below 2^-6 of it change.
     (Tokens that are taken back later leave the scale that they needed.)  Rotated keys are rounded once, to the nearest of the eight bits; a value that is
-    not finite becomes NaN.  Queries are as paged_append_ returns them, in qkv's type."""
+    not finite becomes NaN.  Queries are returned as by paged_append_, in qkv's type; cosines and sines are evaluated in 64 bits here."""
     if not rotate and position_ids is not None:
         raise ValueError("paged_append_q8_: positions are for a rotation")
     if qkv.is_cuda:

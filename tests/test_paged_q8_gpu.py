@@ -155,13 +155,19 @@ def test_append_with_positions_of_its_own(dtype, dev):
 
 
 def test_queries_are_those_of_the_other_cache(dev):
+    """But for cosines that are rounded from 64 bits here and from 32 there: a step of the type of one of them, in either product, and the result's rounding."""
     from odysseus_transformer_amd import ops
     for dtype in (BF16, F32):
         c = q8.make([77, 77, 5], 77, 6, 2, 128, 16, 16, dtype, seed=8)
         g = _to(c, dev)
         k, v = (torch.zeros(c["k8"].shape, dtype=dtype, device=dev) for _ in range(2))
-        a = ops.paged_append_(g["qkv"], 6, k, v, g["table"], g["lengths"])
-        assert torch.equal(a, ops.paged_append_q8_(g["qkv"], 6, *q8.cache(g)))
+        a = ops.paged_append_(g["qkv"], 6, k, v, g["table"], g["lengths"]).double()
+        b = ops.paged_append_q8_(g["qkv"], 6, *q8.cache(g)).double()
+        x = g["qkv"][:, :, :6].double().abs()
+        size = x + torch.cat((x[..., 64:], x[..., :64]), -1)
+        eps = torch.finfo(dtype).eps
+        assert ((a - b).abs() <= eps * size + eps * a.abs()).all()
+        assert (a == b).double().mean() > (0.99 if dtype == BF16 else 0.5)
 
 
 NEW = [
@@ -253,6 +259,51 @@ ATTN = [
     ([3000], 1, 2, 2, 64, 256, 64, F32, "rows"),
     (list(range(0, 260, 2)), 1, 2, 1, 64, 16, 16, BF16, "rows"),      # more sequences than a wavefront has lanes
 ]
+
+
+@pytest.mark.parametrize("D,page,block", [(128, 64, 32), (64, 16, 16), (128, 8, 8), (64, 64, 64)])
+def test_tiles_of_256_rows(D, page, block, dev):
+    """Row tiles of 256, of 64 (sequence, kv head) pairs: lengths around tiles of keys, short and padded sequences, pages of one group of keys and of a tile; all
+    rows of some of the sequences."""
+    from odysseus_transformer_amd import ops
+    lengths, n, Hq, Hkv = [200, 128, 321, 130, 64, 191, 1, 0], 128, 16, 8
+    c = q8.make(lengths, n, Hq, Hkv, D, page, block, BF16, seed=D + page)
+    c["table"][2, 1] = -1
+    g = _to(c, dev)
+    out, lse = ops.paged_attn_q8(g["q"], *q8.cache(g))
+    for heads in (slice(0, 2), slice(14, 16)):
+        part = dict(c, q=c["q"][:, :, heads], k=c["k"][:, :, heads.start // 2:heads.start // 2 + 1], v=c["v"][:, :, heads.start // 2:heads.start // 2 + 1])
+        o, s, mean, dots = ref.attend(part)
+        tol_o, tol_s = ref.attend_bounds(part, o, s, mean, dots)
+        none = s == -math.inf
+        assert ((out[:, :, heads].double().cpu() - o).abs() <= tol_o).all()
+        assert torch.equal(lse[:, heads].cpu() == -math.inf, none) and ((lse[:, heads].double().cpu() - s).abs() <= tol_s)[~none].all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[64], [65, 1], [128, 63], [192, 191], [321, 448, 64], [130 + 64 * 9]], ids=str)
+def test_chunks_of_few_tiles(D, lengths, dev):
+    """As many tiles of keys as a loop with several of them in flight can begin and end with."""
+    for n in (65, 200):
+        c = q8.make(lengths, n, 2, 1, D, 8, 8, BF16, seed=sum(lengths) + n)
+        _check_attn(c, _to(c, dev))
+
+
+@pytest.mark.parametrize("n", [1, 66], ids=["one", "chunk"])
+def test_scores_that_grow(n, dev):
+    """Later keys far above the earlier ones: references follow."""
+    c = q8.make([900, 300], n, 4, 2, 128, 16, 8, BF16, seed=n)
+    grow = torch.exp2(torch.arange(0, 57 + n // 66 * 4) // 8)[: (900 + 15) // 16]
+    for s in range(2):
+        for col in range(c["table"].shape[1]):
+            pg = int(c["table"][s, col])
+            if pg >= 0:
+                z = c["kz"].view(torch.uint8)[pg].int() + int(torch.log2(grow[min(col, len(grow) - 1)]))
+                live = c["kz"].view(torch.uint8)[pg] != 255
+                c["kz"].view(torch.uint8)[pg] = torch.where(live, z.to(torch.uint8), 255)
+    c["k"] = torch.where(torch.isnan(c["k8"].double()), 0.0, c["k8"].double()) * torch.where(
+        c["kz"].view(torch.uint8) == 255, 1.0, torch.exp2(c["kz"].view(torch.uint8).double() - 127)).repeat_interleave(8, 1)[..., None]
+    _check_attn(c, _to(c, dev))
 
 
 @pytest.mark.parametrize("case", ATTN, ids=_ids)
