@@ -232,8 +232,9 @@ class LlamaFlashAttention2TPSP(nn.Module):
         if self.layer_idx is None and cache.num_layers > 1:
             raise ValueError(f"a cache in pages of {cache.num_layers} layers, but this module does not know which one it is: give it a layer_idx")
         scale = 1.0 / math.sqrt(D)
-        k_pages, v_pages = cache.layer(self.layer_idx or 0)
-        where = (k_pages, v_pages, cache.page_table, cache.lengths)
+        index = self.layer_idx or 0
+        append_, attend = (ops.paged_append_q8_, ops.paged_attn_q8) if cache.in_8_bits else (ops.paged_append_, ops.paged_attn)
+        where = (*cache.layer(index), *(cache.scales(index) if cache.in_8_bits else ()), cache.page_table, cache.lengths)
         # nothing but these tokens, as many of every sequence: the rows that the cache would be read back from are at hand.  (A captured step is
         # replayed for steps of which that may not be so.)
         fresh = cache.fresh and not (hidden_states.is_cuda and torch.cuda.is_current_stream_capturing())
@@ -255,11 +256,11 @@ class LlamaFlashAttention2TPSP(nn.Module):
             if rotated:
                 qkv = ops.apply_rope_packed(qkv.view(S, n, nh + 2 * nkv, D), nh + nkv, cache.position_ids, self.rope_theta)
         qkv = qkv.view(S, n, nh + 2 * nkv, D)
-        q = ops.paged_append_(qkv, nh, *where, base=self.rope_theta, rotate=not rotated, new_tokens=cache.new_tokens)
+        q = append_(qkv, nh, *where, base=self.rope_theta, rotate=not rotated, new_tokens=cache.new_tokens)
         if fresh:
             attn_output = ops.flash_attn_func(q, qkv[:, :, nh:nh + nkv], qkv[:, :, nh + nkv:], 0.0, softmax_scale=scale, causal=True)
         else:
-            attn_output = ops.paged_attn(q, *where, scale=scale, new_tokens=cache.new_tokens)[0]
+            attn_output = attend(q, *where, scale=scale, new_tokens=cache.new_tokens)[0]
         y = self._output(attn_output.reshape(1, S * n, nh * D), None if residual is None else residual.reshape(x.shape), cache)
         return (y[0].view(hidden_states.shape), *y[1:])
 

@@ -16,10 +16,14 @@ take it as their `past_key_value(s)`:
 that was captured into a graph is replayed after it.  A step that runs again before the next begin() (a rehearsal in front of a capture) writes its tokens'
 rows anew.  begin() works on the host, once a step for all layers, on the stream that runs the steps; it
 refuses to be captured itself, as free() and truncate() do.
+
+With dtype=torch.float8_e4m3fn the cache holds its values in 8 bits, with a power of two for each `scale_block` tokens of a page and head: half the bytes of bfloat16, which
+are a decoding step's time in attention, and twice the tokens.  Layers use it in the same way, in their own type.  Tokens that are taken back, and those of a step that
+runs again, leave their block the scale that the largest of them needed: what is behind in it has so much less of the small values.
 """
 from __future__ import annotations
 
-from typing import List, Sequence, Union
+from typing import List, Optional, Sequence, Union
 
 import torch
 
@@ -28,19 +32,29 @@ class PagedKVCache:
     is_compileable = False   # a host model asks
 
     def __init__(self, num_layers: int, num_pages: int, *, max_sequences: int, max_length: int, n_kv_heads: int, head_dim: int, page_size: int = 64,
-                 dtype=torch.bfloat16, device="cuda"):
+                 dtype=torch.bfloat16, device="cuda", scale_block: Optional[int] = None):
         for name, value in (("num_layers", num_layers), ("num_pages", num_pages), ("max_sequences", max_sequences), ("max_length", max_length),
                             ("n_kv_heads", n_kv_heads), ("head_dim", head_dim)):
             if value <= 0:
                 raise ValueError(f"{name} must be positive, got {value}")
         if page_size < 8 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two from 8 on, got {page_size}")
-        self.num_layers, self.num_pages, self.page_size = num_layers, num_pages, page_size
+        self.in_8_bits = dtype == torch.float8_e4m3fn
+        if scale_block is None:
+            scale_block = min(32, page_size)
+        elif not self.in_8_bits:
+            raise ValueError(f"scale_block is for a cache in {torch.float8_e4m3fn}, this one is in {dtype}")
+        elif scale_block not in (8, 16, 32, 64) or scale_block > page_size:
+            raise ValueError(f"scale_block must be 8, 16, 32 or 64 and at most a page of {page_size}, got {scale_block}")
+        self.num_layers, self.num_pages, self.page_size, self.scale_block = num_layers, num_pages, page_size, scale_block
         self.max_sequences, self.max_length = max_sequences, max_length
         device = torch.device(device)
         # heads outside of rows: what a block reads of a page is one piece (64 sequences of up to 8192 tokens in pages of 64 171 us a layer, 197 with rows of all heads)
         pools = [torch.empty((2, num_pages, n_kv_heads, page_size, head_dim), dtype=dtype, device=device) for _ in range(num_layers)]
         self._layers = [(p[0].transpose(1, 2), p[1].transpose(1, 2)) for p in pools]
+        scales = [torch.empty((2, num_pages, n_kv_heads, page_size // scale_block), dtype=torch.float8_e8m0fnu, device=device)
+                  for _ in range(num_layers if self.in_8_bits else 0)]
+        self._scales = [(p[0].transpose(1, 2), p[1].transpose(1, 2)) for p in scales]
         self._columns = (max_length + page_size - 1) // page_size
         self.page_table = torch.full((max_sequences, self._columns), -1, dtype=torch.int32, device=device)
         self._counts = torch.zeros((2, max_sequences), dtype=torch.int32, device=device)
@@ -133,6 +147,20 @@ class PagedKVCache:
     def layer(self, index: int):
         """(k_pages, v_pages) of a layer, (pages, page_size, kv heads, head_dim) each."""
         return self._layers[index]
+
+    def scales(self, index: int):
+        """(k_scales, v_scales) of a layer of a cache in 8 bits, (pages, page_size / scale_block, kv heads) each."""
+        if not self.in_8_bits:
+            raise ValueError("scales are those of a cache in 8 bits")
+        return self._scales[index]
+
+    def values(self, index: int, dtype=torch.bfloat16):
+        """What a layer of a cache in 8 bits holds of every sequence: k, v (max_sequences, the longest one's tokens, kv heads, head_dim), 0 behind a sequence's end."""
+        from .. import ops
+        k_scales, v_scales = self.scales(index)
+        self._not_captured()
+        lengths = torch.tensor(self._length, dtype=torch.int32).to(self.page_table.device)
+        return ops.paged_read_q8(*self._layers[index], k_scales, v_scales, self.page_table, lengths, max(self._length), dtype)
 
     def sequence_lengths(self) -> List[int]:
         """Tokens of every sequence, those of the present step included."""
