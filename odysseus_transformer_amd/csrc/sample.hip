@@ -89,12 +89,6 @@ struct Row {
     const unsigned word = sizeof(T) == 2 ? raw[e / 2] : raw[e], bits = sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16;
     return __builtin_bit_cast(float, bits);
   }
-  // Element e, which no constant is.
-  __device__ __forceinline__ static float any_element(const u32x4& raw, int e) {
-    const int at = sizeof(T) == 2 ? e >> 1 : e;
-    const unsigned word = at == 0 ? raw[0] : at == 1 ? raw[1] : at == 2 ? raw[2] : raw[3], bits = sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16;
-    return __builtin_bit_cast(float, bits);
-  }
   __device__ __forceinline__ int index(int at, int e) const { return at * N - head + e; }
   // What vector `at`, which was read, holds of the row.
   __device__ __forceinline__ u32x4 of_row(u32x4 raw, int at) const {
@@ -102,7 +96,6 @@ struct Row {
     return raw;
   }
   __device__ __forceinline__ u32x4 read(int at) const { return of_row(((vector_ptr)base)[min(at, vectors - 1)], at); }
-  // f(vector, its number) for each of a thread's vectors, AHEAD of them under way.  Threads without one in the last turn have what is nowhere in the row.
   // f(vector, turn) for each of a thread's vectors, which are THREADS apart
   template <typename F> __device__ __forceinline__ void each(F f) {
     if constexpr (NV > 0) {
@@ -116,7 +109,11 @@ struct Row {
       again([&](const u32x4& raw, int at) __attribute__((always_inline)) { f(raw, at / THREADS); });
     }
   }
-  template <typename F> __device__ __forceinline__ void again(F f) const {   // from memory; code of one length for all rows
+  // ... from memory, by its number, AHEAD of them under way; code of one length for all rows.  Threads without one in the last turn have what is nowhere in the row.
+  template <typename F> __device__ __forceinline__ void again(F f) const {
+    again(f, [](int) {});
+  }
+  template <typename F, typename G> __device__ __forceinline__ void again(F f, G behind) const {   // behind(turns): now and then, and at the end
     const int tid = threadIdx.x, turns = (vectors + THREADS - 1) / THREADS, last = min(tid, vectors - 1 - (turns - 1) * THREADS);
     auto load = [&](int turn) __attribute__((always_inline)) { return ((vector_ptr)base + min(turn, turns - 1) * THREADS)[turn < turns - 1 ? tid : last]; };
     u32x4 next[AHEAD];
@@ -132,6 +129,7 @@ struct Row {
         if (turn + k == 0 || turn + k == turns - 1) raw = of_row(raw, at);
         f(raw, at);
       }
+      behind(min(turn + AHEAD, turns));
     }
   }
   // f(x, vector, element) for each value
@@ -141,22 +139,28 @@ struct Row {
       for (int e = 0; e < N; e++) f(element(raw, e), at, e);
     });
   }
-  // f(x, index) for every x for which keep(x) holds, which are few
+  // f(x, index) for every x of the row for which keep(x) holds, which are few: a bit for each, of TURNS vectors, so that a wavefront takes as many steps as its
+  // busiest thread has matches.
   template <typename K, typename F> __device__ __forceinline__ void matches(K keep, F f) const {
-    again([&](const u32x4& raw, int at) __attribute__((always_inline)) {
-      bool any = false;
+    constexpr int TURNS = 64 / N;
+    static_assert(TURNS % AHEAD == 0, "the bits of whole turns");
+    u64 mask = 0;
+    again(
+        [&](const u32x4& raw, int at) __attribute__((always_inline)) {
+          unsigned those = 0;
 #pragma unroll
-      for (int e = 0; e < N; e++) any |= keep(element(raw, e));
-      if (!any) return;
-      unsigned mask = 0;
-#pragma unroll
-      for (int e = 0; e < N; e++) mask |= keep(element(raw, e)) ? 1u << e : 0u;
-      while (mask) {
-        const int e = __ffs(mask) - 1;
-        mask &= mask - 1;
-        f(any_element(raw, e), index(at, e));
-      }
-    });
+          for (int e = 0; e < N; e++) those |= keep(element(raw, e)) ? 1u << e : 0u;
+          mask |= (u64)those << at / THREADS % TURNS * N;
+        },
+        [&](int turns) __attribute__((always_inline)) {
+          if (turns % TURNS && turns * THREADS < vectors) return;
+          const int from = (turns - 1) / TURNS * TURNS;
+          while (mask) {
+            const int bit = __ffsll(mask) - 1, at = (from + bit / N) * THREADS + (int)threadIdx.x, e = bit % N, i = index(at, e);
+            mask &= mask - 1;
+            if ((unsigned)i < (unsigned)vocab) f((float)((const T __attribute__((address_space(1)))*)base)[at * N + e], i);
+          }
+        });
   }
   // ---- bf16
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -277,7 +281,7 @@ struct Shared {
   unsigned rank[256];
   u64 wave[WAVES];
   float wave_max[WAVES];
-  u64 found[3], least, small[2];
+  u64 found[3], small[2];
   unsigned words[4], small_tokens;
 };
 static_assert(WAVES <= 16, "a row of 16 lanes sums up the wavefronts");
@@ -643,7 +647,7 @@ __global__ __launch_bounds__(THREADS) void sample_values_kernel(const SamplePara
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   constexpr int EACH = VALUES / THREADS;   // values of a thread, of one exponent
-  static_assert(128 % EACH == 0, "values of one exponent");
+  static_assert(128 % EACH == 0 && EACH == 16, "values of one exponent; lanes of a row sum");
   const int r = blockIdx.x, tid = threadIdx.x;
   Row<bf16, NV> row(static_cast<const bf16*>(p.logits) + r * p.row_stride, p.vocab);
   const Settings set(p, r);
@@ -755,27 +759,27 @@ __global__ __launch_bounds__(THREADS) void sample_values_kernel(const SamplePara
       const bool by_count = step == 0;
       __syncthreads();
       // found: the value's bits and the number of its token, the weights up to and with that one; or the tokens next to 0, with the sums before them
-      if (by_count ? c < target && c + tokens_here >= target : m < target && m + mass_here >= target) {
-        u64 mass = m, count = c;
-        double weight = first;
-#pragma unroll 1
-        for (int k = 0; k < EACH; k++) {
-          const u64 wt = a.w.whole(weight);
-          const unsigned here = s.count[v0 + k];
-          if (by_count ? count + here >= target : mass + wt * here >= target) {
-            unsigned nth = (unsigned)(target - count);
-            if (!by_count) {   // the least with nth wt >= what is missing
-              const u64 missing = target - mass;
-              nth = max(1u, (unsigned)((double)missing * __builtin_amdgcn_rcp((double)wt)));
-              while (nth * wt < missing) nth++;
-              while ((nth - 1) * wt >= missing) nth--;
-            }
-            s.found[0] = (u64)(positive ? bits - k : (bits + k) | 0x8000u) << 32 | nth, s.found[1] = mass + nth * wt, s.words[1] = 0;
-            break;
+      const bool here = by_count ? c < target && c + tokens_here >= target : m < target && m + mass_here >= target;
+      if (const u64 those = __ballot(here)) {   // one thread's: 16 lanes take a value of it each
+        const int lane = tid & 63, from = __ffsll(those) - 1, k = lane & (EACH - 1), skipped = __builtin_amdgcn_readlane(skip, from);
+        const unsigned its_bits = __builtin_amdgcn_readlane(bits, from), its_first = (tid - lane + from) * EACH, number = s.count[its_first + k];
+        const double its_ratio = __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, ratio), from));
+        double weight = __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, first), from));
+#pragma unroll
+        for (int j = 0; j < EACH - 1; j++) weight *= j < skipped || j >= k ? 1.0 : its_ratio;
+        const u64 wt = a.w.whole(weight), mass = wt * number, upto = read_lane(m, from) + row_scan(mass), count = read_lane(c, from) + row_scan(number);
+        if (lane < EACH && (by_count ? count - number < target && count >= target : upto - mass < target && upto >= target)) {
+          unsigned nth = (unsigned)(target - (count - number));
+          if (!by_count) {   // the least with nth wt >= what is missing
+            const u64 missing = target - (upto - mass);
+            nth = max(1u, (unsigned)((double)missing * __builtin_amdgcn_rcp((double)wt)));
+            while (nth * wt < missing) nth++;
+            while ((nth - 1) * wt >= missing) nth--;
           }
-          mass += wt * here, count += here, weight *= k < skip ? 1.0 : ratio;
+          s.found[0] = (u64)(its_first < VALUES / 2 ? its_bits - k : (its_bits + k) | 0x8000u) << 32 | nth, s.found[1] = upto - mass + nth * wt, s.words[1] = 0;
         }
-      } else if (next_to_0 && (by_count ? c + tokens_here < target && c + tokens_here + s.small_tokens >= target : m + mass_here < target && m + mass_here + s.small[0] >= target)) {
+      }
+      if (next_to_0 && !here && (by_count ? c + tokens_here < target && c + tokens_here + s.small_tokens >= target : m + mass_here < target && m + mass_here + s.small[0] >= target)) {
         s.found[0] = c + tokens_here, s.found[1] = m + mass_here, s.words[1] = 1;
       }
       __syncthreads();
@@ -839,16 +843,12 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
         a.find(k, false, set.target_p(kept), 0, upto, was, entry, upto_p);
         kept = min(kept, upto_p);
       }
-      if (set.cut_m) {   // up to the last one that is heavy enough
-        u64 over = set.one;
+      if (set.cut_m) {
+        u64 over = 0, heavy;
 #pragma unroll
-        for (int j = 0; j < a.PER; j++)
-          if (tid * a.PER + j < k && upto[j] - was[j] >= set.least) over = max(over, upto[j]);
-        if (tid == 0) s.least = 0;
-        __syncthreads();
-        atomicMax(&s.least, over);
-        __syncthreads();
-        kept = min(kept, s.least);
+        for (int j = 0; j < a.PER; j++) over += upto[j] - was[j] >= set.least && tid * a.PER + j < k ? upto[j] - was[j] : 0;
+        block_scan(s, over, heavy);
+        kept = min(kept, max(set.one, heavy));   // the first one at any rate
       }
       __syncthreads();
       a.find(k, false, set.target_u(kept), 0, upto, was, entry, upto_p);
@@ -860,20 +860,37 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
   }
   // ---- sums of the weights by buckets of all
   if (!few) {
-    u64 over = 0;   // of weights that are not less than min_p
+    // (many can be in the last bucket, which is everything below 2^-32: it is summed up by each thread)
+    u64 over = 0, tail = 0;   // over: of weights that are not less than min_p
+    const auto put = [&](u64 wt, unsigned b) __attribute__((always_inline)) {
+      if (b == BUCKETS - 1) tail += wt;
+      else atomicAdd(&s.mass[b], wt);
+    };
     if (set.cut_m)
       row.all([&](float x, int, int) {
         unsigned b;
         const u64 wt = a.w.of(x, b);
-        if (wt) atomicAdd(&s.mass[b], wt);
+        put(wt, b);
         over += wt >= set.least ? wt : 0;
       });
     else
       row.all([&](float x, int, int) {
         unsigned b;
-        if (const u64 wt = a.w.of(x, b)) atomicAdd(&s.mass[b], wt);
+        const u64 wt = a.w.of(x, b);
+        put(wt, b);
       });
-    if (set.cut_k) row.all([&](float x, int, int) { if (a.w.of(x)) atomicAdd(&s.count[a.w.bucket(x)], 1u); });
+    tail = wave_scan(tail);
+    if ((tid & 63) == 63) atomicAdd(&s.mass[BUCKETS - 1], tail);
+    if (set.cut_k) {
+      unsigned last = 0;
+      row.all([&](float x, int, int) {
+        unsigned b;
+        const u64 wt = a.w.of(x, b);
+        if (b == BUCKETS - 1) last += wt != 0;
+        else atomicAdd(&s.count[b], 1u);
+      });
+      if (last) atomicAdd(&s.count[BUCKETS - 1], last);
+    }
     __syncthreads();
     constexpr int EACH = BUCKETS / THREADS;
     unsigned tokens[EACH];
