@@ -110,12 +110,16 @@ struct Row {
     }
   }
   // ... from memory, by its number, AHEAD of them under way; code of one length for all rows.  Threads without one in the last turn have what is nowhere in the row.
-  template <typename F> __device__ __forceinline__ void again(F f) const {
-    again(f, [](int) {});
+  template <bool BACK = false, typename F> __device__ __forceinline__ void again(F f) const {
+    again<BACK>(f, [](int) {});
   }
-  template <typename F, typename G> __device__ __forceinline__ void again(F f, G behind) const {   // behind(turns): now and then, and at the end
+  // behind(turns): now and then, and at the end.  BACK: from the row's end, which is what a cache has of a long row that was read before.
+  template <bool BACK = false, typename F, typename G> __device__ __forceinline__ void again(F f, G behind) const {
     const int tid = threadIdx.x, turns = (vectors + THREADS - 1) / THREADS, last = min(tid, vectors - 1 - (turns - 1) * THREADS);
-    auto load = [&](int turn) __attribute__((always_inline)) { return ((vector_ptr)base + min(turn, turns - 1) * THREADS)[turn < turns - 1 ? tid : last]; };
+    auto load = [&](int turn) __attribute__((always_inline)) {
+      turn = BACK ? max(turns - 1 - turn, 0) : min(turn, turns - 1);
+      return ((vector_ptr)base + turn * THREADS)[turn < turns - 1 ? tid : last];
+    };
     u32x4 next[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; k++) next[k] = load(k);
@@ -125,7 +129,7 @@ struct Row {
         if (turn + k >= turns) break;
         u32x4 raw = next[k];
         next[k] = load(turn + k + AHEAD);
-        const int at = (turn + k) * THREADS + tid;
+        const int at = (BACK ? turns - 1 - (turn + k) : turn + k) * THREADS + tid;
         if (turn + k == 0 || turn + k == turns - 1) raw = of_row(raw, at);
         f(raw, at);
       }
@@ -186,34 +190,37 @@ struct Row {
     });
     least = min(l[0], l[1]), most = max(g[0], g[1]);
   }
-  // f(x, index) of every x with these bits, of which there are few: the vectors that have one are read again
+  // f(x, index) of every x with these bits, of which there are few: a bit for each in what four vectors leave clear of 32
   template <typename F> __device__ __forceinline__ void equals(unsigned bits, F f) {
+    static_assert(AHEAD == 4 && NV % 4 == 0, "vectors of a mask");
     const unsigned both = bits << 16 | bits;
-    auto one = [&](const u32x4& raw) __attribute__((always_inline)) {
-      u16x2 l = {1, 1};
-#pragma unroll
-      for (int w = 0; w < 4; w++) l = lower(l, __builtin_bit_cast(u16x2, raw[w] ^ both));
-      return l[0] == 0 || l[1] == 0;
-    };
-    auto take = [&](const u32x4& raw, int at) __attribute__((always_inline)) {
+    auto others = [&](const u32x4& raw) __attribute__((always_inline)) {   // bits w and 16 + w: elements 2 w and 2 w + 1 are others
       unsigned mask = 0;
 #pragma unroll
-      for (int w = 0; w < 4; w++) mask |= ((raw[w] ^ both) << 16 ? 0u : 1u << 2 * w) | ((raw[w] ^ both) >> 16 ? 0u : 2u << 2 * w);
+      for (int w = 0; w < 4; w++) mask |= __builtin_bit_cast(unsigned, lower(__builtin_bit_cast(u16x2, raw[w] ^ both), (u16x2){1, 1})) << w;
+      return mask;
+    };
+    auto take = [&](unsigned mask, auto turn) __attribute__((always_inline)) {
       while (mask) {
-        f(__builtin_bit_cast(float, bits << 16), index(at, __ffs(mask) - 1));
+        const int bit = __ffs(mask) - 1;
         mask &= mask - 1;
+        f(__builtin_bit_cast(float, bits << 16), index(turn(bit >> 2 & 3) * THREADS + (int)threadIdx.x, 2 * (bit & 3) + (bit >> 4)));
       }
     };
     if constexpr (NV > 0) {
-      unsigned those = 0;
-      each([&](const u32x4& raw, int k) __attribute__((always_inline)) { those |= one(raw) ? 1u << k : 0u; });
-      while (those) {
-        const int at = (__ffs(those) - 1) * THREADS + (int)threadIdx.x;
-        those &= those - 1;
-        take(read(at), at);
-      }
+      unsigned mask[NV / 4] = {};
+      each([&](const u32x4& raw, int k) __attribute__((always_inline)) { mask[k / 4] |= others(raw) << 4 * (k % 4); });
+#pragma unroll
+      for (int i = 0; i < NV / 4; i++) take(~mask[i], [&](int k) __attribute__((always_inline)) { return 4 * i + k; });
     } else {
-      again([&](const u32x4& raw, int at) __attribute__((always_inline)) { if (one(raw)) take(raw, at); });
+      const int turns = (vectors + THREADS - 1) / THREADS;
+      unsigned mask = ~0u;
+      int k = 0;
+      again<true>([&](const u32x4& raw, int) __attribute__((always_inline)) { mask ^= (others(raw) ^ 0xf000fu) << 4 * (k++ & 3); },
+                  [&](int behind) __attribute__((always_inline)) {
+                    if (mask != ~0u) take(~mask, [&](int j) __attribute__((always_inline)) { return turns - 1 - ((behind - 1) / 4 * 4 + j); });
+                    mask = ~0u;
+                  });
     }
   }
 };
