@@ -159,22 +159,37 @@ __global__ __launch_bounds__(256) void paged_append_q8_kernel(const AppendParams
 
   // ---- queries: rows (token, head), heads in a row
   if (!ROTATE) return;
-  for (int r = wave * ROWS + sub; r < tokens * p.Hq; r += waves * ROWS) {
-    const int t = ONE ? 0 : r / p.Hq, h = r - t * p.Hq;
-    T* dst = static_cast<T*>(p.q) + s * p.sq.b + (i0 + t) * p.sq.l + h * p.sq.h + col;
-    vec a1{}, b1{};
-    if (t >= real) {
-      const T* src = x + t * p.sx.l + h * p.sx.h;
-      const vec a = *reinterpret_cast<const vec*>(src), b = *reinterpret_cast<const vec*>(src + HALF);
+  constexpr int AHEAD = ONE ? 1 : 4;   // rows of a thread under way
+  const int rows = tokens * p.Hq;
+  for (int r0 = wave * ROWS + sub; r0 < rows; r0 += AHEAD * waves * ROWS) {
+    vec a[AHEAD], b[AHEAD];
+    int t[AHEAD], h[AHEAD];
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        const float c = cs[t][col + e], sine = sn[t][col + e], x1 = (float)a[e], x2 = (float)b[e];
-        a1[e] = (T)(x1 * c - x2 * sine);
-        b1[e] = (T)(x2 * c + x1 * sine);
+    for (int k = 0; k < AHEAD; k++) {
+      const int r = r0 + k * waves * ROWS;
+      t[k] = ONE ? 0 : r / p.Hq, h[k] = r - t[k] * p.Hq;
+      a[k] = b[k] = vec{};
+      if (r < rows && t[k] >= real) {
+        const T* src = x + t[k] * p.sx.l + h[k] * p.sx.h;
+        a[k] = *reinterpret_cast<const vec*>(src), b[k] = *reinterpret_cast<const vec*>(src + HALF);
       }
     }
-    __builtin_nontemporal_store(__builtin_bit_cast(raw, a1), reinterpret_cast<raw*>(dst));
-    __builtin_nontemporal_store(__builtin_bit_cast(raw, b1), reinterpret_cast<raw*>(dst + HALF));
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {
+      if (r0 + k * waves * ROWS >= rows) break;
+      T* dst = static_cast<T*>(p.q) + s * p.sq.b + (i0 + t[k]) * p.sq.l + h[k] * p.sq.h + col;
+      vec a1{}, b1{};
+      if (t[k] >= real) {
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+          const float c = cs[t[k]][col + e], sine = sn[t[k]][col + e], x1 = (float)a[k][e], x2 = (float)b[k][e];
+          a1[e] = (T)(x1 * c - x2 * sine);
+          b1[e] = (T)(x2 * c + x1 * sine);
+        }
+      }
+      __builtin_nontemporal_store(__builtin_bit_cast(raw, a1), reinterpret_cast<raw*>(dst));
+      __builtin_nontemporal_store(__builtin_bit_cast(raw, b1), reinterpret_cast<raw*>(dst + HALF));
+    }
   }
 }
 
