@@ -77,7 +77,9 @@ __global__ __launch_bounds__(256) void paged_append_q8_kernel(const AppendParams
       // rounded to the values' type before use, as ody_rope has them; from 64 bits, for a key on a border of its eight bits would show which way a cosine went
       double sine, cosine;
       sincos((double)th, &sine, &cosine);
-      cs[t][j] = rounded<T>((float)cosine), sn[t][j] = rounded<T>((float)sine);
+      float c = (float)cosine, si = (float)sine;
+      asm("" : "+v"(c), "+v"(si));   // of 32 bits first: the compiler makes one rounding of the two, which differs at ties
+      cs[t][j] = rounded<T>(c), sn[t][j] = rounded<T>(si);
     }
   }
 

@@ -170,6 +170,18 @@ def test_queries_are_those_of_the_other_cache(dev):
         assert (a == b).double().mean() > (0.99 if dtype == BF16 else 0.5)
 
 
+def test_cosines_are_rounded_to_32_bits_first(dev):
+    """Queries of 1 and 0 are the cosines and sines: those of 32 bits, rounded once more to the type.  (Among 2^19 of them a few lie in the middle of two bf16 values then.)"""
+    from odysseus_transformer_amd import ops
+    n, D = 4096, 128
+    c = q8.make([n], n, 1, 1, D, 64, 32, BF16, seed=1)
+    g = _to(c, dev)
+    g["qkv"][:, :, 0, :D // 2], g["qkv"][:, :, 0, D // 2:] = 1.0, 0.0
+    q = ops.paged_append_q8_(g["qkv"], 1, *q8.cache(g), inv_freq=_inv_freq(D).to(dev))[0, :, 0].cpu()
+    th = (torch.arange(n).float()[:, None] * _inv_freq(D)).double()
+    assert torch.equal(q, torch.cat((th.cos(), th.sin()), -1).float().to(BF16))
+
+
 NEW = [
     # lengths, new tokens, n, Hq, Hkv, D, page, block, dtype
     ([40, 300, 7, 90], [1, 1, 0, 1], 1, 8, 2, 128, 16, 8, BF16),
