@@ -31,8 +31,9 @@ __device__ __forceinline__ bf16x8 q8_operand(unsigned lo, unsigned hi, float sca
 }
 #endif
 
-// The kernels of many rows (paged_q8_chunk.hip), by p.tile.
+// The kernels of many rows (paged_q8_chunk.hip, paged_q8_wide.hip), by p.tile.
 int ody_launch_paged_chunk_q8(const PagedAttnParams& p, int D, const PagedCache& c, const PagedScales& z, int blocks, hipStream_t st);
+int ody_launch_paged_wide_q8(const PagedAttnParams& p, const PagedCache& c, const PagedScales& z, int blocks, hipStream_t st);
 
 // Host side: what the entry points of such a cache check, behind paged_check.
 int paged_q8_check(const char* who, const PagedScales& z, int page_size, int block);

@@ -345,7 +345,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_q8_kernel(const Page
   }
 }
 
-// The host knows no lengths: it goes by the places of the table.
+// The host knows no lengths.  Row tiles of 16 or 32 here, the kernels for many rows in bf16 where there is work for them: more than 64 rows, and 2048 in all (32 heads on 8 of 128, us
+// here / in tiles of 128: 17 tokens behind 500 keys 12.3 / 18.7, behind 32768 37.8 / 43.4; of 4 sequences, 2176 rows, behind 2000 24.5 / 24.1, behind 8192 41.0 / 41.3; 33 tokens
+// behind 2000 16.9 / 22.6; 128 tokens, 4096 rows, behind 2000 31.5 / 25.4, behind 8192 48.8 / 43.4; 10 tokens each of 64 sequences, which are read twice here, of up to 8192 keys
+// 209 / 198, of up to 1000 51 / 55).
+// Tiles of 256 for heads of 128 by the rule of paged_attn.hip, where 64 of them keep the chip busy and cover few rows more than tiles of 128 (us in tiles of 128 / 256: 128 tokens, which are
+// 16 units, behind 2000 keys 25.4 / 29.6; 512 tokens, 64 units, 45.7 / 42.0; 512 behind 32768 337 / 290, 2048 behind 8192 384 / 342, 300 each of 64 sequences of up to 3000
+// keys 1424 / 1109; 257 rows of each of 32 heads behind 8192 keys, which are two tiles of 256, 81 / 91).
 struct Plan {
   int tile, row_tiles, step, blocks;
   bool joined;          // a cut may go through a unit
@@ -356,12 +362,14 @@ Plan plan(int S, int n, int group, int Hkv, int D, int page_size, int width, int
   const int64_t most_keys = (int64_t)page_size * width;
   const int64_t rows = (int64_t)n * group;
   const double pairs = (double)S * Hkv;
-  const bool chunk = dtype == ODY_BF16 && (rows > 128 || (rows > 64 ? pairs >= 16 || most_keys > 16384 : rows > 32 && pairs >= 128));
-  const int tile = rows <= 16 ? 16 : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);
+  const bool chunk = dtype == ODY_BF16 && rows > 64 && rows * pairs >= 2048;
+  const int64_t wide_tiles = (rows + PAGED_WIDE_ROWS - 1) / PAGED_WIDE_ROWS, chunk_tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
+  const bool wide = chunk && D == 128 && pairs * wide_tiles >= 64 && 14 * wide_tiles <= 8 * chunk_tiles;
+  const int tile = rows <= 16 ? 16 : wide ? PAGED_WIDE_ROWS : chunk ? PAGED_CHUNK_ROWS : 32, row_tiles = (int)((rows + tile - 1) / tile);
   const int step = chunk ? PAGED_CHUNK_KEYS : WAVES * subs(tile, D) * (dtype == ODY_BF16 ? 32 : 16);
   const int64_t steps = std::max((int64_t)1, (most_keys + step - 1) / step);   // of a unit, at most
   const double all = (double)S * row_tiles * Hkv * (steps + paged_extra(tile));
-  const int blocks = (int)std::min((double)BLOCKS, std::ceil(all / 8) * 8);   // a multiple of 8: paged_range
+  const int blocks = (int)std::min((double)(wide ? BLOCKS / 2 : BLOCKS), std::ceil(all / 8) * 8);   // a multiple of 8: paged_range
   const bool joined = steps > 1;
   const size_t parts = joined ? (size_t)blocks * 2 * tile : 0;
   return Plan{tile, row_tiles, step, blocks, joined, all < 2147483648.0, parts * D * sizeof(float), parts * sizeof(float2)};
@@ -376,7 +384,7 @@ int launch(const PagedAttnParams& p, const PagedCache& c, const PagedScales& z, 
   return rc ? rc : paged_join<T, D, WAVES * subs(16 * NT, D) * Sub<T, D>::KEYS, 1>(p, c, pl.joined, pl.blocks, st);
 }
 int many_rows(const PagedAttnParams& p, int D, const PagedCache& c, const PagedScales& z, const Plan& pl, hipStream_t st) {
-  const int rc = ody_launch_paged_chunk_q8(p, D, c, z, pl.blocks, st);
+  const int rc = pl.tile == PAGED_WIDE_ROWS ? ody_launch_paged_wide_q8(p, c, z, pl.blocks, st) : ody_launch_paged_chunk_q8(p, D, c, z, pl.blocks, st);
   if (rc) return rc;
   return D == 64 ? paged_join<bf16, 64, PAGED_CHUNK_KEYS, PAGED_JOIN_ROWS>(p, c, pl.joined, pl.blocks, st)
                  : paged_join<bf16, 128, PAGED_CHUNK_KEYS, PAGED_JOIN_ROWS>(p, c, pl.joined, pl.blocks, st);

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from odysseus_transformer_amd.utils.paged_cache import PagedKVCache
-from test_product_distances import _assembly, _kernels, M0
+from test_product_distances import _assembly, _kernels, M0, test_wait_states_around_products_by_hand as _wait_states
 
 BF16, F32, F8, E8 = torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -108,6 +108,10 @@ def test_m0_belongs_to_the_direct_loads(tmp_path):
             else:
                 assert not M0.match(op) and not any(re.search(r"\bm0\b|\blds$", o) for o in operands), f"{name}: {op} {operands}"
     assert loads >= 20
+
+
+def test_wait_states_around_products(tmp_path):
+    _wait_states("paged_q8_wide", tmp_path)
 
 
 # ------------------------------------------------------------------------------------------------ on the GPU

@@ -292,6 +292,50 @@ def test_tiles_of_256_rows(D, page, block, dev):
         assert torch.equal(lse[:, heads].cpu() == -math.inf, none) and ((lse[:, heads].double().cpu() - s).abs() <= tol_s)[~none].all()
 
 
+def _check_heads(c, g, dev, heads, **kw):
+    """Some query heads of a case with one for each kv head."""
+    from odysseus_transformer_amd import ops
+    out, lse = ops.paged_attn_q8(g["q"], *q8.cache(g), **kw)
+    for h in heads:
+        part = dict(c, q=c["q"][:, :, h:h + 1], k=c["k"][:, :, h:h + 1], v=c["v"][:, :, h:h + 1])
+        o, s, mean, dots = ref.attend(part)
+        tol_o, tol_s = ref.attend_bounds(part, o, s, mean, dots)
+        none = s == -math.inf
+        assert ((out[:, :, h:h + 1].double().cpu() - o).abs() <= tol_o).all(), h
+        assert torch.equal(lse[:, h:h + 1].cpu() == -math.inf, none) and ((lse[:, h:h + 1].double().cpu() - s).abs() <= tol_s)[~none].all(), h
+
+
+@pytest.mark.parametrize("n,D", [(256, 128), (128, 128), (128, 64)], ids=["256", "128", "128_hd64"])
+@pytest.mark.parametrize("length", [1, 8, 64, 65, 71, 128, 129, 192, 193, 256, 257, 320, 321, 520, 1100])
+def test_many_rows_of_few_tiles(length, n, D, dev):
+    """As many tiles of keys as a loop over them can begin and end with, and groups of keys with one, all or none of theirs there; a page that is not there."""
+    c = q8.make([length], n, 64, 64, D, 16, 8, BF16, seed=length)
+    if length > 100:
+        c["table"][0, 5] = -1
+    _check_heads(c, _to(c, dev), dev, (0, 37, 63))
+
+
+@pytest.mark.parametrize("n", [256, 128])
+def test_many_rows_with_fewer_new_tokens(n, dev):
+    c = q8.make([300, 40, 500], n, 64, 64, 128, 16, 16, BF16, seed=n)
+    c["new"] = torch.tensor([90, 0, n - 1], dtype=torch.int32)
+    g = _to(c, dev)
+    _check_heads(c, g, dev, (2, 63), new_tokens=g["new"])
+
+
+@pytest.mark.parametrize("n", [256, 128])
+def test_many_rows_whose_scores_grow(n, dev):
+    c = q8.make([1000], n, 64, 64, 128, 32, 8, BF16, seed=3)
+    up = torch.arange(c["table"].shape[1]) // 3
+    z = c["kz"].view(torch.uint8)
+    for col in range(c["table"].shape[1]):
+        pg = int(c["table"][0, col])
+        z[pg] = torch.where(z[pg] == 255, 255, z[pg].int() + int(up[col])).to(torch.uint8)
+    held = c["k8"].double()
+    c["k"] = torch.where(torch.isnan(held), 0.0, held) * torch.where(z == 255, 1.0, torch.exp2(z.double() - 127)).repeat_interleave(8, 1)[..., None]
+    _check_heads(c, _to(c, dev), dev, (0, 1, 40))
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("lengths", [[64], [65, 1], [128, 63], [192, 191], [321, 448, 64], [130 + 64 * 9]], ids=str)
 def test_chunks_of_few_tiles(D, lengths, dev):
