@@ -143,9 +143,8 @@ struct Row {
       for (int e = 0; e < N; e++) f(element(raw, e), at, e);
     });
   }
-  // f(x, index) for every x of the row for which keep(x) holds, which are few: a bit for each, of TURNS vectors, so that a wavefront takes as many steps as its
-  // busiest thread has matches.
-  template <typename K, typename F> __device__ __forceinline__ void matches(K keep, F f) const {
+  // f(mask, turn): of TURNS turns of a thread's vectors, from `turn` on, a bit for each x for which keep(x) holds, which are few: a wavefront goes as often over them as its busiest thread has.
+  template <typename K, typename F> __device__ __forceinline__ void masks(K keep, F f) const {
     constexpr int TURNS = 64 / N;
     static_assert(TURNS % AHEAD == 0, "the bits of whole turns");
     u64 mask = 0;
@@ -158,13 +157,20 @@ struct Row {
         },
         [&](int turns) __attribute__((always_inline)) {
           if (turns % TURNS && turns * THREADS < vectors) return;
-          const int from = (turns - 1) / TURNS * TURNS;
-          while (mask) {
-            const int bit = __ffsll(mask) - 1, at = (from + bit / N) * THREADS + (int)threadIdx.x, e = bit % N, i = index(at, e);
-            mask &= mask - 1;
-            if ((unsigned)i < (unsigned)vocab) f((float)((const T __attribute__((address_space(1)))*)base)[at * N + e], i);
-          }
+          f(mask, (turns - 1) / TURNS * TURNS);
+          mask = 0;
         });
+  }
+  __device__ __forceinline__ float value(int i) const { return (float)((const T __attribute__((address_space(1)))*)base)[head + i]; }
+  // f(x, index) for every x of the row for which keep(x) holds, which are few
+  template <typename K, typename F> __device__ __forceinline__ void matches(K keep, F f) const {
+    masks(keep, [&](u64 mask, int turn) __attribute__((always_inline)) {
+      while (mask) {
+        const int bit = __ffsll(mask) - 1, i = index((turn + bit / N) * THREADS + (int)threadIdx.x, bit % N);
+        mask &= mask - 1;
+        if ((unsigned)i < (unsigned)vocab) f(value(i), i);
+      }
+    });
   }
   // ---- bf16
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -242,7 +248,8 @@ struct Weights {
     return bucket_of(nearest(steps(x), r));
   }
   // of a bucket by the value alone: 64 of them for 1
-  __device__ __forceinline__ unsigned plain_bucket(float x) const { return (unsigned)fminf((topf - x) * 64.f, (float)(BUCKETS - 1)); }
+  __device__ __forceinline__ float plain(float x) const { return (topf - x) * 64.f; }
+  __device__ __forceinline__ unsigned plain_bucket(float x) const { return (unsigned)fminf(plain(x), (float)(BUCKETS - 1)); }
   // 2^(-t / OCTAVE), 0 <= t; n: t to the nearest
   __device__ __forceinline__ double power(double t, unsigned& n) const {
     double r;
@@ -348,6 +355,31 @@ struct Sampler {
   // Tokens for which keep(x) holds into s.list, as (falling key, index); how many there are, which may be more than fit.
   template <typename F> __device__ __forceinline__ int gather(F keep) {
     return listed([&](auto take) __attribute__((always_inline)) { row.matches(keep, take); });
+  }
+  // ... for which beyond(x) is not above 0, which it is for -inf
+  template <typename F> __device__ __forceinline__ int gather_within(F beyond) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) s.words[0] = 0;
+    __syncthreads();
+    row.masks([&](float x) __attribute__((always_inline)) { return beyond(x) <= 0.f; }, [&](u64 mask, int turn) __attribute__((always_inline)) {
+      if (mask == 0) return;
+      unsigned to = atomicAdd(&s.words[0], (unsigned)__popcll(mask));
+      for (; mask && to < LIST; to++) {
+        const int bit = __ffsll(mask) - 1;
+        mask &= mask - 1;
+        s.list[to] = (u64)row.index((turn + bit / row.N) * THREADS + tid, bit % row.N);
+      }
+    });
+    __syncthreads();
+    const int n = (int)s.words[0];
+    if (n > LIST) return n;
+    for (int k = tid; k < n; k += THREADS) {   // their values at once
+      const unsigned i = (unsigned)s.list[k];
+      s.list[k] = (u64)~key_of(row.value(i)) << 32 | i;
+    }
+    __syncthreads();
+    return n;
   }
   template <typename F> __device__ __forceinline__ int listed(F walk) {
     __syncthreads();
@@ -517,10 +549,13 @@ struct Sampler {
     lo = of_key(first), hi = of_key(behind - 1);
   }
 
+  // Not above 0 from lo to hi (of which -inf is none: it has no weight); without a branch
+  __device__ __forceinline__ static float outside(float x, float lo, float hi) { return fmaxf(x - hi, fmaxf(lo, -3.4028235e38f) - x); }
+
   // Where the sum reaches the target, among the tokens with logits from `from` to `to`, `count` and `mass` before them: the entry (falling key, index), and the weights up to and with it.
   __device__ __forceinline__ void resolve(float from, float to, bool by_count, u64 target, u64 count, u64 mass, bool want_index, u64& entry, u64& mass_upto) {
     const auto in = [&](float x) __attribute__((always_inline)) { return x >= from && x <= to; };
-    int n = gather(in);
+    int n = gather_within([&](float x) __attribute__((always_inline)) { return outside(x, from, to); });
     if (n <= LIST) {
       order(n);
       reach(n, by_count, target, count, mass, entry, mass_upto);
@@ -625,13 +660,13 @@ template <typename R> __device__ __forceinline__ float largest_of(const R& row, 
 }
 // The largest logit is +inf: those are equals with all of the weight.
 template <typename S> __device__ __forceinline__ void sample_infinite(const SampleParams& p, int r, const Settings& set, S& a, Shared& s) {
-  const u64 number = a.gather([&](float x) __attribute__((always_inline)) { return x == INFINITY; });
-  u64 kept = number << set.frac;
+  const int n = a.gather([&](float x) __attribute__((always_inline)) { return x == INFINITY; });
+  u64 kept = (u64)n << set.frac;
   const auto first_with = [&](u64 sum) { return (sum + set.one - 1) >> set.frac; };
   if (set.cut_k) kept = min(kept, (u64)set.top_k << set.frac);
   if (set.cut_p) kept = min(kept, first_with(set.target_p(kept)) << set.frac);
   if (set.least > set.one) kept = set.one;
-  const u64 entry = a.nth_listed((int)number, INFINITY, (unsigned)first_with(set.target_u(kept)));
+  const u64 entry = a.nth_listed(n, INFINITY, (unsigned)first_with(set.target_u(kept)));
   if (threadIdx.x == 0) p.tokens[r] = (int64_t)(unsigned)entry, p.logprobs[r] = (float)-log((double)(kept >> set.frac));
 }
 // 2^(-j / OCTAVE), by the series of exp around the middle: twelve terms of |x| < 0.35 leave 2^-51.  (Out of memory the table would be the first thing that a block waits for.)
@@ -839,7 +874,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
     __syncthreads();
     const int last = a.bucket_of(nullptr, s.count, true, set.top_k, count, mass);
     int n = LIST + 1;
-    if (last < BUCKETS) n = a.gather([&](float x) { return a.w.plain_bucket(x) <= (unsigned)last; });
+    const float end = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, (float)(last + 1)) - 1);   // up to the number below it, of buckets
+    if (last < BUCKETS) n = a.gather_within([&](float x) { return a.w.plain(x) - end; });
     few = n <= LIST;
     if (few) {
       a.order(n);
@@ -913,12 +949,36 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
       block_scan(s, over, heavy);
       over = max(set.one, heavy);   // the first one at any rate
     }
-    for (int step = set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
+    // top_p and the token in one go: whichever token of its bucket top_p ends with, the random number's is in one or two buckets, which are gathered with it
+    bool both = false;
+    if (set.cut_p && !set.cut_k) {
+      const u64 most = set.cut_m ? over : ~0ull, target = set.target_p(kept);
+      u64 count = 0, mass = 0, mass_u = 0, mass_v = 0, upto_p;
+      const auto bucket_with = [&](u64 sum, u64& before) __attribute__((always_inline)) {
+        return (unsigned)a.template slot_of<EACH>(false, sum, tid * EACH, c, m, tokens, weights, count, before);
+      };
+      // top_p's bucket b; the random number's, from u to v, in front of it or up to it
+      const unsigned b = bucket_with(target, mass), bu = bucket_with(set.target_u(min(most, mass + 1)), mass_u), bv = bucket_with(set.target_u(min(most, mass + s.mass[b])), mass_v);
+      float lo, hi, lo_u, hi_u, none;
+      a.range_of(b, lo, hi), a.range_of(bu, lo_u, hi_u);
+      if (bv != bu) a.range_of(bv, lo_u, none);
+      const int n = a.gather_within([&](float x) __attribute__((always_inline)) { return fminf(a.outside(x, lo, hi), a.outside(x, lo_u, hi_u)); });
+      both = n <= LIST;
+      if (both) {
+        a.order(n);
+        const u64 in_front = (bv == b ? mass : mass_v + s.mass[bv]) - mass_u;   // of the list's part that is bucket b
+        u64 upto[a.PER], was[a.PER];
+        a.sums(n, 0, upto, was);
+        a.find(n, false, target - mass + in_front, 0, upto, was, entry, upto_p);
+        kept = min(min(kept, mass + (upto_p - in_front)), most);
+        __syncthreads();
+        a.find(n, false, set.target_u(kept) - mass_u, 0, upto, was, entry, upto_p);
+      }
+    }
+    for (int step = both ? 3 : set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
       if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
       if (step == 1 && !set.cut_p) continue;
-      if (step == 2) {
-        if (set.cut_m) kept = min(kept, over);
-        }
+      if (step == 2 && set.cut_m) kept = min(kept, over);
       const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
       u64 count = 0, mass = 0, upto;
       const unsigned b = a.template slot_of<EACH>(step == 0, target, tid * EACH, c, m, tokens, weights, count, mass);
