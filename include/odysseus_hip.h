@@ -469,11 +469,12 @@ int ody_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, c
  *             the first, with logprob 0.  NaN logits count as -inf; +inf ones are equals with all of the weight; a row of nothing but -inf gives -1 and -inf.
  *             temperature, top_k, top_p, min_p: (rows) each, or NULL: the number for all.  Sums are of whole multiples of 2^(log2(vocab) - 62) or less, rounded up: the same
  *             for any order of summation.  rows < 2^22, vocab <= 2^21 - 4; logits aligned to their size.
- *             Reads 16-byte pieces that hold at least one logit of the row.
+ *             Reads 16-byte pieces that hold at least one logit of the row.  workspace: ody_sample_workspace_bytes, 0 where a block has a row, 256-byte aligned.
  */
 int ody_sample(const void* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int rows, int vocab,
-               int64_t row_stride, int dtype, void* stream);
+               int64_t row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t ody_sample_workspace_bytes(int rows, int vocab, int dtype);
 
 /* ---- optimizer ------------------------------------------------------------
  * One step of torch.optim.AdamW (the optimizer of the reference's training loop, train.py:170,216) on one

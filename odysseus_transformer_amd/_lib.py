@@ -68,7 +68,8 @@ SIGNATURES = {
     "ody_paged_read_q8": (_i, [_p] * 8 + [_i] * 4 + [_i64] * 12 + [_i] * 4 + [_i64, _i, _p]),
     "ody_paged_attn_q8_workspace_bytes": (_sz, [_i] * 8),
     "ody_paged_attn_q8": (_i, [_p] * 10 + [_i] * 5 + [_i64] * 18 + [_i] * 4 + [_i64, _f, _i, _p, _sz, _p]),
-    "ody_sample": (_i, [_p] * 6 + [_f, _i, _f, _f] + [_p] * 2 + [_i] * 2 + [_i64, _i, _p]),
+    "ody_sample": (_i, [_p] * 6 + [_f, _i, _f, _f] + [_p] * 2 + [_i] * 2 + [_i64, _i, _p, _sz, _p]),
+    "ody_sample_workspace_bytes": (_sz, [_i] * 3),
     "ody_attn_bwd_dropout": (_i, [_p] * 9 + [_i] * 6 + [_i64] * 24 + [_f, _i, _i, _i, _p, _sz, _p, _f, _u64]),
 }
 

@@ -40,7 +40,7 @@ namespace {
   X(ody_linear_dgrad_swiglu_workspace_bytes) X(ody_linear_dgrad_swiglu) X(ody_attn_fwd_workspace_bytes) X(ody_attn_fwd)           \
   X(ody_attn_bwd_workspace_bytes) X(ody_attn_bwd) X(ody_attn_bwd_rope) X(ody_rope) X(ody_rope_table)           \
   X(ody_norm_linear_rope) X(ody_norm_linear_swiglu_h) X(ody_paged_append) X(ody_paged_attn) X(ody_paged_attn_workspace_bytes) \
-  X(ody_paged_append_q8) X(ody_paged_read_q8) X(ody_paged_attn_q8) X(ody_paged_attn_q8_workspace_bytes) X(ody_sample)
+  X(ody_paged_append_q8) X(ody_paged_read_q8) X(ody_paged_attn_q8) X(ody_paged_attn_q8_workspace_bytes) X(ody_sample) X(ody_sample_workspace_bytes)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -710,8 +710,9 @@ PyObject* sample(Call c) {
     }
   }
   at::Tensor tokens = at::empty({rows}, x.options().dtype(at::kLong).requires_grad(false)), logprobs = make_f32({rows}, x);
+  Scratch ws(lib.ody_sample_workspace_bytes((int)rows, (int)vocab, dt(x)), "sample_workspace", x, own_scratch_fn);
   CALL(ody_sample, x.data_ptr(), u, of_rows[0], (const int*)of_rows[1], of_rows[2], of_rows[3], (float)of_all[0], (int)of_all[1], (float)of_all[2], (float)of_all[3],
-       tokens.data_ptr<int64_t>(), logprobs.data_ptr<float>(), (int)rows, (int)vocab, x.stride(0), dt(x), (void*)c.stream);
+       tokens.data_ptr<int64_t>(), logprobs.data_ptr<float>(), (int)rows, (int)vocab, x.stride(0), dt(x), ws.ptr(), ws.bytes, (void*)c.stream);
   return tuple(tokens, logprobs);
 }
 

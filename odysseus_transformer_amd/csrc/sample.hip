@@ -35,6 +35,14 @@ typedef const u32x4 __attribute__((address_space(1)))* vector_ptr;
 constexpr int THREADS = 512, WAVES = THREADS / 64, BUCKETS = 2048, LIST = 4096, OCTAVE = 1024, VALUES = 8192;
 constexpr int MOST = (1 << 21) - 4;   // tokens of a row: nth_of() counts the matches in each 64 vectors, of 4 values or 8, in 2 * LIST numbers
 
+// What finding the token among listed ones takes: top_p's weights, those before its bucket, before the random number's; of the list those before top_p's bucket
+struct Ends {
+  u64 target, mass, mass_u, in_front;
+};
+struct RowEnds {
+  Ends q;
+  u64 kept, most;   // all weights; what min_p keeps of them
+};
 struct SampleParams {
   const void* logits;
   int64_t row_stride;
@@ -45,6 +53,15 @@ struct SampleParams {
   int64_t* tokens;
   float* logprobs;
   int vocab, frac;
+  // a row in `slices` of `slice` tokens: results of the slices, [row][slice][BUCKETS]; of bf16 rows [row][slice][VALUES]
+  int slices, slice;
+  u64 *mass, *over;        // sums of the weights by buckets, or (counts) of the tokens; what min_p keeps of a slice
+  unsigned* counts;
+  int2* ends;              // bf16: the least and the largest bits
+  float* largest;
+  unsigned* listed;        // [row]: entries of its list
+  RowEnds* ends_of_rows;
+  u64* lists;              // [row][LIST]
 };
 
 // x as a number whose order is that of the logits: -0 as 0, NaN as the lowest
@@ -466,6 +483,105 @@ struct Sampler {
     return slot_of<EACH>(by_count, target, threadIdx.x * EACH, c, m, numbers, weights, count, mass);
   }
 
+  // ---- fp32
+  // Tokens by buckets of their values alone
+  __device__ __forceinline__ void count_buckets() {
+    row.all([&](float x, int, int) {
+      const unsigned b = w.plain_bucket(x);
+      if (b < BUCKETS - 1) atomicAdd(&s.count[b], 1u);
+    });
+  }
+  // Sums of the weights by buckets; what a thread has of weights that are not less than `least`, where that is asked for.
+  // (Many can be in the last bucket, which is everything below 2^-32: it is summed up by each thread.)
+  __device__ __forceinline__ u64 add_weights(bool cut_m, u64 least) {
+    u64 over = 0, tail = 0;
+    const auto put = [&](u64 wt, unsigned b) __attribute__((always_inline)) {
+      if (b == BUCKETS - 1) tail += wt;
+      else atomicAdd(&s.mass[b], wt);
+    };
+    if (cut_m)
+      row.all([&](float x, int, int) {
+        unsigned b;
+        const u64 wt = w.of(x, b);
+        put(wt, b);
+        over += wt >= least ? wt : 0;
+      });
+    else
+      row.all([&](float x, int, int) {
+        unsigned b;
+        const u64 wt = w.of(x, b);
+        put(wt, b);
+      });
+    tail = wave_scan(tail);
+    if ((threadIdx.x & 63) == 63) atomicAdd(&s.mass[BUCKETS - 1], tail);
+    return over;
+  }
+  // The few that may be among the first top_k, s.count by buckets: into the list.  More than LIST: not so few.
+  __device__ __forceinline__ int gather_first(int top_k) {
+    u64 count = 0, mass = 0;
+    const int last = bucket_of(nullptr, s.count, true, top_k, count, mass);
+    if (last >= BUCKETS) return LIST + 1;
+    const float end = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, (float)(last + 1)) - 1);   // up to the number below it, of buckets
+    return gather_within([&](float x) __attribute__((always_inline)) { return w.plain(x) - end; });
+  }
+  // ... of which there are n: the token's entry
+  template <typename S> __device__ __forceinline__ u64 among_first(int n, const S& set, u64& kept) {
+    order(n);
+    const int k = min(n, set.top_k);
+    u64 upto[PER], was[PER], upto_p, entry;
+    kept = sums(k, 0, upto, was);
+    if (set.cut_p) {
+      find(k, false, set.target_p(kept), 0, upto, was, entry, upto_p);
+      kept = min(kept, upto_p);
+    }
+    if (set.cut_m) {
+      u64 over = 0, heavy;
+#pragma unroll
+      for (int j = 0; j < PER; j++) over += upto[j] - was[j] >= set.least && (int)threadIdx.x * PER + j < k ? upto[j] - was[j] : 0;
+      block_scan(s, over, heavy);
+      kept = min(kept, max(set.one, heavy));   // the first one at any rate
+    }
+    __syncthreads();
+    find(k, false, set.target_u(kept), 0, upto, was, entry, upto_p);
+    return entry;
+  }
+  // top_p and the token in one go: whichever token of its bucket top_p ends with, the random number's is in one or two buckets, which are gathered with it.  
+  static constexpr int EACH = BUCKETS / THREADS;
+  // Into the list, by a thread's buckets with `m` in front of them, `kept` in all, of which min_p keeps `most`; more than LIST: too many.
+  template <typename S> __device__ __forceinline__ int gather_ends(const S& set, u64 m, const u64 (&weights)[EACH], u64 kept, u64 most, Ends& q) {
+    const unsigned none[EACH] = {};
+    u64 count = 0, mass_v = 0;
+    const auto bucket_with = [&](u64 sum, u64& before) __attribute__((always_inline)) {
+      return (unsigned)slot_of<EACH>(false, sum, (int)threadIdx.x * EACH, 0, m, none, weights, count, before);
+    };
+    float lo, hi, lo_u, hi_u, nothing;
+    q = Ends{};
+    if (!set.cut_p) {
+      range_of(bucket_with(set.target_u(min(kept, most)), q.mass_u), lo, hi);
+      return gather_within([&](float x) __attribute__((always_inline)) { return outside(x, lo, hi); });
+    }
+    q.target = set.target_p(kept);
+    const unsigned b = bucket_with(q.target, q.mass), u = bucket_with(set.target_u(min(most, q.mass + 1)), q.mass_u), v = bucket_with(set.target_u(min(most, q.mass + s.mass[b])), mass_v);
+    q.in_front = (v == b ? q.mass : mass_v + s.mass[v]) - q.mass_u;
+    range_of(b, lo, hi), range_of(u, lo_u, hi_u);
+    if (v != u) range_of(v, lo_u, nothing);
+    return gather_within([&](float x) __attribute__((always_inline)) { return fminf(outside(x, lo, hi), outside(x, lo_u, hi_u)); });
+  }
+  // The token's entry among the n of the list.
+  template <typename S> __device__ __forceinline__ u64 among_ends(int n, const S& set, u64 most, const Ends& q, u64& kept) {
+    u64 upto[PER], was[PER], upto_p, entry;
+    order(n);
+    sums(n, 0, upto, was);
+    if (set.cut_p) {
+      find(n, false, q.target - q.mass + q.in_front, 0, upto, was, entry, upto_p);
+      kept = min(kept, q.mass + (upto_p - q.in_front));
+      __syncthreads();
+    }
+    kept = min(kept, most);
+    find(n, false, set.target_u(kept) - q.mass_u, 0, upto, was, entry, upto_p);
+    return entry;
+  }
+
   // The `nth` (from 1) token with this key, by its index.
   __device__ __forceinline__ int nth_of(unsigned key, unsigned nth) {
     unsigned* counts = reinterpret_cast<unsigned*>(s.list);   // of each 64 vectors
@@ -621,6 +737,8 @@ struct Settings {
       : temperature(p.temperature ? p.temperature[r] : p.temperature_all), top_p(p.top_p ? p.top_p[r] : p.top_p_all), min_p(p.min_p ? p.min_p[r] : p.min_p_all), u(p.u[r]),
         top_k(p.top_k ? p.top_k[r] : p.top_k_all), frac(p.frac), cut_k(top_k > 0 && top_k < p.vocab), cut_p(top_p < 1.f), cut_m(min_p > 0.f), one(1ull << p.frac),
         least(cut_m ? (u64)fmin(ceil((double)min_p * (double)one), 9e18) : 0) {}
+  // all that may be among the first top_k are few, and nothing else need have a weight formed
+  __device__ __forceinline__ bool few() const { return cut_k && top_k <= LIST / 2; }
   // the weights with which top_p is reached, of those kept so far, and the random number's
   __device__ __forceinline__ u64 target_p(u64 kept) const {
     const u64 p64 = part(top_p);
@@ -653,15 +771,15 @@ __device__ __forceinline__ void write(const SampleParams& p, int r, const Weight
   p.logprobs[r] = (float)((log2w + p.frac - y) * 0.6931471805599453 - (d - 0.5 * d * d));
 }
 // The largest of a row, for all threads.
-template <typename R> __device__ __forceinline__ float largest_of(const R& row, Shared& s) {
+template <typename R> __device__ __forceinline__ float largest_of(const R& row, float* wave_max) {
   float x = -INFINITY;
   row.all([&](float y, int, int) { x = fmaxf(x, y); });   // of a NaN and a number the number
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) x = fmaxf(x, __shfl_xor(x, d, 64));
-  if ((threadIdx.x & 63) == 0) s.wave_max[threadIdx.x >> 6] = x;
+  if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = x;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < WAVES; k++) x = fmaxf(x, s.wave_max[k]);
+  for (int k = 0; k < WAVES; k++) x = fmaxf(x, wave_max[k]);
   return x;
 }
 // The largest logit is +inf: those are equals with all of the weight.
@@ -690,15 +808,116 @@ __device__ __forceinline__ void fill_table(Shared& s) {
 __device__ __forceinline__ unsigned base_of(int most) { return (unsigned)max(128, (most + 127) * 128 - VALUES / 2); }
 constexpr int USUAL = 7;   // logits below 128: the largest need not be known to count them
 
+constexpr int VALUES_EACH = VALUES / THREADS;   // values of a thread, of one exponent
+static_assert(128 % VALUES_EACH == 0 && VALUES_EACH == 16, "values of one exponent; lanes of a row sum");
+
+// Tokens nearer to 0 than the window keep weights of their own: their sums to s.small.
+template <typename S, typename R> __device__ __forceinline__ void add_small(const Settings& set, Shared& s, S& a, const R& row, unsigned base) {
+  u64 mass = 0, over = 0;
+  unsigned count = 0;
+  row.matches([&](float x) { return (__builtin_bit_cast(unsigned, x) >> 16 & 0x7fff) < base; }, [&](float x, int) {
+    const u64 wt = a.w.of(x);
+    mass += wt, over += wt >= set.least ? wt : 0, count++;
+  });
+  if (count) {
+    atomicAdd(&s.small[0], mass), atomicAdd(&s.small[1], over);
+    atomicAdd(&s.small_tokens, count);
+  }
+}
+// The cuts, then the token, by the thread's numbers of tokens by value, which s.count has too, in a window from `base` on: its value and its number among those with it, or (`listed`) its
+// entry.  `small`: s.small has what is nearer to 0.  Not WHOLE: false, where a place is among those, which a's row has not all of.
+template <bool WHOLE, typename S>
+__device__ __forceinline__ bool choose_value(const Settings& set, Shared& s, S& a, unsigned base, float top, const unsigned (&tokens)[VALUES_EACH], bool small, float& x, unsigned& nth,
+                                             bool& listed, u64& entry, u64& kept) {
+  constexpr int EACH = VALUES_EACH;
+  const int tid = threadIdx.x;
+  // ---- weights by value: those of a thread are evenly spaced, so that one is a constant times the one before
+  const int v0 = tid * EACH;
+  const bool positive = v0 < VALUES / 2;
+  const unsigned bits = positive ? base + (VALUES / 2 - 1 - v0) : base + (v0 - VALUES / 2);   // of the first one; each has one less, or, among the negative ones, one more
+  const float x0 = __builtin_bit_cast(float, bits << 16 | (positive ? 0u : 0x80000000u));
+  u64 mass_here = 0, m, c = 0, all = 0, over = 0;
+  unsigned tokens_here = 0;
+#pragma unroll
+  for (int k = 0; k < EACH; k++) tokens_here += tokens[k];
+  const int skip = x0 > top ? abs((int)bits - (int)(__builtin_bit_cast(unsigned, top) >> 16 & 0x7fff)) : 0;   // values above the largest: nobody's
+  double first = 0.0, ratio = 0.0;   // of value `skip`; of a step of this exponent
+  if (__any(tokens_here != 0)) {
+    unsigned n;
+    first = a.w.power(a.w.steps(fminf(x0, top)), n);
+    ratio = a.w.power(fmin(__builtin_bit_cast(double, (u64)(1023 - 134 + (bits >> 7)) << 52) * a.w.c, 60.0 * OCTAVE), n);
+    double weight = first;
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const u64 wt = a.w.whole(weight), sum = wt * tokens[k];
+      mass_here += sum, over += wt >= set.least ? sum : 0;
+      weight *= k < skip ? 1.0 : ratio;
+    }
+  }
+  // tokens next to 0 are behind the last positive value's
+  const bool next_to_0 = small && v0 == VALUES / 2 - EACH;
+  m = block_scan(s, mass_here + (next_to_0 ? s.small[0] : 0), kept);
+  if (set.cut_k) c = block_scan(s, tokens_here + (next_to_0 ? s.small_tokens : 0), all);
+  if (set.cut_m) {
+    u64 heavy;
+    block_scan(s, over, heavy);
+    over = max(set.one, heavy + s.small[1]);   // the first one at any rate
+  }
+  // ---- the cuts, then the token
+  for (int step = set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
+    if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
+    if (step == 1 && !set.cut_p) continue;
+    if (step == 2 && set.cut_m) kept = min(kept, over);
+    const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
+    const bool by_count = step == 0;
+    __syncthreads();
+    // found: the value's bits and the number of its token, the weights up to and with that one; or the tokens next to 0, with the sums before them
+    const bool here = by_count ? c < target && c + tokens_here >= target : m < target && m + mass_here >= target;
+    if (const u64 those = __ballot(here)) {   // one thread's: 16 lanes take a value of it each
+      const int lane = tid & 63, from = __ffsll(those) - 1, k = lane & (EACH - 1), skipped = __builtin_amdgcn_readlane(skip, from);
+      const unsigned its_bits = __builtin_amdgcn_readlane(bits, from), its_first = (tid - lane + from) * EACH, number = s.count[its_first + k];
+      const double its_ratio = __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, ratio), from));
+      double weight = __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, first), from));
+#pragma unroll
+      for (int j = 0; j < EACH - 1; j++) weight *= j < skipped || j >= k ? 1.0 : its_ratio;
+      const u64 wt = a.w.whole(weight), mass = wt * number, upto = read_lane(m, from) + row_scan(mass), count = read_lane(c, from) + row_scan(number);
+      if (lane < EACH && (by_count ? count - number < target && count >= target : upto - mass < target && upto >= target)) {
+        unsigned nth = (unsigned)(target - (count - number));
+        if (!by_count) {   // the least with nth wt >= what is missing
+          const u64 missing = target - (upto - mass);
+          nth = max(1u, (unsigned)((double)missing * __builtin_amdgcn_rcp((double)wt)));
+          while (nth * wt < missing) nth++;
+          while ((nth - 1) * wt >= missing) nth--;
+        }
+        s.found[0] = (u64)(its_first < VALUES / 2 ? its_bits - k : (its_bits + k) | 0x8000u) << 32 | nth, s.found[1] = upto - mass + nth * wt, s.words[1] = 0;
+      }
+    }
+    if (next_to_0 && !here && (by_count ? c + tokens_here < target && c + tokens_here + s.small_tokens >= target : m + mass_here < target && m + mass_here + s.small[0] >= target)) {
+      s.found[0] = c + tokens_here, s.found[1] = m + mass_here, s.words[1] = 1;
+    }
+    __syncthreads();
+    u64 upto = s.found[1];
+    const u64 found = s.found[0];
+    if (s.words[1]) {
+      if (!WHOLE) return false;
+      const unsigned key = key_of(__builtin_bit_cast(float, (base - 1) << 16));
+      a.resolve(of_key(~key), of_key(key), by_count, target, found, s.found[1], step == 2, entry, upto);
+      listed = true;
+    } else {
+      x = __builtin_bit_cast(float, (unsigned)(found >> 32) << 16), nth = (unsigned)found;
+      listed = false;
+    }
+    if (step < 2) kept = min(kept, upto);
+  }
+  return true;
+}
+
+// A whole row.
 template <int NV>
-__global__ __launch_bounds__(THREADS) void sample_values_kernel(const SampleParams p) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  Shared& s = *reinterpret_cast<Shared*>(smem);
-  constexpr int EACH = VALUES / THREADS;   // values of a thread, of one exponent
-  static_assert(128 % EACH == 0 && EACH == 16, "values of one exponent; lanes of a row sum");
-  const int r = blockIdx.x, tid = threadIdx.x;
+__device__ __forceinline__ void sample_values_row(const SampleParams& p, int r, const Settings& set, Shared& s) {
+  constexpr int EACH = VALUES_EACH;
+  const int tid = threadIdx.x;
   Row<bf16, NV> row(static_cast<const bf16*>(p.logits) + r * p.row_stride, p.vocab);
-  const Settings set(p, r);
   fill_table(s);
   Sampler<bf16, NV> a{s, row, set.weights(0.f, s.table)};
 
@@ -731,7 +950,7 @@ __global__ __launch_bounds__(THREADS) void sample_values_kernel(const SamplePara
     const unsigned positive = s.words[1];   // bits of the largest one, and 1
     top = __builtin_bit_cast(float, (positive - 1) << 16);
     const bool seen = positive > 0 && positive <= base + VALUES / 2;   // else all are negative, or it is beyond the window: infinite or NaN perhaps
-    if (!seen) top = largest_of(row, s);
+    if (!seen) top = largest_of(row, s.wave_max);
     if (top == -INFINITY) {
       write_first(p, r, true, 0);
       return;
@@ -754,111 +973,30 @@ __global__ __launch_bounds__(THREADS) void sample_values_kernel(const SamplePara
     a.w.top = top, a.w.topf = top;
     const bool small = s.words[0] < base;
     if (small) {   // nearer to 0 than the window
-      u64 mass = 0, over = 0;
-      unsigned count = 0;
-      row.matches([&](float x) { return (__builtin_bit_cast(unsigned, x) >> 16 & 0x7fff) < base; }, [&](float x, int) {
-        const u64 wt = a.w.of(x);
-        mass += wt, over += wt >= set.least ? wt : 0, count++;
-      });
-      if (count) {
-        atomicAdd(&s.small[0], mass), atomicAdd(&s.small[1], over);
-        atomicAdd(&s.small_tokens, count);
-      }
+      add_small(set, s, a, row, base);
       __syncthreads();
     }
-    // ---- weights by value: those of a thread are evenly spaced, so that one is a constant times the one before
-    const int v0 = tid * EACH;
-    const bool positive = v0 < VALUES / 2;
-    const unsigned bits = positive ? base + (VALUES / 2 - 1 - v0) : base + (v0 - VALUES / 2);   // of the first one; each has one less, or, among the negative ones, one more
-    const float x0 = __builtin_bit_cast(float, bits << 16 | (positive ? 0u : 0x80000000u));
-    u64 mass_here = 0, m, c = 0, all = 0, over = 0;
-    unsigned tokens_here = 0;
-#pragma unroll
-    for (int k = 0; k < EACH; k++) tokens_here += tokens[k];
-    const int skip = x0 > top ? abs((int)bits - (int)(__builtin_bit_cast(unsigned, top) >> 16 & 0x7fff)) : 0;   // values above the largest: nobody's
-    double first = 0.0, ratio = 0.0;   // of value `skip`; of a step of this exponent
-    if (__any(tokens_here != 0)) {
-      unsigned n;
-      first = a.w.power(a.w.steps(fminf(x0, top)), n);
-      ratio = a.w.power(fmin(__builtin_bit_cast(double, (u64)(1023 - 134 + (bits >> 7)) << 52) * a.w.c, 60.0 * OCTAVE), n);
-      double weight = first;
-#pragma unroll
-      for (int k = 0; k < EACH; k++) {
-        const u64 wt = a.w.whole(weight), sum = wt * tokens[k];
-        mass_here += sum, over += wt >= set.least ? sum : 0;
-        weight *= k < skip ? 1.0 : ratio;
-      }
-    }
-    // tokens next to 0 are behind the last positive value's
-    const bool next_to_0 = small && v0 == VALUES / 2 - EACH;
-    m = block_scan(s, mass_here + (next_to_0 ? s.small[0] : 0), kept);
-    if (set.cut_k) c = block_scan(s, tokens_here + (next_to_0 ? s.small_tokens : 0), all);
-    if (set.cut_m) {
-      u64 heavy;
-      block_scan(s, over, heavy);
-      over = max(set.one, heavy + s.small[1]);   // the first one at any rate
-    }
-    // ---- the cuts, then the token
-    for (int step = set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
-      if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
-      if (step == 1 && !set.cut_p) continue;
-      if (step == 2 && set.cut_m) kept = min(kept, over);
-      const u64 target = step == 0 ? (u64)set.top_k : step == 1 ? set.target_p(kept) : set.target_u(kept);
-      const bool by_count = step == 0;
-      __syncthreads();
-      // found: the value's bits and the number of its token, the weights up to and with that one; or the tokens next to 0, with the sums before them
-      const bool here = by_count ? c < target && c + tokens_here >= target : m < target && m + mass_here >= target;
-      if (const u64 those = __ballot(here)) {   // one thread's: 16 lanes take a value of it each
-        const int lane = tid & 63, from = __ffsll(those) - 1, k = lane & (EACH - 1), skipped = __builtin_amdgcn_readlane(skip, from);
-        const unsigned its_bits = __builtin_amdgcn_readlane(bits, from), its_first = (tid - lane + from) * EACH, number = s.count[its_first + k];
-        const double its_ratio = __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, ratio), from));
-        double weight = __builtin_bit_cast(double, read_lane(__builtin_bit_cast(u64, first), from));
-#pragma unroll
-        for (int j = 0; j < EACH - 1; j++) weight *= j < skipped || j >= k ? 1.0 : its_ratio;
-        const u64 wt = a.w.whole(weight), mass = wt * number, upto = read_lane(m, from) + row_scan(mass), count = read_lane(c, from) + row_scan(number);
-        if (lane < EACH && (by_count ? count - number < target && count >= target : upto - mass < target && upto >= target)) {
-          unsigned nth = (unsigned)(target - (count - number));
-          if (!by_count) {   // the least with nth wt >= what is missing
-            const u64 missing = target - (upto - mass);
-            nth = max(1u, (unsigned)((double)missing * __builtin_amdgcn_rcp((double)wt)));
-            while (nth * wt < missing) nth++;
-            while ((nth - 1) * wt >= missing) nth--;
-          }
-          s.found[0] = (u64)(its_first < VALUES / 2 ? its_bits - k : (its_bits + k) | 0x8000u) << 32 | nth, s.found[1] = upto - mass + nth * wt, s.words[1] = 0;
-        }
-      }
-      if (next_to_0 && !here && (by_count ? c + tokens_here < target && c + tokens_here + s.small_tokens >= target : m + mass_here < target && m + mass_here + s.small[0] >= target)) {
-        s.found[0] = c + tokens_here, s.found[1] = m + mass_here, s.words[1] = 1;
-      }
-      __syncthreads();
-      u64 upto = s.found[1];
-      const u64 found = s.found[0];
-      if (s.words[1]) {
-        const unsigned key = key_of(__builtin_bit_cast(float, (base - 1) << 16));
-        a.resolve(of_key(~key), of_key(key), by_count, target, found, s.found[1], step == 2, entry, upto);
-        listed = true;
-      } else {
-        x = __builtin_bit_cast(float, (unsigned)(found >> 32) << 16), nth = (unsigned)found;
-        listed = false;
-      }
-      if (step < 2) kept = min(kept, upto);
-    }
+    choose_value<true>(set, s, a, base, top, tokens, small, x, nth, listed, entry, kept);
   }
   if (!listed) entry = a.pick(x, nth);
   if (set.temperature > 0.f) write(p, r, a.w, entry, kept);
   else write_first(p, r, false, entry);
 }
 
-// ---- fp32
-__global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
+template <int NV>
+__global__ __launch_bounds__(THREADS) void sample_values_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  Shared& s = *reinterpret_cast<Shared*>(smem);
-  const int r = blockIdx.x, tid = threadIdx.x;
+  sample_values_row<NV>(p, blockIdx.x, Settings(p, blockIdx.x), *reinterpret_cast<Shared*>(smem));
+}
+
+// ---- fp32
+// A whole row.
+__device__ __forceinline__ void sample_row(const SampleParams& p, int r, const Settings& set, Shared& s) {
+  const int tid = threadIdx.x;
   Row<float> row(static_cast<const float*>(p.logits) + r * p.row_stride, p.vocab);
-  const Settings set(p, r);
   fill_table(s);
   for (int b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0, s.count[b] = 0;
-  float largest = largest_of(row, s);
+  const float largest = largest_of(row, s.wave_max);
   Sampler<float> a{s, row, set.weights(largest, s.table)};
   if (largest == -INFINITY || !(set.temperature > 0.f)) {   // nothing to choose from, or nothing but the first
     write_first(p, r, largest == -INFINITY, largest == -INFINITY ? 0 : a.pick(largest, 1));
@@ -870,37 +1008,14 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
   }
   u64 entry = 0, kept = 0;
   // ---- few: all that may be among the first top_k into the list
-  bool few = set.cut_k && set.top_k <= LIST / 2;
-  if (few) {
-    row.all([&](float x, int, int) {
-      const unsigned b = a.w.plain_bucket(x);
-      if (b < BUCKETS - 1) atomicAdd(&s.count[b], 1u);
-    });
-    u64 count = 0, mass = 0;
+  bool done = false;
+  if (set.few()) {
+    a.count_buckets();
     __syncthreads();
-    const int last = a.bucket_of(nullptr, s.count, true, set.top_k, count, mass);
-    int n = LIST + 1;
-    const float end = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, (float)(last + 1)) - 1);   // up to the number below it, of buckets
-    if (last < BUCKETS) n = a.gather_within([&](float x) { return a.w.plain(x) - end; });
-    few = n <= LIST;
-    if (few) {
-      a.order(n);
-      const int k = min(n, set.top_k);
-      u64 upto[a.PER], was[a.PER], upto_p;
-      kept = a.sums(k, 0, upto, was);
-      if (set.cut_p) {
-        a.find(k, false, set.target_p(kept), 0, upto, was, entry, upto_p);
-        kept = min(kept, upto_p);
-      }
-      if (set.cut_m) {
-        u64 over = 0, heavy;
-#pragma unroll
-        for (int j = 0; j < a.PER; j++) over += upto[j] - was[j] >= set.least && tid * a.PER + j < k ? upto[j] - was[j] : 0;
-        block_scan(s, over, heavy);
-        kept = min(kept, max(set.one, heavy));   // the first one at any rate
-      }
-      __syncthreads();
-      a.find(k, false, set.target_u(kept), 0, upto, was, entry, upto_p);
+    const int n = a.gather_first(set.top_k);
+    done = n <= LIST;
+    if (done) {
+      entry = a.among_first(n, set, kept);
     } else {
       __syncthreads();
       for (int b = tid; b < BUCKETS; b += THREADS) s.count[b] = 0;
@@ -908,28 +1023,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
     }
   }
   // ---- sums of the weights by buckets of all
-  if (!few) {
-    // (many can be in the last bucket, which is everything below 2^-32: it is summed up by each thread)
-    u64 over = 0, tail = 0;   // over: of weights that are not less than min_p
-    const auto put = [&](u64 wt, unsigned b) __attribute__((always_inline)) {
-      if (b == BUCKETS - 1) tail += wt;
-      else atomicAdd(&s.mass[b], wt);
-    };
-    if (set.cut_m)
-      row.all([&](float x, int, int) {
-        unsigned b;
-        const u64 wt = a.w.of(x, b);
-        put(wt, b);
-        over += wt >= set.least ? wt : 0;
-      });
-    else
-      row.all([&](float x, int, int) {
-        unsigned b;
-        const u64 wt = a.w.of(x, b);
-        put(wt, b);
-      });
-    tail = wave_scan(tail);
-    if ((tid & 63) == 63) atomicAdd(&s.mass[BUCKETS - 1], tail);
+  if (!done) {
+    u64 over = a.add_weights(set.cut_m, set.least);
     if (set.cut_k) {
       unsigned last = 0;
       row.all([&](float x, int, int) {
@@ -955,33 +1050,14 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
       block_scan(s, over, heavy);
       over = max(set.one, heavy);   // the first one at any rate
     }
-    // top_p and the token in one go: whichever token of its bucket top_p ends with, the random number's is in one or two buckets, which are gathered with it
-    bool both = false;
-    if (set.cut_p && !set.cut_k) {
-      const u64 most = set.cut_m ? over : ~0ull, target = set.target_p(kept);
-      u64 count = 0, mass = 0, mass_u = 0, mass_v = 0, upto_p;
-      const auto bucket_with = [&](u64 sum, u64& before) __attribute__((always_inline)) {
-        return (unsigned)a.template slot_of<EACH>(false, sum, tid * EACH, c, m, tokens, weights, count, before);
-      };
-      // top_p's bucket b; the random number's, from u to v, in front of it or up to it
-      const unsigned b = bucket_with(target, mass), bu = bucket_with(set.target_u(min(most, mass + 1)), mass_u), bv = bucket_with(set.target_u(min(most, mass + s.mass[b])), mass_v);
-      float lo, hi, lo_u, hi_u, none;
-      a.range_of(b, lo, hi), a.range_of(bu, lo_u, hi_u);
-      if (bv != bu) a.range_of(bv, lo_u, none);
-      const int n = a.gather_within([&](float x) __attribute__((always_inline)) { return fminf(a.outside(x, lo, hi), a.outside(x, lo_u, hi_u)); });
-      both = n <= LIST;
-      if (both) {
-        a.order(n);
-        const u64 in_front = (bv == b ? mass : mass_v + s.mass[bv]) - mass_u;   // of the list's part that is bucket b
-        u64 upto[a.PER], was[a.PER];
-        a.sums(n, 0, upto, was);
-        a.find(n, false, target - mass + in_front, 0, upto, was, entry, upto_p);
-        kept = min(min(kept, mass + (upto_p - in_front)), most);
-        __syncthreads();
-        a.find(n, false, set.target_u(kept) - mass_u, 0, upto, was, entry, upto_p);
-      }
+    if (!set.cut_k) {
+      Ends q;
+      const u64 most = set.cut_m ? over : ~0ull;
+      const int n = a.gather_ends(set, m, weights, kept, most, q);
+      done = n <= LIST;
+      if (done) entry = a.among_ends(n, set, most, q, kept);
     }
-    for (int step = both ? 3 : set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
+    for (int step = done ? 3 : set.cut_k ? 0 : set.cut_p ? 1 : 2; step < 3; step++) {
       if (step == 0 && all < (u64)set.top_k) continue;   // all that have a weight
       if (step == 1 && !set.cut_p) continue;
       if (step == 2 && set.cut_m) kept = min(kept, over);
@@ -997,28 +1073,282 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
   write(p, r, a.w, entry, kept);
 }
 
-template <typename K> int launch(K kernel, const SampleParams& p, int rows, hipStream_t st) {
+__global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  sample_row(p, blockIdx.x, Settings(p, blockIdx.x), *reinterpret_cast<Shared*>(smem));
+}
+
+// ---- few long rows: a row in slices, a block each, in launches between which all slices' results are there
+template <typename T> __device__ __forceinline__ Row<T> slice_of(const SampleParams& p, int r, int j) {
+  return Row<T>(static_cast<const T*>(p.logits) + r * p.row_stride + j * p.slice, min(p.slice, p.vocab - j * p.slice));
+}
+__device__ __forceinline__ float largest_slice(const SampleParams& p, int r) {
+  const int lane = threadIdx.x & 63;
+  float x = lane < p.slices ? p.largest[r * p.slices + lane] : -INFINITY;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x = fmaxf(x, __shfl_xor(x, d, 64));
+  return x;
+}
+// Sums over a row's slices of N vectors of a thread, SIDE slices' loads at once.
+template <int N, typename V> __device__ __forceinline__ void add_slices(V (&sum)[N], const V* from, int pitch, int slices) {
+  constexpr int SIDE = 4;
+  for (int k = 0; k < slices; k += SIDE) {
+    V x[SIDE][N];
+#pragma unroll
+    for (int q = 0; q < SIDE; q++)
+#pragma unroll
+      for (int e = 0; e < N; e++) x[q][e] = from[(int64_t)min(k + q, slices - 1) * pitch + e];
+#pragma unroll
+    for (int q = 0; q < SIDE; q++)
+#pragma unroll
+      for (int e = 0; e < N; e++) sum[e] += k + q < slices ? x[q][e] : V{};
+  }
+}
+// bf16: the slices' tokens by value,
+__global__ __launch_bounds__(THREADS) void sample_counts_kernel(const SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
+  Row<bf16> row = slice_of<bf16>(p, r, j);
+  for (int b = tid; b < VALUES / 4; b += THREADS) reinterpret_cast<u32x4*>(s.count)[b] = u32x4{0, 0, 0, 0};
+  if (tid == 0) s.words[0] = ~0u, s.words[1] = 0;
+  __syncthreads();
+  unsigned least;
+  int greatest;
+  row.count_values(s.count, base_of(USUAL), least, greatest);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) least = min(least, (unsigned)__shfl_xor((int)least, d, 64)), greatest = max(greatest, __shfl_xor(greatest, d, 64));
+  if ((tid & 63) == 0) {
+    atomicMin(&s.words[0], least);
+    if (greatest >= 0) atomicMax(&s.words[1], (unsigned)greatest + 1);
+  }
+  __syncthreads();
+  for (int b = tid; b < VALUES / 4; b += THREADS) reinterpret_cast<u32x4*>(p.counts + (int64_t)blockIdx.x * VALUES)[b] = reinterpret_cast<u32x4*>(s.count)[b];
+  if (tid == 0) p.ends[blockIdx.x] = make_int2((int)s.words[0], (int)s.words[1]);
+}
+// and the token: every block finds its value and the slice that has it, which looks for it.  Rows for which that will not do -- the largest is not a positive one below 128, or the token is
+// one next to 0 -- one block, all of it.
+__global__ __launch_bounds__(THREADS) void sample_counted_kernel(const SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
+  const Settings set(p, r);
+  const unsigned base = base_of(USUAL), *counts = p.counts + (int64_t)r * p.slices * VALUES;
+  const int lane = tid & 63;
+  const int2 ends = p.ends[r * p.slices + min(lane, p.slices - 1)];
+  u32x4 fours[VALUES_EACH / 4] = {};
+  add_slices(fours, reinterpret_cast<const u32x4*>(counts + tid * VALUES_EACH), VALUES / 4, p.slices);
+  unsigned least = (unsigned)ends.x, positive = (unsigned)ends.y, tokens[VALUES_EACH];
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) least = min(least, (unsigned)__shfl_xor((int)least, d, 64)), positive = max(positive, (unsigned)__shfl_xor((int)positive, d, 64));
+#pragma unroll
+  for (int k = 0; k < VALUES_EACH; k++) tokens[k] = fours[k / 4][k % 4];
+  const float top = __builtin_bit_cast(float, (positive - 1) << 16);   // as in a whole row
+  const bool seen = positive > base && positive <= base + VALUES / 2, greedy = !(set.temperature > 0.f);
+  bool whole = !seen || (!greedy && !(top + 36.f * set.temperature < (float)(1 << USUAL)));
+  if (whole && j != 0) return;
+  Row<bf16> row = slice_of<bf16>(p, r, j);
+  Sampler<bf16> a{s, row, set.weights(top, s.table)};
+  float x = top;
+  unsigned nth = 1;
+  u64 entry = 0, kept = 0;
+  if (!greedy && !whole) {
+    bool listed;
+    fill_table(s);
+#pragma unroll
+    for (int q = 0; q < VALUES_EACH / 4; q++) reinterpret_cast<u32x4*>(s.count)[tid * (VALUES_EACH / 4) + q] = fours[q];
+    if (tid == 0) s.small[0] = s.small[1] = 0, s.small_tokens = 0;
+    __syncthreads();
+    for (int k = 0; least < base && k < p.slices; k++)
+      if ((unsigned)p.ends[r * p.slices + k].x < base) add_small(set, s, a, slice_of<bf16>(p, r, k), base);
+    __syncthreads();
+    whole = !choose_value<false>(set, s, a, base, top, tokens, least < base, x, nth, listed, entry, kept);
+  }
+  if (whole) {
+    __syncthreads();
+    if (j == 0) sample_values_row<0>(p, r, set, s);
+    return;
+  }
+  // the slices' numbers of it, in 16 lanes
+  const unsigned bits = __builtin_bit_cast(unsigned, x) >> 16, d = (bits & 0x7fff) - base, place = bits & 0x8000 ? VALUES / 2 + d : VALUES / 2 - 1 - d;
+  const unsigned mine = lane < p.slices ? counts[lane * VALUES + place] : 0, upto = (unsigned)row_scan(mine);
+  const int of = __ffsll(__ballot(lane < p.slices && upto >= nth)) - 1;
+  if (of != j) return;
+  nth -= __builtin_amdgcn_readlane(upto - mine, of);
+  entry = a.pick(x, nth) + (unsigned)(j * p.slice);
+  if (greedy) write_first(p, r, false, entry);
+  else write(p, r, a.w, entry, kept);
+}
+// fp32: the slices' largest,
+__global__ __launch_bounds__(THREADS) void sample_largest_kernel(const SampleParams p) {
+  __shared__ float wave_max[WAVES];
+  const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices;
+  const Row<float> row = slice_of<float>(p, r, j);
+  const float x = largest_of(row, wave_max);
+  if (threadIdx.x == 0) p.largest[blockIdx.x] = x;
+  if (threadIdx.x == 0 && j == 0) p.listed[r] = 0;
+}
+// their sums by buckets,
+__device__ __forceinline__ bool in_slices(const Settings& set, float largest) {
+  return set.temperature > 0.f && fabsf(largest) < INFINITY && (set.few() || !set.cut_k);
+}
+__global__ __launch_bounds__(THREADS) void sample_buckets_kernel(const SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
+  const Settings set(p, r);
+  const float largest = largest_slice(p, r);
+  if (!in_slices(set, largest)) return;
+  const bool few = set.few();
+  Row<float> row = slice_of<float>(p, r, j);
+  Sampler<float> a{s, row, set.weights(largest, s.table)};
+  if (!few) fill_table(s);
+  for (int b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0, s.count[b] = 0;
+  __syncthreads();
+  if (few) {
+    a.count_buckets();
+    __syncthreads();
+    for (int b = tid; b < BUCKETS / 4; b += THREADS) reinterpret_cast<u32x4*>(p.mass + (int64_t)blockIdx.x * BUCKETS)[b] = reinterpret_cast<u32x4*>(s.count)[b];
+  } else {
+    u64 over = a.add_weights(set.cut_m, set.least), heavy;
+    block_scan(s, over, heavy);
+    if (tid == 0) p.over[blockIdx.x] = heavy;
+    for (int b = tid; b < BUCKETS / 2; b += THREADS) reinterpret_cast<u32x4*>(p.mass + (int64_t)blockIdx.x * BUCKETS)[b] = reinterpret_cast<u32x4*>(s.mass)[b];
+  }
+}
+// what each has in the buckets that matter, which every block finds for itself,
+__global__ __launch_bounds__(THREADS) void sample_slices_kernel(const SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
+  const Settings set(p, r);
+  const float largest = largest_slice(p, r);
+  Row<float> row = slice_of<float>(p, r, j);
+  Sampler<float> a{s, row, set.weights(largest, s.table)};
+  if (largest == -INFINITY || !(set.temperature > 0.f)) {   // nothing, or the first: in the first slice that has it
+    int first = 0;
+    while (p.largest[r * p.slices + first] != largest) first++;
+    if (j == first) write_first(p, r, largest == -INFINITY, largest == -INFINITY ? 0 : a.pick(largest, 1) + (unsigned)(j * p.slice));
+    return;
+  }
+  if (!in_slices(set, largest)) return;
+  RowEnds e{};
+  e.most = ~0ull;
+  const u64* mass = p.mass + (int64_t)r * p.slices * BUCKETS;
+  int n;
+  if (set.few()) {
+    u32x4 sum[1] = {};
+    add_slices(sum, reinterpret_cast<const u32x4*>(mass) + tid, BUCKETS / 2, p.slices);
+    reinterpret_cast<u32x4*>(s.count)[tid] = sum[0];
+    __syncthreads();
+    n = a.gather_first(set.top_k);
+  } else {
+    constexpr int EACH = BUCKETS / THREADS;
+    u64 weights[EACH] = {}, here = 0;
+    add_slices(weights, mass + tid * EACH, BUCKETS, p.slices);
+#pragma unroll
+    for (int i = 0; i < EACH; i++) s.mass[tid * EACH + i] = weights[i], here += weights[i];
+    const u64 m = block_scan(s, here, e.kept);
+    if (set.cut_m) {
+      block_scan(s, tid < p.slices ? p.over[r * p.slices + tid] : 0, e.most);
+      e.most = max(set.one, e.most);   // the first one at any rate
+    }
+    n = a.gather_ends(set, m, weights, e.kept, e.most, e.q);
+  }
+  if (tid == 0) s.words[2] = atomicAdd(&p.listed[r], (unsigned)n);
+  if (tid == 0 && j == 0) p.ends_of_rows[r] = e;
+  __syncthreads();
+  const unsigned to = s.words[2];
+  if (n <= LIST && to + n <= LIST)
+    for (int k = tid; k < n; k += THREADS) p.lists[(int64_t)r * LIST + to + k] = s.list[k] + (unsigned)(j * p.slice);
+}
+// and the token among them.  A row for which that will not do: all of it.
+__global__ __launch_bounds__(THREADS) void sample_listed_kernel(const SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const Settings set(p, r);
+  const float largest = largest_slice(p, r);
+  if (largest == -INFINITY || !(set.temperature > 0.f)) return;
+  const unsigned n = p.listed[r];
+  if (!in_slices(set, largest) || n > LIST) {
+    sample_row(p, r, set, s);
+    return;
+  }
+  Row<float> row(static_cast<const float*>(p.logits) + r * p.row_stride, p.vocab);
+  Sampler<float> a{s, row, set.weights(largest, s.table)};
+  for (int k = tid; k < (int)n; k += THREADS) s.list[k] = p.lists[(int64_t)r * LIST + k];
+  const RowEnds e = p.ends_of_rows[r];
+  fill_table(s);
+  __syncthreads();
+  u64 kept = e.kept;
+  const u64 entry = set.few() ? a.among_first((int)n, set, kept) : a.among_ends((int)n, set, e.most, e.q, kept);
+  write(p, r, a.w, entry, kept);
+}
+
+template <typename K> int launch(K kernel, const SampleParams& p, int blocks, hipStream_t st) {
   if (int rc = ody_allow_dynamic_lds(reinterpret_cast<const void*>(kernel), sizeof(Shared), "ody_sample")) return rc;
-  ODY_LAUNCH("sample", st, kernel, dim3((unsigned)rows), dim3(THREADS), sizeof(Shared), p);
+  ODY_LAUNCH("sample", st, kernel, dim3((unsigned)blocks), dim3(THREADS), sizeof(Shared), p);
   return ody_check_launch("sample");
+}
+
+// How rows are divided: long ones into slices, at most one a compute unit; of bf16 fewer, as each block reads the counts of all.  us by a block a row / in slices, top_p 0.9: fp32, one row of
+// 40000 24.7 / 22.4 (with top_k 20 16.1 / 19.3), of 70000 37.0 / 24.0 (22.6 / 19.5), of 250000 108 / 29 (61 / 21); 16 of 128000 64 / 34, 64 68 / 43, 128 73 / 63; bf16, one of 70000
+// 19.8 / 16.9, of 250000 42.9 / 19.5; 8 of 128000 30.0 / 19.9, 64 34.3 / 26.4, 128 35.4 / 28.9.
+struct Plan {
+  int slices, slice;
+  size_t ends, mass, over, largest, listed, bytes;   // places in the workspace, behind the lists (fp32) or the counts (bf16)
+};
+Plan plan(int rows, int vocab, int dtype) {
+  Plan q{};
+  q.slices = std::min(dtype == ODY_F32 ? 16 : rows > 8 ? 4 : 8, 256 / rows);
+  if (q.slices < 2 || vocab < 65536) return Plan{1, vocab, 0, 0, 0, 0, 0, 0};
+  q.slice = ((vocab + q.slices - 1) / q.slices + 7) / 8 * 8;
+  q.slices = (vocab + q.slice - 1) / q.slice;
+  const size_t all = (size_t)rows * q.slices;
+  if (dtype == ODY_BF16) {
+    q.ends = all * VALUES * sizeof(unsigned), q.bytes = q.ends + all * sizeof(int2);
+    return q;
+  }
+  q.mass = (size_t)rows * LIST * sizeof(u64), q.ends = q.mass + all * BUCKETS * sizeof(u64), q.over = q.ends + rows * sizeof(RowEnds);
+  q.largest = q.over + all * sizeof(u64), q.listed = q.largest + all * sizeof(float), q.bytes = q.listed + rows * sizeof(unsigned);
+  return q;
 }
 
 }  // namespace
 
+extern "C" size_t ody_sample_workspace_bytes(int rows, int vocab, int dtype) { return rows > 0 && vocab > 0 ? plan(rows, vocab, dtype).bytes : 0; }
+
 extern "C" int ody_sample(const void* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                           float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int rows, int vocab,
-                          int64_t row_stride, int dtype, void* stream) {
+                          int64_t row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   ODY_REQUIRE(logits && u && tokens && logprobs, ODY_ERR_NULL, "ody_sample: logits, u, tokens or logprobs is NULL");
   ODY_REQUIRE(rows > 0 && vocab > 0 && rows < 1 << 22 && vocab <= MOST, ODY_ERR_BAD_SHAPE, "ody_sample: %d rows of %d logits (fewer than 2^22 of at most %d)", rows, vocab, MOST);
   ODY_REQUIRE(row_stride >= vocab || rows == 1, ODY_ERR_BAD_SHAPE, "ody_sample: rows overlap (stride %lld)", (long long)row_stride);
   ODY_REQUIRE(dtype == ODY_BF16 || dtype == ODY_F32, ODY_ERR_UNSUPPORTED, "ody_sample: dtype %d unknown", dtype);
   ODY_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (dtype == ODY_BF16 ? 1 : 3)) == 0, ODY_ERR_MISALIGNED, "ody_sample: logits are not aligned to their size");
+  const Plan q = plan(rows, vocab, dtype);
+  ODY_REQUIRE(q.bytes == 0 || (workspace && workspace_bytes >= q.bytes && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0), ODY_ERR_WORKSPACE,
+              "ody_sample: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", q.bytes, workspace_bytes);
   int bits = 0;
   while (1 << bits < vocab) bits++;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
   const SampleParams p{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, tokens, logprobs, vocab,
-                       std::min(50, 62 - bits)};
+                       std::min(50, 62 - bits), q.slices, q.slice, reinterpret_cast<u64*>(ws + q.mass), reinterpret_cast<u64*>(ws + q.over), reinterpret_cast<unsigned*>(ws), reinterpret_cast<int2*>(ws + q.ends),
+                       reinterpret_cast<float*>(ws + q.largest), reinterpret_cast<unsigned*>(ws + q.listed), reinterpret_cast<RowEnds*>(ws + q.ends), reinterpret_cast<u64*>(ws)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == ODY_F32) return launch(&sample_kernel, p, rows, st);
+  if (dtype == ODY_F32 && q.slices == 1) return launch(&sample_kernel, p, rows, st);
+  if (dtype == ODY_F32) {
+    ODY_LAUNCH("sample_largest", st, sample_largest_kernel, dim3((unsigned)(rows * q.slices)), dim3(THREADS), 0, p);
+    if (int rc = ody_check_launch("sample_largest")) return rc;
+    if (int rc = launch(&sample_buckets_kernel, p, rows * q.slices, st)) return rc;
+    if (int rc = launch(&sample_slices_kernel, p, rows * q.slices, st)) return rc;
+    return launch(&sample_listed_kernel, p, rows, st);
+  }
+  if (q.slices > 1) {
+    if (int rc = launch(&sample_counts_kernel, p, rows * q.slices, st)) return rc;
+    return launch(&sample_counted_kernel, p, rows * q.slices, st);
+  }
   const int turns = (vocab + 14 + THREADS * 8 - 1) / (THREADS * 8);   // however rows are aligned
   if (turns <= 8) return launch(&sample_values_kernel<8>, p, rows, st);   // longer rows are counted while they arrive (256 of 128000: 45 us, 51 out of registers)
   return launch(&sample_values_kernel<0>, p, rows, st);

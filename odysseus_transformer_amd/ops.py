@@ -721,7 +721,10 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     tokens = torch.empty((rows,), dtype=torch.int64, device=logits.device)
     logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
     if rows:
-        _lib.call("ody_sample", logits.data_ptr(), *pointers, *numbers[1:], tokens.data_ptr(), logprobs.data_ptr(), rows, vocab, logits.stride(0), dt, _stream())
+        ws_bytes = _lib.load().ody_sample_workspace_bytes(rows, vocab, dt)
+        ws = _own_scratch(ws_bytes, "sample_workspace", logits.device) if ws_bytes else None
+        _lib.call("ody_sample", logits.data_ptr(), *pointers, *numbers[1:], tokens.data_ptr(), logprobs.data_ptr(), rows, vocab, logits.stride(0), dt,
+                  ws.data_ptr() if ws is not None else 0, ws_bytes, _stream())
     return tokens, logprobs
 
 

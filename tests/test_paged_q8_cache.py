@@ -88,14 +88,18 @@ def test_tokens_of_one_launch():
 def test_refusals_of_sampling():
     from odysseus_transformer_amd import _lib
 
-    def code(logits=Q, u=Q, tokens=Q, rows=1, vocab=10, stride=10, dtype=0):
+    def code(logits=Q, u=Q, tokens=Q, rows=1, vocab=10, stride=10, dtype=0, workspace=0, space=0):
         with pytest.raises(_lib.OdysseusHipError) as e:
-            _lib.call("ody_sample", logits, u, 0, 0, 0, 0, 1.0, 0, 1.0, 0.0, tokens, Q, rows, vocab, stride, dtype, 0)
+            _lib.call("ody_sample", logits, u, 0, 0, 0, 0, 1.0, 0, 1.0, 0.0, tokens, Q, rows, vocab, stride, dtype, workspace, space, 0)
         return e.value.code
     assert code(logits=0) == code(u=0) == code(tokens=0) == -4
     assert code(rows=0) == code(vocab=0) == code(vocab=2 ** 21 - 3) == code(rows=1 << 22) == code(rows=2, stride=9) == -1
     assert code(dtype=3) == -2
     assert code(logits=17) == code(logits=18, dtype=1) == -3
+    need = _lib.load().ody_sample_workspace_bytes(2, 100000, 1)
+    assert need > 0 and _lib.load().ody_sample_workspace_bytes(2, 1000, 1) == _lib.load().ody_sample_workspace_bytes(0, 100000, 1) == 0
+    for bad in (dict(), dict(workspace=4096, space=need - 1), dict(workspace=4096 + 128, space=need), dict(space=need)):
+        assert code(rows=2, vocab=100000, stride=100000, dtype=1, **bad) == -5, bad
 
 
 def test_m0_belongs_to_the_direct_loads(tmp_path):

@@ -304,3 +304,89 @@ def test_nothing_to_do_and_refusals(dev):
         ops.sample(x.clone().requires_grad_(), v)
     with pytest.raises(_lib.OdysseusHipError, match="rows of"):
         ops.sample(torch.empty((1, 2 ** 21), dtype=BF16, device=dev), v[:1])
+
+
+# ------------------------------------------------------------------------------------------------ few long rows, which are divided among blocks
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [65536, 70001, 131077])
+def test_long_rows_of_all_kinds(vocab, dtype, dev):
+    """Rows side by side that are divided differently: greedy, few of top_k, more, none; of -inf, with +inf, NaN, equals, what one slice alone has."""
+    rows = 30
+    logits, u = _logits(rows, vocab, dtype, seed=vocab)
+    g = torch.Generator().manual_seed(3)
+    pick = lambda *v: torch.tensor(v)[torch.randint(0, len(v), (rows,), generator=g)]  # noqa: E731
+    settings = dict(temperature=pick(0.0, 0.6, 1.0, 1.7), top_k=pick(0, 0, 1, 40, 2048, 2049, vocab - 1).to(torch.int32), top_p=pick(1.0, 0.5, 0.95), min_p=pick(0.0, 0.0, 0.02))
+    logits[1] = -math.inf
+    logits[2, ::vocab // 7] = math.inf
+    logits[3, ::3] = math.nan
+    logits[4] = 1.25
+    logits[5, vocab // 2:] = -math.inf
+    logits[6, :vocab - 5] = -math.inf
+    logits[7] = torch.round(logits[7])
+    logits[8] = 3.0
+    logits[8, vocab - 1] = 4.0
+    logits[9] *= 60.0
+    logits[10] *= 1e-3
+    logits[11, 100:] = -math.inf
+    logits[13], logits[14] = 0.0, -0.0
+    logits[14, ::5] = -1.0
+    logits[15] = -logits[15].abs() - 1.0
+    logits[16, ::2] *= 1e-9
+    logits[12, 1:] = -3e38 if dtype == F32 else -300.0
+    check(logits, u, dev, **settings)
+    for name in settings:
+        check(logits, u, dev, **{name: settings[name]})
+    check(logits, u, dev)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_long_rows_are_equal_in_any_batch(dtype, dev):
+    from odysseus_transformer_amd import ops
+    logits, u = _logits(300, 70003, dtype, seed=5)
+    logits, u = logits.to(dev), u.to(dev)
+    for settings in ({}, dict(top_p=0.9), dict(top_k=100, min_p=0.001), dict(temperature=0.0), dict(min_p=0.01, top_p=0.99)):
+        whole = ops.sample(logits, u, **settings)
+        for part in (slice(0, 1), slice(17, 40), slice(100, 220)):
+            some = ops.sample(logits[part], u[part], **settings)
+            assert torch.equal(some[0], whole[0][part]) and torch.equal(some[1], whole[1][part])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_long_rows_that_are_not_aligned(dtype, dev):
+    logits, u = _logits(5, 66667, dtype, seed=9)
+    for shift in (1, 2, 3, 5):
+        wide = torch.full((5, 66667 + 8), math.inf, dtype=dtype)
+        wide[:, shift:shift + 66667] = logits
+        on = wide.to(dev)[:, shift:shift + 66667]
+        check((on, logits), u, dev, top_p=0.9)
+        check((on, logits), u, dev, top_k=30)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_long_rows_replayed_and_on_two_streams(dtype, dev):
+    from odysseus_transformer_amd import ops
+    sets = [tuple(t.to(dev) for t in _logits(4, 80001, dtype, seed=i)) for i in range(2)]
+    calls = [dict(top_p=0.9), dict(top_k=20), dict()]
+    want = [[ops.sample(*s, **c) for c in calls] for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for _ in range(4):
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append([ops.sample(*s, **c) for c in calls])
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        for (a, b), (c, d) in zip(results, want[i % 2]):
+            assert torch.equal(a, c) and torch.equal(b, d)
+    x, v = (t.clone() for t in sets[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [ops.sample(x, v, **c) for c in calls]
+    for turn in range(4):
+        x.copy_(sets[turn % 2][0])
+        v.copy_(sets[turn % 2][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = [ops.sample(x, v, **c) for c in calls]
+        for (a, b), (c, d), (e, f) in zip(captured, want[turn % 2], eager):
+            assert torch.equal(a, c) and torch.equal(b, d) and torch.equal(e, c) and torch.equal(f, d)
