@@ -10,7 +10,7 @@
 //
 // A turn has one form, for whole tiles and others: with a second one the compiler runs out of registers, and one with reloads from memory takes seven times as long.
 //
-// Bound by the wavefront's instructions, 440 besides 64 products a turn; the matrix cores are busy for 45 % of it.  512 tokens behind 8191 keys, 32 heads on 8: 93.7 us, of which the
+// Bound by the wavefront's instructions, 440 besides 64 products a turn; the matrix cores are busy for 45 % of it, 36 % of the kernel.  512 tokens behind 8191 keys, 32 heads on 8: 93.7 us, of which the
 // join takes 10 (760 TFLOP/s; tiles of 128 106 us, the cache in 16 bits 87); behind 32768 290 us (960 TFLOP/s; 337 and 258).
 #include <cmath>
 #include "attn_rowtile.h"

@@ -22,6 +22,10 @@
 // reading: 256 of 128000, 37.4 us, of which counting takes 11 (8 atomics a vector, 5.5 of their lanes a cycle and compute unit, as they meet in banks; the bytes take 12.9 at a copy's rate) and the
 // second pass 9.  fp32 by the instructions of the weights, 30 for each: 64 rows of 32001, a third of them without top_k, 25.3 us, of which weights take 7.5.
 // 512 threads: 1024 were 5 us faster for the 256 rows and slower for all others.
+//
+// Few long rows would leave most compute units idle: they go in slices, a block each, with what the slices have to know of one another between launches (sums are of whole numbers, so a row's result
+// is the same to the bit).  bf16 in two: counts; then every block adds up the slices' counts, finds the value and whose slice has its token.  fp32 in four: the largest; sums by buckets; what is in the
+// buckets that matter, into a list; the token.  Tried: the list's last writer going on by itself, for the fourth launch; the fences that this takes write back and empty whole caches (64 rows of 128000 83 us, 43 so).
 #include <algorithm>
 #include <cmath>
 #include "ody_common.h"

@@ -390,3 +390,15 @@ def test_long_rows_replayed_and_on_two_streams(dtype, dev):
         eager = [ops.sample(x, v, **c) for c in calls]
         for (a, b), (c, d), (e, f) in zip(captured, want[turn % 2], eager):
             assert torch.equal(a, c) and torch.equal(b, d) and torch.equal(e, c) and torch.equal(f, d)
+
+
+def test_long_rows_by_both_host_paths(dev, monkeypatch):
+    from odysseus_transformer_amd import _native, ops
+    for dtype in (BF16, F32):
+        logits, u = (t.to(dev) for t in _logits(3, 90001, dtype, seed=4))
+        plain = [ops.sample(logits, u, **c) for c in (dict(top_p=0.9), dict(top_k=30))]
+        with monkeypatch.context() as m:
+            m.setattr(ops, "native", _native._Nothing())
+            for c, (a, b) in zip((dict(top_p=0.9), dict(top_k=30)), plain):
+                x, y = ops.sample(logits, u, **c)
+                assert torch.equal(a, x) and torch.equal(b, y)
