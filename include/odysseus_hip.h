@@ -430,7 +430,7 @@ int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, cons
 
 /* ---- a cache in pages that holds its values in 8 bits -----------------------
  * As above, with pages of e4m3 values (1 byte; no infinities, 448 the largest) and a power of two for each block of tokens and head: the value at a place is
- * its e4m3 value times 2^(byte - 127).
+ * its e4m3 value times 2^(byte - 127), bytes from 1 to 254.
  * k_scales, v_scales  (pages, page_size / block, Hkv) bytes, strides s*z_p (page), s*z_b (block of a page), s*z_h (head).  block: a power of two from 8 to 64,
  *                     at most page_size.
  * ody_paged_append_q8 as ody_paged_append.  2^e of a block and head: the least with e >= -126 and max |x| <= 448 * 2^e over the finite values of its tokens there; with

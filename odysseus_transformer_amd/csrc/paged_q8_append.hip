@@ -249,8 +249,12 @@ __global__ __launch_bounds__(256) void paged_read_q8_kernel(T* k, T* v, const Pa
       q8_values(kw[0], ks, a.x), q8_values(kw[1], ks, a.x + 4);
       q8_values(vw[0], vs, b.x), q8_values(vw[1], vs, b.x + 4);
     }
-    reinterpret_cast<Eight<T>*>(k)[s * per_sequence + at] = a;
-    reinterpret_cast<Eight<T>*>(v)[s * per_sequence + at] = b;
+    constexpr int PIECES = sizeof(a) / 16;
+#pragma unroll
+    for (int e = 0; e < PIECES; e++) {
+      __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(&a)[e], reinterpret_cast<u32x4*>(k) + (s * per_sequence + at) * PIECES + e);
+      __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(&b)[e], reinterpret_cast<u32x4*>(v) + (s * per_sequence + at) * PIECES + e);
+    }
   }
 }
 
