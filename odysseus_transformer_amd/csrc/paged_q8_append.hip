@@ -15,6 +15,11 @@ struct AppendParams {
   int blocks;           // of a sequence that n tokens may reach
 };
 
+template <bool PAST, typename V> __device__ __forceinline__ V load(const void* from) {   // 16 bytes; PAST the caches
+  typedef unsigned raw __attribute__((ext_vector_type(4)));
+  if constexpr (PAST) return __builtin_bit_cast(V, __builtin_nontemporal_load(static_cast<const raw*>(from)));
+  else return *static_cast<const V*>(from);
+}
 template <typename T> __device__ __forceinline__ float rounded(float x) { return (float)(T)x; }
 
 // x1 c - x2 s and x2 c + x1 s, rounded once to 32 bits: the products of bf16 are exact there, those of fp32 in 64.
@@ -53,9 +58,9 @@ __device__ __forceinline__ unsigned rescaled(unsigned word, int down) {   // tim
 // holds earlier tokens and the scale rises, their rows are rounded to the new one (by powers of two: only values that fall below 2^-6 of the scale change).
 // ONE token a sequence: ROWS heads in a wavefront at once, each LANES lanes with a scale of their own.
 //
-// Bound by memory: four prompts of 2500 to 4096 tokens, 32 heads on 32 of 128, 157 us for 580 MB, 3.7 TB/s (a copy 5.1; with one row of queries a thread under way 167).  Angles, which each share of the heads
+// Bound by memory: four prompts of 2500 to 4096 tokens, 32 heads on 32 of 128, 137 us for 580 MB, 4.2 TB/s (a copy 5.1; with one row of queries a thread under way 10 more).  Angles, which each share of the heads
 // evaluates for itself, do not show (a shorter evaluation left the time as it was).  Few tokens by latencies: 64 single ones, 32 heads on 8, 4.6 us.
-template <typename T, int D, int BLOCK, bool ROTATE, bool ONE>
+template <typename T, int D, int BLOCK, bool ROTATE, bool ONE, bool PAST>
 __global__ __launch_bounds__(256) void paged_append_q8_kernel(const AppendParams p, const PagedCache cache, const PagedScales z) {
   constexpr int N = Vec16B<T>::N, HALF = D / 2, LANES = HALF / N, ROWS = 64 / LANES, TURNS = ONE ? 1 : (BLOCK + ROWS - 1) / ROWS;
   constexpr int TOKENS = ONE ? 1 : BLOCK;
@@ -114,7 +119,7 @@ __global__ __launch_bounds__(256) void paged_append_q8_kernel(const AppendParams
       a[k] = b[k] = vec{};
       if (mine && t >= real && t < tokens) {
         const T* src = x + t * p.sx.l + (p.Hq + unit) * p.sx.h;
-        a[k] = *reinterpret_cast<const vec*>(src), b[k] = *reinterpret_cast<const vec*>(src + HALF);
+        a[k] = load<PAST, vec>(src), b[k] = load<PAST, vec>(src + HALF);
       }
     }
 #pragma unroll
@@ -176,7 +181,7 @@ __global__ __launch_bounds__(256) void paged_append_q8_kernel(const AppendParams
       a[k] = b[k] = vec{};
       if (r < rows && t[k] >= real) {
         const T* src = x + t[k] * p.sx.l + h[k] * p.sx.h;
-        a[k] = *reinterpret_cast<const vec*>(src), b[k] = *reinterpret_cast<const vec*>(src + HALF);
+        a[k] = load<PAST, vec>(src), b[k] = load<PAST, vec>(src + HALF);
       }
     }
 #pragma unroll
@@ -206,13 +211,19 @@ int launch(const AppendParams& p, const PagedCache& c, const PagedScales& z, hip
   const int64_t turns = (p.q ? (tokens * p.Hq + ROWS - 1) / ROWS : 0) + (p.n == 1 ? (2 * p.Hkv + ROWS - 1) / ROWS : 2 * p.Hkv);
   const unsigned shares = (unsigned)std::max((int64_t)1, std::min({(turns + 3) / 4, (2048 + groups - 1) / groups, (int64_t)65535}));
   const dim3 grid((unsigned)groups, shares);
-#define LAUNCH(R, O) ODY_LAUNCH("paged_append_q8", st, (paged_append_q8_kernel<T, D, BLOCK, R, O>), grid, dim3(256), 0, p, c, z)
+  // A projection that the last-level cache (256 MB) does not hold along with what else a layer touches is read past the caches, which keep the new rows for who reads them next; a smaller
+  // one lies there (four prompts of 4096 and reading back, 403 MB, 208 -> 193 us; 1324 tokens of 8 MB 11.6 -> 12.7).
+  const bool past = (double)p.S * p.n * (p.Hq + 2 * p.Hkv) * D * sizeof(T) >= 128e6;
+#define LAUNCH(R, O, P) ODY_LAUNCH("paged_append_q8", st, (paged_append_q8_kernel<T, D, BLOCK, R, O, P>), grid, dim3(256), 0, p, c, z)
   if (p.n == 1) {
-    if (p.q) LAUNCH(true, true);
-    else LAUNCH(false, true);
+    if (p.q) LAUNCH(true, true, false);
+    else LAUNCH(false, true, false);
+  } else if (past) {
+    if (p.q) LAUNCH(true, false, true);
+    else LAUNCH(false, false, true);
   } else {
-    if (p.q) LAUNCH(true, false);
-    else LAUNCH(false, false);
+    if (p.q) LAUNCH(true, false, false);
+    else LAUNCH(false, false, false);
   }
 #undef LAUNCH
   return ody_check_launch("paged_append_q8");
@@ -228,7 +239,7 @@ int by_block(const AppendParams& p, const PagedCache& c, const PagedScales& z, h
 }
 
 // ---- what the cache holds: a thread takes eight values of keys and of values; consecutive threads the columns of a head, heads, places.  Memory is all of it: 16 sequences of up to
-// 4001 tokens, 16 heads of 64, 62 us for 335 MB, 5.4 TB/s (a copy of such sizes 5.1 to 5.4); one of 8191, 8 heads of 128, 9.7 us, 50 MB out of and into the last-level cache
+// 4001 tokens, 16 heads of 64, 45 us for 335 MB, 7.4 TB/s, of which 262 written past the caches (62 through them); one of 8191, 8 heads of 128, 9.8 us, 50 MB
 template <typename T> struct Eight { T x[8]; };
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_read_q8_kernel(T* k, T* v, const PagedCache cache, const PagedScales z, int places, int Hkv, int S) {

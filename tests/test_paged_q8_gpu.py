@@ -170,6 +170,30 @@ def test_queries_are_those_of_the_other_cache(dev):
         assert (a == b).double().mean() > (0.99 if dtype == BF16 else 0.5)
 
 
+@pytest.mark.parametrize("dtype,n", [(BF16, 2801), (F32, 1403)], ids=["bf16", "f32"])
+def test_large_projections_are_appended_as_small_ones(dtype, n, dev):
+    """A projection of more than 128 MB is read in another way: the same bytes as sequence by sequence."""
+    from odysseus_transformer_amd import ops
+    S, Hq, Hkv, D, page, block = 4, 32, 8, 128, 64, 32
+    assert S * n * (Hq + 2 * Hkv) * D * (2 if dtype == BF16 else 4) >= 128e6
+    lengths = torch.tensor([n, n + 45, 700, n + 7], dtype=torch.int32, device=dev)
+    columns = (n + 45 + page - 1) // page
+    table = torch.randperm(S * columns, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(S, columns).to(dev)
+    qkv = torch.randn((S, n, Hq + 2 * Hkv, D), generator=torch.Generator(device=dev).manual_seed(2), device=dev).to(dtype)
+
+    def caches():
+        return tuple(torch.zeros((S * columns, page, Hkv, D), dtype=torch.uint8, device=dev).view(F8) for _ in range(2)) + \
+            tuple(torch.full((S * columns, page // block, Hkv), 120, dtype=torch.uint8, device=dev).view(E8) for _ in range(2))
+    for rotate in (True, False):
+        a, b = caches(), caches()
+        q = ops.paged_append_q8_(qkv, Hq, *a, table, lengths, rotate=rotate)
+        for s in range(S):
+            one = ops.paged_append_q8_(qkv[s:s + 1], Hq, *b, table[s:s + 1], lengths[s:s + 1], rotate=rotate)
+            assert torch.equal(one[0], q[s])
+        for x, y in zip(a, b):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
 def test_cosines_are_rounded_to_32_bits_first(dev):
     """Queries of 1 and 0 are the cosines and sines: those of 32 bits, rounded once more to the type.  (Among 2^19 of them a few lie in the middle of two bf16 values then.)"""
     from odysseus_transformer_amd import ops
