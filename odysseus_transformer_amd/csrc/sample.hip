@@ -21,7 +21,6 @@
 // Bound by latencies for few rows, a chain of some thirty barriers and LDS reads behind a load: one of 32000 in bf16 13.0 us, of which counting takes 1.8.  For many by LDS atomics and the second
 // reading: 256 of 128000, 37.4 us, of which counting takes 11 (8 atomics a vector, 5.5 of their lanes a cycle and compute unit, as they meet in banks; the bytes take 12.9 at a copy's rate) and the
 // second pass 9.  fp32 by the instructions of the weights, 30 for each: 64 rows of 32001, a third of them without top_k, 25.3 us, of which weights take 7.5.
-// 512 threads: 1024 were 5 us faster for the 256 rows and slower for all others.
 //
 // Few long rows would leave most compute units idle: they go in slices, a block each, with what the slices have to know of one another between launches (sums are of whole numbers, so a row's result
 // is the same to the bit).  bf16 in two: counts; then every block adds up the slices' counts, finds the value and whose slice has its token.  fp32 in four: the largest; sums by buckets; what is in the
@@ -36,7 +35,10 @@ typedef unsigned long long u64;
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef const u32x4 __attribute__((address_space(1)))* vector_ptr;
 
-constexpr int THREADS = 512, WAVES = THREADS / 64, BUCKETS = 2048, LIST = 4096, OCTAVE = 1024, VALUES = 8192;
+constexpr int BUCKETS = 2048, LIST = 4096, OCTAVE = 1024, VALUES = 8192;
+// Threads of a block.  fp32 rows are read and weighed by all that a compute unit has (256 rows of 128000 78 us, 84 by 512; 64 of 32001 23.4 and 25.6).  bf16 by 512, in whose registers short rows stay (512 rows of
+// 32000 30 us, 45 by 1024; 256 of 128000 37.5 and 35.4).
+template <typename T> constexpr int THREADS_OF = sizeof(T) == 4 ? 1024 : 512;
 constexpr int MOST = (1 << 21) - 4;   // tokens of a row: nth_of() counts the matches in each 64 vectors, of 4 values or 8, in 2 * LIST numbers
 
 // What finding the token among listed ones takes: top_p's weights, those before its bucket, before the random number's; of the list those before top_p's bucket
@@ -79,7 +81,7 @@ __device__ __forceinline__ float of_key(unsigned k) { return __builtin_bit_cast(
 // A row, in vectors of 16 bytes that hold at least one value of it.  What is not the row's counts as -inf, which has no weight and so is never a result.
 template <typename T, int NV = 0>
 struct Row {
-  static constexpr int N = 16 / (int)sizeof(T), AHEAD = 4;   // values of a vector; vectors under way, where they are read for each pass
+  static constexpr int THREADS = THREADS_OF<T>, N = 16 / (int)sizeof(T), AHEAD = 4;   // values of a vector; vectors under way, where they are read for each pass
   static constexpr unsigned LOWEST = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
   const T* base;      // 16-byte aligned, at most N - 1 values before the row
   int head, vocab, vectors;
@@ -320,15 +322,16 @@ struct Shared {
   unsigned count[VALUES], finer_count[BUCKETS];
   u64 list[LIST], ordered[LIST];
   unsigned rank[256];
-  u64 wave[WAVES];
-  float wave_max[WAVES];
+  u64 wave[16];
+  float wave_max[16];
   u64 found[3], small[2];
   unsigned words[4], small_tokens;
 };
-static_assert(WAVES <= 16, "a row of 16 lanes sums up the wavefronts");
 
 // Exclusive sum over the block; `all`: of all threads.
-__device__ __forceinline__ u64 block_scan(Shared& s, u64 x, u64& all) {
+template <typename T> __device__ __forceinline__ u64 block_scan(Shared& s, u64 x, u64& all) {
+  constexpr int WAVES = THREADS_OF<T> / 64;
+  static_assert(WAVES <= 16, "a row of 16 lanes sums up the wavefronts");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const u64 upto = wave_scan(x);
   __syncthreads();   // a sum before this one has been read
@@ -342,6 +345,7 @@ __device__ __forceinline__ u64 block_scan(Shared& s, u64 x, u64& all) {
 
 template <typename T, int NV = 0>
 struct Sampler {
+  static constexpr int THREADS = THREADS_OF<T>, WAVES = THREADS / 64;
   Shared& s;
   Row<T, NV>& row;
   Weights w;
@@ -430,7 +434,7 @@ struct Sampler {
       if (i < n) sum += w.of(of_key(~(unsigned)(s.ordered[i] >> 32)));
       mine[k] = sum;
     }
-    const u64 before = mass + block_scan(s, sum, all);
+    const u64 before = mass + block_scan<T>(s, sum, all);
 #pragma unroll
     for (int k = 0; k < PER; k++) upto[k] = before + mine[k], was[k] = k ? upto[k - 1] : before;
     return mass + all;
@@ -482,7 +486,7 @@ struct Sampler {
       weights[k] = masses ? masses[b] : 0, numbers[k] = counts[b];
       sum += weights[k], tokens += numbers[k];
     }
-    const u64 m = masses ? mass + block_scan(s, sum, all) : 0, c = count + block_scan(s, tokens, all);
+    const u64 m = masses ? mass + block_scan<T>(s, sum, all) : 0, c = count + block_scan<T>(s, tokens, all);
     if (by_count && count + all < target) return BUCKETS;   // fewer than that are counted
     return slot_of<EACH>(by_count, target, threadIdx.x * EACH, c, m, numbers, weights, count, mass);
   }
@@ -542,7 +546,7 @@ struct Sampler {
       u64 over = 0, heavy;
 #pragma unroll
       for (int j = 0; j < PER; j++) over += upto[j] - was[j] >= set.least && (int)threadIdx.x * PER + j < k ? upto[j] - was[j] : 0;
-      block_scan(s, over, heavy);
+      block_scan<T>(s, over, heavy);
       kept = min(kept, max(set.one, heavy));   // the first one at any rate
     }
     __syncthreads();
@@ -783,7 +787,7 @@ template <typename R> __device__ __forceinline__ float largest_of(const R& row, 
   if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = x;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < WAVES; k++) x = fmaxf(x, wave_max[k]);
+  for (int k = 0; k < R::THREADS / 64; k++) x = fmaxf(x, wave_max[k]);
   return x;
 }
 // The largest logit is +inf: those are equals with all of the weight.
@@ -798,8 +802,8 @@ template <typename S> __device__ __forceinline__ void sample_infinite(const Samp
   if (threadIdx.x == 0) p.tokens[r] = (int64_t)(unsigned)entry, p.logprobs[r] = (float)-log((double)(kept >> set.frac));
 }
 // 2^(-j / OCTAVE), by the series of exp around the middle: twelve terms of |x| < 0.35 leave 2^-51.  (Out of memory the table would be the first thing that a block waits for.)
-__device__ __forceinline__ void fill_table(Shared& s) {
-  for (int j = threadIdx.x; j < OCTAVE; j += THREADS) {
+template <typename T> __device__ __forceinline__ void fill_table(Shared& s) {
+  for (int j = threadIdx.x; j < OCTAVE; j += THREADS_OF<T>) {
     const double x = (OCTAVE / 2 - j) * (0.6931471805599453 / OCTAVE);
     double y = 1.0;
 #pragma unroll
@@ -812,7 +816,7 @@ __device__ __forceinline__ void fill_table(Shared& s) {
 __device__ __forceinline__ unsigned base_of(int most) { return (unsigned)max(128, (most + 127) * 128 - VALUES / 2); }
 constexpr int USUAL = 7;   // logits below 128: the largest need not be known to count them
 
-constexpr int VALUES_EACH = VALUES / THREADS;   // values of a thread, of one exponent
+constexpr int VALUES_EACH = VALUES / THREADS_OF<bf16>;   // values of a thread, of one exponent
 static_assert(128 % VALUES_EACH == 0 && VALUES_EACH == 16, "values of one exponent; lanes of a row sum");
 
 // Tokens nearer to 0 than the window keep weights of their own: their sums to s.small.
@@ -860,11 +864,11 @@ __device__ __forceinline__ bool choose_value(const Settings& set, Shared& s, S& 
   }
   // tokens next to 0 are behind the last positive value's
   const bool next_to_0 = small && v0 == VALUES / 2 - EACH;
-  m = block_scan(s, mass_here + (next_to_0 ? s.small[0] : 0), kept);
-  if (set.cut_k) c = block_scan(s, tokens_here + (next_to_0 ? s.small_tokens : 0), all);
+  m = block_scan<bf16>(s, mass_here + (next_to_0 ? s.small[0] : 0), kept);
+  if (set.cut_k) c = block_scan<bf16>(s, tokens_here + (next_to_0 ? s.small_tokens : 0), all);
   if (set.cut_m) {
     u64 heavy;
-    block_scan(s, over, heavy);
+    block_scan<bf16>(s, over, heavy);
     over = max(set.one, heavy + s.small[1]);   // the first one at any rate
   }
   // ---- the cuts, then the token
@@ -922,7 +926,7 @@ __device__ __forceinline__ void sample_values_row(const SampleParams& p, int r, 
   constexpr int EACH = VALUES_EACH;
   const int tid = threadIdx.x;
   Row<bf16, NV> row(static_cast<const bf16*>(p.logits) + r * p.row_stride, p.vocab);
-  fill_table(s);
+  fill_table<bf16>(s);
   Sampler<bf16, NV> a{s, row, set.weights(0.f, s.table)};
 
   // ---- tokens by value, in a window that may have to be another one once the largest value is known
@@ -931,7 +935,7 @@ __device__ __forceinline__ void sample_values_row(const SampleParams& p, int r, 
   int most = USUAL;
   for (bool again = false;; again = true) {
     base = base_of(most);
-    for (int b = tid; b < VALUES / 4; b += THREADS) reinterpret_cast<u32x4*>(s.count)[b] = u32x4{0, 0, 0, 0};
+    for (int b = tid; b < VALUES / 4; b += THREADS_OF<bf16>) reinterpret_cast<u32x4*>(s.count)[b] = u32x4{0, 0, 0, 0};
     if (tid == 0) s.words[0] = ~0u, s.words[1] = 0, s.small[0] = s.small[1] = 0, s.small_tokens = 0;
     __syncthreads();
     unsigned least;
@@ -988,7 +992,7 @@ __device__ __forceinline__ void sample_values_row(const SampleParams& p, int r, 
 }
 
 template <int NV>
-__global__ __launch_bounds__(THREADS) void sample_values_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS_OF<bf16>) void sample_values_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   sample_values_row<NV>(p, blockIdx.x, Settings(p, blockIdx.x), *reinterpret_cast<Shared*>(smem));
 }
@@ -998,8 +1002,8 @@ __global__ __launch_bounds__(THREADS) void sample_values_kernel(const SamplePara
 __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const Settings& set, Shared& s) {
   const int tid = threadIdx.x;
   Row<float> row(static_cast<const float*>(p.logits) + r * p.row_stride, p.vocab);
-  fill_table(s);
-  for (int b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0, s.count[b] = 0;
+  fill_table<float>(s);
+  for (int b = tid; b < BUCKETS; b += THREADS_OF<float>) s.mass[b] = 0, s.count[b] = 0;
   const float largest = largest_of(row, s.wave_max);
   Sampler<float> a{s, row, set.weights(largest, s.table)};
   if (largest == -INFINITY || !(set.temperature > 0.f)) {   // nothing to choose from, or nothing but the first
@@ -1022,7 +1026,7 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
       entry = a.among_first(n, set, kept);
     } else {
       __syncthreads();
-      for (int b = tid; b < BUCKETS; b += THREADS) s.count[b] = 0;
+      for (int b = tid; b < BUCKETS; b += THREADS_OF<float>) s.count[b] = 0;
       __syncthreads();
     }
   }
@@ -1040,7 +1044,7 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
       if (last) atomicAdd(&s.count[BUCKETS - 1], last);
     }
     __syncthreads();
-    constexpr int EACH = BUCKETS / THREADS;
+    constexpr int EACH = BUCKETS / THREADS_OF<float>;
     unsigned tokens[EACH];
     u64 weights[EACH], mass_here = 0, tokens_here = 0, m, c = 0, all = 0, heavy;
 #pragma unroll
@@ -1048,10 +1052,10 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
       weights[k] = s.mass[tid * EACH + k], tokens[k] = s.count[tid * EACH + k];
       mass_here += weights[k], tokens_here += tokens[k];
     }
-    m = block_scan(s, mass_here, kept);
-    if (set.cut_k) c = block_scan(s, tokens_here, all);
+    m = block_scan<float>(s, mass_here, kept);
+    if (set.cut_k) c = block_scan<float>(s, tokens_here, all);
     if (set.cut_m) {
-      block_scan(s, over, heavy);
+      block_scan<float>(s, over, heavy);
       over = max(set.one, heavy);   // the first one at any rate
     }
     if (!set.cut_k) {
@@ -1077,7 +1081,7 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
   write(p, r, a.w, entry, kept);
 }
 
-__global__ __launch_bounds__(THREADS) void sample_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS_OF<float>) void sample_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   sample_row(p, blockIdx.x, Settings(p, blockIdx.x), *reinterpret_cast<Shared*>(smem));
 }
@@ -1109,12 +1113,12 @@ template <int N, typename V> __device__ __forceinline__ void add_slices(V (&sum)
   }
 }
 // bf16: the slices' tokens by value,
-__global__ __launch_bounds__(THREADS) void sample_counts_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS_OF<bf16>) void sample_counts_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
   Row<bf16> row = slice_of<bf16>(p, r, j);
-  for (int b = tid; b < VALUES / 4; b += THREADS) reinterpret_cast<u32x4*>(s.count)[b] = u32x4{0, 0, 0, 0};
+  for (int b = tid; b < VALUES / 4; b += THREADS_OF<bf16>) reinterpret_cast<u32x4*>(s.count)[b] = u32x4{0, 0, 0, 0};
   if (tid == 0) s.words[0] = ~0u, s.words[1] = 0;
   __syncthreads();
   unsigned least;
@@ -1127,12 +1131,12 @@ __global__ __launch_bounds__(THREADS) void sample_counts_kernel(const SamplePara
     if (greatest >= 0) atomicMax(&s.words[1], (unsigned)greatest + 1);
   }
   __syncthreads();
-  for (int b = tid; b < VALUES / 4; b += THREADS) reinterpret_cast<u32x4*>(p.counts + (int64_t)blockIdx.x * VALUES)[b] = reinterpret_cast<u32x4*>(s.count)[b];
+  for (int b = tid; b < VALUES / 4; b += THREADS_OF<bf16>) reinterpret_cast<u32x4*>(p.counts + (int64_t)blockIdx.x * VALUES)[b] = reinterpret_cast<u32x4*>(s.count)[b];
   if (tid == 0) p.ends[blockIdx.x] = make_int2((int)s.words[0], (int)s.words[1]);
 }
 // and the token: every block finds its value and the slice that has it, which looks for it.  Rows for which that will not do -- the largest is not a positive one below 128, or the token is
 // one next to 0 -- one block, all of it.
-__global__ __launch_bounds__(THREADS) void sample_counted_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS_OF<bf16>) void sample_counted_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
@@ -1158,7 +1162,7 @@ __global__ __launch_bounds__(THREADS) void sample_counted_kernel(const SamplePar
   u64 entry = 0, kept = 0;
   if (!greedy && !whole) {
     bool listed;
-    fill_table(s);
+    fill_table<bf16>(s);
 #pragma unroll
     for (int q = 0; q < VALUES_EACH / 4; q++) reinterpret_cast<u32x4*>(s.count)[tid * (VALUES_EACH / 4) + q] = fours[q];
     if (tid == 0) s.small[0] = s.small[1] = 0, s.small_tokens = 0;
@@ -1184,8 +1188,8 @@ __global__ __launch_bounds__(THREADS) void sample_counted_kernel(const SamplePar
   else write(p, r, a.w, entry, kept);
 }
 // fp32: the slices' largest,
-__global__ __launch_bounds__(THREADS) void sample_largest_kernel(const SampleParams p) {
-  __shared__ float wave_max[WAVES];
+__global__ __launch_bounds__(THREADS_OF<float>) void sample_largest_kernel(const SampleParams p) {
+  __shared__ float wave_max[THREADS_OF<float> / 64];
   const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices;
   const Row<float> row = slice_of<float>(p, r, j);
   const float x = largest_of(row, wave_max);
@@ -1196,7 +1200,7 @@ __global__ __launch_bounds__(THREADS) void sample_largest_kernel(const SamplePar
 __device__ __forceinline__ bool in_slices(const Settings& set, float largest) {
   return set.temperature > 0.f && fabsf(largest) < INFINITY && (set.few() || !set.cut_k);
 }
-__global__ __launch_bounds__(THREADS) void sample_buckets_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS_OF<float>) void sample_buckets_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
@@ -1206,22 +1210,22 @@ __global__ __launch_bounds__(THREADS) void sample_buckets_kernel(const SamplePar
   const bool few = set.few();
   Row<float> row = slice_of<float>(p, r, j);
   Sampler<float> a{s, row, set.weights(largest, s.table)};
-  if (!few) fill_table(s);
-  for (int b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0, s.count[b] = 0;
+  if (!few) fill_table<float>(s);
+  for (int b = tid; b < BUCKETS; b += THREADS_OF<float>) s.mass[b] = 0, s.count[b] = 0;
   __syncthreads();
   if (few) {
     a.count_buckets();
     __syncthreads();
-    for (int b = tid; b < BUCKETS / 4; b += THREADS) reinterpret_cast<u32x4*>(p.mass + (int64_t)blockIdx.x * BUCKETS)[b] = reinterpret_cast<u32x4*>(s.count)[b];
+    for (int b = tid; b < BUCKETS / 4; b += THREADS_OF<float>) reinterpret_cast<u32x4*>(p.mass + (int64_t)blockIdx.x * BUCKETS)[b] = reinterpret_cast<u32x4*>(s.count)[b];
   } else {
     u64 over = a.add_weights(set.cut_m, set.least), heavy;
-    block_scan(s, over, heavy);
+    block_scan<float>(s, over, heavy);
     if (tid == 0) p.over[blockIdx.x] = heavy;
-    for (int b = tid; b < BUCKETS / 2; b += THREADS) reinterpret_cast<u32x4*>(p.mass + (int64_t)blockIdx.x * BUCKETS)[b] = reinterpret_cast<u32x4*>(s.mass)[b];
+    for (int b = tid; b < BUCKETS / 2; b += THREADS_OF<float>) reinterpret_cast<u32x4*>(p.mass + (int64_t)blockIdx.x * BUCKETS)[b] = reinterpret_cast<u32x4*>(s.mass)[b];
   }
 }
 // what each has in the buckets that matter, which every block finds for itself,
-__global__ __launch_bounds__(THREADS) void sample_slices_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS_OF<float>) void sample_slices_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   const int r = blockIdx.x / p.slices, j = blockIdx.x - r * p.slices, tid = threadIdx.x;
@@ -1241,20 +1245,21 @@ __global__ __launch_bounds__(THREADS) void sample_slices_kernel(const SamplePara
   const u64* mass = p.mass + (int64_t)r * p.slices * BUCKETS;
   int n;
   if (set.few()) {
-    u32x4 sum[1] = {};
-    add_slices(sum, reinterpret_cast<const u32x4*>(mass) + tid, BUCKETS / 2, p.slices);
-    reinterpret_cast<u32x4*>(s.count)[tid] = sum[0];
+    typedef unsigned part __attribute__((ext_vector_type(BUCKETS / THREADS_OF<float>)));
+    part sum[1] = {};
+    add_slices(sum, reinterpret_cast<const part*>(mass) + tid, BUCKETS * (int)(sizeof(u64) / sizeof(part)), p.slices);
+    reinterpret_cast<part*>(s.count)[tid] = sum[0];
     __syncthreads();
     n = a.gather_first(set.top_k);
   } else {
-    constexpr int EACH = BUCKETS / THREADS;
+    constexpr int EACH = BUCKETS / THREADS_OF<float>;
     u64 weights[EACH] = {}, here = 0;
     add_slices(weights, mass + tid * EACH, BUCKETS, p.slices);
 #pragma unroll
     for (int i = 0; i < EACH; i++) s.mass[tid * EACH + i] = weights[i], here += weights[i];
-    const u64 m = block_scan(s, here, e.kept);
+    const u64 m = block_scan<float>(s, here, e.kept);
     if (set.cut_m) {
-      block_scan(s, tid < p.slices ? p.over[r * p.slices + tid] : 0, e.most);
+      block_scan<float>(s, tid < p.slices ? p.over[r * p.slices + tid] : 0, e.most);
       e.most = max(set.one, e.most);   // the first one at any rate
     }
     n = a.gather_ends(set, m, weights, e.kept, e.most, e.q);
@@ -1264,10 +1269,10 @@ __global__ __launch_bounds__(THREADS) void sample_slices_kernel(const SamplePara
   __syncthreads();
   const unsigned to = s.words[2];
   if (n <= LIST && to + n <= LIST)
-    for (int k = tid; k < n; k += THREADS) p.lists[(int64_t)r * LIST + to + k] = s.list[k] + (unsigned)(j * p.slice);
+    for (int k = tid; k < n; k += THREADS_OF<float>) p.lists[(int64_t)r * LIST + to + k] = s.list[k] + (unsigned)(j * p.slice);
 }
 // and the token among them.  A row for which that will not do: all of it.
-__global__ __launch_bounds__(THREADS) void sample_listed_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS_OF<float>) void sample_listed_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   const int r = blockIdx.x, tid = threadIdx.x;
@@ -1281,18 +1286,18 @@ __global__ __launch_bounds__(THREADS) void sample_listed_kernel(const SamplePara
   }
   Row<float> row(static_cast<const float*>(p.logits) + r * p.row_stride, p.vocab);
   Sampler<float> a{s, row, set.weights(largest, s.table)};
-  for (int k = tid; k < (int)n; k += THREADS) s.list[k] = p.lists[(int64_t)r * LIST + k];
+  for (int k = tid; k < (int)n; k += THREADS_OF<float>) s.list[k] = p.lists[(int64_t)r * LIST + k];
   const RowEnds e = p.ends_of_rows[r];
-  fill_table(s);
+  fill_table<float>(s);
   __syncthreads();
   u64 kept = e.kept;
   const u64 entry = set.few() ? a.among_first((int)n, set, kept) : a.among_ends((int)n, set, e.most, e.q, kept);
   write(p, r, a.w, entry, kept);
 }
 
-template <typename K> int launch(K kernel, const SampleParams& p, int blocks, hipStream_t st) {
+template <typename T, typename K> int launch(K kernel, const SampleParams& p, int blocks, hipStream_t st) {
   if (int rc = ody_allow_dynamic_lds(reinterpret_cast<const void*>(kernel), sizeof(Shared), "ody_sample")) return rc;
-  ODY_LAUNCH("sample", st, kernel, dim3((unsigned)blocks), dim3(THREADS), sizeof(Shared), p);
+  ODY_LAUNCH("sample", st, kernel, dim3((unsigned)blocks), dim3(THREADS_OF<T>), sizeof(Shared), p);
   return ody_check_launch("sample");
 }
 
@@ -1341,19 +1346,19 @@ extern "C" int ody_sample(const void* logits, const float* u, const float* tempe
                        std::min(50, 62 - bits), q.slices, q.slice, reinterpret_cast<u64*>(ws + q.mass), reinterpret_cast<u64*>(ws + q.over), reinterpret_cast<unsigned*>(ws), reinterpret_cast<int2*>(ws + q.ends),
                        reinterpret_cast<float*>(ws + q.largest), reinterpret_cast<unsigned*>(ws + q.listed), reinterpret_cast<RowEnds*>(ws + q.ends), reinterpret_cast<u64*>(ws)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == ODY_F32 && q.slices == 1) return launch(&sample_kernel, p, rows, st);
+  if (dtype == ODY_F32 && q.slices == 1) return launch<float>(&sample_kernel, p, rows, st);
   if (dtype == ODY_F32) {
-    ODY_LAUNCH("sample_largest", st, sample_largest_kernel, dim3((unsigned)(rows * q.slices)), dim3(THREADS), 0, p);
+    ODY_LAUNCH("sample_largest", st, sample_largest_kernel, dim3((unsigned)(rows * q.slices)), dim3(THREADS_OF<float>), 0, p);
     if (int rc = ody_check_launch("sample_largest")) return rc;
-    if (int rc = launch(&sample_buckets_kernel, p, rows * q.slices, st)) return rc;
-    if (int rc = launch(&sample_slices_kernel, p, rows * q.slices, st)) return rc;
-    return launch(&sample_listed_kernel, p, rows, st);
+    if (int rc = launch<float>(&sample_buckets_kernel, p, rows * q.slices, st)) return rc;
+    if (int rc = launch<float>(&sample_slices_kernel, p, rows * q.slices, st)) return rc;
+    return launch<float>(&sample_listed_kernel, p, rows, st);
   }
   if (q.slices > 1) {
-    if (int rc = launch(&sample_counts_kernel, p, rows * q.slices, st)) return rc;
-    return launch(&sample_counted_kernel, p, rows * q.slices, st);
+    if (int rc = launch<bf16>(&sample_counts_kernel, p, rows * q.slices, st)) return rc;
+    return launch<bf16>(&sample_counted_kernel, p, rows * q.slices, st);
   }
-  const int turns = (vocab + 14 + THREADS * 8 - 1) / (THREADS * 8);   // however rows are aligned
-  if (turns <= 8) return launch(&sample_values_kernel<8>, p, rows, st);   // longer rows are counted while they arrive (256 of 128000: 45 us, 51 out of registers)
-  return launch(&sample_values_kernel<0>, p, rows, st);
+  const int turns = (vocab + 14 + THREADS_OF<bf16> * 8 - 1) / (THREADS_OF<bf16> * 8);   // however rows are aligned
+  if (turns <= 8) return launch<bf16>(&sample_values_kernel<8>, p, rows, st);   // longer rows are counted while they arrive (256 of 128000: 45 us, 51 out of registers)
+  return launch<bf16>(&sample_values_kernel<0>, p, rows, st);
 }
