@@ -20,11 +20,11 @@
 //
 // Bound by latencies for few rows, a chain of some thirty barriers and LDS reads behind a load: one of 32000 in bf16 13.0 us, of which counting takes 1.8.  For many by LDS atomics and the second
 // reading: 256 of 128000, 37.4 us, of which counting takes 11 (8 atomics a vector, 5.5 of their lanes a cycle and compute unit, as they meet in banks; the bytes take 12.9 at a copy's rate) and the
-// second pass 9.  fp32 by the instructions of the weights, 30 for each: 64 rows of 32001, a third of them without top_k, 25.3 us, of which weights take 7.5.
+// second pass 9.  fp32 by the instructions of the weights, 30 for each: 64 rows of 32001, a third of them without top_k, 23.4 us, of which weights take some 6.
 //
 // Few long rows would leave most compute units idle: they go in slices, a block each, with what the slices have to know of one another between launches (sums are of whole numbers, so a row's result
 // is the same to the bit).  bf16 in two: counts; then every block adds up the slices' counts, finds the value and whose slice has its token.  fp32 in four: the largest; sums by buckets; what is in the
-// buckets that matter, into a list; the token.  Tried: the list's last writer going on by itself, for the fourth launch; the fences that this takes write back and empty whole caches (64 rows of 128000 83 us, 43 so).
+// buckets that matter, into a list; the token.  Tried: the list's last writer going on by itself, for the fourth launch; the fences that this takes write back and empty whole caches (64 rows of 128000 83 us, 41 so).
 #include <algorithm>
 #include <cmath>
 #include "ody_common.h"
@@ -1301,9 +1301,9 @@ template <typename T, typename K> int launch(K kernel, const SampleParams& p, in
   return ody_check_launch("sample");
 }
 
-// How rows are divided: long ones into slices, at most one a compute unit; of bf16 fewer, as each block reads the counts of all.  us by a block a row / in slices, top_p 0.9: fp32, one row of
-// 40000 24.7 / 22.4 (with top_k 20 16.1 / 19.3), of 70000 37.0 / 24.0 (22.6 / 19.5), of 250000 108 / 29 (61 / 21); 16 of 128000 64 / 34, 64 68 / 43, 128 73 / 63; bf16, one of 70000
-// 19.8 / 16.9, of 250000 42.9 / 19.5; 8 of 128000 30.0 / 19.9, 64 34.3 / 26.4, 128 35.4 / 28.9.
+// How rows are divided: long ones into slices, at most one a compute unit; of bf16 fewer, as each block reads the counts of all.  us by a block a row / in slices, top_p 0.9 (fp32 also with top_k 20): fp32,
+// one row of 70000 32.8 / 25.0 (19.1 / 20.2), of 250000 87.5 / 28.0 (47.3 / 21.1); 16 of 128000 52.6 / 32.8, 64 54.6 / 40.6, 128 61.6 / 59.8 (36.5 / 45.1); bf16, one of 70000 19.8 / 16.9, of 250000
+// 42.9 / 19.5; 8 of 128000 30.0 / 19.9, 64 34.3 / 26.4, 128 35.4 / 28.9.
 struct Plan {
   int slices, slice;
   size_t ends, mass, over, largest, listed, bytes;   // places in the workspace, behind the lists (fp32) or the counts (bf16)
@@ -1311,7 +1311,7 @@ struct Plan {
 Plan plan(int rows, int vocab, int dtype) {
   Plan q{};
   q.slices = std::min(dtype == ODY_F32 ? 16 : rows > 8 ? 4 : 8, 256 / rows);
-  if (q.slices < 2 || vocab < 65536) return Plan{1, vocab, 0, 0, 0, 0, 0, 0};
+  if (dtype == ODY_F32 ? q.slices < 4 || vocab < 98304 : q.slices < 2 || vocab < 65536) return Plan{1, vocab, 0, 0, 0, 0, 0, 0};
   q.slice = ((vocab + q.slices - 1) / q.slices + 7) / 8 * 8;
   q.slices = (vocab + q.slice - 1) / q.slice;
   const size_t all = (size_t)rows * q.slices;

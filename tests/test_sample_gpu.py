@@ -308,7 +308,7 @@ def test_nothing_to_do_and_refusals(dev):
 
 # ------------------------------------------------------------------------------------------------ few long rows, which are divided among blocks
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
-@pytest.mark.parametrize("vocab", [65536, 70001, 131077])
+@pytest.mark.parametrize("vocab", [65536, 98304, 131077])
 def test_long_rows_of_all_kinds(vocab, dtype, dev):
     """Rows side by side that are divided differently: greedy, few of top_k, more, none; of -inf, with +inf, NaN, equals, what one slice alone has."""
     rows = 30
@@ -342,7 +342,7 @@ def test_long_rows_of_all_kinds(vocab, dtype, dev):
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 def test_long_rows_are_equal_in_any_batch(dtype, dev):
     from odysseus_transformer_amd import ops
-    logits, u = _logits(300, 70003, dtype, seed=5)
+    logits, u = _logits(300, 100003, dtype, seed=5)
     logits, u = logits.to(dev), u.to(dev)
     for settings in ({}, dict(top_p=0.9), dict(top_k=100, min_p=0.001), dict(temperature=0.0), dict(min_p=0.01, top_p=0.99)):
         whole = ops.sample(logits, u, **settings)
@@ -353,11 +353,11 @@ def test_long_rows_are_equal_in_any_batch(dtype, dev):
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 def test_long_rows_that_are_not_aligned(dtype, dev):
-    logits, u = _logits(5, 66667, dtype, seed=9)
+    logits, u = _logits(5, 98333, dtype, seed=9)
     for shift in (1, 2, 3, 5):
-        wide = torch.full((5, 66667 + 8), math.inf, dtype=dtype)
-        wide[:, shift:shift + 66667] = logits
-        on = wide.to(dev)[:, shift:shift + 66667]
+        wide = torch.full((5, 98333 + 8), math.inf, dtype=dtype)
+        wide[:, shift:shift + 98333] = logits
+        on = wide.to(dev)[:, shift:shift + 98333]
         check((on, logits), u, dev, top_p=0.9)
         check((on, logits), u, dev, top_k=30)
 
@@ -365,7 +365,7 @@ def test_long_rows_that_are_not_aligned(dtype, dev):
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 def test_long_rows_replayed_and_on_two_streams(dtype, dev):
     from odysseus_transformer_amd import ops
-    sets = [tuple(t.to(dev) for t in _logits(4, 80001, dtype, seed=i)) for i in range(2)]
+    sets = [tuple(t.to(dev) for t in _logits(4, 100001, dtype, seed=i)) for i in range(2)]
     calls = [dict(top_p=0.9), dict(top_k=20), dict()]
     want = [[ops.sample(*s, **c) for c in calls] for s in sets]
     torch.cuda.synchronize()
@@ -395,7 +395,7 @@ def test_long_rows_replayed_and_on_two_streams(dtype, dev):
 def test_long_rows_by_both_host_paths(dev, monkeypatch):
     from odysseus_transformer_amd import _native, ops
     for dtype in (BF16, F32):
-        logits, u = (t.to(dev) for t in _logits(3, 90001, dtype, seed=4))
+        logits, u = (t.to(dev) for t in _logits(3, 100001, dtype, seed=4))
         plain = [ops.sample(logits, u, **c) for c in (dict(top_p=0.9), dict(top_k=30))]
         with monkeypatch.context() as m:
             m.setattr(ops, "native", _native._Nothing())
