@@ -38,7 +38,11 @@ typedef const u32x4 __attribute__((address_space(1)))* vector_ptr;
 constexpr int BUCKETS = 2048, LIST = 4096, OCTAVE = 1024, VALUES = 8192;
 // Threads of a block.  fp32 rows are read and weighed by all that a compute unit has (256 rows of 128000 78 us, 84 by 512; 64 of 32001 23.4 and 25.6).  bf16 by 512, in whose registers short rows stay (512 rows of
 // 32000 30 us, 45 by 1024; 256 of 128000 37.5 and 35.4).
-template <typename T> constexpr int THREADS_OF = sizeof(T) == 4 ? 1024 : 512;
+struct ShortRow {   // fp32, of a short row
+  float x;
+};
+template <typename T> constexpr int THREADS_OF = 512;
+template <> constexpr int THREADS_OF<float> = 1024;
 constexpr int MOST = (1 << 21) - 4;   // tokens of a row: nth_of() counts the matches in each 64 vectors, of 4 values or 8, in 2 * LIST numbers
 
 // What finding the token among listed ones takes: top_p's weights, those before its bucket, before the random number's; of the list those before top_p's bucket
@@ -190,7 +194,10 @@ struct Row {
           mask = 0;
         });
   }
-  __device__ __forceinline__ float value(int i) const { return (float)((const T __attribute__((address_space(1)))*)base)[head + i]; }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (sizeof(T) == 4) return ((const float __attribute__((address_space(1)))*)base)[head + i];
+    else return (float)((const T __attribute__((address_space(1)))*)base)[head + i];
+  }
   // f(x, index) for every x of the row for which keep(x) holds, which are few
   template <typename K, typename F> __device__ __forceinline__ void matches(K keep, F f) const {
     masks(keep, [&](u64 mask, int turn) __attribute__((always_inline)) {
@@ -999,13 +1006,14 @@ __global__ __launch_bounds__(THREADS_OF<bf16>) void sample_values_kernel(const S
 
 // ---- fp32
 // A whole row.
+template <typename T>
 __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const Settings& set, Shared& s) {
   const int tid = threadIdx.x;
-  Row<float> row(static_cast<const float*>(p.logits) + r * p.row_stride, p.vocab);
-  fill_table<float>(s);
-  for (int b = tid; b < BUCKETS; b += THREADS_OF<float>) s.mass[b] = 0, s.count[b] = 0;
+  Row<T> row(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
+  fill_table<T>(s);
+  for (int b = tid; b < BUCKETS; b += THREADS_OF<T>) s.mass[b] = 0, s.count[b] = 0;
   const float largest = largest_of(row, s.wave_max);
-  Sampler<float> a{s, row, set.weights(largest, s.table)};
+  Sampler<T> a{s, row, set.weights(largest, s.table)};
   if (largest == -INFINITY || !(set.temperature > 0.f)) {   // nothing to choose from, or nothing but the first
     write_first(p, r, largest == -INFINITY, largest == -INFINITY ? 0 : a.pick(largest, 1));
     return;
@@ -1026,7 +1034,7 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
       entry = a.among_first(n, set, kept);
     } else {
       __syncthreads();
-      for (int b = tid; b < BUCKETS; b += THREADS_OF<float>) s.count[b] = 0;
+      for (int b = tid; b < BUCKETS; b += THREADS_OF<T>) s.count[b] = 0;
       __syncthreads();
     }
   }
@@ -1044,7 +1052,7 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
       if (last) atomicAdd(&s.count[BUCKETS - 1], last);
     }
     __syncthreads();
-    constexpr int EACH = BUCKETS / THREADS_OF<float>;
+    constexpr int EACH = BUCKETS / THREADS_OF<T>;
     unsigned tokens[EACH];
     u64 weights[EACH], mass_here = 0, tokens_here = 0, m, c = 0, all = 0, heavy;
 #pragma unroll
@@ -1052,10 +1060,10 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
       weights[k] = s.mass[tid * EACH + k], tokens[k] = s.count[tid * EACH + k];
       mass_here += weights[k], tokens_here += tokens[k];
     }
-    m = block_scan<float>(s, mass_here, kept);
-    if (set.cut_k) c = block_scan<float>(s, tokens_here, all);
+    m = block_scan<T>(s, mass_here, kept);
+    if (set.cut_k) c = block_scan<T>(s, tokens_here, all);
     if (set.cut_m) {
-      block_scan<float>(s, over, heavy);
+      block_scan<T>(s, over, heavy);
       over = max(set.one, heavy);   // the first one at any rate
     }
     if (!set.cut_k) {
@@ -1081,9 +1089,10 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int r, const S
   write(p, r, a.w, entry, kept);
 }
 
-__global__ __launch_bounds__(THREADS_OF<float>) void sample_kernel(const SampleParams p) {
+template <typename T>
+__global__ __launch_bounds__(THREADS_OF<T>) void sample_kernel(const SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  sample_row(p, blockIdx.x, Settings(p, blockIdx.x), *reinterpret_cast<Shared*>(smem));
+  sample_row<T>(p, blockIdx.x, Settings(p, blockIdx.x), *reinterpret_cast<Shared*>(smem));
 }
 
 // ---- few long rows: a row in slices, a block each, in launches between which all slices' results are there
@@ -1281,7 +1290,7 @@ __global__ __launch_bounds__(THREADS_OF<float>) void sample_listed_kernel(const 
   if (largest == -INFINITY || !(set.temperature > 0.f)) return;
   const unsigned n = p.listed[r];
   if (!in_slices(set, largest) || n > LIST) {
-    sample_row(p, r, set, s);
+    sample_row<float>(p, r, set, s);
     return;
   }
   Row<float> row(static_cast<const float*>(p.logits) + r * p.row_stride, p.vocab);
@@ -1301,6 +1310,8 @@ template <typename T, typename K> int launch(K kernel, const SampleParams& p, in
   return ody_check_launch("sample");
 }
 
+// fp32 rows of fewer logits go by 512 threads, whose barriers and joined results cost less (us by 512 / 1024: 64 rows of 4000 10.6 / 12.0, of 12000 14.7 / 14.9, of 24000 19.8 / 19.1).
+constexpr int SHORT = 12288;
 // How rows are divided: long ones into slices, at most one a compute unit; of bf16 fewer, as each block reads the counts of all.  us by a block a row / in slices, top_p 0.9 (fp32 also with top_k 20): fp32,
 // one row of 70000 32.8 / 25.0 (19.1 / 20.2), of 250000 87.5 / 28.0 (47.3 / 21.1); 16 of 128000 52.6 / 32.8, 64 54.6 / 40.6, 128 61.6 / 59.8 (36.5 / 45.1); bf16, one of 70000 19.8 / 16.9, of 250000
 // 42.9 / 19.5; 8 of 128000 30.0 / 19.9, 64 34.3 / 26.4, 128 35.4 / 28.9.
@@ -1346,7 +1357,7 @@ extern "C" int ody_sample(const void* logits, const float* u, const float* tempe
                        std::min(50, 62 - bits), q.slices, q.slice, reinterpret_cast<u64*>(ws + q.mass), reinterpret_cast<u64*>(ws + q.over), reinterpret_cast<unsigned*>(ws), reinterpret_cast<int2*>(ws + q.ends),
                        reinterpret_cast<float*>(ws + q.largest), reinterpret_cast<unsigned*>(ws + q.listed), reinterpret_cast<RowEnds*>(ws + q.ends), reinterpret_cast<u64*>(ws)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == ODY_F32 && q.slices == 1) return launch<float>(&sample_kernel, p, rows, st);
+  if (dtype == ODY_F32 && q.slices == 1) return vocab < SHORT ? launch<ShortRow>(&sample_kernel<ShortRow>, p, rows, st) : launch<float>(&sample_kernel<float>, p, rows, st);
   if (dtype == ODY_F32) {
     ODY_LAUNCH("sample_largest", st, sample_largest_kernel, dim3((unsigned)(rows * q.slices)), dim3(THREADS_OF<float>), 0, p);
     if (int rc = ody_check_launch("sample_largest")) return rc;
