@@ -467,8 +467,9 @@ int ody_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, c
  *             of all that top_k keeps (1 or more: all), and their own is at least min_p (0 or less: all).  tokens (rows): the first in the order with which the
  *             weights kept so far sum up to more than u times all that are kept; logprobs (rows): the logarithm of its share of those.  temperature 0, below 0 or NaN:
  *             the first, with logprob 0.  NaN logits count as -inf; +inf ones are equals with all of the weight; a row of nothing but -inf gives -1 and -inf.
- *             temperature, top_k, top_p, min_p: (rows) each, or NULL: the number for all.  Sums are of whole multiples of 2^(log2(vocab) - 62) or less, rounded up: the same
- *             for any order of summation.  rows < 2^22, vocab <= 2^21 - 4; logits aligned to their size.
+ *             temperature, top_k, top_p, min_p: (rows) each, or NULL: the number for all.  Weights are whole multiples of 2^-f, f the largest up to 50 with
+ *             (vocab + 1) 2^f < 2^64 (47 for 128000), so sums are the same for any order of summation; a sum is off by 2^-37 of itself and vocab 2^-(f + 1) at most, of a largest
+ *             weight of 1, and a token's share ends as near to where it should.  rows < 2^22, vocab <= 2^21 - 4; logits aligned to their size.
  *             Reads 16-byte pieces that hold at least one logit of the row.  workspace: ody_sample_workspace_bytes, 0 where a block has a row, 256-byte aligned.
  */
 int ody_sample(const void* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p,

@@ -11,9 +11,10 @@
 //
 // What is gathered and too many to be ordered is divided by the bits of x, until it is few or has one value.
 //
-// Weights are whole numbers of 2^-FRAC (FRAC = 62 - log2 of the row's length, 45 for a vocabulary of 128000): sums in any order, by atomics too, are the same.  They are formed in 64 bits, whose
-// vector rate is that of 32 here, as 2^-(n / 1024) 2^(-r / 1024), |r| <= 1 / 2, from a table and a polynomial of the second degree: off by 2^-37 of themselves, so that a place is
-// missed where a random number is as near to a border of its share as that.
+// Weights are whole numbers of 2^-FRAC: sums in any order, by atomics too, are the same.  FRAC is 50, or, for rows beyond 16382, what is left of 64 bits for a sum of all weights, of at most 1, and one more:
+// 47 for a vocabulary of 128000, 43 for the longest rows.  They are formed in 64 bits, whose vector rate is that of 32 here, as 2^-(n / 1024) 2^(-r / 1024), |r| <= 1 / 2, from a table and a polynomial of the
+// second degree: off by 2^-37 of themselves and by half of 2^-FRAC.  Both can have one direction in all of a tail of equals, so that a sum is off by 2^-37 of itself and vocab 2^-(FRAC + 1), 2^-31 for
+// 128000 and 2^-23 for the longest rows, where the largest weight is 1: as near to a border of its share a random number may give the token on its other side.
 //
 // A block has a row.  bf16: counting is one pass, finding the tokens of the value that the place is in another; up to 32 754 tokens the row stays in registers between them, a longer one is read again
 // from its end, of which the caches have more.  fp32: the largest, then sums (or counts), then what is gathered, each a pass.
@@ -1350,11 +1351,10 @@ extern "C" int ody_sample(const void* logits, const float* u, const float* tempe
   const Plan q = plan(rows, vocab, dtype);
   ODY_REQUIRE(q.bytes == 0 || (workspace && workspace_bytes >= q.bytes && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0), ODY_ERR_WORKSPACE,
               "ody_sample: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", q.bytes, workspace_bytes);
-  int bits = 0;
-  while (1 << bits < vocab) bits++;
+  const int frac = std::min(50, __builtin_clzll((u64)vocab + 1));   // (vocab + 1) 2^frac is below 2^64
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const SampleParams p{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, tokens, logprobs, vocab,
-                       std::min(50, 62 - bits), q.slices, q.slice, reinterpret_cast<u64*>(ws + q.mass), reinterpret_cast<u64*>(ws + q.over), reinterpret_cast<unsigned*>(ws), reinterpret_cast<int2*>(ws + q.ends),
+                       frac, q.slices, q.slice, reinterpret_cast<u64*>(ws + q.mass), reinterpret_cast<u64*>(ws + q.over), reinterpret_cast<unsigned*>(ws), reinterpret_cast<int2*>(ws + q.ends),
                        reinterpret_cast<float*>(ws + q.largest), reinterpret_cast<unsigned*>(ws + q.listed), reinterpret_cast<RowEnds*>(ws + q.ends), reinterpret_cast<u64*>(ws)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == ODY_F32 && q.slices == 1) return vocab < SHORT ? launch<ShortRow>(&sample_kernel<ShortRow>, p, rows, st) : launch<float>(&sample_kernel<float>, p, rows, st);

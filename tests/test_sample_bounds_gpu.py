@@ -1,0 +1,58 @@
+"""How near a chosen token is to the border of its share."""
+import pytest
+import torch
+
+from test_sample_gpu import BF16, F32, check
+
+pytestmark = pytest.mark.gpu
+
+
+def unit(vocab):
+    """What a weight is a whole number of: 2^-50, or what the sums of a long row leave of 64 bits -- its weights, of at most 1, and one more."""
+    frac = 50
+    while (vocab + 1) << frac >= 1 << 64:
+        frac -= 1
+    return 2.0 ** -frac
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [2 ** 21 - 4, 262144, 131072, 128000, 40000])
+def test_a_peak_and_a_flat_tail(vocab, dtype, dev):
+    """A token of weight 1 and many of one small weight, which are all off in the same direction: by half a unit each, and by 2^-37 of themselves.  So is a sum by as much
+    for each of its weights, of a total of 1 at least; a share by that twice, the log-probability once."""
+    from odysseus_transformer_amd import ops
+    d = 29.0
+    falls = torch.arange(32.55, 47.0, 0.5, dtype=torch.float64)                      # the tail's weights are 2^-these
+    temperature = (d / (falls * torch.log(torch.tensor(2.0, dtype=torch.float64)))).float()
+    draws = torch.tensor([1 - 2 ** -24, 1 - 2 ** -23, 1 - 2 ** -20, 0.5, 0.0])
+    for u in draws:
+        x = torch.full((1, vocab), 1.0, dtype=dtype)
+        x[0, vocab // 3] = 1.0 + d
+        on = x.to(dev)
+        for t in temperature:
+            tokens, logs = (y.cpu() for y in ops.sample(on, u[None].to(dev), temperature=float(t)))
+            w = torch.exp(torch.tensor(-d, dtype=torch.float64) / t.double())
+            tail = (vocab - 1) * w
+            total = 1 + tail
+            off = (vocab - 1) * unit(vocab) / 2 + tail * 2 ** -37
+            token = int(tokens[0])
+            if token == vocab // 3:
+                before, upto, log = 0.0, 1.0 / total, -torch.log1p(tail)
+            else:
+                rank = token + 1 if token < vocab // 3 else token                  # in the tail, from 1
+                before, upto, log = (1 + (rank - 1) * w) / total, (1 + rank * w) / total, torch.log(w) - torch.log1p(tail)
+            assert before - 2 * off <= float(u) <= upto + 2 * off, (vocab, float(t), float(u), token)
+            # half a step of 32 bits; the power that the total's logarithm is corrected by is off by 2^-37 too
+            assert abs(float(logs[0].double() - log)) <= off + 2 ** -24 * abs(float(log)) + 2 ** -36.5, (vocab, float(t), float(u), float(logs[0]), float(log))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [2 ** 16 - 1, 2 ** 17 - 2, 2 ** 17 - 1, 2 ** 17, 2 ** 20 - 1])
+def test_sums_of_nearly_64_bits(vocab, dtype, dev):
+    """Rows of equals, whose weights are all 1, and of infinite ones: their sums are the largest that a row of its length can have."""
+    u = torch.tensor([0.0, 0.25, 0.5, 0.99, 1 - 2 ** -24, 1.0])
+    zeros = torch.zeros((6, vocab), dtype=dtype)
+    for logits in (zeros, zeros + 3.5, zeros - 200.0, torch.full_like(zeros, float("inf"))):
+        check(logits, u, dev)
+        check(logits, u, dev, top_p=0.75)
+        check(logits, u, dev, top_k=vocab - 1, min_p=1.0)
