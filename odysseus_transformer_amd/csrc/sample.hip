@@ -13,7 +13,7 @@
 //
 // Weights are whole numbers of 2^-FRAC: sums in any order, by atomics too, are the same.  FRAC is 50, or, for rows beyond 16382, what is left of 64 bits for a sum of all weights, of at most 1, and one more:
 // 47 for a vocabulary of 128000, 43 for the longest rows.  They are formed in 64 bits, whose vector rate is that of 32 here, as 2^-(n / 1024) 2^(-r / 1024), |r| <= 1 / 2, from a table and a polynomial of the
-// second degree: off by 2^-37 of themselves and by half of 2^-FRAC.  Both can have one direction in all of a tail of equals, so that a sum is off by 2^-37 of itself and vocab 2^-(FRAC + 1), 2^-31 for
+// second degree (bf16: of the third, for what a value's weight is times a factor for each of up to fifteen steps): off by 2^-37 of themselves at most and by half of 2^-FRAC.  Both can have one direction in all of a tail of equals, so that a sum is off by 2^-37 of itself and vocab 2^-(FRAC + 1), 2^-31 for
 // 128000 and 2^-23 for the longest rows, where the largest weight is 1: as near to a border of its share a random number may give the token on its other side.
 //
 // A block has a row.  bf16: counting is one pass, finding the tokens of the value that the place is in another; up to 32 754 tokens the row stays in registers between them, a longer one is read again
@@ -287,12 +287,12 @@ struct Weights {
   // of a bucket by the value alone: 64 of them for 1
   __device__ __forceinline__ float plain(float x) const { return (topf - x) * 64.f; }
   __device__ __forceinline__ unsigned plain_bucket(float x) const { return (unsigned)fminf(plain(x), (float)(BUCKETS - 1)); }
-  // 2^(-t / OCTAVE), 0 <= t; n: t to the nearest
-  __device__ __forceinline__ double power(double t, unsigned& n) const {
+  // 2^(-t / OCTAVE), 0 <= t; n: t to the nearest.  TERMS of the series: two leave 2^-37, three 2^-48
+  template <int TERMS = 2> __device__ __forceinline__ double power(double t, unsigned& n) const {
     double r;
     n = nearest(t, r);
     constexpr double L = -0.6931471805599453 / OCTAVE;
-    const double p = fma(fma(L * L / 2, r, L), r, 1.0);
+    const double p = fma(fma(TERMS == 3 ? fma(L * L * L / 6, r, L * L / 2) : L * L / 2, r, L), r, 1.0);
     u64 e = __builtin_bit_cast(u64, table[n % OCTAVE]);
     e = (u64)((unsigned)(e >> 32) - (n / OCTAVE << 20)) << 32 | (unsigned)e;
     return __builtin_bit_cast(double, e) * p;
@@ -860,8 +860,9 @@ __device__ __forceinline__ bool choose_value(const Settings& set, Shared& s, S& 
   double first = 0.0, ratio = 0.0;   // of value `skip`; of a step of this exponent
   if (__any(tokens_here != 0)) {
     unsigned n;
-    first = a.w.power(a.w.steps(fminf(x0, top)), n);
-    ratio = a.w.power(fmin(__builtin_bit_cast(double, (u64)(1023 - 134 + (bits >> 7)) << 52) * a.w.c, 60.0 * OCTAVE), n);
+    // (up to fifteen factors' errors add up in a weight: three terms, for 2^-44)
+    first = a.w.template power<3>(a.w.steps(fminf(x0, top)), n);
+    ratio = a.w.template power<3>(fmin(__builtin_bit_cast(double, (u64)(1023 - 134 + (bits >> 7)) << 52) * a.w.c, 60.0 * OCTAVE), n);
     double weight = first;
 #pragma unroll
     for (int k = 0; k < EACH; k++) {

@@ -56,3 +56,28 @@ def test_sums_of_nearly_64_bits(vocab, dtype, dev):
         check(logits, u, dev)
         check(logits, u, dev, top_p=0.75)
         check(logits, u, dev, top_k=vocab - 1, min_p=1.0)
+
+
+def _near_borders(steps, least, most, seed=1):
+    """Rows of one token of 1 + 15/128 and `others` of 1.0, and a random number of 32 bits that is between 2^least and 2^most of the first one's share away from its border.
+    (The two values lie at the ends of 16 that the kernel for bf16 forms weights of by 15 products with one factor.)"""
+    g = torch.Generator().manual_seed(seed)
+    n = 1 << 21
+    others = torch.randint(50, 3000, (n,), generator=g).double()
+    temperature = (0.3 + 1.2 * torch.rand((n,), generator=g)).float()
+    border = 1 / (1 + others * torch.exp(-(steps / 128.0) / temperature.double()))
+    u = border.float()
+    away = (u.double() / border - 1).abs()
+    those = ((away >= 2.0 ** least) & (away <= 2.0 ** most)).nonzero().flatten()[:400]
+    return others[those].long(), temperature[those], u[those]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_borders_of_shares(dtype, dev):
+    """Random numbers that are 2^-37 to 2^-35.5 of a share away from its border are on the side where 64 bits have them."""
+    others, temperature, u = _near_borders(15, -37.0, -35.5)
+    assert len(u) > 100
+    logits = torch.full((len(u), 3000), -float("inf"))
+    logits[:, 1:] = torch.where(torch.arange(2999)[None, :] < others[:, None], 1.0, -float("inf"))
+    logits[:, 0] = 1.0 + 15 / 128
+    check(logits.to(dtype), u, dev, temperature=temperature)
