@@ -470,7 +470,8 @@ int ody_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, c
  *             temperature, top_k, top_p, min_p: (rows) each, or NULL: the number for all.  Weights are whole multiples of 2^-f, f the largest up to 50 with
  *             (vocab + 1) 2^f < 2^64 (47 for 128000), so sums are the same for any order of summation; a sum is off by 2^-37 of itself and vocab 2^-(f + 1) at most, of a largest
  *             weight of 1, and a token's share ends as near to where it should.  rows < 2^22, vocab <= 2^21 - 4; logits aligned to their size.
- *             Reads 16-byte pieces that hold at least one logit of the row.  workspace: ody_sample_workspace_bytes, 0 where a block has a row, 256-byte aligned.
+ *             Reads 16-byte pieces that hold at least one logit of the row.  workspace: ody_sample_workspace_bytes (for any settings), 0 where
+ *             a block has a row whatever they are, 256-byte aligned.
  */
 int ody_sample(const void* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int rows, int vocab,

@@ -1314,17 +1314,26 @@ template <typename T, typename K> int launch(K kernel, const SampleParams& p, in
 
 // fp32 rows of fewer logits go by 512 threads, whose barriers and joined results cost less (us by 512 / 1024: 64 rows of 4000 10.6 / 12.0, of 12000 14.7 / 14.9, of 24000 19.8 / 19.1).
 constexpr int SHORT = 12288;
-// How rows are divided: long ones into slices, at most one a compute unit; of bf16 fewer, as each block reads the counts of all.  us by a block a row / in slices, top_p 0.9 (fp32 also with top_k 20): fp32,
-// one row of 70000 32.8 / 25.0 (19.1 / 20.2), of 250000 87.5 / 28.0 (47.3 / 21.1); 16 of 128000 52.6 / 32.8, 64 54.6 / 40.6, 128 61.6 / 59.8 (36.5 / 45.1); bf16, one of 70000 19.8 / 16.9, of 250000
-// 42.9 / 19.5; 8 of 128000 30.0 / 19.9, 64 34.3 / 26.4, 128 35.4 / 28.9.
+// How rows are divided: long ones into slices, at most one a compute unit; of bf16 fewer, as each block reads the counts of all.  us by a block a row / in slices, top_p 0.9: fp32,
+// one row of 66000 31.8 / 24.3, of 80000 34.6 / 23.7, of 250000 87.5 / 28.0; 16 of 66000 32.0 / 32.2, of 80000 35.8 / 32.3, of 128000 52.6 / 32.8; 64 of 80000 37.2 / 32.5, of 128000 54.6 / 40.6, 128 61.6 / 59.8;
+// bf16, one of 70000 19.8 / 16.9, of 250000 42.9 / 19.5; 8 of 128000 30.0 / 19.9, 64 34.3 / 26.4, 128 35.4 / 28.9.
+// fp32 rows of a small top_k and greedy ones are read twice and little else: in slices from FEW on (one of 66000 with top_k 20 18.5 / 19.5, of 98000 22.9 / 19.6, of 250000 47.3 / 21.1; 16 of 66000 19.1 / 24.4,
+// of 98000 23.4 / 24.5; greedy, one of 70000 10.3 / 12.1), if one number for all says so; where each has its own they may all be such, and many rows lose more so than others gain (4 of 66000, top_k 0 and 20 in
+// turn 28.7 / 23.7, all 20 18.8 / 20.6; 16 28.9 / 27.7 and 19.0 / 24.4; 64 29.0 / 29.6 and 19.0 / 23.6).  A large top_k for all is nothing for slices (in_slices): one row of 70000 with top_k 4000 57.3 / 65.8.
+constexpr int LONG = 65536, FEW = 98304;
+int least_of(int rows, int vocab, bool greedy, bool each, int top_k) {   // the least of fp32 rows that go in slices
+  if (greedy || (each && rows >= 16)) return FEW;
+  if (each || top_k <= 0 || top_k >= vocab) return LONG;
+  return top_k <= LIST / 2 ? FEW : vocab + 1;
+}
 struct Plan {
   int slices, slice;
   size_t ends, mass, over, largest, listed, bytes;   // places in the workspace, behind the lists (fp32) or the counts (bf16)
 };
-Plan plan(int rows, int vocab, int dtype) {
+Plan plan(int rows, int vocab, int dtype, int least) {
   Plan q{};
   q.slices = std::min(dtype == ODY_F32 ? 16 : rows > 8 ? 4 : 8, 256 / rows);
-  if (dtype == ODY_F32 ? q.slices < 4 || vocab < 98304 : q.slices < 2 || vocab < 65536) return Plan{1, vocab, 0, 0, 0, 0, 0, 0};
+  if (vocab < least || q.slices < (dtype == ODY_F32 ? 4 : 2)) return Plan{1, vocab, 0, 0, 0, 0, 0, 0};
   q.slice = ((vocab + q.slices - 1) / q.slices + 7) / 8 * 8;
   q.slices = (vocab + q.slice - 1) / q.slice;
   const size_t all = (size_t)rows * q.slices;
@@ -1339,7 +1348,7 @@ Plan plan(int rows, int vocab, int dtype) {
 
 }  // namespace
 
-extern "C" size_t ody_sample_workspace_bytes(int rows, int vocab, int dtype) { return rows > 0 && vocab > 0 ? plan(rows, vocab, dtype).bytes : 0; }
+extern "C" size_t ody_sample_workspace_bytes(int rows, int vocab, int dtype) { return rows > 0 && vocab > 0 ? plan(rows, vocab, dtype, LONG).bytes : 0; }
 
 extern "C" int ody_sample(const void* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                           float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int rows, int vocab,
@@ -1349,7 +1358,7 @@ extern "C" int ody_sample(const void* logits, const float* u, const float* tempe
   ODY_REQUIRE(row_stride >= vocab || rows == 1, ODY_ERR_BAD_SHAPE, "ody_sample: rows overlap (stride %lld)", (long long)row_stride);
   ODY_REQUIRE(dtype == ODY_BF16 || dtype == ODY_F32, ODY_ERR_UNSUPPORTED, "ody_sample: dtype %d unknown", dtype);
   ODY_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (dtype == ODY_BF16 ? 1 : 3)) == 0, ODY_ERR_MISALIGNED, "ody_sample: logits are not aligned to their size");
-  const Plan q = plan(rows, vocab, dtype);
+  const Plan q = plan(rows, vocab, dtype, dtype == ODY_F32 ? least_of(rows, vocab, !temperature && !(temperature_all > 0.f), top_k != nullptr, top_k_all) : LONG);
   ODY_REQUIRE(q.bytes == 0 || (workspace && workspace_bytes >= q.bytes && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0), ODY_ERR_WORKSPACE,
               "ody_sample: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", q.bytes, workspace_bytes);
   const int frac = std::min(50, __builtin_clzll((u64)vocab + 1));   // (vocab + 1) 2^frac is below 2^64

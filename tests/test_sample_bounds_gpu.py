@@ -1,8 +1,8 @@
-"""How near a chosen token is to the border of its share."""
+"""How near a chosen token is to the border of its share, and which launches a call makes."""
 import pytest
 import torch
 
-from test_sample_gpu import BF16, F32, check
+from test_sample_gpu import BF16, F32, _logits, check
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,28 @@ def test_borders_of_shares(dtype, dev):
     logits[:, 1:] = torch.where(torch.arange(2999)[None, :] < others[:, None], 1.0, -float("inf"))
     logits[:, 0] = 1.0 + 15 / 128
     check(logits.to(dtype), u, dev, temperature=temperature)
+
+
+@pytest.mark.parametrize("rows,vocab,settings,sliced", [
+    (1, 70000, dict(), True), (1, 70000, dict(top_p=0.9), True), (16, 70000, dict(top_p=0.9), True), (65, 70000, dict(), False), (1, 70000, dict(top_k=20), False),
+    (1, 70000, dict(top_k=2049), False), (1, 65535, dict(), False), (3, 70000, dict(top_k="each"), True), (16, 70000, dict(top_k="each"), False), (16, 98304, dict(top_k="each"), True),
+    (1, 98304, dict(top_k=20), True), (1, 98303, dict(top_k=2048), False), (1, 250000, dict(top_k=4000), False), (1, 250000, dict(top_k=250000), True),
+    (1, 250000, dict(top_k=2 ** 31 - 1), True), (1, 250000, dict(temperature=0.0, top_k=4000), True), (1, 70000, dict(temperature=0.0), False),
+    (2, 250000, dict(temperature="each", top_k=4000), False)], ids=str)
+def test_which_rows_go_in_slices(rows, vocab, settings, sliced, dev):
+    """Long fp32 rows: from 65536 logits on, from 98304 on where they are known to be read and little else, not with a top_k that slices can do nothing with."""
+    from odysseus_transformer_amd import _lib, ops
+    logits, u = _logits(rows, vocab, F32, seed=vocab)
+    own = torch.arange(rows)
+    given = {"top_k": (own % 3 * 30).to(torch.int32), "temperature": 1.0 - own % 2}
+    settings = {k: given[k] if v == "each" else v for k, v in settings.items()}
+    check(logits, u, dev, **settings)
+    on = logits.to(dev), u.to(dev), {k: v.to(dev) if torch.is_tensor(v) else v for k, v in settings.items()}
+    _lib.profile_enable(True)
+    try:
+        ops.sample(on[0], on[1], **on[2])
+        torch.cuda.synchronize()
+        launches = _lib.profile_collect()
+    finally:
+        _lib.profile_enable(False)
+    assert ("sample_largest" in launches) == sliced and sum(n for n, _, _ in launches.values()) == (4 if sliced else 1), launches
