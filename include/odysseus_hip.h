@@ -430,16 +430,17 @@ int ody_paged_attn(const void* q, const void* k_pages, const void* v_pages, cons
 
 /* ---- a cache in pages that holds its values in 8 bits -----------------------
  * As above, with pages of e4m3 values (1 byte; no infinities, 448 the largest) and a power of two for each block of tokens and head: the value at a place is
- * its e4m3 value times 2^(byte - 127), bytes from 1 to 254.
+ * its e4m3 value times 2^(byte - 127), bytes from 1 to 254.  fp32 has them all, bf16 those of bytes from 3 on (under 1 and 2 some multiples of 2^-135 and 2^-134 lie between its
+ * smallest numbers); values of 2^128 and more, under bytes from 247 on, are infinite in both.
  * k_scales, v_scales  (pages, page_size / block, Hkv) bytes, strides s*z_p (page), s*z_b (block of a page), s*z_h (head).  block: a power of two from 8 to 64,
  *                     at most page_size.
  * ody_paged_append_q8 as ody_paged_append.  2^e of a block and head: the least with e >= -126 and max |x| <= 448 * 2^e over the finite values of its tokens there; with
  *                     earlier tokens in the block at least what it was.  Values x 2^-e are rounded to the nearest e4m3 value, half way to the even one; one that is
- *                     not finite becomes NaN.  Rotated keys are rounded to 32 bits in between and not to `dtype`.  Where earlier tokens are in a block whose e rises, their
+ *                     not finite becomes NaN (a finite one from 1.9375 * 2^127 on 2^128).  Rotated keys are rounded to 32 bits in between and not to `dtype`.  Where earlier tokens are in a block whose e rises, their
  *                     rows are rounded to the new one (exact, but for values below 2^-6 of the scale).  Fewer than 2^24 tokens and 2^23 blocks of them a call.
- * ody_paged_read_q8   k, v (S, places, Hkv, D) of `dtype`, contiguous: the values of places 0 .. places - 1, exactly; 0 behind a sequence's length and where there
- *                     is no page.  S < 65536, places * Hkv < 2^31.
- * ody_paged_attn_q8   as ody_paged_attn, q and out of `dtype`; values are converted to it, exactly, in front of the products.
+ * ody_paged_read_q8   k, v (S, places, Hkv, D) of `dtype`, contiguous: the values of places 0 .. places - 1, exactly where `dtype` has them and else the nearest number
+ *                     of it, half way to the even one; 0 behind a sequence's length and where there is no page.  S < 65536, places * Hkv < 2^31.
+ * ody_paged_attn_q8   as ody_paged_attn, q and out of `dtype`; values are converted to it, as they are read back, in front of the products.
  * Pages and their strides on 16 bytes, pages and the rows of a page less than 4 GiB apart, as above; scales need no alignment.
  */
 int ody_paged_append_q8(const void* qkv, void* q, void* k_pages, void* v_pages, uint8_t* k_scales, uint8_t* v_scales, const int* page_table,

@@ -13,7 +13,8 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float q8_scale(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
-// Four values, exactly: an e4m3 value has four bits, a power of two moves its exponent.
+// Four values, exactly but at the ends of the type: an e4m3 value has four bits, a power of two moves its exponent.  Below bf16's smallest number (scales of 2^-126 and 2^-125) the nearest one,
+// from 2^128 on infinite.
 __device__ __forceinline__ void q8_values(unsigned word, float scale, bf16* to) {
   *reinterpret_cast<bf16x2*>(to) = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, false);
   *reinterpret_cast<bf16x2*>(to + 2) = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, true);

@@ -2,7 +2,7 @@
 //
 // The products and their operands are those of paged_attn.hip, and so is the division of the work: nothing but registers lies between memory and the matrix
 // cores, and a wavefront takes a tile of keys for all rows of a row tile.  A value is converted where it becomes an operand, to the queries' type and with its
-// block's power of two: exactly.  Half the bytes make a tile of twice the keys, two sub-tiles of which each is the contraction of one product with V, so that as many bytes
+// block's power of two: exactly (paged_q8.h: but for the ends of the type).  Half the bytes make a tile of twice the keys, two sub-tiles of which each is the contraction of one product with V, so that as many bytes
 // are under way:
 //
 //      S^T = K Q^T          A: K rows, 16 columns a lane in 16 bytes, which are the lane's of two products (bf16) or sixteen (fp32); Q^T is read in the same order

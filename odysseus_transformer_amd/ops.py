@@ -614,8 +614,9 @@ def paged_append_q8_(qkv, n_heads: int, k_pages, v_pages, k_scales, v_scales, pa
 
 
 def paged_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, lengths, places: int, dtype=torch.bfloat16):
-    """What a cache in 8 bits holds (paged_append_q8_ says what the arguments are): -> k, v (S, places, Hkv, D) of `dtype` (bfloat16 or float32, exactly), the
-    values of each sequence's places 0 .. places - 1, 0 behind its length and where it has no page."""
+    """What a cache in 8 bits holds (paged_append_q8_ says what the arguments are): -> k, v (S, places, Hkv, D) of `dtype` (bfloat16 or float32), the
+    values of each sequence's places 0 .. places - 1, 0 behind its length and where it has no page: exactly where `dtype` has them, which float32 does, and bfloat16 but for some
+    under the two smallest scales, rounded to its smallest numbers.  Values of 2^128 and more are infinite."""
     if k_pages.is_cuda:
         plain = native.paged_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, lengths, places, dtype == torch.float32) \
             if dtype in (torch.bfloat16, torch.float32) else None
