@@ -1,4 +1,4 @@
-"""A cache in 8 bits to the byte: every value under every scale."""
+"""A cache in 8 bits to the byte: every value under every scale, tiles of 256 rows over pages of each size."""
 import math
 
 import pytest
@@ -7,7 +7,7 @@ import torch
 import paged_q8_reference as q8
 import paged_reference as ref
 from paged_q8_reference import E8, F8
-from test_paged_q8_gpu import _to
+from test_paged_q8_gpu import _check_heads, _to
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -72,3 +72,26 @@ def test_attention_over_the_smallest_scales(byte, n, H, D, dtype, dev):
     # beside them half a step of the smallest numbers for the values and for the result
     least = 2.0 ** (-133 + 100) if dtype == BF16 else 2.0 ** (-149 + 100)
     assert ((out[:, :, :1].double().cpu() * 2.0 ** 100 - o).abs() <= ref.attend_bounds(part, o, s, mean, dots)[0] + least).all()
+
+
+@pytest.mark.parametrize("D,page,block", [(128, 16, 16), (128, 64, 64), (128, 64, 32), (128, 8, 8), (128, 128, 64)])
+def test_tiles_of_256_rows_over_pages_of_each_size(D, page, block, dev):
+    """Row tiles of 256, of 64 (sequence, kv head) pairs, which the workspace's size shows: a scale for a whole tile of keys, for half of one, for a group of eight."""
+    from odysseus_transformer_amd import _lib
+    lengths, n, H = [256 + 64, 300, 517, 64, 191, 1, 0, 256 + 65], 256, 8
+    c = q8.make(lengths, n, H, H, D, page, block, BF16, seed=page)
+    c["table"][2, 1] = -1
+    width = c["table"].shape[1]
+    parts = _lib.load().ody_paged_attn_q8_workspace_bytes(len(lengths), n, H, H, D, page, width, 0)
+    assert parts == 256 * 2 * 256 * (D * 4 + 8)                    # 256 blocks, two units each, of 256 rows
+    _check_heads(c, _to(c, dev), dev, (0, 5))
+
+
+@pytest.mark.parametrize("D,page,block", [(64, 16, 16), (64, 64, 64), (64, 8, 8)])
+def test_tiles_of_128_rows_of_heads_of_64(D, page, block, dev):
+    from odysseus_transformer_amd import _lib
+    lengths, n, H = [200, 128, 321, 130, 64, 191, 1, 0], 128, 8
+    c = q8.make(lengths, n, H, H, D, page, block, BF16, seed=page)
+    parts = _lib.load().ody_paged_attn_q8_workspace_bytes(len(lengths), n, H, H, D, page, c["table"].shape[1], 0)
+    assert parts % (2 * 128 * (D * 4 + 8)) == 0 and parts // (2 * 128 * (D * 4 + 8)) == 512
+    _check_heads(c, _to(c, dev), dev, (0, 5))
