@@ -1,4 +1,4 @@
-"""A cache in 8 bits to the byte: every value under every scale, tiles of 256 rows over pages of each size."""
+"""A cache in 8 bits to the byte: every value under every scale, rotated keys as the definition has them, tiles of 256 rows over pages of each size."""
 import math
 
 import pytest
@@ -7,7 +7,7 @@ import torch
 import paged_q8_reference as q8
 import paged_reference as ref
 from paged_q8_reference import E8, F8
-from test_paged_q8_gpu import _check_heads, _to
+from test_paged_q8_gpu import _bytes, _check_heads, _inv_freq, _rows, _to
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -95,3 +95,27 @@ def test_tiles_of_128_rows_of_heads_of_64(D, page, block, dev):
     parts = _lib.load().ody_paged_attn_q8_workspace_bytes(len(lengths), n, H, H, D, page, c["table"].shape[1], 0)
     assert parts % (2 * 128 * (D * 4 + 8)) == 0 and parts // (2 * 128 * (D * 4 + 8)) == 512
     _check_heads(c, _to(c, dev), dev, (0, 5))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("lengths,n,D,block", [([100, 37, 64], 1, 128, 32), ([300, 131, 70], 67, 128, 16), ([700, 513], 500, 64, 64), ([2100], 2100, 128, 8)], ids=str)
+def test_rotated_keys_to_the_byte(lengths, n, D, block, dtype, dev):
+    """The angle is the 32-bit product; its cosine and sine, of 64 bits, are rounded to 32 and then to the type; the rotated key is rounded to 32 bits and then to eight.  (Where 64
+    bits of a cosine come out a last place apart on two machines, one in 2^28 of those of 32 bits differs.)"""
+    from odysseus_transformer_amd import ops
+    Hq, Hkv, page = 3, 3, 64
+    c = q8.make(lengths, n, Hq, Hkv, D, page, block, dtype, seed=n)
+    g, f = _to(c, dev), _inv_freq(D)
+    x, half = c["qkv"], D // 2
+    place = torch.tensor(lengths)[:, None] - n + torch.arange(n)
+    th = (place.clamp(min=0).float()[:, :, None] * f).double()
+    cos, sin = (t(th).float().to(dtype).double()[:, :, None] for t in (torch.cos, torch.sin))
+    keys = x[:, :, Hq:Hq + Hkv].double()
+    a, b = keys[..., :half], keys[..., half:]
+    c["qkv"] = x.double()
+    c["qkv"][:, :, Hq:Hq + Hkv] = torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+    # as they are: rounded to 32 bits, then to eight
+    _, (k_rows, k_scales, _, _), (v_rows, v_scales, _) = q8.append(c, Hq)
+    ops.paged_append_q8_(x.to(dev), Hq, *q8.cache(g), inv_freq=f.to(dev))
+    assert torch.equal(_bytes(g["kz"]), k_scales) and torch.equal(_bytes(g["vz"]), v_scales)
+    assert torch.equal(_rows(g["k8"]), _rows(k_rows)) and torch.equal(_rows(g["v8"]), _rows(v_rows))
