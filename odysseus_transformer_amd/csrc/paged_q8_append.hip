@@ -238,40 +238,37 @@ int by_block(const AppendParams& p, const PagedCache& c, const PagedScales& z, h
   }
 }
 
-// ---- what the cache holds: a thread takes eight values of keys and of values; consecutive threads the columns of a head, heads, places.  Memory is all of it: 16 sequences of up to
-// 4001 tokens, 16 heads of 64, 45 us for 335 MB, 7.4 TB/s, of which 262 written past the caches (62 through them); one of 8191, 8 heads of 128, 9.8 us, 50 MB
-template <typename T> struct Eight { T x[8]; };
+// ---- what the cache holds: a thread takes the keys and the values that make 16 bytes, so that a wavefront writes whole lines; consecutive threads the columns of a head, heads, places.  Memory is all of it:
+// 16 sequences of up to 4001 tokens, 16 heads of 64, 45 us for 335 MB, 7.4 TB/s, of which 262 written past the caches (62 through them); in fp32 89 (eight values a
+// thread, of which either half of a line is a store: 244, and 139 through the caches); one of 8191, 8 heads of 128, 7.3 us, in fp32 13
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_read_q8_kernel(T* k, T* v, const PagedCache cache, const PagedScales z, int places, int Hkv, int S) {
-  constexpr int LANES = D / 8;
+  constexpr int N = 16 / (int)sizeof(T), LANES = D / N;
+  typedef unsigned piece __attribute__((ext_vector_type(N / 4)));
   const int64_t per_sequence = (int64_t)places * Hkv * LANES;
   const int s = blockIdx.y;
   const int length = paged_length(cache, s);
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < per_sequence; at += (int64_t)gridDim.x * 256) {
-    const int row = (int)(at / LANES), col = (int)(at % LANES) * 8, place = row / Hkv, h = row - place * Hkv;
+    const int row = (int)(at / LANES), col = (int)(at % LANES) * N, place = row / Hkv, h = row - place * Hkv;
     int page = -1;
     if (place < length && place >> cache.shift < cache.width) page = cache.table[s * cache.table_stride + (place >> cache.shift)];
-    Eight<T> a{}, b{};
+    T a[N] = {}, b[N] = {};
     if ((unsigned)page < (unsigned)cache.pages) {
       const int r = place & ((1 << cache.shift) - 1);
-      const u32x2 kw = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(cache.k) + page * cache.sk.p + r * cache.sk.r + h * cache.sk.h + col);
-      const u32x2 vw = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(cache.v) + page * cache.sv.p + r * cache.sv.r + h * cache.sv.h + col);
+      const piece kw = *reinterpret_cast<const piece*>(static_cast<const uint8_t*>(cache.k) + page * cache.sk.p + r * cache.sk.r + h * cache.sk.h + col);
+      const piece vw = *reinterpret_cast<const piece*>(static_cast<const uint8_t*>(cache.v) + page * cache.sv.p + r * cache.sv.r + h * cache.sv.h + col);
       const float ks = q8_scale(z.k[page * z.sk.p + (r >> z.shift) * z.sk.r + h * z.sk.h]), vs = q8_scale(z.v[page * z.sv.p + (r >> z.shift) * z.sv.r + h * z.sv.h]);
-      q8_values(kw[0], ks, a.x), q8_values(kw[1], ks, a.x + 4);
-      q8_values(vw[0], vs, b.x), q8_values(vw[1], vs, b.x + 4);
-    }
-    constexpr int PIECES = sizeof(a) / 16;
 #pragma unroll
-    for (int e = 0; e < PIECES; e++) {
-      __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(&a)[e], reinterpret_cast<u32x4*>(k) + (s * per_sequence + at) * PIECES + e);
-      __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(&b)[e], reinterpret_cast<u32x4*>(v) + (s * per_sequence + at) * PIECES + e);
+      for (int e = 0; e < N / 4; e++) q8_values(kw[e], ks, a + 4 * e), q8_values(vw[e], vs, b + 4 * e);
     }
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, a), reinterpret_cast<u32x4*>(k) + s * per_sequence + at);
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, b), reinterpret_cast<u32x4*>(v) + s * per_sequence + at);
   }
 }
 
 template <typename T, int D>
 int launch_read(void* k, void* v, const PagedCache& c, const PagedScales& z, int S, int places, int Hkv, hipStream_t st) {
-  const int64_t blocks = ((int64_t)places * Hkv * (D / 8) + 255) / 256;
+  const int64_t blocks = ((int64_t)places * Hkv * (D * sizeof(T) / 16) + 255) / 256;
   const dim3 grid((unsigned)std::min(blocks, (int64_t)1 << 16), (unsigned)S);
   ODY_LAUNCH("paged_read_q8", st, (paged_read_q8_kernel<T, D>), grid, dim3(256), 0, static_cast<T*>(k), static_cast<T*>(v), c, z, places, Hkv, S);
   return ody_check_launch("paged_read_q8");

@@ -1,0 +1,14 @@
+"""What reading a cache in 8 bits writes past the caches: whole lines."""
+from test_product_distances import _assembly, _kernels
+
+
+def test_reading_back_writes_whole_lines(tmp_path):
+    """A store past the caches is written as it is: the threads of a wavefront write 16 bytes beside one another, one store of keys and one of values each (two stores of a thread
+    that lie side by side leave holes in each other's lines)."""
+    seen = 0
+    for name, code, _ in _kernels(_assembly("paged_q8_append", tmp_path)):
+        if "paged_read_q8" in name:
+            stores = [(op, operands) for op, operands, _ in code if op.startswith(("global_store", "flat_store", "buffer_store"))]
+            assert len(stores) == 2 and all(op == "global_store_dwordx4" and operands[-1].split()[-1] == "nt" for op, operands in stores), (name, stores)
+            seen += 1
+    assert seen == 4
