@@ -212,15 +212,18 @@ int launch(const AppendParams& p, const PagedCache& c, const PagedScales& z, hip
   const unsigned shares = (unsigned)std::max((int64_t)1, std::min({(turns + 3) / 4, (2048 + groups - 1) / groups, (int64_t)65535}));
   const dim3 grid((unsigned)groups, shares);
   // A projection that the last-level cache (256 MB) does not hold along with what else a layer touches is read past the caches, which keep the new rows for who reads them next; a smaller
-  // one lies there (four prompts of 4096 and reading back, 403 MB, 208 -> 193 us; 1324 tokens of 8 MB 11.6 -> 12.7).
-  const bool past = (double)p.S * p.n * (p.Hq + 2 * p.Hkv) * D * sizeof(T) >= 128e6;
+  // one lies there (1324 tokens of 8 MB 11.6 -> 12.7 us so).  Behind the product that writes it, through / past the caches: 402 MB 150.9 / 130.4, 201 MB 76.4 / 73.5, 132 MB 52.0 / 51.7.  Not where half a row,
+  // which a load of several rows takes, is half a line (heads of 64 in bf16, 201 MB: 73.2 / 95.4, each line comes twice).  What is not rotated is read by attention next: past the caches only where they
+  // have none of it then (with reading it once more, 201 MB 123.9 / 129.5, 255 MB 154.3 / 161.6, 294 MB 205.7 / 206.9, 402 MB 287.7 / 282.6).
+  constexpr bool LINES = D / 2 * sizeof(T) >= 128;
+  const bool past = LINES && (double)p.S * p.n * (p.Hq + 2 * p.Hkv) * D * sizeof(T) >= (p.q ? 128e6 : 268e6);
 #define LAUNCH(R, O, P) ODY_LAUNCH("paged_append_q8", st, (paged_append_q8_kernel<T, D, BLOCK, R, O, P>), grid, dim3(256), 0, p, c, z)
   if (p.n == 1) {
     if (p.q) LAUNCH(true, true, false);
     else LAUNCH(false, true, false);
   } else if (past) {
-    if (p.q) LAUNCH(true, false, true);
-    else LAUNCH(false, false, true);
+    if (p.q) LAUNCH(true, false, LINES);
+    else LAUNCH(false, false, LINES);
   } else {
     if (p.q) LAUNCH(true, false, false);
     else LAUNCH(false, false, false);
