@@ -10,10 +10,11 @@
 //
 // on v_mfma_f32_32x32x16_bf16.  The conversions are exact and apply a block's power of two for nothing.  (The product of e4m3 values with scales of their own,
 // v_mfma_scale_f32_32x32x64_f8f6f4, would take K as it is and a query as the sum of two such rows, which is exact; but its sums of 64 come out 2^-18.7 of the sum of
-// their sizes off, root mean square, where this one's are at 2^-27.)
+// their sizes off, root mean square, where this one's are at 2^-27: for rows of unit size less than the 2^-8 by which P is rounded, but all of what lse is off by.  Not taken up.)
 //
 // Each of a block's wavefronts converts all of a tile, half of the vector work: 512 tokens behind 8191 keys, 32 heads on 8 of 128, 106 us (670 TFLOP/s; paged_q8_wide.hip, which converts a value once, 94);
-// heads of 64 65 us.
+// heads of 64 65 us; 128 tokens 43.
+// Of heads of 128, 47 registers go to memory: the loop of plain turns has two accesses a turn, whose wait is one for the direct loads before them too, the other one twelve.
 //
 // P is rounded to bf16 for its product and summed up in fp32 unrounded, as in the attention over contiguous keys.
 #include <cmath>

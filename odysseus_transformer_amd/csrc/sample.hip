@@ -21,7 +21,10 @@
 //
 // Bound by latencies for few rows, a chain of some thirty barriers and LDS reads behind a load: one of 32000 in bf16 13.0 us, of which counting takes 1.8.  For many by LDS atomics and the second
 // reading: 256 of 128000, 37.4 us, of which counting takes 11 (8 atomics a vector, 5.5 of their lanes a cycle and compute unit, as they meet in banks; the bytes take 12.9 at a copy's rate) and the
-// second pass 9.  fp32 by the instructions of the weights, 30 for each: 64 rows of 32001, a third of them without top_k, 23.4 us, of which weights take some 6.
+// second pass 9.  fp32 by the instructions of the weights, 30 for each: 64 rows of 32001, a third of them without top_k, 23.4 us, of which weights take some 6.  A block has
+// 145 KB of LDS, so that a compute unit has one: of more rows than there are the others wait for whole chains (512 rows of 32000 in bf16 28 us, 490 of 11166 in fp32 27).  Lists of more than 256 are sorted with a
+// barrier for each of 45 steps and more (two fp32 rows of 81959, top_k 351 32 us, 1000 37; top_k 200 24.7); an fp32 row with a top_k above 2048 is one block's (250000 logits 148 us).  The blocks of 1024 threads leave 128
+// registers: 18 go to memory.
 //
 // Few long rows would leave most compute units idle: they go in slices, a block each, with what the slices have to know of one another between launches (sums are of whole numbers, so a row's result
 // is the same to the bit).  bf16 in two: counts; then every block adds up the slices' counts, finds the value and whose slice has its token.  fp32 in four: the largest; sums by buckets; what is in the
